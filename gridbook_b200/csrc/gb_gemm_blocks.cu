@@ -1,0 +1,974 @@
+// GEMMs of block-scaled E4M3: D[m, n] = sum over blocks b of 128 columns of
+//     a_scale[m, b] * b_scale[n / 128, b] * sum over k in b of A[m, k] W[n, k],
+// dense, or grouped over expert segments (rows seg[e] .. seg[e + 1] of A times expert e's weights).
+//
+// The scales differ from block to block, so a sum on the tensor cores goes over one block only (four instructions of
+// kind::f8f6f4) and the blocks are added in fp32 registers: every block has an accumulator of its own in tensor memory, a ring
+// of them, and the read-out warps turn each into one multiply-add per element while the next blocks are multiplied.
+//
+// Two kernels.  gemm_blocks_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x 256 or 128 features, activations on
+// the M side, so that a thread holds one row and its scale is one number per block.  gemm_blocks_rows_kernel: few rows; the
+// WEIGHTS are the M side (128 features a CTA, one scale per block for the whole tile), the rows the N side in steps of
+// sixteen, K sliced over a thread-block cluster where there are fewer tiles than SMs.
+#include "gb_common.cuh"
+
+#include <cuda.h>
+#include <atomic>
+#include <mutex>
+
+namespace {
+
+constexpr int kSlab = 128;                           // columns of a block = bytes of K of a stage (one swizzle span)
+constexpr int kBM = 128;                             // rows of an operand tile of a CTA on the M side
+constexpr int kMaxGroups = 1024;                     // experts of one grouped launch
+constexpr int kSegBytes = 2 * (kMaxGroups + 1) * 4 + 8;
+
+struct BlocksParams {
+  int64_t M, N;              // rows of A (grouped: all of them), features (grouped: of an expert)
+  int kb, nb;                // blocks along K, along the features (of an expert)
+  int m_tiles, n_tiles;
+  const float* a_scale;      // [M][kb]
+  const float* b_scale;      // [E][nb][kb]
+  void* D;
+  int out;                   // GB_DTYPE_*
+  int vec4;                  // rows of both scales are whole aligned 16-byte pieces
+  int out_tma, out16;        // 16-bit rows of D that TMA takes; rows of D are whole 16-byte pieces
+  const int32_t* seg;        // [E + 1], or null
+  int E;
+  int beside;                // W, its scales and seg are not written by the launch ahead: read before it has finished
+  uint32_t idesc;            // without M and N
+  int* status;
+  // rows kernel
+  int rows_per_pass, passes, per_slice, slices, stages;
+};
+
+// ---- waits, copies, MMAs -------------------------------------------------------------------------------------
+template <bool kOfPair>
+GB_DEVINL bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  if (kOfPair)
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// A bounded wait that remembers a timeout for the rest of the CTA: later waits return at once.
+template <bool kOfPair>
+__device__ __noinline__ void wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 0; !*abort_flag; ++spin) {
+    if (try_wait<kOfPair>(bar, parity)) return;
+    if ((spin & 255u) == 255u) {
+      const uint64_t now = gb_globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 2000000000ull) { *abort_flag = 1; atomicExch(status, code); }
+    }
+  }
+}
+// By a whole warp that goes on together; false: given up.
+template <bool kOfPair = false>
+GB_DEVINL bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, try_wait<kOfPair>(bar, parity))) return true;
+  wait_slow<kOfPair>(bar, parity, abort_flag, status, code);
+  return !__any_sync(0xffffffffu, *abort_flag != 0);
+}
+GB_DEVINL int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+GB_DEVINL void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+GB_DEVINL void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+GB_DEVINL void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Hands tensor memory from read-out warps of both CTAs to the leader's MMA issuer: ordered by the tensor-memory fences on
+// both sides, so the arrive itself may be relaxed (one that released would wait for the output stores in flight).
+GB_DEVINL void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+GB_DEVINL uint32_t leader_addr(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+GB_DEVINL void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+GB_DEVINL void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+// K-major operand tile stored as rows of 128 bytes with the 128-byte swizzle.
+GB_DEVINL uint64_t desc_sw128(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <int kGroup>
+GB_DEVINL void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
+  if (kGroup == 2)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+template <int kGroup>
+GB_DEVINL void commit_to(uint32_t bar) {
+  if (kGroup == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+GB_DEVINL void commit_pair(uint32_t bar, uint32_t to_peer) {
+  commit_to<2>(bar);
+  commit_to<2>(bar + to_peer);
+}
+GB_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+GB_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr));
+}
+GB_DEVINL void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+GB_DEVINL void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+GB_DEVINL void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Scales of four consecutive blocks, kt .. kt + 3, of a row of `kb`; zeros past its end and for a null row.
+GB_DEVINL float4 scales4(const float* row, int kt, int kb, bool vec4) {
+  if (row == nullptr) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (vec4 && (kt & 3) == 0) return __ldg(reinterpret_cast<const float4*>(row + kt));      // kb is a multiple of four
+  return make_float4(kt < kb ? __ldg(row + kt) : 0.0f, kt + 1 < kb ? __ldg(row + kt + 1) : 0.0f,
+                     kt + 2 < kb ? __ldg(row + kt + 2) : 0.0f, kt + 3 < kb ? __ldg(row + kt + 3) : 0.0f);
+}
+GB_DEVINL float pick(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+GB_DEVINL uint32_t pack2(float a, float b, int out) {
+  if (out == GB_DTYPE_BF16) return gb_pack_bf16x2(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+GB_DEVINL void store1(void* D, int64_t at, float v, int out) {
+  if (out == GB_DTYPE_FP32) static_cast<float*>(D)[at] = v;
+  else if (out == GB_DTYPE_BF16) static_cast<uint16_t*>(D)[at] = (uint16_t)gb_f32_to_bf16_bits(v);
+  else static_cast<uint16_t*>(D)[at] = __half_as_ushort(__float2half_rn(v));
+}
+
+// Segment starts and the number of row tiles in front of each expert, into shared memory, by one warp.
+GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, int* base_s) {
+  const int lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    const int lo = e < p.E ? p.seg[e] : 0, hi = e < p.E ? p.seg[e + 1] : 0;
+    const int tiles = (hi - lo + tile_rows - 1) / tile_rows;
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (e < p.E) {
+      seg_s[e] = lo;
+      base_s[e] = carry + incl - tiles;
+      if (e == p.E - 1) { seg_s[p.E] = hi; base_s[p.E] = carry + incl; }
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+// ======================================== CTA pairs ========================================================
+constexpr int kPairM = 256;                          // rows of a pair's tile
+constexpr int kEpiWarps = 8;                         // two per lane quarter, half of the columns each
+constexpr int kOutChunk = 2048;                      // 32 rows x 32 16-bit columns on their way out
+constexpr int kPairThreads = 32 * (kEpiWarps + 2);
+constexpr int kTmemCols = 512;
+constexpr int kGroupM = 16;                          // row tiles walked together before the next columns (see gb_gemm_pair.cu)
+
+template <int kBN, bool kGrouped>
+struct Pair {
+  static constexpr int kABytes = kBM * kSlab, kBBytes = kBN / 2 * kSlab, kStageBytes = kABytes + kBBytes;
+  static constexpr int kOutBytes = kEpiWarps * 2 * kOutChunk + (kGrouped ? kSegBytes : 0);
+  static constexpr int kStages = (227 * 1024 - 2048 - kOutBytes) / kStageBytes;
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 2048;
+  static constexpr int kAccs = kTmemCols / kBN;
+};
+
+// The tiles of a pair: first, first + stride, ...
+template <int kBN, bool kGrouped>
+struct PairTiles {
+  int tile, stride, e = 0;
+  int m0 = 0, n0 = 0, w0 = 0, end = 0;               // first row, first feature, first weight row, end of the rows that count
+  GB_DEVINL PairTiles(int first, int stride_) : tile(first - stride_), stride(stride_) {}
+  GB_DEVINL bool next(const BlocksParams& p, int total, const int* seg_s, const int* base_s) {
+    tile += stride;
+    if (tile >= total) return false;
+    if (kGrouped) {                                  // features fastest: a row tile's columns run together
+      const int gp = tile / p.n_tiles, nt = tile - gp * p.n_tiles;
+      while (base_s[e + 1] <= gp) ++e;               // experts without rows are stepped over
+      m0 = seg_s[e] + (gp - base_s[e]) * kPairM;
+      end = seg_s[e + 1];
+      n0 = nt * kBN;
+      w0 = e * (int)p.N + n0;
+    } else {
+      const int per = kGroupM * p.n_tiles, g = tile / per, in = tile - g * per;
+      const int rows = min(kGroupM, p.m_tiles - g * kGroupM);
+      m0 = (g * kGroupM + in % rows) * kPairM;
+      n0 = in / rows * kBN;
+      w0 = n0;
+      end = (int)p.M;
+    }
+    return true;
+  }
+};
+
+template <int kBN, bool kGrouped>
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
+                        const __grid_constant__ BlocksParams p) {
+  using S = Pair<kBN, kGrouped>;
+  constexpr int kStages = S::kStages, kAccs = S::kAccs;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
+  uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
+  const uint32_t out_ring = ring + kStages * S::kStageBytes;             // two chunks per read-out warp
+  const uint32_t full_bar = out_ring + (S::kOutBytes + 7) / 8 * 8;       // leader: both CTAs' operand tiles have landed
+  const uint32_t empty_bar = full_bar + 8 * kStages;                     // the MMAs that read the stage are done
+  const uint32_t acc_full = empty_bar + 8 * kStages;                     // [kAccs] a block's sums are complete
+  const uint32_t acc_empty = acc_full + 8 * kAccs;                       // [kAccs] leader: read out by both CTAs
+  const uint32_t slot = acc_empty + 8 * kAccs;
+  volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(ring_ptr + (slot - ring));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
+  int* seg_s = reinterpret_cast<int*>(ring_ptr + (out_ring - ring) + kEpiWarps * 2 * kOutChunk);
+  int* base_s = seg_s + kMaxGroups + 1;
+
+  const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  gb_pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(full_bar + 8 * s, 1);
+      bar_init(empty_bar + 8 * s, 1);
+    }
+    for (int b = 0; b < kAccs; ++b) {
+      bar_init(acc_full + 8 * b, 1);
+      bar_init(acc_empty + 8 * b, 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    gb_fence_barrier_init();
+  }
+  if (warp == kEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"((uint32_t)kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  gb_pdl_wait();
+  if (kGrouped && warp == 0) load_segments(p, kPairM, seg_s, base_s);
+  tmem_fence_before();
+  __syncthreads();
+  gb_cluster_sync();                                                     // both CTAs' barriers exist
+  tmem_fence_after();
+  const uint32_t tmem_base = *slot_ptr;
+  const int total = kGrouped ? base_s[p.E] * p.n_tiles : p.m_tiles * p.n_tiles;
+  const int stride = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
+
+  if (warp == kEpiWarps) {
+    // ------------------------------- producer (each CTA) -------------------------------
+    const uint32_t full_pair = (uint32_t)uniform((int)leader_addr(full_bar));
+    const int me = uniform((int)rank);
+    const bool one = gb_elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (PairTiles<kBN, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+      const int m0 = uniform(T.m0) + me * kBM, w0 = uniform(T.w0) + me * (kBN / 2);
+      for (int kt = 0; kt < p.kb; ++kt) {
+        ok = warp_wait<true>(empty_bar + 8 * s, ph, abort_flag, p.status, 91);
+        if (!ok) break;
+        if (one) {
+          const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
+          if (me == 0) expect_tx(full_bar + 8 * s, 2 * S::kStageBytes);
+          tma_load_pair(st, &map_a, kt * kSlab, m0, full_pair + 8 * s);
+          tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);
+        }
+        __syncwarp();
+        if (++s == kStages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // --------------------------- MMA issuer (the leader's) ------------------------------
+    if (uniform((int)rank) == 0) {
+      uint32_t to_peer;                                      // distance of the peer's barriers
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
+      to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
+      const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
+      const int tiles = uniform(total > first ? (total - first + stride - 1) / stride : 0);
+      const bool one = gb_elect_one();
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 1;
+      for (int64_t left = (int64_t)tiles * p.kb; left > 0; --left) {
+        if (!warp_wait<true>(acc_empty + 8 * buf, acc_ph, abort_flag, p.status, 92)) break;
+        if (!warp_wait<true>(full_bar + 8 * s, ph, abort_flag, p.status, 93)) break;
+        tmem_fence_after();
+        const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
+        const uint64_t da = desc_sw128(st), db = desc_sw128(st + S::kABytes);
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)                        // 32 columns of K per instruction
+            mma<2>(tmem + (uint32_t)(buf * kBN), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), p.idesc, k > 0);
+          commit_pair(empty_bar + 8 * s, to_peer);
+          commit_pair(acc_full + 8 * buf, to_peer);
+        }
+        __syncwarp();
+        if (++s == kStages) { s = 0; ph ^= 1; }
+        if (++buf == kAccs) { buf = 0; acc_ph ^= 1; }
+      }
+    }
+  } else {
+    // ------------------------------- read-out (each CTA) --------------------------------
+    const uint32_t acc_empty_pair = leader_addr(acc_empty);
+    constexpr int kCols = kBN / 2, kChunks = kCols / 32;
+    const int quarter = warp & 3, c_lo = (warp >> 2) * kCols;
+    const uint32_t out = out_ring + (uint32_t)warp * 2 * kOutChunk;
+    const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c_lo;
+    int buf = 0, flip = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (PairTiles<kBN, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+      const int row0 = T.m0 + (int)rank * kBM + quarter * 32, row = row0 + lane, n0 = T.n0 + c_lo;
+      const bool row_ok = row < T.end;
+      const float* as = row_ok ? p.a_scale + (int64_t)row * p.kb : nullptr;
+      // a tile's half lies within one block of features; one past the last is not stored
+      const float* bs = p.b_scale + ((int64_t)(kGrouped ? T.e : 0) * p.nb + min(n0 / kSlab, p.nb - 1)) * p.kb;
+      float acc[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+      float4 as4 = scales4(as, 0, p.kb, p.vec4), bs4 = scales4(bs, 0, p.kb, p.vec4);
+      for (int kt0 = 0; ok && kt0 < p.kb; kt0 += 4) {
+        const float4 sc = make_float4(as4.x * bs4.x, as4.y * bs4.y, as4.z * bs4.z, as4.w * bs4.w);
+        if (kt0 + 4 < p.kb) {                                // the next four blocks' while these are added
+          as4 = scales4(as, kt0 + 4, p.kb, p.vec4);
+          bs4 = scales4(bs, kt0 + 4, p.kb, p.vec4);
+        }
+#pragma unroll 1
+        for (int j = 0; j < 4 && kt0 + j < p.kb; ++j) {
+          const float scale = pick(sc, j);
+          ok = warp_wait<true>(acc_full + 8 * buf, ph, abort_flag, p.status, 94);
+          if (!ok) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t v[32];
+            tmem_ld32(at + (uint32_t)(buf * kBN + 32 * c), v);
+            tmem_wait_ld();
+            if (c == kChunks - 1) {
+              tmem_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_cluster(acc_empty_pair + 8 * buf);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(v[i]), scale, acc[32 * c + i]);
+          }
+          if (++buf == kAccs) { buf = 0; ph ^= 1; }
+        }
+      }
+      if (!ok) break;
+      if (p.out_tma && (!kGrouped || row0 + 32 <= T.end)) {  // dense: what sticks out is not written
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const uint32_t dst = out + (uint32_t)flip * kOutChunk;
+          flip ^= 1;
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");       // the chunk before last has left its buffer
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {                      // 64-byte swizzle: eight rows touch eight bank groups
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack2(acc[32 * c + 8 * q + 2 * i], acc[32 * c + 8 * q + 2 * i + 1], p.out);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(dst + (uint32_t)lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && row0 < T.end && n0 + 32 * c < p.N)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                         ::"l"(reinterpret_cast<uint64_t>(&map_d)), "r"(n0 + 32 * c), "r"(row0), "r"(dst) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else if (row_ok) {
+        const int64_t d = (int64_t)row * p.N + n0;
+        const int cols = (int)min((int64_t)kCols, p.N - n0);
+        if (p.out16 && p.out != GB_DTYPE_FP32) {             // whole 16-byte pieces
+#pragma unroll
+          for (int c = 0; c < kCols; c += 8)
+            if (c < cols)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.D) + d + c) =
+                  make_uint4(pack2(acc[c], acc[c + 1], p.out), pack2(acc[c + 2], acc[c + 3], p.out), pack2(acc[c + 4], acc[c + 5], p.out),
+                             pack2(acc[c + 6], acc[c + 7], p.out));
+        } else if (p.out16) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 4)
+            if (c < cols) *reinterpret_cast<float4*>(static_cast<float*>(p.D) + d + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if (c < cols) store1(p.D, d + c, acc[c], p.out);
+        }
+      }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  tmem_fence_before();
+  __syncthreads();
+  if (*abort_flag) __nanosleep(1000000);                   // loads and MMAs still in flight end before the memory goes
+  gb_cluster_sync();                                       // the peer may still signal barriers here
+  if (warp == kEpiWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols) : "memory");
+}
+
+// ======================================== few rows =========================================================
+constexpr int kMaxStages = 12, kMaxSlices = 8;
+constexpr int kScaleSlots = 4;                       // groups of four blocks whose scales are there ahead of their sums
+
+template <int kR>
+struct Rows {
+  static constexpr int kRead = kR == 16 ? 4 : 8;     // read-out warps: two per lane quarter where there are columns for both
+  static constexpr int kThreads = 32 * (kRead + 3);
+  static constexpr int kMine = kR / 16 / (kRead / 4);          // chunks of sixteen columns of a warp
+  static constexpr int kAccs = kR <= 64 ? 8 : 512 / kR;
+  static constexpr uint32_t kTmem = kAccs * kR < 32 ? 32 : kAccs * kR;
+  static constexpr int kStageBytes = kBM * kSlab + kR * kSlab;
+};
+constexpr int kSmemMax = 224 * 1024;                 // with the static arrays within the 227 KB of a CTA
+
+template <int kR, bool kGrouped>
+__global__ void __launch_bounds__(Rows<kR>::kThreads, 1)
+gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ BlocksParams p) {
+  using S = Rows<kR>;
+  constexpr int kRead = S::kRead, kAccs = S::kAccs, kMine = S::kMine;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_s[kMaxStages], empty_s[kMaxStages], acc_full_s[kAccs], acc_empty_s[kAccs], sc_full_s[kScaleSlots], sc_empty_s[kScaleSlots];
+  __shared__ uint32_t slot_s;
+  __shared__ volatile int abort_s;
+  const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of a cluster
+  uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
+  float* scale_s = reinterpret_cast<float*>(ring_ptr + p.stages * S::kStageBytes);      // [slot][4][kR]
+  int* seg_s = reinterpret_cast<int*>(scale_s + kScaleSlots * 4 * kR);
+  int* base_s = seg_s + kMaxGroups + 1;
+  const uint32_t full_bar = gb_smem_u32(full_s), empty_bar = gb_smem_u32(empty_s), acc_full = gb_smem_u32(acc_full_s),
+                 acc_empty = gb_smem_u32(acc_empty_s), sc_full = gb_smem_u32(sc_full_s), sc_empty = gb_smem_u32(sc_empty_s);
+
+  const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  gb_pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      gb_mbar_init(&full_s[s], 1);
+      gb_mbar_init(&empty_s[s], 1);
+    }
+    for (int b = 0; b < kAccs; ++b) {
+      gb_mbar_init(&acc_full_s[b], 1);
+      gb_mbar_init(&acc_empty_s[b], kRead);
+    }
+    for (int b = 0; b < kScaleSlots; ++b) {
+      gb_mbar_init(&sc_full_s[b], 1);
+      gb_mbar_init(&sc_empty_s[b], kRead);
+    }
+    abort_s = 0;
+    gb_fence_barrier_init();
+  }
+  if (warp == kRead + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gb_smem_u32(&slot_s)), "r"(S::kTmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (!p.beside) gb_pdl_wait();
+  if (kGrouped && warp == 0) load_segments(p, kR, seg_s, base_s);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = (uint32_t)uniform((int)slot_s);
+  // sliced: one item per cluster; otherwise the CTA walks items
+  const int total = kGrouped ? base_s[p.E] * p.n_tiles : p.passes * p.n_tiles;
+  const int slice = (int)blockIdx.y, k_begin = slice * p.per_slice, k_end = min(p.kb, k_begin + p.per_slice), k_n = k_end - k_begin;
+  const int first = (int)blockIdx.x, stride = (int)gridDim.x;
+
+  // What an item is: rows [m0, m0 + rows) of A, features [n0, n0 + 128), weight row of the first.
+  struct Item { int m0, rows, n0, w0, e; };
+  auto item_at = [&](int item, int e) {
+    Item t;
+    if (kGrouped) {
+      const int gp = item / p.n_tiles;
+      while (base_s[e + 1] <= gp) ++e;
+      t.m0 = seg_s[e] + (gp - base_s[e]) * kR;
+      t.rows = min(kR, seg_s[e + 1] - t.m0);
+      t.n0 = (item - gp * p.n_tiles) * kBM;
+      t.e = e;
+      t.w0 = e * (int)p.N + t.n0;
+    } else {
+      const int tile = item / p.passes, pass = item - tile * p.passes;
+      t.m0 = pass * p.rows_per_pass;
+      t.rows = (int)min((int64_t)p.rows_per_pass, p.M - t.m0);
+      t.n0 = t.w0 = tile * kBM;
+      t.e = 0;
+    }
+    return t;
+  };
+
+  float acc[kMine][16];
+  Item last{};
+  if (warp == kRead) {
+    // ------------------------------- producer -----------------------------------
+    const bool one = gb_elect_one();
+    int s = 0, e = 0;
+    uint32_t ph = 1;
+    bool ok = true, waited = !p.beside;
+    for (int item = first; ok && item < total; item += stride) {
+      const Item t = item_at(item, e);
+      e = t.e;
+      const int m0 = uniform(t.m0), w0 = uniform(t.w0);
+      int ahead = 0;                                       // slabs whose weights are on their way already
+      if (!waited) {
+        // the launch ahead still writes the rows: the weights of the first stages need not wait for it
+        for (; ok && ahead < min(p.stages, k_n); ++ahead) {
+          ok = warp_wait(empty_bar + 8 * ahead, 1, &abort_s, p.status, 95);
+          if (ok && one) {
+            expect_tx(full_bar + 8 * ahead, S::kStageBytes);
+            tma_load_2d(ring + (uint32_t)ahead * S::kStageBytes, &map_w, (k_begin + ahead) * kSlab, w0, full_bar + 8 * ahead);
+          }
+          __syncwarp();
+        }
+        gb_pdl_wait();
+        waited = true;
+      }
+      for (int kt = 0; ok && kt < k_n; ++kt) {
+        if (kt >= ahead) ok = warp_wait(empty_bar + 8 * s, ph, &abort_s, p.status, 95);
+        if (!ok) break;
+        if (one) {
+          const uint32_t st = ring + (uint32_t)s * S::kStageBytes, bar = full_bar + 8 * s;
+          if (kt >= ahead) {
+            expect_tx(bar, S::kStageBytes);
+            tma_load_2d(st, &map_w, (k_begin + kt) * kSlab, w0, bar);
+          }
+          tma_load_2d(st + kBM * kSlab, &map_x, (k_begin + kt) * kSlab, m0, bar);
+        }
+        __syncwarp();
+        if (++s == p.stages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == kRead + 1) {
+    // ------------------------------- MMA issuer ---------------------------------
+    const bool one = gb_elect_one();
+    int s = 0, buf = 0, e = 0;
+    uint32_t ph = 0, acc_ph = 1;
+    bool ok = true;
+    for (int item = first; ok && item < total; item += stride) {
+      const Item t = item_at(item, e);
+      e = t.e;
+      const uint32_t idesc = p.idesc | (uint32_t)((uniform(t.rows) + 15) / 16 * 2) << 17 | (uint32_t)(kBM >> 4) << 24;
+      for (int kt = 0; kt < k_n; ++kt) {
+        ok = warp_wait(acc_empty + 8 * buf, acc_ph, &abort_s, p.status, 96);
+        if (!ok) break;
+        ok = warp_wait(full_bar + 8 * s, ph, &abort_s, p.status, 97);
+        if (!ok) break;
+        tmem_fence_after();
+        if (one) {
+          const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
+          const uint64_t dw = desc_sw128(st), dx = desc_sw128(st + kBM * kSlab);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)                      // 32 columns of K per instruction
+            mma<1>(tmem + (uint32_t)(buf * kR), dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, k > 0);
+          commit_to<1>(empty_bar + 8 * s);
+          commit_to<1>(acc_full + 8 * buf);
+        }
+        __syncwarp();
+        if (++s == p.stages) { s = 0; ph ^= 1; }
+        if (++buf == kAccs) { buf = 0; acc_ph ^= 1; }
+      }
+    }
+  } else if (warp == kRead + 2) {
+    // ------------------- scales of the rows times the tile's, four blocks at a time --------------------
+    if (p.beside) gb_pdl_wait();
+    int slot = 0, e = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int item = first; ok && item < total; item += stride) {
+      const Item t = item_at(item, e);
+      e = t.e;
+      const float* bs = p.b_scale + ((int64_t)t.e * p.nb + t.n0 / kSlab) * p.kb;
+      for (int kt = k_begin; kt < k_end; kt += 4) {
+        const float4 b = scales4(bs, kt, p.kb, p.vec4);
+        float4 a[(kR + 31) / 32];
+#pragma unroll
+        for (int i = 0; i < (kR + 31) / 32; ++i) {
+          const int r = i * 32 + lane;
+          a[i] = scales4(r < t.rows ? p.a_scale + (int64_t)(t.m0 + r) * p.kb : nullptr, kt, p.kb, p.vec4);
+        }
+        ok = warp_wait(sc_empty + 8 * slot, ph, &abort_s, p.status, 98);
+        if (!ok) break;
+        float* to = scale_s + slot * 4 * kR;
+#pragma unroll
+        for (int i = 0; i < (kR + 31) / 32; ++i) {
+          const int r = i * 32 + lane;
+          if (r < kR) {
+            to[r] = a[i].x * b.x;
+            to[kR + r] = a[i].y * b.y;
+            to[2 * kR + r] = a[i].z * b.z;
+            to[3 * kR + r] = a[i].w * b.w;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) arrive(sc_full + 8 * slot);
+        if (++slot == kScaleSlots) { slot = 0; ph ^= 1; }
+      }
+    }
+  } else {
+    // ------------------------------- read-out -----------------------------------
+    if (p.beside) gb_pdl_wait();                           // nothing is written before the launch ahead has finished
+    const int quarter = warp & 3, group = warp >> 2;
+    const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
+    int buf = 0, slot = 0, e = 0;
+    uint32_t ph = 0, sc_ph = 0;
+    bool ok = true;
+    for (int item = first; ok && item < total; item += stride) {
+      const Item t = item_at(item, e);
+      e = t.e;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+#pragma unroll
+        for (int c = 0; c < 16; ++c) acc[i][c] = 0.0f;
+      for (int kt = 0; ok && kt < k_n; ++kt) {
+        if ((kt & 3) == 0) {
+          ok = warp_wait(sc_full + 8 * slot, sc_ph, &abort_s, p.status, 99);
+          if (!ok) break;
+        }
+        ok = warp_wait(acc_full + 8 * buf, ph, &abort_s, p.status, 100);
+        if (!ok) break;
+        tmem_fence_after();
+        const float* sc = scale_s + (slot * 4 + (kt & 3)) * kR;
+        uint32_t v[kMine][16];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) tmem_ld16(at + (uint32_t)(buf * kR + (i * (kRead / 4) + group) * 16), v[i]);
+        tmem_wait_ld();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(acc_empty + 8 * buf);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const float4* s4 = reinterpret_cast<const float4*>(sc + (i * (kRead / 4) + group) * 16);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float4 f = s4[c];
+            acc[i][4 * c] = fmaf(__uint_as_float(v[i][4 * c]), f.x, acc[i][4 * c]);
+            acc[i][4 * c + 1] = fmaf(__uint_as_float(v[i][4 * c + 1]), f.y, acc[i][4 * c + 1]);
+            acc[i][4 * c + 2] = fmaf(__uint_as_float(v[i][4 * c + 2]), f.z, acc[i][4 * c + 2]);
+            acc[i][4 * c + 3] = fmaf(__uint_as_float(v[i][4 * c + 3]), f.w, acc[i][4 * c + 3]);
+          }
+        }
+        if (++buf == kAccs) { buf = 0; ph ^= 1; }
+        if ((kt & 3) == 3 || kt + 1 == k_n) {
+          __syncwarp();
+          if (lane == 0) arrive(sc_empty + 8 * slot);
+          if (++slot == kScaleSlots) { slot = 0; sc_ph ^= 1; }
+        }
+      }
+      if (!ok) break;
+      last = t;
+      if (p.slices == 1) {                                 // lane = feature: 64 contiguous bytes a warp and row
+        const int feature = t.n0 + quarter * 32 + lane;
+        if (feature < p.N) {
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const int r0 = (i * (kRead / 4) + group) * 16;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (r0 + c < t.rows) store1(p.D, (int64_t)(t.m0 + r0 + c) * p.N + feature, acc[i][c], p.out);
+          }
+        }
+      }
+    }
+    if (p.slices > 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * kRead) : "memory");     // all of them see the same flag behind it
+  }
+
+  if (p.slices > 1) {
+    // Sums into the shared memory of the CTA that owns the row, [slice][own row][feature], over the operand ring: every CTA
+    // of the cluster has finished its MMAs, and with them its loads.  Rows are owned in sixteens.
+    const bool live = warp < kRead && !abort_s && first < total;
+    const int rows = live ? last.rows : 0, cols = (rows + 15) / 16 * 16;
+    const int own = (cols / 16 + p.slices - 1) / p.slices * 16;
+    const int quarter = warp & 3, group = warp >> 2, feature = quarter * 32 + lane;
+    gb_cluster_sync();
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r0 = (i * (kRead / 4) + group) * 16;
+        if (r0 >= cols) continue;
+        const int to = r0 / own, off = r0 - to * own;
+        uint32_t dst;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                     : "=r"(dst) : "r"(ring + (uint32_t)((slice * own + off) * kBM + feature) * 4u), "r"(to));
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (r0 + c < rows)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + (uint32_t)c * kBM * 4u), "r"(__float_as_uint(acc[i][c])) : "memory");
+      }
+    }
+    gb_cluster_sync();                                     // the last access to another CTA's memory lies in front of it
+    if (live) {
+      const int f = lane * 4, left = (int)min((int64_t)kBM, p.N - last.n0) - f, end = min(own, rows - slice * own);
+      for (int r = warp; r < end; r += kRead) {
+        float sum[4] = {};
+#pragma unroll 4
+        for (int q = 0; q < p.slices; ++q) {
+          float v[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(ring + (uint32_t)((q * own + r) * kBM + f) * 4u));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] += v[i];
+        }
+        const int64_t d = (int64_t)(last.m0 + slice * own + r) * p.N + last.n0 + f;
+        if (p.out16 && left > 0 && p.out != GB_DTYPE_FP32) {
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.D) + d) = make_uint2(pack2(sum[0], sum[1], p.out), pack2(sum[2], sum[3], p.out));
+        } else if (p.out16 && left > 0) {
+          *reinterpret_cast<float4*>(static_cast<float*>(p.D) + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < left) store1(p.D, d + i, sum[i], p.out);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tmem_fence_before();
+  __syncthreads();
+  if (abort_s) __nanosleep(1000000);                       // loads and MMAs still in flight end before the memory goes
+  if (warp == kRead + 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmem) : "memory");
+}
+
+// ======================================== host =============================================================
+std::mutex g_mutex;
+int g_pairs[64][4];                                        // pairs that run at once, per device and kernel (0: not asked)
+std::atomic<bool> g_ready[64];                             // shared-memory limits of the device's kernels are set
+GbClusters g_clusters[8];
+
+int set_limits() {
+#define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)(k), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+  GB_ATTR((gemm_blocks_pair_kernel<256, false>), (Pair<256, false>::kSmem));
+  GB_ATTR((gemm_blocks_pair_kernel<128, false>), (Pair<128, false>::kSmem));
+  GB_ATTR((gemm_blocks_pair_kernel<256, true>), (Pair<256, true>::kSmem));
+  GB_ATTR((gemm_blocks_pair_kernel<128, true>), (Pair<128, true>::kSmem));
+  GB_ATTR((gemm_blocks_rows_kernel<16, false>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<32, false>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<64, false>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<128, false>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, true>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<32, true>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<64, true>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<128, true>), kSmemMax);
+#undef GB_ATTR
+  return GB_OK;
+}
+
+// The limits of the current device, once; callers need not have gone through gb_prepare.
+int ready() {
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  GB_REQUIRE(dev >= 0 && dev < 64, "device %d out of range", dev);
+  if (g_ready[dev].load(std::memory_order_acquire)) return GB_OK;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  const int rc = set_limits();
+  if (rc == GB_OK) g_ready[dev].store(true, std::memory_order_release);
+  return rc;
+}
+
+template <int kBN, bool kGrouped>
+int resident_pairs() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  int& n = g_pairs[dev][(kBN == 256) + 2 * kGrouped];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * 256);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = Pair<kBN, kGrouped>::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_blocks_pair_kernel<kBN, kGrouped>, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
+  }
+  return n;
+}
+
+template <int kBN, bool kGrouped>
+int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
+  using S = Pair<kBN, kGrouped>;
+  const int pairs = resident_pairs<kBN, kGrouped>();
+  if (pairs <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+  p.n_tiles = (int)((p.N + kBN - 1) / kBN);
+  p.m_tiles = (int)((p.M + kPairM - 1) / kPairM);
+  p.idesc = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24);
+  p.out_tma = p.N % 8 == 0 && p.out != GB_DTYPE_FP32;
+  CUtensorMap map_a, map_b, map_d = {};
+  int rc = gb_tensor_map_operand(&map_a, A, p.M, K, 1, kBM);
+  if (rc != GB_OK) return rc;
+  rc = gb_tensor_map_operand(&map_b, W, (kGrouped ? p.E : 1) * p.N, K, 1, kBN / 2);
+  if (rc != GB_OK) return rc;
+  if (p.out_tma) {
+    rc = gb_tensor_map_out(&map_d, p.D, p.M, p.N);
+    if (rc != GB_OK) return rc;
+  }
+  const int64_t tiles = (int64_t)(p.m_tiles + (kGrouped ? p.E : 0)) * p.n_tiles;      // grouped: at least as many as the routing can make
+  GB_REQUIRE(tiles < (1ll << 31), "too many output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
+  gb_count_launch();
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_pair_kernel<kBN, kGrouped>, map_a, map_b, map_d, p));
+  return GB_OK;
+}
+
+template <int kR, bool kGrouped>
+int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
+  using S = Rows<kR>;
+  const int64_t sms = gb_sm_count();
+  if (sms <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+  p.n_tiles = (int)((p.N + kBM - 1) / kBM);
+  int64_t most;                                            // items there can be
+  if (kGrouped) {
+    const int64_t hit = p.M < p.E ? p.M : p.E;
+    most = (p.M / kR + hit) * p.n_tiles;
+  } else {
+    p.passes = (int)((p.M + kR - 1) / kR);
+    p.rows_per_pass = (int)(((p.M + p.passes - 1) / p.passes + 15) / 16 * 16);
+    p.passes = (int)((p.M + p.rows_per_pass - 1) / p.rows_per_pass);
+    most = (int64_t)p.passes * p.n_tiles;
+  }
+  GB_REQUIRE(most < (1ll << 31), "too many output tiles");
+  // K slices: as many as the SMs take, at least four blocks each
+  GbClusters& clusters = g_clusters[(kR == 16 ? 0 : kR == 32 ? 1 : kR == 64 ? 2 : 3) + 4 * kGrouped];
+  int want = 1;
+  for (int n = 2; n <= (kR <= 64 ? kMaxSlices : 4) && most * n <= sms && n * 4 <= p.kb; ++n)
+    if (most <= clusters.ask((const void*)gemm_blocks_rows_kernel<kR, kGrouped>, S::kThreads, kSmemMax, n)) want = n;
+  p.per_slice = (p.kb + want - 1) / want;
+  p.slices = (p.kb + p.per_slice - 1) / p.per_slice;
+  constexpr int kFixed = 1024 + kScaleSlots * 4 * kR * 4 + (kGrouped ? kSegBytes : 0);
+  p.stages = (kSmemMax - kFixed) / S::kStageBytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.idesc = 1u << 4;
+  CUtensorMap map_w, map_x;
+  int rc = gb_tensor_map_operand(&map_w, W, (kGrouped ? p.E : 1) * p.N, K, 1, kBM);
+  if (rc != GB_OK) return rc;
+  rc = gb_tensor_map_operand(&map_x, A, p.M, K, 1, kR);
+  if (rc != GB_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.slices > 1 || most < sms ? most : sms), (unsigned)p.slices);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = kFixed + p.stages * S::kStageBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (gb_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.slices > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1; attr[n].val.clusterDim.y = (unsigned)p.slices; attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  gb_count_launch();
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_rows_kernel<kR, kGrouped>, map_w, map_x, p));
+  return GB_OK;
+}
+
+template <bool kGrouped>
+int run_few(const void* A, const void* W, int64_t K, const BlocksParams& p, int64_t rows, cudaStream_t stream) {
+  if (rows <= 16) return run_rows<16, kGrouped>(A, W, K, p, stream);
+  if (rows <= 32) return run_rows<32, kGrouped>(A, W, K, p, stream);
+  if (rows <= 64) return run_rows<64, kGrouped>(A, W, K, p, stream);
+  return run_rows<128, kGrouped>(A, W, K, p, stream);
+}
+
+int check_blocks(const void* A, const float* as, const void* W, const float* bs, const void* D, int out, int64_t M, int64_t N, int64_t K, int64_t E) {
+  GB_REQUIRE(out >= GB_DTYPE_BF16 && out <= GB_DTYPE_FP32, "unknown dtype %d", out);
+  GB_REQUIRE(M >= 0 && N > 0 && K > 0, "bad shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  GB_REQUIRE(K % 16 == 0, "K=%lld must be a multiple of 16: rows of both operands are fetched in 16-byte pieces", (long long)K);
+  GB_REQUIRE(M < (1ll << 30) && N < (1ll << 30) && K < (1ll << 30) && E * N < (1ll << 31), "dimension too large");
+  if (M == 0) return GB_OK;
+  GB_REQUIRE(A && as && W && bs && D, "null pointer argument");
+  GB_REQUIRE(((uintptr_t)A & 15u) == 0 && ((uintptr_t)W & 15u) == 0, "operands must be 16-byte aligned");
+  GB_REQUIRE(((uintptr_t)D & 15u) == 0, "the output must be 16-byte aligned");
+  GB_REQUIRE((((uintptr_t)as | (uintptr_t)bs) & 3u) == 0, "misaligned scales");
+  return ready();
+}
+
+BlocksParams params(const float* as, const float* bs, void* D, int out, int64_t M, int64_t N, int64_t K, int beside) {
+  BlocksParams p = {};
+  p.M = M; p.N = N;
+  p.kb = (int)((K + kSlab - 1) / kSlab);
+  p.nb = (int)((N + kSlab - 1) / kSlab);
+  p.a_scale = as; p.b_scale = bs;
+  p.D = D; p.out = out;
+  p.vec4 = p.kb % 4 == 0 && (((uintptr_t)as | (uintptr_t)bs) & 15u) == 0;
+  p.out16 = N * (out == GB_DTYPE_FP32 ? 4 : 2) % 16 == 0;
+  p.beside = beside;
+  p.status = gb_status_word();
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const float* w_scale, void* D, int out, int64_t M, int64_t N, int64_t K,
+                       int beside, void* stream) {
+  const int rc = check_blocks(A, a_scale, W, w_scale, D, out, M, N, K, 1);
+  if (rc != GB_OK || M == 0) return rc;
+  const BlocksParams p = params(a_scale, w_scale, D, out, M, N, K, beside);
+  if (M <= 128) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
+  return run_pair<256, false>(A, W, K, p, (cudaStream_t)stream);
+}
+
+int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* W, const float* w_scale, const int32_t* seg_offsets, int64_t E, void* D,
+                               int out, int64_t P, int64_t N, int64_t K, int beside, void* stream) {
+  GB_REQUIRE(E > 0 && E <= kMaxGroups, "expert count %lld outside [1, %d]", (long long)E, kMaxGroups);
+  const int rc = check_blocks(A, a_scale, W, w_scale, D, out, P, N, K, E);
+  if (rc != GB_OK || P == 0) return rc;
+  GB_REQUIRE(seg_offsets != nullptr, "null pointer argument");
+  BlocksParams p = params(a_scale, w_scale, D, out, P, N, K, beside);
+  p.seg = seg_offsets;
+  p.E = (int)E;
+  const int64_t mean = P / E;
+  if (mean <= 64) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
+  return run_pair<256, true>(A, W, K, p, (cudaStream_t)stream);
+}
+
+}  // extern "C"

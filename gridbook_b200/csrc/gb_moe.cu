@@ -24,6 +24,7 @@ moe_route_kernel(const int32_t* __restrict__ ids, int P, int E, int first_expert
     const int id = ids[i] - first_expert;
     const bool live = id >= 0 && id < E;
     if (live) atomicAdd(&cnt[id], 1);
+    else if (inv) inv[i] = -1;
     // combine weight of the pair: the router weight rounded to bf16, zero for a dropped pair
     if (pair_w) pair_w[i] = live ? gb_bf16_bits_to_f32(gb_f32_to_bf16_bits(weights[i])) : 0.0f;
   }
@@ -186,7 +187,10 @@ moe_route_few_kernel(const int32_t* __restrict__ ids, int P, int E, int first_ex
   for (int e = tid; e <= E; e += kRouteThreads) offsets[e] = off[e];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    if (id[j] < 0) continue;
+    if (id[j] < 0) {
+      if (inv && first + 32 * j < P) inv[first + 32 * j] = -1;
+      continue;
+    }
     const int at = off[id[j]] + mine[id[j]] + rank[j];
     order[at] = first + 32 * j;
     if (inv) inv[first + 32 * j] = at;
@@ -303,6 +307,8 @@ route_scatter_kernel(const int32_t* __restrict__ ids, int P, int E, int first_ex
     const int at = wcnt[id * nwarps + warp] + rank;
     order[at] = i;
     if (inv) inv[i] = at;
+  } else if (inv && i < P) {
+    inv[i] = -1;
   }
 }
 

@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <atomic>
@@ -43,7 +44,8 @@ namespace {
   F(gb_moe_gather_rows) F(gb_moe_swiglu_rows) F(gb_moe_gemv) F(gb_moe_gemv_sorted) F(gb_moe_mlp_pairs) \
   F(gb_moe_mlp_pairs_workspace_bytes) F(gb_moe_combine) F(gb_gemv_hinted) F(gb_scales_e4m3) F(gb_moe_route_inv) \
   F(gb_moe_fp4_pass_rows) F(gb_moe_fp4_operand_bytes) F(gb_moe_fp4_rows) F(gb_moe_fp4_swiglu_rows) \
-  F(gb_moe_gemv_fp4) F(gb_moe_gemm_fp4)
+  F(gb_moe_gemv_fp4) F(gb_moe_gemm_fp4) F(gb_fp8_quantize_blocks) F(gb_moe_swiglu_fp8) F(gb_moe_permute_fp8) \
+  F(gb_gemm_fp8_blocks) F(gb_gemm_fp8_blocks_grouped) F(gb_moe_permute) F(gb_moe_unpermute) F(gb_moe_unpermute_grad)
 
 struct Lib {
 #define GB_FN(name) decltype(&::name) name = nullptr;
@@ -693,6 +695,319 @@ struct MoEPlan {
   }
 };
 
+// ------------------------------------------------------------------ block-scaled E4M3
+constexpr int64_t kBlock = 128;
+int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+void need(bool ok, const std::string& what) {
+  if (!ok) throw std::runtime_error(what);
+}
+
+int dtype_code(at::ScalarType t, const char* what) {
+  if (t == at::kBFloat16) return GB_DTYPE_BF16;
+  if (t == at::kHalf) return GB_DTYPE_FP16;
+  if (t == at::kFloat) return GB_DTYPE_FP32;
+  throw py::type_error(std::string(what) + " takes bfloat16, float16 or float32");
+}
+
+// Every tensor of a call lies on the first one's device.
+void same_device(const at::Tensor& first, std::initializer_list<const at::Tensor*> others) {
+  need_cuda(first);
+  for (const at::Tensor* t : others) need(t->device() == first.device(), "all tensors of a call must be on one CUDA device");
+}
+
+// Rows of x's last dimension as the kernels take them: `ld` elements apart, copied where they are not.
+struct RowsOf {
+  at::Tensor t;
+  int64_t M, K, ld;
+  explicit RowsOf(const at::Tensor& x) {
+    need(x.dim() >= 1 && x.size(-1) > 0, "rows of at least one value expected");
+    K = x.size(-1);
+    M = x.numel() / K;
+    const bool rows = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= K;
+    t = rows ? x : x.contiguous();
+    ld = rows ? x.stride(0) : K;
+  }
+};
+
+std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = last;
+  return shape;
+}
+
+using Two = std::tuple<at::Tensor, at::Tensor>;
+
+Two fp8_quantize_blocks(const at::Tensor& x, int rule) {
+  need_cuda(x);
+  const int dt = dtype_code(x.scalar_type(), "the block quantiser");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const RowsOf r(x);
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty(with_last(x, blocks(r.K)), x.options().dtype(at::kFloat));
+  check(L.gb_fp8_quantize_blocks(r.t.data_ptr(), dt, r.ld, r.M, r.K, rule, q.data_ptr(), scale.data_ptr<float>(),
+                                 c10::cuda::getCurrentCUDAStream().stream()));
+  return {q, scale};
+}
+
+const int32_t* offsets_of(const at::Tensor& offsets, const at::Tensor& like, int64_t E) {
+  same_device(like, {&offsets});
+  need(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.is_contiguous() && offsets.numel() >= 2 && (E < 0 || offsets.numel() == E + 1),
+       "offsets: a contiguous int32 tensor of one entry per expert and one more expected");
+  return offsets.data_ptr<int32_t>();
+}
+
+Two moe_swiglu_fp8(const at::Tensor& h, const Opt& offsets, int rule) {
+  need_cuda(h);
+  const int dt = dtype_code(h.scalar_type(), "moe_swiglu_fp8");
+  need(h.dim() == 2 && h.size(1) > 0 && h.size(1) % 2 == 0, "rows of [gate | up] expected");
+  const c10::cuda::CUDAGuard guard(h.device());
+  const RowsOf r(h);
+  const int64_t inter = r.K / 2;
+  const int32_t* live = nullptr;
+  if (offsets.has_value() && offsets->defined()) live = offsets_of(*offsets, h, -1) + offsets->numel() - 1;
+  at::Tensor q = at::empty({r.M, inter}, h.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty({r.M, blocks(inter)}, h.options().dtype(at::kFloat));
+  check(L.gb_moe_swiglu_fp8(r.t.data_ptr(), dt, r.ld, live, r.M, inter, rule, q.data_ptr(), scale.data_ptr<float>(),
+                            c10::cuda::getCurrentCUDAStream().stream()));
+  return {q, scale};
+}
+
+void need_operand(const at::Tensor& v, const at::Tensor& scale, int64_t lead, const std::string& what, bool weight) {
+  if (v.scalar_type() != at::kFloat8_e4m3fn) throw py::type_error(what + ": float8_e4m3fn values expected");
+  if (scale.scalar_type() != at::kFloat) throw py::type_error(what + ": float32 scales expected");
+  need(v.dim() == lead && scale.dim() == lead, what + ": " + std::to_string(lead) + " dimensions expected");
+  for (int64_t i = 0; i < lead; ++i) {
+    const int64_t want = i == lead - 1 || (weight && i == lead - 2) ? blocks(v.size(i)) : v.size(i);
+    need(scale.size(i) == want, what + ": a scale of " + std::to_string(want) + " along dimension " + std::to_string(i) + " expected, got " +
+                                    std::to_string(scale.size(i)));
+  }
+}
+
+at::ScalarType out_type(const c10::optional<at::ScalarType>& given, at::ScalarType otherwise) { return given.has_value() ? *given : otherwise; }
+
+// [.., N] = rows [.., K] . w^T, the rows quantised by the launch in front of the product.
+at::Tensor linear_fp8_blocks(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale, const c10::optional<at::ScalarType>& out_dtype, int rule) {
+  same_device(x, {&w, &w_scale});
+  const int dt = dtype_code(x.scalar_type(), "the block-scaled linear");
+  need_operand(w, w_scale, 2, "weight", true);
+  need(x.dim() >= 1 && x.size(-1) == w.size(1), "activations are rows of " + std::to_string(w.size(1)) + " values");
+  const at::ScalarType ot = out_type(out_dtype, x.scalar_type());
+  const int odt = dtype_code(ot, "the block-scaled linear's output");
+  const c10::cuda::CUDAGuard guard(x.device());
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const int64_t N = w.size(0), K = w.size(1);
+  at::Tensor out = at::empty(with_last(x, N), x.options().dtype(ot));
+  if (out.numel() == 0) return out;
+  const RowsOf r(x);
+  const at::Tensor wc = w.contiguous(), wsc = w_scale.contiguous();
+  Arena a;
+  const int q = a.add(r.M * K), s = a.add(r.M * blocks(K) * 4);
+  a.alloc(x);
+  check(L.gb_fp8_quantize_blocks(r.t.data_ptr(), dt, r.ld, r.M, K, rule, a.ptr(q), a.ptr<float>(s), stream));
+  // copies of the weights were made by the work in front of the quantiser, which waits for it
+  check(L.gb_gemm_fp8_blocks(a.ptr(q), a.ptr<float>(s), wc.data_ptr(), wsc.data_ptr<float>(), out.data_ptr(), odt, r.M, N, K, 1, stream));
+  return out;
+}
+
+at::Tensor gemm_fp8_blocks(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, at::ScalarType out_dtype) {
+  same_device(a, {&a_scale, &b, &b_scale});
+  need_operand(a, a_scale, 2, "a", false);
+  need_operand(b, b_scale, 2, "b", true);
+  need(a.size(1) == b.size(1), "gemm_fp8_blocks: K mismatch " + std::to_string(a.size(1)) + " vs " + std::to_string(b.size(1)));
+  const int odt = dtype_code(out_dtype, "gemm_fp8_blocks' output");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const at::Tensor ac = a.contiguous(), asc = a_scale.contiguous(), bc = b.contiguous(), bsc = b_scale.contiguous();
+  at::Tensor out = at::empty({a.size(0), b.size(0)}, a.options().dtype(out_dtype));
+  if (out.numel() == 0) return out;
+  check(L.gb_gemm_fp8_blocks(ac.data_ptr(), asc.data_ptr<float>(), bc.data_ptr(), bsc.data_ptr<float>(), out.data_ptr(), odt, a.size(0), b.size(0),
+                             a.size(1), 0, c10::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+at::Tensor gemm_fp8_blocks_grouped(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, const at::Tensor& offsets,
+                                   const Opt& given, at::ScalarType out_dtype) {
+  same_device(a, {&a_scale, &b, &b_scale});
+  need_operand(a, a_scale, 2, "a", false);
+  need_operand(b, b_scale, 3, "b", true);
+  need(a.size(1) == b.size(2), "gemm_fp8_blocks_grouped: K mismatch " + std::to_string(a.size(1)) + " vs " + std::to_string(b.size(2)));
+  const int64_t P = a.size(0), E = b.size(0), N = b.size(1), K = a.size(1);
+  const int32_t* seg = offsets_of(offsets, a, E);
+  const c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor out;
+  if (given.has_value() && given->defined()) {
+    out = *given;
+    same_device(a, {&out});
+    need(out.dim() == 2 && out.size(0) == P && out.size(1) == N && out.is_contiguous(), "out: a contiguous [" + std::to_string(P) + ", " + std::to_string(N) + "] expected");
+  } else {
+    out = at::empty({P, N}, a.options().dtype(out_dtype));
+  }
+  const int odt = dtype_code(out.scalar_type(), "gemm_fp8_blocks_grouped's output");
+  if (out.numel() == 0) return out;
+  const at::Tensor ac = a.contiguous(), asc = a_scale.contiguous(), bc = b.contiguous(), bsc = b_scale.contiguous();
+  check(L.gb_gemm_fp8_blocks_grouped(ac.data_ptr(), asc.data_ptr<float>(), bc.data_ptr(), bsc.data_ptr<float>(), seg, E, out.data_ptr(), odt, P, N, K, 0,
+                                     c10::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+// ------------------------------------------------------------------ tokens sorted by expert and back
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& topk_ids, int64_t E, int64_t base) {
+  need_cuda(topk_ids);
+  need(topk_ids.dim() == 2, "expert ids of shape [tokens, top-k] expected");
+  need(!topk_ids.is_floating_point() && !topk_ids.is_complex() && topk_ids.scalar_type() != at::kBool, "expert ids are whole numbers");
+  const int64_t T = topk_ids.size(0), topk = topk_ids.size(1), P = T * topk;
+  need(E >= 1 && E <= 4096 && topk >= 1 && P < (1ll << 30), "1 to 4096 experts, at least one a token and fewer than 2^30 pairs expected");
+  const c10::cuda::CUDAGuard guard(topk_ids.device());
+  const at::Tensor ids = topk_ids.to(at::kInt).contiguous();
+  const auto opt = ids.options();
+  if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
+  at::Tensor counts = at::empty({E}, opt), offsets = at::empty({E + 1}, opt), order = at::empty({P}, opt), place = at::empty({P}, opt), ws;
+  const int64_t bytes = L.gb_moe_route_workspace_bytes(T, topk, E);
+  if (bytes) ws = at::empty({bytes}, opt.dtype(at::kByte));
+  check(L.gb_moe_route_inv(ids.data_ptr<int32_t>(), T, topk, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(),
+                           place.data_ptr<int32_t>(), nullptr, nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+                           c10::cuda::getCurrentCUDAStream().stream()));
+  return {counts, offsets, order, place};
+}
+
+// The sort as the row kernels take it, checked against the rows that come with it.
+struct Sorted {
+  const int32_t *place, *live;
+  int64_t T, topk, P;
+  Sorted(const at::Tensor& places, const at::Tensor& offsets, int64_t topk_, const at::Tensor& like) : topk(topk_), P(places.numel()) {
+    live = offsets_of(offsets, like, -1) + offsets.numel() - 1;
+    same_device(like, {&places});
+    need(places.scalar_type() == at::kInt && places.is_contiguous() && topk >= 1 && P % topk == 0, "place: a contiguous int32 tensor of tokens x top-k expected");
+    T = P / topk;
+    place = places.data_ptr<int32_t>();
+  }
+};
+
+Two moe_permute_fp8(const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk, int rule) {
+  need_cuda(x);
+  const int dt = dtype_code(x.scalar_type(), "moe_permute_fp8");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Sorted s(place, offsets, topk, x);
+  const RowsOf r(x);
+  need(r.M == s.T, std::to_string(s.T) + " tokens expected, got " + std::to_string(r.M));
+  at::Tensor q = at::empty({s.P, r.K}, x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty({s.P, blocks(r.K)}, x.options().dtype(at::kFloat));
+  check(L.gb_moe_permute_fp8(r.t.data_ptr(), dt, r.ld, s.place, s.live, s.T, topk, r.K, rule, q.data_ptr(), scale.data_ptr<float>(),
+                             c10::cuda::getCurrentCUDAStream().stream()));
+  return {q, scale};
+}
+
+at::Tensor permute_rows(const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Sorted s(place, offsets, topk, x);
+  const RowsOf r(x);
+  need(r.M == s.T, std::to_string(s.T) + " tokens expected, got " + std::to_string(r.M));
+  at::Tensor rows = at::empty({s.P, r.K}, x.options());
+  check(L.gb_moe_permute(r.t.data_ptr(), x.element_size(), r.ld, s.place, s.live, s.T, topk, r.K, rows.data_ptr(),
+                         c10::cuda::getCurrentCUDAStream().stream()));
+  return rows;
+}
+
+at::Tensor unpermute_rows(const at::Tensor& y, const at::Tensor& place, const at::Tensor& offsets, int64_t topk, const at::Tensor& w) {
+  const c10::cuda::CUDAGuard guard(y.device());
+  const Sorted s(place, offsets, topk, y);
+  need(y.dim() == 2 && y.size(0) == s.P && y.size(1) > 0, std::to_string(s.P) + " rows expected");
+  const at::Tensor yc = y.contiguous();
+  at::Tensor out = at::empty({s.T, y.size(1)}, y.options());
+  check(L.gb_moe_unpermute(yc.data_ptr(), dtype_code(y.scalar_type(), "moe_unpermute"), s.place, w.defined() ? w.data_ptr<float>() : nullptr, s.T, topk,
+                           y.size(1), out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+void first_derivatives_only() {
+  need(!at::GradMode::is_enabled(), "the sorted rows' gradients have no derivatives of their own (create_graph)");
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct PermuteFn : torch::autograd::Function<PermuteFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+    ctx->save_for_backward({place, offsets});
+    ctx->saved_data["topk"] = topk;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return permute_rows(x, place, offsets, topk);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_derivatives_only();
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor dx;
+    if (grads[0].defined())
+      dx = unpermute_rows(grads[0], saved[0], saved[1], ctx->saved_data["topk"].toInt(), at::Tensor()).view(ctx->saved_data["shape"].toIntVector());
+    return {dx, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+struct UnpermuteOnesFn : torch::autograd::Function<UnpermuteOnesFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+    ctx->save_for_backward({place, offsets});
+    ctx->saved_data["topk"] = topk;
+    return unpermute_rows(y, place, offsets, topk, at::Tensor());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_derivatives_only();
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor dy;
+    if (grads[0].defined()) dy = permute_rows(grads[0], saved[0], saved[1], ctx->saved_data["topk"].toInt());
+    return {dy, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& w, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+    const bool need_y = w.requires_grad();                         // y is kept for the weights' gradient alone
+    ctx->save_for_backward({place, offsets, w, need_y ? y : at::Tensor()});
+    ctx->saved_data["topk"] = topk;
+    return unpermute_rows(y, place, offsets, topk, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_derivatives_only();
+    at::Tensor dy, dw;
+    if (grads[0].defined()) {
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &place = saved[0], &offsets = saved[1], &w = saved[2], g = grads[0].contiguous();
+      const int64_t topk = ctx->saved_data["topk"].toInt(), H = g.size(-1);
+      const c10::cuda::CUDAGuard guard(g.device());
+      const Sorted s(place, offsets, topk, g);
+      at::Tensor y;
+      if (saved[3].defined()) {
+        y = saved[3].contiguous();
+        dw = at::empty(w.sizes(), w.options());
+      }
+      if (ctx->needs_input_grad(0)) dy = at::empty({s.P, H}, g.options());
+      check(L.gb_moe_unpermute_grad(g.data_ptr(), y.defined() ? y.data_ptr() : nullptr, dtype_code(g.scalar_type(), "moe_unpermute"), s.place, s.live,
+                                    w.data_ptr<float>(), s.T, topk, H, dy.defined() ? dy.data_ptr() : nullptr,
+                                    dw.defined() ? dw.data_ptr<float>() : nullptr, c10::cuda::getCurrentCUDAStream().stream()));
+    }
+    return {dy, dw, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor moe_permute(const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+  need_cuda(x);
+  dtype_code(x.scalar_type(), "moe_permute");
+  if (!(at::GradMode::is_enabled() && x.requires_grad())) return permute_rows(x, place, offsets, topk);
+  return PermuteFn::apply(x, place, offsets, topk);
+}
+
+at::Tensor moe_unpermute(const at::Tensor& y, const at::Tensor& place, const at::Tensor& offsets, int64_t topk, const Opt& weights) {
+  need_cuda(y);
+  dtype_code(y.scalar_type(), "moe_unpermute");
+  at::Tensor w;
+  if (weights.has_value() && weights->defined()) {
+    same_device(y, {&*weights});
+    need(weights->is_floating_point() && weights->numel() == place.numel(), "one weight for each of " + std::to_string(place.numel()) + " pairs expected");
+    w = weights->to(at::kFloat).contiguous();
+  }
+  if (!(at::GradMode::is_enabled() && (y.requires_grad() || (w.defined() && w.requires_grad())))) return unpermute_rows(y, place, offsets, topk, w);
+  if (!w.defined()) return UnpermuteOnesFn::apply(y, place, offsets, topk);
+  return UnpermuteFn::apply(y, w, place, offsets, topk);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gb_torch, m) {
@@ -709,5 +1024,15 @@ PYBIND11_MODULE(_gb_torch, m) {
       .def_property_readonly("fp4", &MoEPlan::fp4)
       .def("__call__", &MoEPlan::forward, py::call_guard<py::gil_scoped_release>())
       .def_property_readonly("route", [](const MoEPlan& p) { return p.route.load(); });
+  using Free = py::call_guard<py::gil_scoped_release>;
+  m.def("fp8_quantize_blocks", &fp8_quantize_blocks, Free());
+  m.def("moe_swiglu_fp8", &moe_swiglu_fp8, Free());
+  m.def("moe_permute_fp8", &moe_permute_fp8, Free());
+  m.def("linear_fp8_blocks", &linear_fp8_blocks, Free());
+  m.def("gemm_fp8_blocks", &gemm_fp8_blocks, Free());
+  m.def("gemm_fp8_blocks_grouped", &gemm_fp8_blocks_grouped, Free());
+  m.def("moe_sort", &moe_sort, Free());
+  m.def("moe_permute", &moe_permute, Free());
+  m.def("moe_unpermute", &moe_unpermute, Free());
   m.def("shared_row", &shared_row, py::arg("plans"), py::arg("x"), py::arg("rule"), py::arg("routes") = py::none());
 }

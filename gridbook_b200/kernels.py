@@ -625,3 +625,81 @@ def moe_gemv_sorted(x_sorted: torch.Tensor, w: PackedWeight, offsets: torch.Tens
                                      ctypes.byref(peer_rows) if peer_rows is not None else None,
                                      nat.stream_ptr(x_sorted.device)), lib)
     return out if peer_rows is None else True
+
+
+# ------------------------------------------------------------------ block-scaled E4M3
+# Weights [N, K] float8_e4m3fn with one fp32 scale per 128 x 128 block, activations [M, K] with one per 1 x 128
+# block; the last blocks may be short.  Compiled host path: csrc/gb_torch.cpp.
+FP8_BLOCK = 128
+
+
+def fp8_quantize_blocks(x: torch.Tensor, scale_rule: str = "recip"):
+    """E4M3 quantisation in blocks of 128 columns: x [..., K] bf16, fp16 or fp32 -> (q [..., K] float8_e4m3fn, scale
+    [..., ceil(K / 128)] fp32), x ~ q * scale with scale = max(amax, 1e-10) / 448.  A NaN or an infinity
+    spreads over its block."""
+    return nat.host("block quantiser").fp8_quantize_blocks(x, _rule(scale_rule))
+
+
+def gemm_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
+                    out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """D[M, N] = (a * a_scale) . (b * b_scale)^T: ``a`` [M, K] with ``a_scale`` [M, ceil(K/128)], ``b`` [N, K] with
+    ``b_scale`` [ceil(N/128), ceil(K/128)].  Sums in fp32, one rounding to ``out_dtype`` (bf16, fp16 or fp32).  K is a
+    multiple of 16."""
+    return nat.host("block-scaled GEMM").gemm_fp8_blocks(a, a_scale, b, b_scale, out_dtype)
+
+
+def linear_fp8_blocks(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *, out_dtype: torch.dtype | None = None,
+                      scale_rule: str = "recip") -> torch.Tensor:
+    """y[..., N] = quantised(x)[..., K] . (weight * weight_scale)^T: :func:`fp8_quantize_blocks` and
+    :func:`gemm_fp8_blocks` in one call, ``x`` bf16, fp16 or fp32, y of its type unless ``out_dtype`` names another."""
+    return nat.host("block-scaled linear").linear_fp8_blocks(x, weight, weight_scale, out_dtype, _rule(scale_rule))
+
+
+def gemm_fp8_blocks_grouped(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                            offsets: torch.Tensor, *, out: torch.Tensor | None = None,
+                            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`gemm_fp8_blocks` over expert segments: rows ``offsets[e]:offsets[e+1]`` of ``a`` [P, K] times ``b[e]`` of [E, N, K]
+    with ``b_scale`` [E, ceil(N/128), ceil(K/128)], up to 1024 experts.  Rows past ``offsets[E]`` are left unwritten."""
+    return nat.host("grouped block-scaled GEMM").gemm_fp8_blocks_grouped(a, a_scale, b, b_scale, offsets, out, out_dtype)
+
+
+# ------------------------------------------------------------------ tokens sorted by expert and back
+@dataclass
+class MoESort:
+    """Routed pairs p = token * top-k + slot in expert order (stable); those of experts that are held elsewhere are dropped."""
+    counts: torch.Tensor      # int32 [E]
+    offsets: torch.Tensor     # int32 [E + 1], expert e owns sorted rows offsets[e]:offsets[e+1]
+    order: torch.Tensor       # int32 [P], pair of a sorted row; 0 past offsets[E]
+    place: torch.Tensor       # int32 [P], sorted row of a pair; -1 for a dropped one
+    topk: int
+
+
+def moe_sort(topk_ids: torch.Tensor, E: int, *, expert_base: int = 0) -> MoESort:
+    """Sorts the pairs of ``topk_ids`` [T, top-k] by expert, on the device and without a host read.  The ``E`` experts held
+    here are the global ids [expert_base, expert_base + E); others, -1 among them, are dropped."""
+    counts, offsets, order, place = nat.host("MoE routing").moe_sort(topk_ids, E, expert_base)
+    return MoESort(counts, offsets, order, place, topk_ids.shape[1])
+
+
+def moe_permute(x: torch.Tensor, s: MoESort) -> torch.Tensor:
+    """Token rows [T, H] (bf16, fp16 or fp32) in expert order: out[j] = x[order[j] // top-k], zero past offsets[E].
+    Differentiable in ``x``."""
+    return nat.host("routed row permutation").moe_permute(x, s.place, s.offsets, s.topk)
+
+
+def moe_unpermute(y: torch.Tensor, s: MoESort, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """Sorted rows back to their tokens: out[t] = sum over slots of weights[t, slot] * y[place[t, slot]], in fp32 and slot order,
+    rounded once; dropped pairs count nothing, ``weights`` None: ones.  Differentiable in ``y`` and ``weights``."""
+    return nat.host("routed row combination").moe_unpermute(y, s.place, s.offsets, s.topk, weights)
+
+
+def moe_permute_fp8(x: torch.Tensor, s: MoESort, scale_rule: str = "recip"):
+    """:func:`fp8_quantize_blocks` of the token rows [T, K], written in expert order: (q [P, K], scale
+    [P, ceil(K / 128)]), zero past offsets[E]."""
+    return nat.host("routed block quantiser").moe_permute_fp8(x, s.place, s.offsets, s.topk, _rule(scale_rule))
+
+
+def moe_swiglu_fp8(h: torch.Tensor, offsets: torch.Tensor | None = None, scale_rule: str = "recip"):
+    """:func:`fp8_quantize_blocks` of silu(gate) * up, taken in fp32, over rows h [P, 2 I] = [gate | up]: (q [P, I], scale).
+    ``offsets``: rows past offsets[-1] are left unset."""
+    return nat.host("routed SwiGLU and block quantiser").moe_swiglu_fp8(h, offsets, _rule(scale_rule))

@@ -37,6 +37,8 @@ enum { GB_SCALE_NONE = 0, GB_SCALE_V1 = 1, GB_SCALE_V2 = 2 };
  * (gridbook/csrc/cb_gemv.cu:88-91,485-511), or a true division (torch-on-CPU) */
 enum { GB_SCALE_RULE_RECIP = 0, GB_SCALE_RULE_DIV = 1 };
 enum { GB_ACT_NONE = 0, GB_ACT_FP4_GROUP16 = 1, GB_ACT_FP8_TOKEN = 2 };
+/* element types of the block-scaled and sorted-row entries */
+enum { GB_DTYPE_BF16 = 0, GB_DTYPE_FP16 = 1, GB_DTYPE_FP32 = 2 };
 
 /* One packed format (the `scheme` dict of gridbook/config.py:803-957). */
 typedef struct gb_format {
@@ -315,7 +317,7 @@ GB_API int gb_moe_route_ws(const int32_t* topk_ids, int64_t T, int64_t topk, int
                            int32_t* counts, int32_t* offsets, int32_t* order, const float* topk_weights,
                            float* pair_w, void* workspace, int64_t ws_bytes, void* stream);
 
-/* gb_moe_route_ws that also writes the inverse permutation: inv[p] = sorted position of pair p (unset for
+/* gb_moe_route_ws that also writes the inverse permutation: inv[p] = sorted position of pair p (-1 for
  * a dropped pair). */
 GB_API int gb_moe_route_inv(const int32_t* topk_ids, int64_t T, int64_t topk, int64_t E, int64_t expert_base,
                             int32_t* counts, int32_t* offsets, int32_t* order, int32_t* inv, const float* topk_weights,
@@ -419,6 +421,57 @@ GB_API int gb_moe_mlp_pairs(const void* x_bf16, const int32_t* x_row, const gb_w
 GB_API int gb_moe_combine(const void* y_bf16, const float* pair_w, const int32_t* topk_ids,
                    int64_t E, int64_t T, int64_t topk, int64_t H, int round_weights,
                    void* out_bf16, void* stream);
+
+/* ---- block-scaled E4M3 --------------------------------------------------------- */
+/* The form in which FP8 checkpoints ship the layers that a codebook artifact leaves at their source
+ * precision (the reference serves them outside its codebook path, gridbook/csrc/fp8_source_w8a16.cu):
+ * weights [N, K] E4M3 with one fp32 scale per 128 x 128 block, w_scale [ceil(N/128), ceil(K/128)];
+ * activations [M, K] E4M3 with one per 1 x 128 block, a_scale [M, ceil(K/128)].  Last blocks may be
+ * short.  No counterpart among the reference's native ops: its lane multiplies bf16 activations.
+ *
+ * gb_fp8_quantize_blocks: scale = max(amax, 1e-10) / 448 (scale_rule as elsewhere), q = E4M3(x / scale),
+ * nearest, ties to even; a NaN or an infinity spreads over its block.  x [M, K] of `dtype`, rows `ld`
+ * elements apart; q [M, K] and scale contiguous.
+ * gb_moe_swiglu_fp8: the same of silu(gate) * up in fp32, h [P, 2 * inter] = [gate | up]; `live`
+ * (optional): a device count of the rows that matter (offsets[E]), later ones are left as they are.
+ * gb_moe_permute_fp8: quantises each of T token rows once and writes it to place[t * topk + s] (from
+ * gb_moe_route_inv; negative: dropped) of q [T * topk, K]; rows from *live on become zero. */
+GB_API int gb_fp8_quantize_blocks(const void* x, int dtype, int64_t ld, int64_t M, int64_t K, int scale_rule, void* q,
+                                  float* scale, void* stream);
+GB_API int gb_moe_swiglu_fp8(const void* h, int dtype, int64_t ld, const int32_t* live, int64_t P, int64_t inter,
+                             int scale_rule, void* q, float* scale, void* stream);
+GB_API int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_t* place, const int32_t* live, int64_t T,
+                              int64_t topk, int64_t K, int scale_rule, void* q, float* scale, void* stream);
+
+/* D[m, n] = sum over blocks b of a_scale[m, b] w_scale[n / 128, b] * sum over k in b of A[m, k] W[n, k]; the
+ * inner sums in fp32 on the tensor cores, the outer in fp32 registers, one rounding to `out` (GB_DTYPE_*).
+ * K a multiple of 16, operands and D 16-byte aligned.  Grouped: A [P, K] rows sorted by expert (expert e
+ * owns seg_offsets[e] .. seg_offsets[e + 1]), W [E, N, K], w_scale [E, ceil(N/128), ceil(K/128)], E <= 1024;
+ * rows of D from seg_offsets[E] on are left as they are.
+ * beside: W, its scales and seg_offsets are not written by the launch right ahead on the stream, and that
+ * launch lets this one start only behind its own wait (the quantisers above do): W is then fetched while
+ * that launch still runs.  0 is always right. */
+GB_API int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const float* w_scale, void* D, int out,
+                              int64_t M, int64_t N, int64_t K, int beside, void* stream);
+GB_API int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* W, const float* w_scale,
+                                      const int32_t* seg_offsets, int64_t E, void* D, int out, int64_t P, int64_t N,
+                                      int64_t K, int beside, void* stream);
+
+/* ---- tokens sorted by expert and back -------------------------------------------- */
+/* place [T * topk] and *live = offsets[E] from gb_moe_route_inv.
+ * gb_moe_permute: rows[place[p]] = x[p / topk], x [T, H] with rows `ld` elements of elem_bytes (2 or 4)
+ * apart; rows from *live on become zero.
+ * gb_moe_unpermute: out[t] = sum over slots of weights[p] * y[place[p]] (weights NULL: ones; dropped pairs
+ * count nothing), fp32, one rounding; with NULL weights the gradient of gb_moe_permute.
+ * gb_moe_unpermute_grad: d_y[place[p]] = weights[p] * d_out[p / topk], rows from *live on zero, and
+ * d_w[p] = <y[place[p]], d_out[p / topk]> in fp32, zero for a dropped pair; either may be NULL. */
+GB_API int gb_moe_permute(const void* x, int64_t elem_bytes, int64_t ld, const int32_t* place, const int32_t* live, int64_t T,
+                          int64_t topk, int64_t H, void* rows, void* stream);
+GB_API int gb_moe_unpermute(const void* y, int dtype, const int32_t* place, const float* weights, int64_t T, int64_t topk,
+                            int64_t H, void* out, void* stream);
+GB_API int gb_moe_unpermute_grad(const void* d_out, const void* y, int dtype, const int32_t* place, const int32_t* live,
+                                 const float* weights, int64_t T, int64_t topk, int64_t H, void* d_y, float* d_w,
+                                 void* stream);
 
 /* Kernel launches this library has issued in this process so far (launches recorded into a
  * CUDA graph count once, at capture).  No reference counterpart; used by the benchmark to
