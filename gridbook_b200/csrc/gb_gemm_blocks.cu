@@ -43,11 +43,18 @@ struct BlocksParams {
 };
 
 // ---- waits, copies, MMAs -------------------------------------------------------------------------------------
-template <bool kOfPair>
+// What a wait hands over: this CTA's writes or copies; those of either CTA of the pair; tensor memory alone, which the
+// tcgen05 fences on both sides order, so that the wait itself may be relaxed (an acquire at cluster scope took 150 clocks
+// with the barrier already complete).
+enum Scope { kOfCta, kOfPair, kTensorMemory };
+template <Scope kScope>
 GB_DEVINL bool try_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
-  if (kOfPair)
+  if (kScope == kOfPair)
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  else if (kScope == kTensorMemory)
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   else
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
@@ -55,11 +62,11 @@ GB_DEVINL bool try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 // A bounded wait that remembers a timeout for the rest of the CTA: later waits return at once.
-template <bool kOfPair>
-__device__ __noinline__ void wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+template <Scope kScope>
+GB_DEVINL void wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   uint64_t t0 = 0;
   for (uint32_t spin = 0; !*abort_flag; ++spin) {
-    if (try_wait<kOfPair>(bar, parity)) return;
+    if (try_wait<kScope>(bar, parity)) return;
     if ((spin & 255u) == 255u) {
       const uint64_t now = gb_globaltimer_ns();
       if (t0 == 0) t0 = now;
@@ -68,10 +75,10 @@ __device__ __noinline__ void wait_slow(uint32_t bar, uint32_t parity, volatile i
   }
 }
 // By a whole warp that goes on together; false: given up.
-template <bool kOfPair = false>
+template <Scope kScope = kOfCta>
 GB_DEVINL bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  if (__all_sync(0xffffffffu, try_wait<kOfPair>(bar, parity))) return true;
-  wait_slow<kOfPair>(bar, parity, abort_flag, status, code);
+  if (__all_sync(0xffffffffu, try_wait<kScope>(bar, parity))) return true;
+  wait_slow<kScope>(bar, parity, abort_flag, status, code);
   return !__any_sync(0xffffffffu, *abort_flag != 0);
 }
 GB_DEVINL int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
@@ -84,8 +91,8 @@ GB_DEVINL void expect_tx(uint32_t bar, uint32_t bytes) {
 GB_DEVINL void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // Hands tensor memory from read-out warps of both CTAs to the leader's MMA issuer: ordered by the tensor-memory fences on
 // both sides, so the arrive itself may be relaxed (one that released would wait for the output stores in flight).
-GB_DEVINL void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+GB_DEVINL void arrive_cluster(uint32_t addr, bool mine) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %1, 0;\n@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n}\n" ::"r"(addr), "r"((uint32_t)mine) : "memory");
 }
 GB_DEVINL uint32_t leader_addr(uint32_t addr) {
   uint32_t r;
@@ -142,16 +149,50 @@ GB_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr));
 }
+// Two fp32 in one register pair: one instruction multiplies and adds both, each rounded as fmaf.
+GB_DEVINL uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+GB_DEVINL void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+GB_DEVINL void fma_f32x2(uint64_t& d, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
+template <int kRegs>
+GB_DEVINL void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+GB_DEVINL void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+// The loads issued so far have arrived; `v`, loaded by them, is read behind this only.
+GB_DEVINL void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]),
+                 "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31]) ::"memory");
+}
 GB_DEVINL void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 GB_DEVINL void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 GB_DEVINL void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Scales of four consecutive blocks, kt .. kt + 3, of a row of `kb`; zeros past its end and for a null row.
+// Scales of four consecutive blocks, kt .. kt + 3, of a row of `kb`; zeros past its end and for a null row.  The loads are
+// volatile so that they stay where they are issued, four blocks ahead: free to move, they were sunk to their use, and every
+// fourth block waited some 1900 clocks for them (333 rows of 5120 x 17408: 78 us, 65 with them in flight).
+GB_DEVINL float load1(const float* at) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(at));
+  return v;
+}
 GB_DEVINL float4 scales4(const float* row, int kt, int kb, bool vec4) {
-  if (row == nullptr) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (vec4 && (kt & 3) == 0) return __ldg(reinterpret_cast<const float4*>(row + kt));      // kb is a multiple of four
-  return make_float4(kt < kb ? __ldg(row + kt) : 0.0f, kt + 1 < kb ? __ldg(row + kt + 1) : 0.0f,
-                     kt + 2 < kb ? __ldg(row + kt + 2) : 0.0f, kt + 3 < kb ? __ldg(row + kt + 3) : 0.0f);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (row == nullptr) return v;
+  if (vec4 && (kt & 3) == 0) {                             // kb is a multiple of four
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(row + kt));
+    return v;
+  }
+  if (kt < kb) v.x = load1(row + kt);
+  if (kt + 1 < kb) v.y = load1(row + kt + 1);
+  if (kt + 2 < kb) v.z = load1(row + kt + 2);
+  if (kt + 3 < kb) v.w = load1(row + kt + 3);
+  return v;
 }
 GB_DEVINL float pick(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -193,21 +234,25 @@ GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, i
 constexpr int kPairM = 256;                          // rows of a pair's tile
 constexpr int kEpiWarps = 8;                         // two per lane quarter, half of the columns each
 constexpr int kOutChunk = 2048;                      // 32 rows x 32 16-bit columns on their way out
-constexpr int kPairThreads = 32 * (kEpiWarps + 2);
+constexpr int kPairThreads = 32 * (kEpiWarps + 4);     // three warpgroups, the last two warps idle
+// A thread of the read-out holds 128 sums and has 64 more on their way; 168 registers a thread at launch.
+constexpr int kReadRegs = 224, kOtherRegs = 56;
+static_assert(256 * kReadRegs + 128 * kOtherRegs <= 384 * 168, "a register split draws on what the block was launched with");
 constexpr int kTmemCols = 512;
+constexpr int kBN = 256, kPart = 128, kParts = 2;    // features of a tile, of a part: one block of features, an accumulator
+constexpr int kAccs = kTmemCols / kPart;
 constexpr int kGroupM = 16;                          // row tiles walked together before the next columns (see gb_gemm_pair.cu)
 
-template <int kBN, bool kGrouped>
+template <bool kGrouped>
 struct Pair {
   static constexpr int kABytes = kBM * kSlab, kBBytes = kBN / 2 * kSlab, kStageBytes = kABytes + kBBytes;
   static constexpr int kOutBytes = kEpiWarps * 2 * kOutChunk + (kGrouped ? kSegBytes : 0);
   static constexpr int kStages = (227 * 1024 - 2048 - kOutBytes) / kStageBytes;
   static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 2048;
-  static constexpr int kAccs = kTmemCols / kBN;
 };
 
 // The tiles of a pair: first, first + stride, ...
-template <int kBN, bool kGrouped>
+template <bool kGrouped>
 struct PairTiles {
   int tile, stride, e = 0;
   int m0 = 0, n0 = 0, w0 = 0, end = 0;               // first row, first feature, first weight row, end of the rows that count
@@ -234,12 +279,23 @@ struct PairTiles {
   }
 };
 
-template <int kBN, bool kGrouped>
+// fmaf, kept where it stands between the loads and the waits.
+GB_DEVINL void add_scaled(float& acc, uint32_t v, float scale) {
+  asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(v)), "f"(scale));
+}
+GB_DEVINL void read64(uint32_t at, uint32_t (&v)[2][32]) {
+  tmem_ld32(at, v[0]);
+  tmem_ld32(at + 32u, v[1]);
+  tmem_wait_ld(v[0]);
+  tmem_wait_ld(v[1]);
+}
+
+template <bool kGrouped>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
                         const __grid_constant__ BlocksParams p) {
-  using S = Pair<kBN, kGrouped>;
-  constexpr int kStages = S::kStages, kAccs = S::kAccs;
+  using S = Pair<kGrouped>;
+  constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
   uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
@@ -265,7 +321,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     for (int b = 0; b < kAccs; ++b) {
       bar_init(acc_full + 8 * b, 1);
-      bar_init(acc_empty + 8 * b, 2 * kEpiWarps);
+      bar_init(acc_empty + 8 * b, kEpiWarps);
     }
     *abort_flag = 0;
     gb_fence_barrier_init();
@@ -286,75 +342,92 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
 
   if (warp == kEpiWarps) {
     // ------------------------------- producer (each CTA) -------------------------------
+    fewer_registers<kOtherRegs>();
     const uint32_t full_pair = (uint32_t)uniform((int)leader_addr(full_bar));
     const int me = uniform((int)rank);
     const bool one = gb_elect_one();
     int s = 0;
     uint32_t ph = 1;
     bool ok = true;
-    for (PairTiles<kBN, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
-      const int m0 = uniform(T.m0) + me * kBM, w0 = uniform(T.w0) + me * (kBN / 2);
+    for (PairTiles<kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+      const int m0 = uniform(T.m0) + me * kBM, w0 = uniform(T.w0) + me * (kPart / 2);
       for (int kt = 0; kt < p.kb; ++kt) {
-        ok = warp_wait<true>(empty_bar + 8 * s, ph, abort_flag, p.status, 91);
+        ok = warp_wait<kTensorMemory>(empty_bar + 8 * s, ph, abort_flag, p.status, 91);
         if (!ok) break;
         if (one) {
           const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
           if (me == 0) expect_tx(full_bar + 8 * s, 2 * S::kStageBytes);
           tma_load_pair(st, &map_a, kt * kSlab, m0, full_pair + 8 * s);
-          tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);
+          tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);                          // half of a part's
+          tma_load_pair(st + S::kABytes + S::kBBytes / 2, &map_b, kt * kSlab, w0 + kPart, full_pair + 8 * s);  // features each
         }
         __syncwarp();
         if (++s == kStages) { s = 0; ph ^= 1; }
       }
     }
-  } else if (warp == kEpiWarps + 1) {
-    // --------------------------- MMA issuer (the leader's) ------------------------------
+  } else if (warp == kEpiWarps + 1 || warp == kEpiWarps + 2) {
+    // ------ MMA issuers (the leader's): the waits, MMAs and commits of a slab take one some 700 clocks, so two share the slabs
+    // in turn; every slab has accumulators of its own, so that their order does not matter ------
+    fewer_registers<kOtherRegs>();
     if (uniform((int)rank) == 0) {
       uint32_t to_peer;                                      // distance of the peer's barriers
       asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
       to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
       const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
-      const int tiles = uniform(total > first ? (total - first + stride - 1) / stride : 0);
+      const int tiles = uniform(total > first ? (total - first + stride - 1) / stride : 0), turn = warp - kEpiWarps - 1;
+      const int64_t slabs = (int64_t)tiles * p.kb;
       const bool one = gb_elect_one();
-      int s = 0, buf = 0;
-      uint32_t ph = 0, acc_ph = 1;
-      for (int64_t left = (int64_t)tiles * p.kb; left > 0; --left) {
-        if (!warp_wait<true>(acc_empty + 8 * buf, acc_ph, abort_flag, p.status, 92)) break;
-        if (!warp_wait<true>(full_bar + 8 * s, ph, abort_flag, p.status, 93)) break;
-        tmem_fence_after();
+      int s = turn % kStages;
+      uint32_t ph = turn >= kStages ? 1 : 0, acc_ph = 1;
+      bool ok = true;
+      for (int64_t slab = turn; ok && slab < slabs; slab += 2) {
+        ok = warp_wait(full_bar + 8 * s, ph, abort_flag, p.status, 93);
+        if (!ok) break;
         const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
-        const uint64_t da = desc_sw128(st), db = desc_sw128(st + S::kABytes);
-        if (one) {
+        const uint64_t da = desc_sw128(st);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)                        // 32 columns of K per instruction
-            mma<2>(tmem + (uint32_t)(buf * kBN), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), p.idesc, k > 0);
-          commit_pair(empty_bar + 8 * s, to_peer);
-          commit_pair(acc_full + 8 * buf, to_peer);
+        for (int h = 0; h < kParts; ++h) {
+          const int buf = turn * kParts + h;
+          ok = warp_wait<kTensorMemory>(acc_empty + 8 * buf, acc_ph, abort_flag, p.status, 92);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint64_t db = desc_sw128(st + S::kABytes + (uint32_t)h * (S::kBBytes / 2));
+          if (one) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)                      // 32 columns of K per instruction
+              mma<2>(tmem + (uint32_t)(buf * kPart), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), p.idesc, k > 0);
+            commit_pair(acc_full + 8 * buf, to_peer);
+            if (h == kParts - 1) commit_pair(empty_bar + 8 * s, to_peer);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (++s == kStages) { s = 0; ph ^= 1; }
-        if (++buf == kAccs) { buf = 0; acc_ph ^= 1; }
+        acc_ph ^= 1;
+        s += 2;
+        if (s >= kStages) { s -= kStages; ph ^= 1; }
       }
     }
-  } else {
+  } else if (warp < kEpiWarps) {
     // ------------------------------- read-out (each CTA) --------------------------------
+    more_registers<kReadRegs>();
     const uint32_t acc_empty_pair = leader_addr(acc_empty);
-    constexpr int kCols = kBN / 2, kChunks = kCols / 32;
-    const int quarter = warp & 3, c_lo = (warp >> 2) * kCols;
+    // Four warps for each part, one per lane quarter: while one of a scheduler's two adds, the other waits or loads.  (All
+    // eight on half of every part wait together and then add together.)
+    constexpr int kChunks = kPart / 32;
+    const int quarter = warp & 3, part = warp >> 2, c_lo = part * kPart;
     const uint32_t out = out_ring + (uint32_t)warp * 2 * kOutChunk;
-    const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c_lo;
-    int buf = 0, flip = 0;
+    const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    int buf = part, flip = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (PairTiles<kBN, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+    for (PairTiles<kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
       const int row0 = T.m0 + (int)rank * kBM + quarter * 32, row = row0 + lane, n0 = T.n0 + c_lo;
       const bool row_ok = row < T.end;
       const float* as = row_ok ? p.a_scale + (int64_t)row * p.kb : nullptr;
-      // a tile's half lies within one block of features; one past the last is not stored
+      // a part is one block of features; one past the last is not stored
       const float* bs = p.b_scale + ((int64_t)(kGrouped ? T.e : 0) * p.nb + min(n0 / kSlab, p.nb - 1)) * p.kb;
-      float acc[kCols];
+      float acc[kPart];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+      for (int c = 0; c < kPart; ++c) acc[c] = 0.0f;
       float4 as4 = scales4(as, 0, p.kb, p.vec4), bs4 = scales4(bs, 0, p.kb, p.vec4);
       for (int kt0 = 0; ok && kt0 < p.kb; kt0 += 4) {
         const float4 sc = make_float4(as4.x * bs4.x, as4.y * bs4.y, as4.z * bs4.z, as4.w * bs4.w);
@@ -362,26 +435,25 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
           as4 = scales4(as, kt0 + 4, p.kb, p.vec4);
           bs4 = scales4(bs, kt0 + 4, p.kb, p.vec4);
         }
-#pragma unroll 1
-        for (int j = 0; j < 4 && kt0 + j < p.kb; ++j) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!ok || kt0 + j >= p.kb) break;
           const float scale = pick(sc, j);
-          ok = warp_wait<true>(acc_full + 8 * buf, ph, abort_flag, p.status, 94);
+          ok = warp_wait<kTensorMemory>(acc_full + 8 * buf, ph, abort_flag, p.status, 94);
           if (!ok) break;
           tmem_fence_after();
+          uint32_t v[2][32];
+          read64(at + (uint32_t)(buf * kPart), v);
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint32_t v[32];
-            tmem_ld32(at + (uint32_t)(buf * kBN + 32 * c), v);
-            tmem_wait_ld();
-            if (c == kChunks - 1) {
-              tmem_fence_before();
-              __syncwarp();
-              if (lane == 0) arrive_cluster(acc_empty_pair + 8 * buf);
-            }
+          for (int c = 0; c < 64; ++c) add_scaled(acc[c], v[c >> 5][c & 31], scale);
+          read64(at + (uint32_t)(buf * kPart + 64), v);
+          tmem_fence_before();
+          __syncwarp();
+          arrive_cluster(acc_empty_pair + 8 * buf, lane == 0);
+          buf += kParts;
+          if (buf >= kAccs) { buf -= kAccs; ph ^= 1; }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(v[i]), scale, acc[32 * c + i]);
-          }
-          if (++buf == kAccs) { buf = 0; ph ^= 1; }
+          for (int c = 0; c < 64; ++c) add_scaled(acc[64 + c], v[c >> 5][c & 31], scale);
         }
       }
       if (!ok) break;
@@ -410,26 +482,28 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         }
       } else if (row_ok) {
         const int64_t d = (int64_t)row * p.N + n0;
-        const int cols = (int)min((int64_t)kCols, p.N - n0);
+        const int cols = (int)min((int64_t)kPart, p.N - n0);
         if (p.out16 && p.out != GB_DTYPE_FP32) {             // whole 16-byte pieces
 #pragma unroll
-          for (int c = 0; c < kCols; c += 8)
+          for (int c = 0; c < kPart; c += 8)
             if (c < cols)
               *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.D) + d + c) =
                   make_uint4(pack2(acc[c], acc[c + 1], p.out), pack2(acc[c + 2], acc[c + 3], p.out), pack2(acc[c + 4], acc[c + 5], p.out),
                              pack2(acc[c + 6], acc[c + 7], p.out));
         } else if (p.out16) {
 #pragma unroll
-          for (int c = 0; c < kCols; c += 4)
+          for (int c = 0; c < kPart; c += 4)
             if (c < cols) *reinterpret_cast<float4*>(static_cast<float*>(p.D) + d + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
         } else {
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
+          for (int c = 0; c < kPart; ++c)
             if (c < cols) store1(p.D, d + c, acc[c], p.out);
         }
       }
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  } else {
+    fewer_registers<kOtherRegs>();
   }
   __syncwarp();
   tmem_fence_before();
@@ -761,16 +835,14 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 
 // ======================================== host =============================================================
 std::mutex g_mutex;
-int g_pairs[64][4];                                        // pairs that run at once, per device and kernel (0: not asked)
+int g_pairs[64][2];                                        // pairs that run at once, per device and kernel (0: not asked)
 std::atomic<bool> g_ready[64];                             // shared-memory limits of the device's kernels are set
 GbClusters g_clusters[8];
 
 int set_limits() {
-#define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)(k), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
-  GB_ATTR((gemm_blocks_pair_kernel<256, false>), (Pair<256, false>::kSmem));
-  GB_ATTR((gemm_blocks_pair_kernel<128, false>), (Pair<128, false>::kSmem));
-  GB_ATTR((gemm_blocks_pair_kernel<256, true>), (Pair<256, true>::kSmem));
-  GB_ATTR((gemm_blocks_pair_kernel<128, true>), (Pair<128, true>::kSmem));
+#define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+  GB_ATTR(gemm_blocks_pair_kernel<false>, Pair<false>::kSmem);
+  GB_ATTR(gemm_blocks_pair_kernel<true>, Pair<true>::kSmem);
   GB_ATTR((gemm_blocks_rows_kernel<16, false>), kSmemMax);
   GB_ATTR((gemm_blocks_rows_kernel<32, false>), kSmemMax);
   GB_ATTR((gemm_blocks_rows_kernel<64, false>), kSmemMax);
@@ -795,40 +867,40 @@ int ready() {
   return rc;
 }
 
-template <int kBN, bool kGrouped>
+template <bool kGrouped>
 int resident_pairs() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   std::lock_guard<std::mutex> lock(g_mutex);
-  int& n = g_pairs[dev][(kBN == 256) + 2 * kGrouped];
+  int& n = g_pairs[dev][kGrouped];
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * 256);
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = Pair<kBN, kGrouped>::kSmem;
+    cfg.dynamicSmemBytes = Pair<kGrouped>::kSmem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_blocks_pair_kernel<kBN, kGrouped>, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_blocks_pair_kernel<kGrouped>, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
   }
   return n;
 }
 
-template <int kBN, bool kGrouped>
+template <bool kGrouped>
 int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
-  using S = Pair<kBN, kGrouped>;
-  const int pairs = resident_pairs<kBN, kGrouped>();
+  using S = Pair<kGrouped>;
+  const int pairs = resident_pairs<kGrouped>();
   if (pairs <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
   p.n_tiles = (int)((p.N + kBN - 1) / kBN);
   p.m_tiles = (int)((p.M + kPairM - 1) / kPairM);
-  p.idesc = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24);
+  p.idesc = (1u << 4) | ((uint32_t)(kPart >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24);
   p.out_tma = p.N % 8 == 0 && p.out != GB_DTYPE_FP32;
   CUtensorMap map_a, map_b, map_d = {};
   int rc = gb_tensor_map_operand(&map_a, A, p.M, K, 1, kBM);
   if (rc != GB_OK) return rc;
-  rc = gb_tensor_map_operand(&map_b, W, (kGrouped ? p.E : 1) * p.N, K, 1, kBN / 2);
+  rc = gb_tensor_map_operand(&map_b, W, (kGrouped ? p.E : 1) * p.N, K, 1, kPart / 2);
   if (rc != GB_OK) return rc;
   if (p.out_tma) {
     rc = gb_tensor_map_out(&map_d, p.D, p.M, p.N);
@@ -849,7 +921,7 @@ int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   cfg.attrs = attr;
   cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
   gb_count_launch();
-  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_pair_kernel<kBN, kGrouped>, map_a, map_b, map_d, p));
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_pair_kernel<kGrouped>, map_a, map_b, map_d, p));
   return GB_OK;
 }
 
@@ -954,7 +1026,7 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
   if (rc != GB_OK || M == 0) return rc;
   const BlocksParams p = params(a_scale, w_scale, D, out, M, N, K, beside);
   if (M <= 128) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
-  return run_pair<256, false>(A, W, K, p, (cudaStream_t)stream);
+  return run_pair<false>(A, W, K, p, (cudaStream_t)stream);
 }
 
 int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* W, const float* w_scale, const int32_t* seg_offsets, int64_t E, void* D,
@@ -968,7 +1040,7 @@ int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* 
   p.E = (int)E;
   const int64_t mean = P / E;
   if (mean <= 64) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
-  return run_pair<256, true>(A, W, K, p, (cudaStream_t)stream);
+  return run_pair<true>(A, W, K, p, (cudaStream_t)stream);
 }
 
 }  // extern "C"
