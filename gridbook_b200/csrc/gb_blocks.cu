@@ -8,105 +8,60 @@
 //
 // Sixteen lanes take a block, eight columns each: the maximum is four shuffles away, a warp reads 512 contiguous bytes of
 // 16-bit rows and writes 256 of the result.
-#include "gb_common.cuh"
+#include "gb_blocks.cuh"
 
 namespace {
 
-constexpr int kBlock = 128, kThreads = 256, kHalfWarps = kThreads / 16;
-constexpr float kAmaxFloor = 1e-10f;
+using namespace gb_blocks;
+
+constexpr int kThreads = 256, kHalfWarps = kThreads / 16;
 
 enum Source { kRows = 0, kSorted = 1, kSwiglu = 2 };
 
-struct Bf16 { using word = uint16_t; };
-struct Fp16 { using word = uint16_t; };
-struct Fp32 { using word = uint32_t; };
-
-template <typename T>
-GB_DEVINL float to_f32(typename T::word w);
-template <> GB_DEVINL float to_f32<Bf16>(uint16_t w) { return gb_bf16_bits_to_f32(w); }
-template <> GB_DEVINL float to_f32<Fp16>(uint16_t w) { return __half2float(__ushort_as_half(w)); }
-template <> GB_DEVINL float to_f32<Fp32>(uint32_t w) { return __uint_as_float(w); }
-template <typename T>
-GB_DEVINL typename T::word from_f32(float v);
-template <> GB_DEVINL uint16_t from_f32<Bf16>(float v) { return (uint16_t)gb_f32_to_bf16_bits(v); }
-template <> GB_DEVINL uint16_t from_f32<Fp16>(float v) { return __half_as_ushort(__float2half_rn(v)); }
-template <> GB_DEVINL uint32_t from_f32<Fp32>(float v) { return __float_as_uint(v); }
-
-// Sixteen bytes of a row as fp32.
-template <typename T>
-GB_DEVINL void unpack16(const uint4& q, float* v) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(typename T::word) == 2) {
-      v[2 * i] = to_f32<T>((uint16_t)(w[i] & 0xFFFFu));
-      v[2 * i + 1] = to_f32<T>((uint16_t)(w[i] >> 16));
-    } else {
-      v[i] = to_f32<T>(w[i]);
-    }
-  }
-}
-template <typename T>
-GB_DEVINL uint4 pack16(const float* v) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(typename T::word) == 2)
-      w[i] = (uint32_t)from_f32<T>(v[2 * i]) | (uint32_t)from_f32<T>(v[2 * i + 1]) << 16;
-    else
-      w[i] = from_f32<T>(v[i]);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Eight consecutive columns from `c` of a row of `K`, zeros past its end.  kVec: rows of whole 16-byte pieces, K a multiple of 8.
+// Eight consecutive columns as they lie in memory, zeros past the row's end.  kVec: rows of whole 16-byte pieces, K a multiple
+// of 8.
 template <typename T, bool kVec>
-GB_DEVINL void load8(const typename T::word* row, int64_t c, int64_t K, float (&v)[8]) {
-  if constexpr (kVec) {
-    if (c < K) {
-      if constexpr (sizeof(typename T::word) == 2) {
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + c)), v);
-      } else {
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + c)), v);
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + c + 4)), v + 4);
-      }
-      return;
+struct Eight {
+  static constexpr int kPieces = sizeof(typename T::word) / 2;
+  using word = typename T::word;
+  uint4 v[kVec ? kPieces : 1];
+  word w[kVec ? 1 : 8];
+  GB_DEVINL void load(const word* row, int64_t c, int64_t K) {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) v[i] = c < K ? __ldg(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = c + i < K ? row[c + i] : word(0);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32<T>(row[c + i]) : 0.0f;
   }
-}
+  GB_DEVINL void clear() {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = word(0);
+    }
+  }
+  GB_DEVINL void unpack(float (&f)[8]) const {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) unpack16<T>(v[i], f + i * (8 / kPieces));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(w[i]);
+    }
+  }
+};
 
-GB_DEVINL float max_nan(float a, float b) {
+// gate / (1 + exp(-gate)): the reciprocal is off by a unit at most, the exponential by 2 + 1.2 |gate|; a gate far below zero
+// gives zero, whose exponential is infinite.
+GB_DEVINL float silu(float gate) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-gate)));
+  return gate * r;
 }
-
-// The eight values' E4M3 bytes and the block's scale; the sixteen lanes of the block call it together.
-GB_DEVINL uint2 quantize8(const float (&v)[8], int scale_rule, float& scale) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[i]));
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  amax = max_nan(amax, kAmaxFloor);
-  scale = scale_rule == GB_SCALE_RULE_DIV ? __fdiv_rn(amax, 448.0f) : __fmul_rn(amax, 1.0f / 448.0f);
-  uint32_t q[4];
-  if (gb_plain_division(scale)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = gb_cvt_e4m3x2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale));
-  } else {
-    const float rinv = __frcp_rn(scale);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = gb_cvt_e4m3x2(gb_div(v[2 * i], scale, rinv), gb_div(v[2 * i + 1], scale, rinv));
-  }
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-}
-
 template <bool kVec>
 GB_DEVINL void store8(uint8_t* row, int64_t c, int64_t K, uint2 q) {
   if constexpr (kVec) {
@@ -122,6 +77,7 @@ struct QuantizeParams {
   const void* x;
   int64_t ld, rows, K;        // of the result; a swiglu row is [gate | up]
   uint32_t blocks;            // of a row
+  uint32_t step_rows, step_blocks;      // sixteen blocks further on
   int64_t units;              // rows * blocks
   int scale_rule;
   uint8_t* q;
@@ -141,43 +97,55 @@ quantize_blocks_kernel(const __grid_constant__ QuantizeParams p) {
   const typename T::word* x = static_cast<const typename T::word*>(p.x);
   int64_t rows = p.rows;
   if (kSource == kSwiglu && p.live) rows = min(rows, (int64_t)*p.live);
-  float v[kPer][8];
+  // every block's bytes are on their way before the first is looked at
+  Eight<T, kVec> raw[kPer], up[kSource == kSwiglu ? kPer : 1];
   int64_t row[kPer];
   uint32_t block[kPer];
+  const int64_t unit = (int64_t)blockIdx.x * (kPer * kHalfWarps) + half;
+  row[0] = (uint32_t)unit / p.blocks;
+  block[0] = (uint32_t)unit - (uint32_t)row[0] * p.blocks;
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) {         // sixteen blocks on
+    row[i] = row[i - 1] + p.step_rows;
+    block[i] = block[i - 1] + p.step_blocks;
+    if (block[i] >= p.blocks) { block[i] -= p.blocks; ++row[i]; }
+  }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int64_t unit = ((int64_t)blockIdx.x * kPer + i) * kHalfWarps + half;
-    row[i] = unit < p.units ? (int64_t)((uint32_t)unit / p.blocks) : p.rows;
-    block[i] = (uint32_t)unit - (uint32_t)row[i] * p.blocks;
     const int64_t c = (int64_t)block[i] * kBlock + lane * 8;
     if (row[i] < rows) {
-      const typename T::word* at = x + row[i] * p.ld;
-      load8<T, kVec>(at, c, p.K, v[i]);
-      if constexpr (kSource == kSwiglu) {
-        float up[8];
-        load8<T, kVec>(at + p.K, c, p.K, up);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = c + k < p.K ? gb_silu(v[i][k]) * up[k] : 0.0f;
-      }
+      raw[i].load(x + row[i] * p.ld, c, p.K);
+      if constexpr (kSource == kSwiglu) up[i].load(x + row[i] * p.ld + p.K, c, p.K);
     } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
+      raw[i].clear();
+      if constexpr (kSource == kSwiglu) up[i].clear();
     }
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int64_t c = (int64_t)block[i] * kBlock + lane * 8;
-    float scale;
-    const uint2 q = quantize8(v[i], p.scale_rule, scale);
-    if (row[i] >= rows) continue;
+    int to_lane = -1;
+    if (kSource == kSorted && row[i] < rows && lane < p.topk) to_lane = p.place[row[i] * p.topk + lane];
+    float v[8], scale;
+    raw[i].unpack(v);
+    if constexpr (kSource == kSwiglu) {    // zeros past the row's end stay zeros
+      float u[8];
+      up[i].unpack(u);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = silu(v[k]) * u[k];
+    }
+    uint32_t w[2];
+    quantize_block<8, 16>(v, p.scale_rule, scale, w);
+    const uint2 q = make_uint2(w[0], w[1]);
     if constexpr (kSource == kSorted) {
-      for (int s = 0; s < p.topk; ++s) {
-        const int64_t to = p.place[row[i] * p.topk + s];
+      for (int s = 0; s < p.topk; ++s) {   // the same for all sixteen lanes
+        int64_t to = __shfl_sync(0xffffffffu, to_lane, s & 15, 16);
+        if (s >= 16) to = row[i] < rows ? p.place[row[i] * p.topk + s] : -1;
         if (to < 0) continue;
         store8<kVec>(p.q + to * p.K, c, p.K, q);
         if (lane == 0) p.scale[to * p.blocks + block[i]] = scale;
       }
-    } else {
+    } else if (row[i] < rows) {
       store8<kVec>(p.q + row[i] * p.K, c, p.K, q);
       if (lane == 0) p.scale[row[i] * p.blocks + block[i]] = scale;
     }
@@ -194,13 +162,18 @@ quantize_blocks_kernel(const __grid_constant__ QuantizeParams p) {
 
 template <typename T, Source kSource>
 int launch_quantize(const QuantizeParams& p, bool vec, cudaStream_t stream) {
-  // one block each while that leaves SMs idle, four from some waves on
+  // one block each for less than a wave of them, two from there on (8192 rows of 5120 bf16: 32.3 us, 31.2, four 32.9); one where every
+  // block is written several times (4096 tokens x 8 x 2048 columns: 23 us, four 27)
   const int64_t few = 8ll * gb_sm_count() * kHalfWarps;
-  const int per = p.units > few ? 4 : 1;
+  const int per = kSource != kSorted && p.units > few ? 2 : 1;
   const dim3 grid((unsigned)((p.units + per * kHalfWarps - 1) / (per * kHalfWarps)));
 #define GB_Q(v, n) GB_CUDA_OK(gb_launch(quantize_blocks_kernel<T, kSource, v, n>, grid, dim3(kThreads), 0, stream, p))
-  if (vec) { if (per == 4) GB_Q(true, 4); else GB_Q(true, 1); }
-  else { if (per == 4) GB_Q(false, 4); else GB_Q(false, 1); }
+  if constexpr (kSource == kSorted) {
+    if (vec) GB_Q(true, 1); else GB_Q(false, 1);
+  } else {
+    if (vec) { if (per == 2) GB_Q(true, 2); else GB_Q(true, 1); }
+    else { if (per == 2) GB_Q(false, 2); else GB_Q(false, 1); }
+  }
 #undef GB_Q
   return GB_OK;
 }
@@ -217,6 +190,8 @@ int quantize(QuantizeParams p, int dtype, cudaStream_t stream) {
   GB_REQUIRE(p.x && p.q && p.scale, "null pointer argument");
   GB_REQUIRE(((uintptr_t)p.scale & 3u) == 0 && (uintptr_t)p.x % elem_bytes(dtype) == 0, "misaligned pointer");
   p.blocks = (uint32_t)((p.K + kBlock - 1) / kBlock);
+  p.step_rows = kHalfWarps / p.blocks;
+  p.step_blocks = kHalfWarps % p.blocks;
   p.units = p.rows * p.blocks;
   GB_REQUIRE(p.units < (1ll << 31), "too many blocks");
   const int eb = elem_bytes(dtype);
@@ -225,6 +200,157 @@ int quantize(QuantizeParams p, int dtype, cudaStream_t stream) {
   if (dtype == GB_DTYPE_BF16) return launch_quantize<Bf16, kSource>(p, vec, stream);
   if (dtype == GB_DTYPE_FP16) return launch_quantize<Fp16, kSource>(p, vec, stream);
   return launch_quantize<Fp32, kSource>(p, vec, stream);
+}
+
+// ---- the sort itself -------------------------------------------------------------------------------------------
+// Pairs by expert, stable, in ONE launch: a cluster of up to eight CTAs, a warp 32 kPer consecutive pairs.  A pair's place =
+// the expert's segment start + its pairs in earlier CTAs + in earlier warps + in earlier steps of its warp + its rank among
+// the step's lanes.  Every CTA counts its own pairs; the counts of the others are read through the cluster's shared memory.
+// The same order as gb_moe_route's, which takes three launches from 4096 pairs on.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortExperts = 1024, kSortMostCtas = 8, kSortMostPer = 8;
+
+GB_DEVINL int load_cluster(uint32_t addr, int rank) {
+  uint32_t from, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+  return (int)v;
+}
+// Exclusive prefix of v over the CTA's threads, and the sum, by shuffles within the warps and one warp over them.
+GB_DEVINL int prefix_sum(int v, int* warp_sums, int& sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += n;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  int others = warp_sums[lane];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, others, d);
+    if (lane >= d) others += n;
+  }
+  sum = __shfl_sync(0xffffffffu, others, 31);
+  const int before = __shfl_sync(0xffffffffu, others, (warp + 31) & 31);
+  return incl - v + (warp ? before : 0);
+}
+
+template <typename Id, int kPer>
+__global__ void __launch_bounds__(kSortThreads)
+sort_pairs_kernel(const Id* __restrict__ ids, int P, int E, int64_t first_expert, int per_cta, int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
+                  int32_t* __restrict__ order, int32_t* __restrict__ place) {
+  extern __shared__ int32_t sh[];          // [warp][E] counts, then starts; [E] the CTA's counts; [E] starts of its pairs
+  __shared__ int32_t warp_sums[32];
+  int32_t* mine = sh + (threadIdx.x >> 5) * E;
+  int32_t *total = sh + kSortWarps * E, *start = total + E;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int rank, ctas;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  gb_pdl_launch_dependents();
+  for (int k = tid; k < E * kSortWarps; k += kSortThreads) sh[k] = 0;
+  gb_pdl_wait();
+  const int base = rank * per_cta, end = min(P, base + per_cta), first = base + warp * 32 * kPer + lane;
+  int id[kPer], at[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = first + 32 * j;
+    const int64_t e = i < end ? (int64_t)ids[i] - first_expert : -1;
+    id[j] = e >= 0 && e < E ? (int)e : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const unsigned same = __match_any_sync(0xffffffffu, id[j]);
+    const int before = id[j] >= 0 ? mine[id[j]] : 0;
+    at[j] = before + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (id[j] >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[id[j]] = before + __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  const int warps = min(kSortWarps, (end - base + 32 * kPer - 1) / (32 * kPer));       // the others hold no pair
+  for (int e = tid; e < E; e += kSortThreads) {
+    int run = 0;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) {
+      const int v = sh[w * E + e];
+      sh[w * E + e] = run;
+      run += v;
+    }
+    total[e] = run;
+  }
+  gb_cluster_sync();                       // E is at most the CTA's threads: one expert each from here on
+  int all = 0, before = 0;
+  if (tid < E)
+    for (int r = 0; r < ctas; ++r) {
+      const int v = load_cluster(gb_smem_u32(total + tid), r);
+      before += r < rank ? v : 0;
+      all += v;
+    }
+  int live;
+  const int off = prefix_sum(all, warp_sums, live);
+  if (tid < E) {
+    start[tid] = off + before;
+    if (rank == 0) {
+      counts[tid] = all;
+      offsets[tid] = off;
+    }
+  }
+  if (rank == 0 && tid == 0) offsets[E] = live;
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // nothing of another CTA is read behind this
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = first + 32 * j;
+    if (id[j] >= 0) {
+      const int to = start[id[j]] + mine[id[j]] + at[j];
+      order[to] = i;
+      place[i] = to;
+    } else if (i < end) {
+      place[i] = -1;
+    }
+  }
+  for (int i = live + rank * kSortThreads + tid; i < P; i += ctas * kSortThreads) order[i] = 0;     // dropped pairs
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <typename Id>
+int launch_sort(const void* ids, int P, int E, int64_t base, int32_t* counts, int32_t* offsets, int32_t* order, int32_t* place, cudaStream_t stream) {
+  // CTAs while each has at least 512 pairs, then pairs per thread
+  int ctas = 1, per = 1;
+  while (ctas < kSortMostCtas && P > ctas * 512) ctas *= 2;
+  while (P > ctas * per * kSortThreads) per *= 2;
+  const int per_cta = (P + ctas - 1) / ctas;
+  const size_t smem = (size_t)(kSortWarps + 2) * E * sizeof(int32_t);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
+  gb_count_launch();
+#define GB_SORT(n)                                                                                                                          \
+  do {                                                                                                                                      \
+    if (smem > 48 * 1024)                                                                                                                   \
+      GB_CUDA_OK(cudaFuncSetAttribute((const void*)sort_pairs_kernel<Id, n>, cudaFuncAttributeMaxDynamicSharedMemorySize,                  \
+                                      (int)((kSortWarps + 2) * kSortExperts * sizeof(int32_t))));                                          \
+    GB_CUDA_OK(cudaLaunchKernelEx(&cfg, sort_pairs_kernel<Id, n>, (const Id*)ids, P, E, base, per_cta, counts, offsets, order, place));     \
+  } while (0)
+  if (per == 1) GB_SORT(1);
+  else if (per == 2) GB_SORT(2);
+  else if (per == 4) GB_SORT(4);
+  else GB_SORT(8);
+#undef GB_SORT
+  return GB_OK;
 }
 
 // ---- tokens into expert order and back ---------------------------------------------------------------------
@@ -280,25 +406,28 @@ unpermute_kernel(const typename T::word* __restrict__ y, const int32_t* __restri
   gb_pdl_wait();
   const int64_t H = (int64_t)vecs * P::n, t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (t >= tokens) return;
-  constexpr int kInFlight = 4;
+  constexpr int kInFlight = 4;           // eight: 37 us instead of 29 for 4096 tokens x 8 x 2048 columns, fewer CTAs being resident
   for (int c = threadIdx.x; c < vecs; c += blockDim.x) {
     float acc[P::n] = {};
     for (int s0 = 0; s0 < topk; s0 += kInFlight) {
       typename P::raw r[kInFlight];
-      int64_t at[kInFlight];
+      int at[kInFlight];
+      float weight[kInFlight];
 #pragma unroll
       for (int j = 0; j < kInFlight; ++j) {
-        at[j] = s0 + j < topk ? (int64_t)place[t * topk + s0 + j] : -1;
-        if (at[j] >= 0) r[j] = reinterpret_cast<const typename P::raw*>(y + at[j] * H)[c];
+        at[j] = s0 + j < topk ? place[t * topk + s0 + j] : -1;
+        weight[j] = w && s0 + j < topk ? w[t * topk + s0 + j] : 1.0f;
       }
+#pragma unroll
+      for (int j = 0; j < kInFlight; ++j)
+        if (at[j] >= 0) r[j] = reinterpret_cast<const typename P::raw*>(y + at[j] * H)[c];
 #pragma unroll
       for (int j = 0; j < kInFlight; ++j) {
         if (at[j] < 0) continue;
-        const float weight = w ? w[t * topk + s0 + j] : 1.0f;
         float v[P::n];
         P::unpack(r[j], v);
 #pragma unroll
-        for (int i = 0; i < P::n; ++i) acc[i] = fmaf(weight, v[i], acc[i]);
+        for (int i = 0; i < P::n; ++i) acc[i] = fmaf(weight[j], v[i], acc[i]);
       }
     }
     reinterpret_cast<typename P::raw*>(out + t * H)[c] = P::pack(acc);
@@ -307,14 +436,15 @@ unpermute_kernel(const typename T::word* __restrict__ y, const int32_t* __restri
 
 // The weighted sum's gradients, with g = d_out[t]: d_y[place[t, s]] = w[t, s] * g, d_w[t, s] = <y[place[t, s]], g>; a dropped
 // pair's weight gets zero, rows of d_y that no pair has become zero.  A token's lanes are whole warps of one CTA: sums by
-// shuffles, then over the warps in order.  kSlots of a token's slots at a time.
+// shuffles, then over the warps in order.  kSlots of a token's slots at a time: the gradient's row comes out of L1 again for the
+// next ones, which costs less than the registers of more (4096 tokens x 8 x 2048 columns: 59 us with eight, 53 with four).
 template <typename T, bool kVec, int kSlots>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 unpermute_grad_kernel(const typename T::word* __restrict__ d_out, const typename T::word* __restrict__ y, const int32_t* __restrict__ place,
                       const int32_t* __restrict__ live, const float* __restrict__ w, int64_t tokens, int topk, int vecs,
                       typename T::word* __restrict__ d_y, float* __restrict__ d_w) {
   using P = Piece<T, kVec>;
-  __shared__ float part[8][kSlots];
+  __shared__ float part[4][kSlots];
   gb_pdl_launch_dependents();
   gb_pdl_wait();
   const int64_t H = (int64_t)vecs * P::n, t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -378,11 +508,11 @@ unpermute_grad_kernel(const typename T::word* __restrict__ d_out, const typename
   }
 }
 
-// Lanes of a token: whole warps, no more than the row has vectors; 256 threads a CTA.
-dim3 token_block(int vecs) {
+// Lanes of a token: whole warps, no more than the row has vectors, up to all `threads` of a CTA.
+dim3 token_block(int vecs, unsigned threads) {
   unsigned x = 32;
-  while (x < 256 && x < (unsigned)vecs) x *= 2;
-  return dim3(x, 256 / x);
+  while (x < threads && x < (unsigned)vecs) x *= 2;
+  return dim3(x, threads / x);
 }
 
 int check_sorted(const void* place, int64_t T, int64_t topk, int64_t H) {
@@ -421,6 +551,17 @@ int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_t* plac
   return quantize<kSorted>(p, dtype, (cudaStream_t)stream);
 }
 
+int gb_moe_sort_applies(int64_t P, int64_t E) { return P >= 1 && P <= (int64_t)kSortMostCtas * kSortThreads * kSortMostPer && E >= 1 && E <= kSortExperts; }
+
+int gb_moe_sort(const void* ids, int id_bytes, int64_t P, int64_t E, int64_t expert_base, int32_t* counts, int32_t* offsets, int32_t* order,
+                int32_t* place, void* stream) {
+  GB_REQUIRE(id_bytes == 4 || id_bytes == 8, "ids of %d bytes", id_bytes);
+  if (!gb_moe_sort_applies(P, E)) return gb_fail(GB_EUNSUPPORTED, "%lld pairs of %lld experts: gb_moe_route_inv sorts them", (long long)P, (long long)E);
+  GB_REQUIRE(ids && counts && offsets && order && place, "null pointer argument");
+  if (id_bytes == 8) return launch_sort<int64_t>(ids, (int)P, (int)E, expert_base, counts, offsets, order, place, (cudaStream_t)stream);
+  return launch_sort<int32_t>(ids, (int)P, (int)E, expert_base, counts, offsets, order, place, (cudaStream_t)stream);
+}
+
 int gb_moe_permute(const void* x, int64_t elem_bytes, int64_t ld, const int32_t* place, const int32_t* live, int64_t T, int64_t topk, int64_t H,
                    void* rows, void* stream) {
   const int rc = check_sorted(place, T, topk, H);
@@ -434,7 +575,7 @@ int gb_moe_permute(const void* x, int64_t elem_bytes, int64_t ld, const int32_t*
   GB_REQUIRE(all % elem_bytes == 0, "misaligned pointer");
 #define GB_PERMUTE(V)                                                                                                                \
   do {                                                                                                                               \
-    const dim3 block = token_block((int)(bytes / (int64_t)sizeof(V)));                                                               \
+    const dim3 block = token_block((int)(bytes / (int64_t)sizeof(V)), 256);                                                               \
     GB_CUDA_OK(gb_launch(permute_kernel<V>, dim3((unsigned)((T + block.y - 1) / block.y)), block, 0, (cudaStream_t)stream,           \
                          (const uint8_t*)x, pitch, place, live, T, (int)topk, (int)(bytes / (int64_t)sizeof(V)), (uint8_t*)rows));   \
   } while (0)
@@ -457,7 +598,7 @@ int gb_moe_unpermute(const void* y, int dtype, const int32_t* place, const float
   GB_REQUIRE(all % eb == 0, "misaligned pointer");
   const bool vec = H % per == 0 && all % 16 == 0;
   const int vecs = (int)(vec ? H / per : H);
-  const dim3 block = token_block(vecs), grid((unsigned)((T + block.y - 1) / block.y));
+  const dim3 block = token_block(vecs, 256), grid((unsigned)((T + block.y - 1) / block.y));
 #define GB_UNPERMUTE(D, V)                                                                                                         \
   GB_CUDA_OK(gb_launch(unpermute_kernel<D, V>, grid, block, 0, (cudaStream_t)stream, (const D::word*)y, place, weights, T, (int)topk, vecs, \
                        (D::word*)out))
@@ -480,11 +621,11 @@ int gb_moe_unpermute_grad(const void* d_out, const void* y, int dtype, const int
   GB_REQUIRE(all % eb == 0, "misaligned pointer");
   const bool vec = H % per == 0 && all % 16 == 0;
   const int vecs = (int)(vec ? H / per : H);
-  const dim3 block = token_block(vecs), grid((unsigned)((T + block.y - 1) / block.y));
+  const dim3 block = token_block(vecs, 128), grid((unsigned)((T + block.y - 1) / block.y));
 #define GB_GRAD(D, V, S)                                                                                                                    \
   GB_CUDA_OK(gb_launch(unpermute_grad_kernel<D, V, S>, grid, block, 0, (cudaStream_t)stream, (const D::word*)d_out, (const D::word*)y, place, live, \
                        weights, T, (int)topk, vecs, (D::word*)d_y, d_w))
-#define GB_GRAD_SLOTS(D, V) do { if (topk > 4) GB_GRAD(D, V, 8); else GB_GRAD(D, V, 4); } while (0)
+#define GB_GRAD_SLOTS(D, V) do { if (topk > 2) GB_GRAD(D, V, 4); else GB_GRAD(D, V, 2); } while (0)
   if (dtype == GB_DTYPE_BF16) { if (vec) GB_GRAD_SLOTS(Bf16, true); else GB_GRAD_SLOTS(Bf16, false); }
   else if (dtype == GB_DTYPE_FP16) { if (vec) GB_GRAD_SLOTS(Fp16, true); else GB_GRAD_SLOTS(Fp16, false); }
   else { if (vec) GB_GRAD_SLOTS(Fp32, true); else GB_GRAD_SLOTS(Fp32, false); }

@@ -10,7 +10,7 @@
 // the M side, so that a thread holds one row and its scale is one number per block.  gemm_blocks_rows_kernel: few rows; the
 // WEIGHTS are the M side (128 features a CTA, one scale per block for the whole tile), the rows the N side in steps of
 // sixteen, K sliced over a thread-block cluster where there are fewer tiles than SMs.
-#include "gb_common.cuh"
+#include "gb_blocks.cuh"
 
 #include <cuda.h>
 #include <atomic>
@@ -40,6 +40,11 @@ struct BlocksParams {
   int* status;
   // rows kernel
   int rows_per_pass, passes, per_slice, slices, stages;
+  int overlay, sums_at;      // sums of a sliced K lie over the ring, or that far behind its start
+  // rows quantised by the kernel itself: M of them, ld elements apart
+  const void* x;
+  int64_t ld, K;
+  int scale_rule;
 };
 
 // ---- waits, copies, MMAs -------------------------------------------------------------------------------------
@@ -149,14 +154,6 @@ GB_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr));
 }
-// Two fp32 in one register pair: one instruction multiplies and adds both, each rounded as fmaf.
-GB_DEVINL uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-GB_DEVINL void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-GB_DEVINL void fma_f32x2(uint64_t& d, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
 template <int kRegs>
 GB_DEVINL void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs>
@@ -207,27 +204,27 @@ GB_DEVINL void store1(void* D, int64_t at, float v, int out) {
   else static_cast<uint16_t*>(D)[at] = __half_as_ushort(__float2half_rn(v));
 }
 
-// Segment starts and the number of row tiles in front of each expert, into shared memory, by one warp.
+// Segment starts and the number of row tiles in front of each expert, into shared memory, by one warp: a lane takes consecutive
+// experts, so that their loads are in flight together.
 GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, int* base_s) {
-  const int lane = threadIdx.x & 31;
-  int carry = 0;
-  for (int e0 = 0; e0 < p.E; e0 += 32) {
-    const int e = e0 + lane;
-    const int lo = e < p.E ? p.seg[e] : 0, hi = e < p.E ? p.seg[e + 1] : 0;
-    const int tiles = (hi - lo + tile_rows - 1) / tile_rows;
-    int incl = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (e < p.E) {
-      seg_s[e] = lo;
-      base_s[e] = carry + incl - tiles;
-      if (e == p.E - 1) { seg_s[p.E] = hi; base_s[p.E] = carry + incl; }
-    }
-    carry += __shfl_sync(0xffffffffu, incl, 31);
+  const int lane = threadIdx.x & 31, per = (p.E + 31) / 32, e0 = lane * per, e1 = min(p.E, e0 + per);
+  int tiles = 0;
+#pragma unroll 8
+  for (int e = e0; e < e1; ++e) {
+    const int lo = p.seg[e], hi = p.seg[e + 1];
+    seg_s[e] = lo;
+    base_s[e] = tiles;
+    tiles += (hi - lo + tile_rows - 1) / tile_rows;
+    if (e == p.E - 1) seg_s[p.E] = hi;
   }
+  int incl = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  for (int e = e0; e < e1; ++e) base_s[e] += incl - tiles;
+  if (lane == 31) base_s[p.E] = incl;
 }
 
 // ======================================== CTA pairs ========================================================
@@ -246,8 +243,10 @@ constexpr int kGroupM = 16;                          // row tiles walked togethe
 template <bool kGrouped>
 struct Pair {
   static constexpr int kABytes = kBM * kSlab, kBBytes = kBN / 2 * kSlab, kStageBytes = kABytes + kBBytes;
-  static constexpr int kOutBytes = kEpiWarps * 2 * kOutChunk + (kGrouped ? kSegBytes : 0);
-  static constexpr int kStages = (227 * 1024 - 2048 - kOutBytes) / kStageBytes;
+  static constexpr int kChunks = kGrouped ? 1 : 2;     // on their way out, of a warp
+  static constexpr int kOutBytes = kEpiWarps * kChunks * kOutChunk + (kGrouped ? kSegBytes : 0);
+  // an even number: each of the two MMA issuers meets every phase of the stages that it waits for
+  static constexpr int kStages = (227 * 1024 - 2048 - kOutBytes) / kStageBytes / 2 * 2;
   static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 2048;
 };
 
@@ -299,7 +298,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
   uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
-  const uint32_t out_ring = ring + kStages * S::kStageBytes;             // two chunks per read-out warp
+  const uint32_t out_ring = ring + kStages * S::kStageBytes;             // one or two chunks per read-out warp
   const uint32_t full_bar = out_ring + (S::kOutBytes + 7) / 8 * 8;       // leader: both CTAs' operand tiles have landed
   const uint32_t empty_bar = full_bar + 8 * kStages;                     // the MMAs that read the stage are done
   const uint32_t acc_full = empty_bar + 8 * kStages;                     // [kAccs] a block's sums are complete
@@ -307,23 +306,24 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   const uint32_t slot = acc_empty + 8 * kAccs;
   volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(ring_ptr + (slot - ring));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
-  int* seg_s = reinterpret_cast<int*>(ring_ptr + (out_ring - ring) + kEpiWarps * 2 * kOutChunk);
+  int* seg_s = reinterpret_cast<int*>(ring_ptr + (out_ring - ring) + kEpiWarps * S::kChunks * kOutChunk);
   int* base_s = seg_s + kMaxGroups + 1;
 
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   gb_pdl_launch_dependents();
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      bar_init(full_bar + 8 * s, 1);
-      bar_init(empty_bar + 8 * s, 1);
+  {                                                        // a barrier of each kind per thread
+    const uint32_t i = threadIdx.x;
+    if (i < kStages) {
+      bar_init(full_bar + 8 * i, 1);
+      bar_init(empty_bar + 8 * i, 1);
     }
-    for (int b = 0; b < kAccs; ++b) {
-      bar_init(acc_full + 8 * b, 1);
-      bar_init(acc_empty + 8 * b, kEpiWarps);
+    if (i < kAccs) {
+      bar_init(acc_full + 8 * i, 1);
+      bar_init(acc_empty + 8 * i, kEpiWarps);
     }
-    *abort_flag = 0;
+    if (i == 0) *abort_flag = 0;
     gb_fence_barrier_init();
   }
   if (warp == kEpiWarps + 1) {
@@ -331,7 +331,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   gb_pdl_wait();
-  if (kGrouped && warp == 0) load_segments(p, kPairM, seg_s, base_s);
+  if (kGrouped && warp == kEpiWarps) load_segments(p, kPairM, seg_s, base_s);
   tmem_fence_before();
   __syncthreads();
   gb_cluster_sync();                                                     // both CTAs' barriers exist
@@ -412,9 +412,9 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     const uint32_t acc_empty_pair = leader_addr(acc_empty);
     // Four warps for each part, one per lane quarter: while one of a scheduler's two adds, the other waits or loads.  (All
     // eight on half of every part wait together and then add together.)
-    constexpr int kChunks = kPart / 32;
+    constexpr int kOuts = kPart / 32;
     const int quarter = warp & 3, part = warp >> 2, c_lo = part * kPart;
-    const uint32_t out = out_ring + (uint32_t)warp * 2 * kOutChunk;
+    const uint32_t out = out_ring + (uint32_t)warp * S::kChunks * kOutChunk;
     const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16);
     int buf = part, flip = 0;
     uint32_t ph = 0;
@@ -459,10 +459,10 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       if (!ok) break;
       if (p.out_tma && (!kGrouped || row0 + 32 <= T.end)) {  // dense: what sticks out is not written
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < kOuts; ++c) {
           const uint32_t dst = out + (uint32_t)flip * kOutChunk;
-          flip ^= 1;
-          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");       // the chunk before last has left its buffer
+          if (S::kChunks == 2) flip ^= 1;
+          asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(S::kChunks - 1) : "memory");     // the buffer's last chunk has left it
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {                      // 64-byte swizzle: eight rows touch eight bank groups
@@ -517,11 +517,15 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
 // ======================================== few rows =========================================================
 constexpr int kMaxStages = 12, kMaxSlices = 8;
 constexpr int kScaleSlots = 4;                       // groups of four blocks whose scales are there ahead of their sums
+constexpr int kQuantWarps = 4, kQuantStages = 10, kScaleRing = 32;    // rows quantised here: warps that do, fewest stages, blocks whose scales are kept
 
-template <int kR>
+// In: the type of rows that the kernel quantises itself, or void: A is E4M3 with its scales.
+template <int kR, typename In = void>
 struct Rows {
+  static constexpr bool kQuantize = !std::is_void<In>::value;
   static constexpr int kRead = kR == 16 ? 4 : 8;     // read-out warps: two per lane quarter where there are columns for both
-  static constexpr int kThreads = 32 * (kRead + 3);
+  static constexpr int kThreads = 32 * (kRead + 3 + (kQuantize ? kQuantWarps : 1));
+  static constexpr int kBox = kR < 32 ? kR : 32;     // rows of a copy of A
   static constexpr int kMine = kR / 16 / (kRead / 4);          // chunks of sixteen columns of a warp
   static constexpr int kAccs = kR <= 64 ? 8 : 512 / kR;
   static constexpr uint32_t kTmem = kAccs * kR < 32 ? 32 : kAccs * kR;
@@ -529,47 +533,50 @@ struct Rows {
 };
 constexpr int kSmemMax = 224 * 1024;                 // with the static arrays within the 227 KB of a CTA
 
-template <int kR, bool kGrouped>
-__global__ void __launch_bounds__(Rows<kR>::kThreads, 1)
+template <int kR, bool kGrouped, typename In>
+__global__ void __launch_bounds__(Rows<kR, In>::kThreads, 1)
 gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ BlocksParams p) {
-  using S = Rows<kR>;
+  using S = Rows<kR, In>;
+  constexpr bool kQuantize = S::kQuantize;
+  constexpr int kScaleBars = kQuantize ? kScaleRing : kScaleSlots, kScaleRows = kQuantize ? kScaleRing : 4 * kScaleSlots;
   constexpr int kRead = S::kRead, kAccs = S::kAccs, kMine = S::kMine;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_s[kMaxStages], empty_s[kMaxStages], acc_full_s[kAccs], acc_empty_s[kAccs], sc_full_s[kScaleSlots], sc_empty_s[kScaleSlots];
+  __shared__ uint64_t full_s[kMaxStages], empty_s[kMaxStages], acc_full_s[kAccs], acc_empty_s[kAccs], sc_full_s[kScaleBars], sc_empty_s[kScaleSlots];
   __shared__ uint32_t slot_s;
   __shared__ volatile int abort_s;
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of a cluster
   uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
-  float* scale_s = reinterpret_cast<float*>(ring_ptr + p.stages * S::kStageBytes);      // [slot][4][kR]
-  int* seg_s = reinterpret_cast<int*>(scale_s + kScaleSlots * 4 * kR);
+  float* scale_s = reinterpret_cast<float*>(ring_ptr + p.stages * S::kStageBytes);      // [slot][4][kR], or [block % kScaleRing][kR]
+  int* seg_s = reinterpret_cast<int*>(scale_s + kScaleRows * kR);
   int* base_s = seg_s + kMaxGroups + 1;
   const uint32_t full_bar = gb_smem_u32(full_s), empty_bar = gb_smem_u32(empty_s), acc_full = gb_smem_u32(acc_full_s),
                  acc_empty = gb_smem_u32(acc_empty_s), sc_full = gb_smem_u32(sc_full_s), sc_empty = gb_smem_u32(sc_empty_s);
 
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   gb_pdl_launch_dependents();
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      gb_mbar_init(&full_s[s], 1);
-      gb_mbar_init(&empty_s[s], 1);
+  {                                                        // a barrier of each kind per thread: one thread took 600 clocks
+    const int i = (int)threadIdx.x;
+    if (i < p.stages) {
+      gb_mbar_init(&full_s[i], kQuantize ? 1 + (uint32_t)p.M : 1);       // and every row's block
+      gb_mbar_init(&empty_s[i], 1);
     }
-    for (int b = 0; b < kAccs; ++b) {
-      gb_mbar_init(&acc_full_s[b], 1);
-      gb_mbar_init(&acc_empty_s[b], kRead);
+    if (i < kAccs) {
+      gb_mbar_init(&acc_full_s[i], 1);
+      gb_mbar_init(&acc_empty_s[i], kRead);
     }
-    for (int b = 0; b < kScaleSlots; ++b) {
-      gb_mbar_init(&sc_full_s[b], 1);
-      gb_mbar_init(&sc_empty_s[b], kRead);
-    }
-    abort_s = 0;
+    if (i < kScaleBars) gb_mbar_init(&sc_full_s[i], kQuantize ? (uint32_t)p.M : 1);
+    if (i < kScaleSlots) gb_mbar_init(&sc_empty_s[i], kRead);
+    if (i == 0) abort_s = 0;
     gb_fence_barrier_init();
   }
   if (warp == kRead + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gb_smem_u32(&slot_s)), "r"(S::kTmem) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the sums of a sliced K have a place of their own: that the others have started is all that a CTA has to know, by the end
+  if (p.slices > 1 && !p.overlay) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   if (!p.beside) gb_pdl_wait();
-  if (kGrouped && warp == 0) load_segments(p, kR, seg_s, base_s);
+  if (kGrouped && warp == kRead) load_segments(p, kR, seg_s, base_s);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -612,14 +619,15 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     for (int item = first; ok && item < total; item += stride) {
       const Item t = item_at(item, e);
       e = t.e;
-      const int m0 = uniform(t.m0), w0 = uniform(t.w0);
+      const int m0 = uniform(t.m0), w0 = uniform(t.w0), boxes = kQuantize ? 0 : (uniform(t.rows) + S::kBox - 1) / S::kBox;
+      const uint32_t bytes = kBM * kSlab + (uint32_t)boxes * (S::kBox * kSlab);
       int ahead = 0;                                       // slabs whose weights are on their way already
       if (!waited) {
         // the launch ahead still writes the rows: the weights of the first stages need not wait for it
         for (; ok && ahead < min(p.stages, k_n); ++ahead) {
           ok = warp_wait(empty_bar + 8 * ahead, 1, &abort_s, p.status, 95);
           if (ok && one) {
-            expect_tx(full_bar + 8 * ahead, S::kStageBytes);
+            expect_tx(full_bar + 8 * ahead, bytes);
             tma_load_2d(ring + (uint32_t)ahead * S::kStageBytes, &map_w, (k_begin + ahead) * kSlab, w0, full_bar + 8 * ahead);
           }
           __syncwarp();
@@ -633,27 +641,30 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         if (one) {
           const uint32_t st = ring + (uint32_t)s * S::kStageBytes, bar = full_bar + 8 * s;
           if (kt >= ahead) {
-            expect_tx(bar, S::kStageBytes);
+            expect_tx(bar, bytes);
             tma_load_2d(st, &map_w, (k_begin + kt) * kSlab, w0, bar);
           }
-          tma_load_2d(st + kBM * kSlab, &map_x, (k_begin + kt) * kSlab, m0, bar);
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d(st + kBM * kSlab + (uint32_t)i * (S::kBox * kSlab), &map_x, (k_begin + kt) * kSlab, m0 + i * S::kBox, bar);
         }
         __syncwarp();
         if (++s == p.stages) { s = 0; ph ^= 1; }
       }
     }
-  } else if (warp == kRead + 1) {
-    // ------------------------------- MMA issuer ---------------------------------
+  } else if (warp == kRead + 1 || warp == kRead + 2) {
+    // ------ MMA issuers: the waits, MMAs and commits of a slab take one some 450 clocks, so two share the slabs in turn; every
+    // slab has an accumulator of its own.  Stages and accumulators are even in number: each issuer meets all phases of its ones. ------
     const bool one = gb_elect_one();
-    int s = 0, buf = 0, e = 0;
+    const int mine = warp - kRead - 1;
+    int s = mine, buf = mine, e = 0, kt = mine;
     uint32_t ph = 0, acc_ph = 1;
     bool ok = true;
-    for (int item = first; ok && item < total; item += stride) {
+    for (int item = first; ok && item < total; item += stride, kt -= k_n) {
       const Item t = item_at(item, e);
       e = t.e;
       const uint32_t idesc = p.idesc | (uint32_t)((uniform(t.rows) + 15) / 16 * 2) << 17 | (uint32_t)(kBM >> 4) << 24;
-      for (int kt = 0; kt < k_n; ++kt) {
-        ok = warp_wait(acc_empty + 8 * buf, acc_ph, &abort_s, p.status, 96);
+      for (; kt < k_n; kt += 2) {
+        ok = warp_wait<kTensorMemory>(acc_empty + 8 * buf, acc_ph, &abort_s, p.status, 96);
         if (!ok) break;
         ok = warp_wait(full_bar + 8 * s, ph, &abort_s, p.status, 97);
         if (!ok) break;
@@ -664,15 +675,80 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 #pragma unroll
           for (int k = 0; k < 4; ++k)                      // 32 columns of K per instruction
             mma<1>(tmem + (uint32_t)(buf * kR), dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, k > 0);
-          commit_to<1>(empty_bar + 8 * s);
           commit_to<1>(acc_full + 8 * buf);
+          commit_to<1>(empty_bar + 8 * s);
         }
         __syncwarp();
-        if (++s == p.stages) { s = 0; ph ^= 1; }
-        if (++buf == kAccs) { buf = 0; acc_ph ^= 1; }
+        s += 2;
+        if (s >= p.stages) { s -= p.stages; ph ^= 1; }
+        buf += 2;
+        if (buf >= kAccs) { buf -= kAccs; acc_ph ^= 1; }
       }
     }
-  } else if (warp == kRead + 2) {
+  } else if (kQuantize && warp >= kRead + 3) {
+    // ------- rows -> E4M3 in the operand's place, their scales times the tile's: eight lanes take a row's block, sixteen columns
+    // each; items (block, row) in that order, up to sixteen a step, loaded two steps ahead -------
+    if constexpr (kQuantize) {
+      constexpr int kPieces = sizeof(typename In::word);       // of sixteen bytes, in sixteen columns
+      const int mine = (warp - kRead - 3) * 4 + (lane >> 3), c = lane & 7, rows = (int)p.M, step = min(4 * kQuantWarps, 4 * rows);
+      const uint32_t total_items = (uint32_t)k_n * (uint32_t)rows;
+      struct Raw { uint4 v[kPieces]; float bs; int kt, row; };
+      int before = 0;                                      // slabs of the items before this one
+      bool ok = true;
+      for (int item = first; ok && item < total; item += stride) {
+        const Item t = item_at(item, 0);
+        const float* bs = p.b_scale + (int64_t)(t.n0 / kSlab) * p.kb;
+        auto load = [&](uint32_t i, Raw& r) {
+          const bool live = mine < step && i < total_items;
+          r.kt = live ? (int)(i / (uint32_t)rows) : -1;
+          r.row = live ? (int)(i - (uint32_t)r.kt * (uint32_t)rows) : 0;
+          const int64_t col = (int64_t)(k_begin + r.kt) * kSlab + c * 16;
+          const uint4* at = reinterpret_cast<const uint4*>(static_cast<const typename In::word*>(p.x) + r.row * p.ld + col);
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q) r.v[q] = live && col < p.K ? at[q] : make_uint4(0u, 0u, 0u, 0u);
+          r.bs = live ? bs[k_begin + r.kt] : 0.0f;
+        };
+        Raw cur, next;
+        load((uint32_t)mine, cur);
+        load((uint32_t)(mine + step), next);
+        for (uint32_t i0 = 0; i0 < total_items; i0 += (uint32_t)step) {
+          Raw after;
+          load(i0 + (uint32_t)(mine + 2 * step), after);
+          float v[16], scale;
+          uint32_t q[4];
+#pragma unroll
+          for (int k = 0; k < kPieces; ++k) gb_blocks::unpack16<In>(cur.v[k], v + k * (16 / kPieces));
+          gb_blocks::quantize_block<16, 8>(v, p.scale_rule, scale, q);
+          const bool live = cur.kt >= 0;
+          const int n = before + cur.kt, turn = n / p.stages, s = n - turn * p.stages;
+          // The stage is free once the MMAs that read it last are done.  A barrier's parity tells a phase from the next one only:
+          // this wait's phase cannot be over, for its MMAs need the block that is written below, and the phase before the last is,
+          // for the warp has waited, a step or two ago, for a slab at most `stages` before this one (steps of no more than four slabs).
+          const bool there = !live || try_wait<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u);
+          if (!__all_sync(0xffffffffu, there)) {
+            if (!there) wait_slow<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u, &abort_s, p.status, 98);
+            ok = !__any_sync(0xffffffffu, abort_s != 0);
+            if (!ok) break;
+          }
+          if (live) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(ring + (uint32_t)s * S::kStageBytes + kBM * kSlab + (uint32_t)(cur.row * kSlab + ((c ^ (cur.row & 7)) * 16))), "r"(q[0]),
+                           "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
+            if (c == 0) scale_s[(n % kScaleRing) * kR + cur.row] = scale * cur.bs;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (live && c == 0) {
+            arrive(full_bar + 8 * s);
+            arrive(sc_full + 8 * (n % kScaleRing));
+          }
+          cur = next;
+          next = after;
+        }
+        before += k_n;
+      }
+    }
+  } else if (warp == kRead + 3) {
     // ------------------- scales of the rows times the tile's, four blocks at a time --------------------
     if (p.beside) gb_pdl_wait();
     int slot = 0, e = 0;
@@ -719,28 +795,31 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     for (int item = first; ok && item < total; item += stride) {
       const Item t = item_at(item, e);
       e = t.e;
+      const int cols = (t.rows + 15) / 16;                 // sixteens that hold rows
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[i][c] = 0.0f;
       for (int kt = 0; ok && kt < k_n; ++kt) {
-        if ((kt & 3) == 0) {
+        if (kQuantize || (kt & 3) == 0) {
           ok = warp_wait(sc_full + 8 * slot, sc_ph, &abort_s, p.status, 99);
           if (!ok) break;
         }
-        ok = warp_wait(acc_full + 8 * buf, ph, &abort_s, p.status, 100);
+        ok = warp_wait<kTensorMemory>(acc_full + 8 * buf, ph, &abort_s, p.status, 100);
         if (!ok) break;
         tmem_fence_after();
-        const float* sc = scale_s + (slot * 4 + (kt & 3)) * kR;
+        const float* sc = scale_s + (kQuantize ? slot : slot * 4 + (kt & 3)) * kR;
         uint32_t v[kMine][16];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) tmem_ld16(at + (uint32_t)(buf * kR + (i * (kRead / 4) + group) * 16), v[i]);
+        for (int i = 0; i < kMine; ++i)
+          if (kMine == 1 || i * (kRead / 4) + group < cols) tmem_ld16(at + (uint32_t)(buf * kR + (i * (kRead / 4) + group) * 16), v[i]);
         tmem_wait_ld();
         tmem_fence_before();
         __syncwarp();
         if (lane == 0) arrive(acc_empty + 8 * buf);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
+          if (kMine > 1 && i * (kRead / 4) + group >= cols) break;
           const float4* s4 = reinterpret_cast<const float4*>(sc + (i * (kRead / 4) + group) * 16);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -752,7 +831,11 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
           }
         }
         if (++buf == kAccs) { buf = 0; ph ^= 1; }
-        if ((kt & 3) == 3 || kt + 1 == k_n) {
+        if (kQuantize) {
+          // no arrival: an entry is written again 32 slabs on, behind a stage that was freed by MMAs whose accumulators this
+          // warp had released long after (stages + accumulators <= 20 slabs)
+          if (++slot == kScaleRing) { slot = 0; sc_ph ^= 1; }
+        } else if ((kt & 3) == 3 || kt + 1 == k_n) {
           __syncwarp();
           if (lane == 0) arrive(sc_empty + 8 * slot);
           if (++slot == kScaleSlots) { slot = 0; sc_ph ^= 1; }
@@ -777,13 +860,19 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   }
 
   if (p.slices > 1) {
-    // Sums into the shared memory of the CTA that owns the row, [slice][own row][feature], over the operand ring: every CTA
-    // of the cluster has finished its MMAs, and with them its loads.  Rows are owned in sixteens.
+    // Sums into the shared memory of the CTA that owns the row, [slice][own row][feature]; where that lies over the operand
+    // ring, every CTA of the cluster has finished its MMAs first, and with them its loads.  Rows are owned in sixteens.
     const bool live = warp < kRead && !abort_s && first < total;
     const int rows = live ? last.rows : 0, cols = (rows + 15) / 16 * 16;
     const int own = (cols / 16 + p.slices - 1) / p.slices * 16;
     const int quarter = warp & 3, group = warp >> 2, feature = quarter * 32 + lane;
-    gb_cluster_sync();
+    const uint32_t sums = p.overlay ? ring : ring + (uint32_t)p.sums_at;
+    if (p.overlay) {
+      gb_cluster_sync();
+    } else {
+      __syncwarp();
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
     if (live) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -792,7 +881,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         const int to = r0 / own, off = r0 - to * own;
         uint32_t dst;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                     : "=r"(dst) : "r"(ring + (uint32_t)((slice * own + off) * kBM + feature) * 4u), "r"(to));
+                     : "=r"(dst) : "r"(sums + (uint32_t)((slice * own + off) * kBM + feature) * 4u), "r"(to));
 #pragma unroll
         for (int c = 0; c < 16; ++c)
           if (r0 + c < rows)
@@ -808,7 +897,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         for (int q = 0; q < p.slices; ++q) {
           float v[4];
           asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(ring + (uint32_t)((q * own + r) * kBM + f) * 4u));
+                       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(sums + (uint32_t)((q * own + r) * kBM + f) * 4u));
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] += v[i];
         }
@@ -837,20 +926,22 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 std::mutex g_mutex;
 int g_pairs[64][2];                                        // pairs that run at once, per device and kernel (0: not asked)
 std::atomic<bool> g_ready[64];                             // shared-memory limits of the device's kernels are set
-GbClusters g_clusters[8];
 
 int set_limits() {
 #define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
   GB_ATTR(gemm_blocks_pair_kernel<false>, Pair<false>::kSmem);
   GB_ATTR(gemm_blocks_pair_kernel<true>, Pair<true>::kSmem);
-  GB_ATTR((gemm_blocks_rows_kernel<16, false>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<32, false>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<64, false>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<128, false>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<16, true>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<32, true>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<64, true>), kSmemMax);
-  GB_ATTR((gemm_blocks_rows_kernel<128, true>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, false, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<32, false, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<64, false, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<128, false, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, true, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<32, true, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<64, true, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<128, true, void>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, false, gb_blocks::Bf16>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, false, gb_blocks::Fp16>), kSmemMax);
+  GB_ATTR((gemm_blocks_rows_kernel<16, false, gb_blocks::Fp32>), kSmemMax);
 #undef GB_ATTR
   return GB_OK;
 }
@@ -925,9 +1016,9 @@ int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   return GB_OK;
 }
 
-template <int kR, bool kGrouped>
+template <int kR, bool kGrouped, typename In = void>
 int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
-  using S = Rows<kR>;
+  using S = Rows<kR, In>;
   const int64_t sms = gb_sm_count();
   if (sms <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
   p.n_tiles = (int)((p.N + kBM - 1) / kBM);
@@ -943,25 +1034,34 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   }
   GB_REQUIRE(most < (1ll << 31), "too many output tiles");
   // K slices: as many as the SMs take, at least four blocks each
-  GbClusters& clusters = g_clusters[(kR == 16 ? 0 : kR == 32 ? 1 : kR == 64 ? 2 : 3) + 4 * kGrouped];
+  static GbClusters clusters;
   int want = 1;
   for (int n = 2; n <= (kR <= 64 ? kMaxSlices : 4) && most * n <= sms && n * 4 <= p.kb; ++n)
-    if (most <= clusters.ask((const void*)gemm_blocks_rows_kernel<kR, kGrouped>, S::kThreads, kSmemMax, n)) want = n;
+    if (most <= clusters.ask((const void*)gemm_blocks_rows_kernel<kR, kGrouped, In>, S::kThreads, kSmemMax, n)) want = n;
   p.per_slice = (p.kb + want - 1) / want;
   p.slices = (p.kb + p.per_slice - 1) / p.per_slice;
-  constexpr int kFixed = 1024 + kScaleSlots * 4 * kR * 4 + (kGrouped ? kSegBytes : 0);
-  p.stages = (kSmemMax - kFixed) / S::kStageBytes;
+  constexpr int kFixed = 1024 + (S::kQuantize ? kScaleRing : 4 * kScaleSlots) * kR * 4 + (kGrouped ? kSegBytes : 0);
+  // the sums take up to 64 KB: of their own where that leaves enough stages
+  constexpr int kLeast = S::kQuantize ? kQuantStages : 8;
+  const int own = (kR / 16 + p.slices - 1) / p.slices * 16, sums = p.slices > 1 ? p.slices * own * kBM * 4 : 0;
+  p.overlay = (kSmemMax - kFixed - sums) / S::kStageBytes < kLeast;
+  p.stages = (kSmemMax - kFixed - (p.overlay ? 0 : sums)) / S::kStageBytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.stages &= ~1;
+  static_assert(!S::kQuantize || (kSmemMax - kFixed) / S::kStageBytes >= kLeast, "the quantising warps count on so many stages");
+  p.sums_at = kFixed - 1024 + p.stages * S::kStageBytes;
   p.idesc = 1u << 4;
-  CUtensorMap map_w, map_x;
+  CUtensorMap map_w, map_x = {};
   int rc = gb_tensor_map_operand(&map_w, W, (kGrouped ? p.E : 1) * p.N, K, 1, kBM);
   if (rc != GB_OK) return rc;
-  rc = gb_tensor_map_operand(&map_x, A, p.M, K, 1, kR);
-  if (rc != GB_OK) return rc;
+  if (!S::kQuantize) {
+    rc = gb_tensor_map_operand(&map_x, A, p.M, K, 1, S::kBox);
+    if (rc != GB_OK) return rc;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.slices > 1 || most < sms ? most : sms), (unsigned)p.slices);
   cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = kFixed + p.stages * S::kStageBytes;
+  cfg.dynamicSmemBytes = kFixed + p.stages * S::kStageBytes + (p.overlay ? 0 : sums);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -977,7 +1077,7 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   cfg.attrs = attr;
   cfg.numAttrs = n;
   gb_count_launch();
-  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_rows_kernel<kR, kGrouped>, map_w, map_x, p));
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_rows_kernel<kR, kGrouped, In>, map_w, map_x, p));
   return GB_OK;
 }
 
@@ -1027,6 +1127,29 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
   const BlocksParams p = params(a_scale, w_scale, D, out, M, N, K, beside);
   if (M <= 128) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
   return run_pair<false>(A, W, K, p, (cudaStream_t)stream);
+}
+
+// us, two launches / one: 1 row of 34816 x 5120 34.9 / 32.9, 4 rows 35.7 / 33.7, 8 rows 36.7 / 43.0; 4 rows of 4096 x 4096 10.3 / 8.4, 16 rows
+// 10.3 / 12.3: every CTA quantises all rows, four blocks at a time and warp.
+static constexpr int64_t kQuantMaxRows = 4;
+
+int gb_linear_fp8_blocks(const void* x, int dtype, int64_t ld, int scale_rule, const void* W, const float* w_scale, void* D, int out, int64_t M, int64_t N,
+                         int64_t K, void* stream) {
+  GB_REQUIRE(dtype >= GB_DTYPE_BF16 && dtype <= GB_DTYPE_FP32, "unknown dtype %d", dtype);
+  GB_REQUIRE(scale_rule == GB_SCALE_RULE_RECIP || scale_rule == GB_SCALE_RULE_DIV, "unknown scale rule %d", scale_rule);
+  const int eb = dtype == GB_DTYPE_FP32 ? 4 : 2;
+  GB_REQUIRE(ld >= K || M <= 1, "row stride %lld is shorter than the row", (long long)ld);
+  if (M > kQuantMaxRows || ((uintptr_t)x & 15u) != 0 || (M > 1 && ld * eb % 16 != 0))
+    return gb_fail(GB_EUNSUPPORTED, "more than 4 rows, or rows off the 16-byte alignment: quantise them first");
+  const int rc = check_blocks(W, w_scale, W, w_scale, D, out, M, N, K, 1);
+  if (rc != GB_OK || M == 0) return rc;
+  GB_REQUIRE(x != nullptr, "null pointer argument");
+  BlocksParams p = params(w_scale, w_scale, D, out, M, N, K, 0);
+  p.x = x; p.ld = ld; p.K = K; p.scale_rule = scale_rule;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == GB_DTYPE_BF16) return run_rows<16, false, gb_blocks::Bf16>(nullptr, W, K, p, st);
+  if (dtype == GB_DTYPE_FP16) return run_rows<16, false, gb_blocks::Fp16>(nullptr, W, K, p, st);
+  return run_rows<16, false, gb_blocks::Fp32>(nullptr, W, K, p, st);
 }
 
 int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* W, const float* w_scale, const int32_t* seg_offsets, int64_t E, void* D,

@@ -11,6 +11,7 @@
 // The library is reached through dlsym on the path the ctypes loader uses, so that both bind the
 // same file and a missing symbol fails closed.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -45,7 +46,7 @@ namespace {
   F(gb_moe_mlp_pairs_workspace_bytes) F(gb_moe_combine) F(gb_gemv_hinted) F(gb_scales_e4m3) F(gb_moe_route_inv) \
   F(gb_moe_fp4_pass_rows) F(gb_moe_fp4_operand_bytes) F(gb_moe_fp4_rows) F(gb_moe_fp4_swiglu_rows) \
   F(gb_moe_gemv_fp4) F(gb_moe_gemm_fp4) F(gb_fp8_quantize_blocks) F(gb_moe_swiglu_fp8) F(gb_moe_permute_fp8) \
-  F(gb_gemm_fp8_blocks) F(gb_gemm_fp8_blocks_grouped) F(gb_moe_permute) F(gb_moe_unpermute) F(gb_moe_unpermute_grad)
+  F(gb_gemm_fp8_blocks) F(gb_gemm_fp8_blocks_grouped) F(gb_linear_fp8_blocks) F(gb_moe_sort) F(gb_moe_sort_applies) F(gb_moe_permute) F(gb_moe_unpermute) F(gb_moe_unpermute_grad)
 
 struct Lib {
 #define GB_FN(name) decltype(&::name) name = nullptr;
@@ -738,13 +739,18 @@ std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
 
 using Two = std::tuple<at::Tensor, at::Tensor>;
 
+// An uninitialised tensor on `like`'s device, past the dispatcher (0.8 us a call).
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
+}
+
 Two fp8_quantize_blocks(const at::Tensor& x, int rule) {
   need_cuda(x);
   const int dt = dtype_code(x.scalar_type(), "the block quantiser");
   const c10::cuda::CUDAGuard guard(x.device());
   const RowsOf r(x);
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scale = at::empty(with_last(x, blocks(r.K)), x.options().dtype(at::kFloat));
+  at::Tensor q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+  at::Tensor scale = fresh(with_last(x, blocks(r.K)), at::kFloat, x);
   check(L.gb_fp8_quantize_blocks(r.t.data_ptr(), dt, r.ld, r.M, r.K, rule, q.data_ptr(), scale.data_ptr<float>(),
                                  c10::cuda::getCurrentCUDAStream().stream()));
   return {q, scale};
@@ -766,8 +772,8 @@ Two moe_swiglu_fp8(const at::Tensor& h, const Opt& offsets, int rule) {
   const int64_t inter = r.K / 2;
   const int32_t* live = nullptr;
   if (offsets.has_value() && offsets->defined()) live = offsets_of(*offsets, h, -1) + offsets->numel() - 1;
-  at::Tensor q = at::empty({r.M, inter}, h.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scale = at::empty({r.M, blocks(inter)}, h.options().dtype(at::kFloat));
+  at::Tensor q = fresh({r.M, inter}, at::kFloat8_e4m3fn, h);
+  at::Tensor scale = fresh({r.M, blocks(inter)}, at::kFloat, h);
   check(L.gb_moe_swiglu_fp8(r.t.data_ptr(), dt, r.ld, live, r.M, inter, rule, q.data_ptr(), scale.data_ptr<float>(),
                             c10::cuda::getCurrentCUDAStream().stream()));
   return {q, scale};
@@ -797,10 +803,15 @@ at::Tensor linear_fp8_blocks(const at::Tensor& x, const at::Tensor& w, const at:
   const c10::cuda::CUDAGuard guard(x.device());
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   const int64_t N = w.size(0), K = w.size(1);
-  at::Tensor out = at::empty(with_last(x, N), x.options().dtype(ot));
+  at::Tensor out = fresh(with_last(x, N), ot, x);
   if (out.numel() == 0) return out;
   const RowsOf r(x);
   const at::Tensor wc = w.contiguous(), wsc = w_scale.contiguous();
+  if (r.M <= 4) {                                          // quantised inside the product
+    const int rc = L.gb_linear_fp8_blocks(r.t.data_ptr(), dt, r.ld, rule, wc.data_ptr(), wsc.data_ptr<float>(), out.data_ptr(), odt, r.M, N, K, stream);
+    if (rc == GB_OK) return out;
+    if (rc != GB_EUNSUPPORTED) check(rc);
+  }
   Arena a;
   const int q = a.add(r.M * K), s = a.add(r.M * blocks(K) * 4);
   a.alloc(x);
@@ -818,7 +829,7 @@ at::Tensor gemm_fp8_blocks(const at::Tensor& a, const at::Tensor& a_scale, const
   const int odt = dtype_code(out_dtype, "gemm_fp8_blocks' output");
   const c10::cuda::CUDAGuard guard(a.device());
   const at::Tensor ac = a.contiguous(), asc = a_scale.contiguous(), bc = b.contiguous(), bsc = b_scale.contiguous();
-  at::Tensor out = at::empty({a.size(0), b.size(0)}, a.options().dtype(out_dtype));
+  at::Tensor out = fresh({a.size(0), b.size(0)}, out_dtype, a);
   if (out.numel() == 0) return out;
   check(L.gb_gemm_fp8_blocks(ac.data_ptr(), asc.data_ptr<float>(), bc.data_ptr(), bsc.data_ptr<float>(), out.data_ptr(), odt, a.size(0), b.size(0),
                              a.size(1), 0, c10::cuda::getCurrentCUDAStream().stream()));
@@ -840,7 +851,7 @@ at::Tensor gemm_fp8_blocks_grouped(const at::Tensor& a, const at::Tensor& a_scal
     same_device(a, {&out});
     need(out.dim() == 2 && out.size(0) == P && out.size(1) == N && out.is_contiguous(), "out: a contiguous [" + std::to_string(P) + ", " + std::to_string(N) + "] expected");
   } else {
-    out = at::empty({P, N}, a.options().dtype(out_dtype));
+    out = fresh({P, N}, out_dtype, a);
   }
   const int odt = dtype_code(out.scalar_type(), "gemm_fp8_blocks_grouped's output");
   if (out.numel() == 0) return out;
@@ -858,15 +869,25 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Te
   const int64_t T = topk_ids.size(0), topk = topk_ids.size(1), P = T * topk;
   need(E >= 1 && E <= 4096 && topk >= 1 && P < (1ll << 30), "1 to 4096 experts, at least one a token and fewer than 2^30 pairs expected");
   const c10::cuda::CUDAGuard guard(topk_ids.device());
-  const at::Tensor ids = topk_ids.to(at::kInt).contiguous();
-  const auto opt = ids.options();
+  const auto opt = topk_ids.options().dtype(at::kInt);
   if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
-  at::Tensor counts = at::empty({E}, opt), offsets = at::empty({E + 1}, opt), order = at::empty({P}, opt), place = at::empty({P}, opt), ws;
+  at::Tensor counts = fresh({E}, at::kInt, topk_ids), offsets = fresh({E + 1}, at::kInt, topk_ids), order = fresh({P}, at::kInt, topk_ids),
+             place = fresh({P}, at::kInt, topk_ids);
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const bool wide = topk_ids.scalar_type() == at::kLong;
+  if (L.gb_moe_sort_applies(P, E)) {
+    const at::Tensor ids = (wide || topk_ids.scalar_type() == at::kInt ? topk_ids : topk_ids.to(at::kInt)).contiguous();
+    check(L.gb_moe_sort(ids.data_ptr(), wide ? 8 : 4, P, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(),
+                        place.data_ptr<int32_t>(), stream));
+    return {counts, offsets, order, place};
+  }
+  // in 32 bits, ids that do not fit them dropped like others that are held elsewhere
+  const at::Tensor ids = (wide ? topk_ids.clamp(-1, std::numeric_limits<int32_t>::max()) : topk_ids).to(at::kInt).contiguous();
+  at::Tensor ws;
   const int64_t bytes = L.gb_moe_route_workspace_bytes(T, topk, E);
   if (bytes) ws = at::empty({bytes}, opt.dtype(at::kByte));
   check(L.gb_moe_route_inv(ids.data_ptr<int32_t>(), T, topk, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(),
-                           place.data_ptr<int32_t>(), nullptr, nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
-                           c10::cuda::getCurrentCUDAStream().stream()));
+                           place.data_ptr<int32_t>(), nullptr, nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream));
   return {counts, offsets, order, place};
 }
 
@@ -890,7 +911,7 @@ Two moe_permute_fp8(const at::Tensor& x, const at::Tensor& place, const at::Tens
   const Sorted s(place, offsets, topk, x);
   const RowsOf r(x);
   need(r.M == s.T, std::to_string(s.T) + " tokens expected, got " + std::to_string(r.M));
-  at::Tensor q = at::empty({s.P, r.K}, x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty({s.P, blocks(r.K)}, x.options().dtype(at::kFloat));
+  at::Tensor q = fresh({s.P, r.K}, at::kFloat8_e4m3fn, x), scale = fresh({s.P, blocks(r.K)}, at::kFloat, x);
   check(L.gb_moe_permute_fp8(r.t.data_ptr(), dt, r.ld, s.place, s.live, s.T, topk, r.K, rule, q.data_ptr(), scale.data_ptr<float>(),
                              c10::cuda::getCurrentCUDAStream().stream()));
   return {q, scale};
@@ -901,7 +922,7 @@ at::Tensor permute_rows(const at::Tensor& x, const at::Tensor& place, const at::
   const Sorted s(place, offsets, topk, x);
   const RowsOf r(x);
   need(r.M == s.T, std::to_string(s.T) + " tokens expected, got " + std::to_string(r.M));
-  at::Tensor rows = at::empty({s.P, r.K}, x.options());
+  at::Tensor rows = fresh({s.P, r.K}, x.scalar_type(), x);
   check(L.gb_moe_permute(r.t.data_ptr(), x.element_size(), r.ld, s.place, s.live, s.T, topk, r.K, rows.data_ptr(),
                          c10::cuda::getCurrentCUDAStream().stream()));
   return rows;
@@ -912,7 +933,7 @@ at::Tensor unpermute_rows(const at::Tensor& y, const at::Tensor& place, const at
   const Sorted s(place, offsets, topk, y);
   need(y.dim() == 2 && y.size(0) == s.P && y.size(1) > 0, std::to_string(s.P) + " rows expected");
   const at::Tensor yc = y.contiguous();
-  at::Tensor out = at::empty({s.T, y.size(1)}, y.options());
+  at::Tensor out = fresh({s.T, y.size(1)}, y.scalar_type(), y);
   check(L.gb_moe_unpermute(yc.data_ptr(), dtype_code(y.scalar_type(), "moe_unpermute"), s.place, w.defined() ? w.data_ptr<float>() : nullptr, s.T, topk,
                            y.size(1), out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()));
   return out;
@@ -976,9 +997,9 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
       at::Tensor y;
       if (saved[3].defined()) {
         y = saved[3].contiguous();
-        dw = at::empty(w.sizes(), w.options());
+        dw = fresh(w.sizes(), at::kFloat, w);
       }
-      if (ctx->needs_input_grad(0)) dy = at::empty({s.P, H}, g.options());
+      if (ctx->needs_input_grad(0)) dy = fresh({s.P, H}, g.scalar_type(), g);
       check(L.gb_moe_unpermute_grad(g.data_ptr(), y.defined() ? y.data_ptr() : nullptr, dtype_code(g.scalar_type(), "moe_unpermute"), s.place, s.live,
                                     w.data_ptr<float>(), s.T, topk, H, dy.defined() ? dy.data_ptr() : nullptr,
                                     dw.defined() ? dw.data_ptr<float>() : nullptr, c10::cuda::getCurrentCUDAStream().stream()));

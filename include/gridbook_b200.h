@@ -453,18 +453,27 @@ GB_API int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_
  * that launch still runs.  0 is always right. */
 GB_API int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const float* w_scale, void* D, int out,
                               int64_t M, int64_t N, int64_t K, int beside, void* stream);
+/* gb_fp8_quantize_blocks and gb_gemm_fp8_blocks of up to 4 rows in one launch, the same values; x 16-byte aligned, rows
+ * whole 16-byte pieces apart (GB_EUNSUPPORTED otherwise: call the two). */
+GB_API int gb_linear_fp8_blocks(const void* x, int dtype, int64_t ld, int scale_rule, const void* W, const float* w_scale, void* D,
+                                int out, int64_t M, int64_t N, int64_t K, void* stream);
 GB_API int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* W, const float* w_scale,
                                       const int32_t* seg_offsets, int64_t E, void* D, int out, int64_t P, int64_t N,
                                       int64_t K, int beside, void* stream);
 
 /* ---- tokens sorted by expert and back -------------------------------------------- */
-/* place [T * topk] and *live = offsets[E] from gb_moe_route_inv.
+/* gb_moe_sort: gb_moe_route_inv without weights in one launch of one cluster, ids int32 or int64 (id_bytes), for up
+ * to 65536 pairs and 1024 experts (gb_moe_sort_applies; GB_EUNSUPPORTED past them: use gb_moe_route_inv).
+ * place [T * topk] and *live = offsets[E] from either.
  * gb_moe_permute: rows[place[p]] = x[p / topk], x [T, H] with rows `ld` elements of elem_bytes (2 or 4)
  * apart; rows from *live on become zero.
  * gb_moe_unpermute: out[t] = sum over slots of weights[p] * y[place[p]] (weights NULL: ones; dropped pairs
  * count nothing), fp32, one rounding; with NULL weights the gradient of gb_moe_permute.
  * gb_moe_unpermute_grad: d_y[place[p]] = weights[p] * d_out[p / topk], rows from *live on zero, and
  * d_w[p] = <y[place[p]], d_out[p / topk]> in fp32, zero for a dropped pair; either may be NULL. */
+GB_API int gb_moe_sort_applies(int64_t P, int64_t E);
+GB_API int gb_moe_sort(const void* topk_ids, int id_bytes, int64_t P, int64_t E, int64_t expert_base, int32_t* counts,
+                       int32_t* offsets, int32_t* order, int32_t* place, void* stream);
 GB_API int gb_moe_permute(const void* x, int64_t elem_bytes, int64_t ld, const int32_t* place, const int32_t* live, int64_t T,
                           int64_t topk, int64_t H, void* rows, void* stream);
 GB_API int gb_moe_unpermute(const void* y, int dtype, const int32_t* place, const float* weights, int64_t T, int64_t topk,

@@ -50,6 +50,14 @@ def test_grouped_gemm_refuses(lib, args, word):
     assert word in _text(lib)
 
 
+def test_one_launch_linear_refuses(lib):
+    def call(x=P, dtype=0, ld=128, rule=0, out=0, M=4, N=8, K=128):
+        return lib.gb_linear_fp8_blocks(x, dtype, ld, rule, P, P, P, out, M, N, K, NULL)
+    for kw, code, word in ((dict(M=5), 3, "4 rows"), (dict(x=ODD), 3, "4 rows"), (dict(ld=132), 3, "4 rows"), (dict(dtype=4), 1, "dtype"), (dict(rule=2), 1, "rule"),
+                           (dict(ld=64), 1, "shorter"), (dict(K=24), 1, "multiple of 16"), (dict(out=9), 1, "dtype"), (dict(N=0), 1, "shape")):
+        assert call(**kw) == code and word in _text(lib), kw
+
+
 def test_empty_calls_launch_nothing(lib):
     before = lib.gb_launch_count()
     assert lib.gb_gemm_fp8_blocks(NULL, NULL, NULL, NULL, NULL, 0, 0, 8, 128, 0, NULL) == 0
@@ -86,6 +94,13 @@ def test_sorted_rows_refuse(lib):
     assert lib.gb_moe_unpermute_grad(P, NULL, 0, P, P, P, 4, 2, 64, NULL, P, NULL) != 0 and "null" in _text(lib)
     assert lib.gb_moe_swiglu_fp8(P, 0, 64, NULL, 4, 64, 0, P, P, NULL) != 0 and "shorter" in _text(lib)
     assert lib.gb_moe_permute_fp8(P, 0, 64, P, NULL, 4, 2, 64, 0, P, P, NULL) != 0 and "null" in _text(lib)
+
+
+def test_one_launch_sort_refuses(lib):
+    assert [lib.gb_moe_sort_applies(*a) for a in ((0, 4), (1, 0), (1, 1), (65536, 1024), (65537, 4), (8, 1025))] == [0, 0, 1, 1, 0, 0]
+    assert lib.gb_moe_sort(P, 2, 8, 4, 0, P, P, P, P, NULL) != 0 and "bytes" in _text(lib)
+    assert lib.gb_moe_sort(P, 4, 65537, 4, 0, P, P, P, P, NULL) == 3 and "gb_moe_route_inv" in _text(lib)
+    assert lib.gb_moe_sort(P, 8, 8, 4, 0, P, P, P, NULL, NULL) != 0 and "null" in _text(lib)
 
 
 def test_host_tensors_are_refused():

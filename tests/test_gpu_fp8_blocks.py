@@ -162,7 +162,8 @@ def test_product_scales_far_apart_and_special_values(dev):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (1, 136, 144), (4, 300, 400), (16, 1024, 1536), (40, 256, 4096), (200, 520, 640)])
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (1, 136, 144), (4, 300, 400), (16, 1024, 1536), (40, 256, 4096), (200, 520, 640), (3, 520, 272),
+                                   (13, 129, 2064), (7, 64, 16), (2, 256, 5120), (5, 40000, 256), (16, 33000, 400), (1, 30000, 4240), (9, 1, 7168)])
 def test_linear(dev, dtype, M, N, K):
     from gridbook_b200 import kernels
     g = _gen(dev, M * N + K)

@@ -24,7 +24,8 @@ def _gen(dev, seed):
     return torch.Generator(device=dev).manual_seed(seed)
 
 
-@pytest.mark.parametrize("T,topk,H,E,base", CASES + [(3000, 2, 8, 20, 5), (1100, 4, 8, 256, 3), (1, 1, 8, 4096, 0), (1500, 3, 8, 700, 9)])
+@pytest.mark.parametrize("T,topk,H,E,base", CASES + [(3000, 2, 8, 20, 5), (1100, 4, 8, 256, 3), (1, 1, 8, 4096, 0), (1500, 3, 8, 700, 9), (513, 1, 8, 9, 0), (4100, 2, 8, 1024, 1),
+                                                  (8192, 8, 8, 128, 0), (5000, 4, 8, 256, 100), (9000, 8, 8, 64, 3), (6000, 1, 8, 1500, 0)])
 def test_sort(dev, T, topk, H, E, base):
     from gridbook_b200 import kernels
     ids = _ids(T, topk, E, base, _gen(dev, T + topk), dev)
@@ -33,6 +34,18 @@ def test_sort(dev, T, topk, H, E, base):
         counts, offsets, order, place = B.sort(ids, E, base)
         assert r.counts.tolist() == counts and r.offsets.tolist() == offsets and r.order.tolist() == order and r.place.tolist() == place
         assert r.topk == topk and r.place.dtype is torch.int32
+
+
+def test_ids_of_other_types_and_past_32_bits(dev):
+    from gridbook_b200 import kernels
+    for T in (3, 40000):
+        ids = torch.randint(0, 6, (T, 2), generator=_gen(dev, T), device=dev)
+        want = kernels.moe_sort(ids.int(), 4, expert_base=1)
+        far = torch.where(ids == 0, ids + (1 << 32) + 2, ids)        # held nowhere, whatever the low half says
+        for i in (ids, far, ids.to(torch.int16), ids.to(torch.uint8)):
+            got = kernels.moe_sort(i, 4, expert_base=1)
+            for a, b in ((got.counts, want.counts), (got.offsets, want.offsets), (got.order, want.order), (got.place, want.place)):
+                assert torch.equal(a, b)
 
 
 def test_nothing_to_sort(dev):
