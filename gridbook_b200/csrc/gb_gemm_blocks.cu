@@ -531,7 +531,7 @@ struct Rows {
   static constexpr uint32_t kTmem = kAccs * kR < 32 ? 32 : kAccs * kR;
   static constexpr int kStageBytes = kBM * kSlab + kR * kSlab;
 };
-constexpr int kSmemMax = 224 * 1024;                 // with the static arrays within the 227 KB of a CTA
+constexpr int kSmemMax = 217 * 1024;                 // with the static arrays within the 227 KB of a CTA
 
 template <int kR, bool kGrouped, typename In>
 __global__ void __launch_bounds__(Rows<kR, In>::kThreads, 1)
@@ -542,6 +542,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   constexpr int kRead = S::kRead, kAccs = S::kAccs, kMine = S::kMine;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_s[kMaxStages], empty_s[kMaxStages], acc_full_s[kAccs], acc_empty_s[kAccs], sc_full_s[kScaleBars], sc_empty_s[kScaleSlots];
+  __shared__ __align__(16) uint8_t out_s[kRead * 1024];
   __shared__ uint32_t slot_s;
   __shared__ volatile int abort_s;
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of a cluster
@@ -843,15 +844,52 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       }
       if (!ok) break;
       last = t;
-      if (p.slices == 1) {                                 // lane = feature: 64 contiguous bytes a warp and row
-        const int feature = t.n0 + quarter * 32 + lane;
-        if (feature < p.N) {
+      if (p.slices == 1) {
+        // lane = feature; out through a KB of shared memory per warp, so that four lanes store 64 contiguous bytes of a row
+        // (one value a lane and store: 7400 clocks for 128 features of 70 rows, more than half of what their sums took)
+        const uint32_t out = gb_smem_u32(out_s) + (uint32_t)warp * 1024u;
+        const int f0 = t.n0 + quarter * 32;
 #pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            const int r0 = (i * (kRead / 4) + group) * 16;
+        for (int i = 0; i < kMine; ++i) {
+          const int r0 = (i * (kRead / 4) + group) * 16;
+          if (r0 >= t.rows) break;
+          if (p.out16 && p.out != GB_DTYPE_FP32) {
 #pragma unroll
             for (int c = 0; c < 16; ++c)
-              if (r0 + c < t.rows) store1(p.D, (int64_t)(t.m0 + r0 + c) * p.N + feature, acc[i][c], p.out);
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(out + (uint32_t)(c * 64 + lane * 2)), "h"((uint16_t)pack2(acc[i][c], 0.0f, p.out)) : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = h * 8 + (lane >> 2), f = f0 + (lane & 3) * 8;
+              uint4 q;
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(out + (uint32_t)(h * 512 + lane * 16)) : "memory");
+              if (r0 + r < t.rows && f < p.N) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.D) + (int64_t)(t.m0 + r0 + r) * p.N + f) = q;
+            }
+            __syncwarp();
+          } else if (p.out16) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(out + (uint32_t)(c * 128 + lane * 4)), "f"(acc[i][half * 8 + c]) : "memory");
+              __syncwarp();
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int r = half * 8 + h * 4 + (lane >> 3), f = f0 + (lane & 7) * 4;
+                uint4 q;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(out + (uint32_t)(h * 512 + lane * 16)) : "memory");
+                if (r0 + r < t.rows && f < p.N) *reinterpret_cast<uint4*>(static_cast<float*>(p.D) + (int64_t)(t.m0 + r0 + r) * p.N + f) = q;
+              }
+              __syncwarp();
+            }
+          } else if (f0 + lane < p.N) {                    // rows of D that are no multiple of 16 bytes
+            for (int c = 0; c < 16; ++c)
+              if (r0 + c < t.rows) {
+                float v = acc[i][0];
+#pragma unroll
+                for (int k = 1; k < 16; ++k) v = c == k ? acc[i][k] : v;
+                store1(p.D, (int64_t)(t.m0 + r0 + c) * p.N + f0 + lane, v, p.out);
+              }
           }
         }
       }
@@ -1116,6 +1154,14 @@ BlocksParams params(const float* as, const float* bs, void* D, int out, int64_t 
   return p;
 }
 
+// Where the rows kernel is the faster one: up to 128 rows, and past them where its tiles are one wave (the pairs' tiles, a
+// quarter as many, leave more of the GPU idle).  us, pairs / rows kernel: 100 rows of 4096 x 4096 20.0 / 12.3, 128 of 5120 x 17408
+// 61.5 / 28.7, of 34816 x 5120 46.5 / 42.1, 160 of 5120 x 17408 61.5 / 49.4, 333 of 2048 x 5120 22.6 / 16.4, of 5120 x 17408 62.8 / 59.4; but 200 of
+// 34816 x 5120 48.2 / 72.2, 512 of 5120 x 5120 24.4 / 40.3.
+bool few_rows(int64_t M, int64_t N) {
+  return M <= 128 || ((M + 127) / 128) * ((N + kBM - 1) / kBM) <= gb_sm_count();
+}
+
 }  // namespace
 
 extern "C" {
@@ -1125,7 +1171,7 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
   const int rc = check_blocks(A, a_scale, W, w_scale, D, out, M, N, K, 1);
   if (rc != GB_OK || M == 0) return rc;
   const BlocksParams p = params(a_scale, w_scale, D, out, M, N, K, beside);
-  if (M <= 128) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
+  if (few_rows(M, N)) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
   return run_pair<false>(A, W, K, p, (cudaStream_t)stream);
 }
 
@@ -1161,8 +1207,10 @@ int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* 
   BlocksParams p = params(a_scale, w_scale, D, out, P, N, K, beside);
   p.seg = seg_offsets;
   p.E = (int)E;
+  // us, pairs / rows kernel, 128 experts of 1536 x 2048: 69 rows an expert on average 113 / 80, 96 116 / 91, 128 119 / 122, 256 165 / 198;
+  // 32 of 4096 x 7168: 100 240 / 187, 150 243 / 303.  A pass holds twice the average where that is at most 128.
   const int64_t mean = P / E;
-  if (mean <= 64) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
+  if (mean <= 112) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
   return run_pair<true>(A, W, K, p, (cudaStream_t)stream);
 }
 
