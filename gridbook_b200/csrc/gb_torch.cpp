@@ -862,32 +862,41 @@ at::Tensor gemm_fp8_blocks_grouped(const at::Tensor& a, const at::Tensor& a_scal
 }
 
 // ------------------------------------------------------------------ tokens sorted by expert and back
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& topk_ids, int64_t E, int64_t base) {
+int64_t check_ids(const at::Tensor& topk_ids, int64_t E) {
   need_cuda(topk_ids);
   need(topk_ids.dim() == 2, "expert ids of shape [tokens, top-k] expected");
   need(!topk_ids.is_floating_point() && !topk_ids.is_complex() && topk_ids.scalar_type() != at::kBool, "expert ids are whole numbers");
-  const int64_t T = topk_ids.size(0), topk = topk_ids.size(1), P = T * topk;
+  const int64_t topk = topk_ids.size(1), P = topk_ids.size(0) * topk;
   need(E >= 1 && E <= 4096 && topk >= 1 && P < (1ll << 30), "1 to 4096 experts, at least one a token and fewer than 2^30 pairs expected");
-  const c10::cuda::CUDAGuard guard(topk_ids.device());
-  const auto opt = topk_ids.options().dtype(at::kInt);
-  if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
-  at::Tensor counts = fresh({E}, at::kInt, topk_ids), offsets = fresh({E + 1}, at::kInt, topk_ids), order = fresh({P}, at::kInt, topk_ids),
-             place = fresh({P}, at::kInt, topk_ids);
-  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  return P;
+}
+
+void sort_pairs(const at::Tensor& topk_ids, int64_t E, int64_t base, int32_t* counts, int32_t* offsets, int32_t* order, int32_t* place, void* stream) {
+  const int64_t T = topk_ids.size(0), topk = topk_ids.size(1), P = T * topk;
   const bool wide = topk_ids.scalar_type() == at::kLong;
   if (L.gb_moe_sort_applies(P, E)) {
     const at::Tensor ids = (wide || topk_ids.scalar_type() == at::kInt ? topk_ids : topk_ids.to(at::kInt)).contiguous();
-    check(L.gb_moe_sort(ids.data_ptr(), wide ? 8 : 4, P, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(),
-                        place.data_ptr<int32_t>(), stream));
-    return {counts, offsets, order, place};
+    check(L.gb_moe_sort(ids.data_ptr(), wide ? 8 : 4, P, E, base, counts, offsets, order, place, stream));
+    return;
   }
   // in 32 bits, ids that do not fit them dropped like others that are held elsewhere
   const at::Tensor ids = (wide ? topk_ids.clamp(-1, std::numeric_limits<int32_t>::max()) : topk_ids).to(at::kInt).contiguous();
   at::Tensor ws;
   const int64_t bytes = L.gb_moe_route_workspace_bytes(T, topk, E);
-  if (bytes) ws = at::empty({bytes}, opt.dtype(at::kByte));
-  check(L.gb_moe_route_inv(ids.data_ptr<int32_t>(), T, topk, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(),
-                           place.data_ptr<int32_t>(), nullptr, nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  if (bytes) ws = at::empty({bytes}, topk_ids.options().dtype(at::kByte));
+  check(L.gb_moe_route_inv(ids.data_ptr<int32_t>(), T, topk, E, base, counts, offsets, order, place, nullptr, nullptr, bytes ? ws.data_ptr() : nullptr,
+                           bytes, stream));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& topk_ids, int64_t E, int64_t base) {
+  const int64_t P = check_ids(topk_ids, E);
+  const c10::cuda::CUDAGuard guard(topk_ids.device());
+  const auto opt = topk_ids.options().dtype(at::kInt);
+  if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
+  at::Tensor counts = fresh({E}, at::kInt, topk_ids), offsets = fresh({E + 1}, at::kInt, topk_ids), order = fresh({P}, at::kInt, topk_ids),
+             place = fresh({P}, at::kInt, topk_ids);
+  sort_pairs(topk_ids, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(), place.data_ptr<int32_t>(),
+             c10::cuda::getCurrentCUDAStream().stream());
   return {counts, offsets, order, place};
 }
 
@@ -915,6 +924,42 @@ Two moe_permute_fp8(const at::Tensor& x, const at::Tensor& place, const at::Tens
   check(L.gb_moe_permute_fp8(r.t.data_ptr(), dt, r.ld, s.place, s.live, s.T, topk, r.K, rule, q.data_ptr(), scale.data_ptr<float>(),
                              c10::cuda::getCurrentCUDAStream().stream()));
   return {q, scale};
+}
+
+// The routed layer: six launches.  Each product comes right behind a quantiser, which lets it start only once all work further
+// ahead (the sort among it) has finished: it may fetch its weights and the segments while the quantiser runs.
+at::Tensor moe_fp8_blocks(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& s13, const at::Tensor& w2, const at::Tensor& s2,
+                          const at::Tensor& topk_weights, const at::Tensor& topk_ids, int64_t base, int rule) {
+  same_device(x, {&w13, &s13, &w2, &s2, &topk_weights, &topk_ids});
+  const int dt = dtype_code(x.scalar_type(), "the routed block-scaled layer");
+  need_operand(w13, s13, 3, "w13", true);
+  need_operand(w2, s2, 3, "w2", true);
+  const int64_t E = w13.size(0), H = w13.size(2), I = w2.size(2);
+  need(w2.size(0) == E && w2.size(1) == H && w13.size(1) == 2 * I, "w13 [E, 2 inter, hidden] and w2 [E, hidden, inter] expected");
+  const int64_t P = check_ids(topk_ids, E), T = topk_ids.size(0), topk = topk_ids.size(1);
+  need(x.dim() >= 1 && x.size(-1) == H && x.numel() == T * H, std::to_string(T) + " tokens of " + std::to_string(H) + " values expected");
+  need(topk_weights.is_floating_point() && topk_weights.numel() == P, "one router weight for each of " + std::to_string(P) + " pairs expected");
+  const c10::cuda::CUDAGuard guard(x.device());
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  at::Tensor out = fresh(x.sizes(), x.scalar_type(), x);
+  if (P == 0) return out;
+  const RowsOf r(x);
+  const at::Tensor w13c = w13.contiguous(), s13c = s13.contiguous(), w2c = w2.contiguous(), s2c = s2.contiguous(),
+                   tw = topk_weights.to(at::kFloat).contiguous();
+  const int64_t size = x.element_size();
+  Arena a;
+  const int counts = a.add(E * 4), offsets = a.add((E + 1) * 4), order = a.add(P * 4), place = a.add(P * 4);
+  const int q = a.add(P * H), qs = a.add(P * blocks(H) * 4), h = a.add(P * 2 * I * size), v = a.add(P * I), vs = a.add(P * blocks(I) * 4),
+            y = a.add(P * H * size);
+  a.alloc(x);
+  int32_t *seg = a.ptr<int32_t>(offsets), *at_ = a.ptr<int32_t>(place);
+  sort_pairs(topk_ids, E, base, a.ptr<int32_t>(counts), seg, a.ptr<int32_t>(order), at_, stream);
+  check(L.gb_moe_permute_fp8(r.t.data_ptr(), dt, r.ld, at_, seg + E, T, topk, H, rule, a.ptr(q), a.ptr<float>(qs), stream));
+  check(L.gb_gemm_fp8_blocks_grouped(a.ptr(q), a.ptr<float>(qs), w13c.data_ptr(), s13c.data_ptr<float>(), seg, E, a.ptr(h), dt, P, 2 * I, H, 1, stream));
+  check(L.gb_moe_swiglu_fp8(a.ptr(h), dt, 2 * I, seg + E, P, I, rule, a.ptr(v), a.ptr<float>(vs), stream));
+  check(L.gb_gemm_fp8_blocks_grouped(a.ptr(v), a.ptr<float>(vs), w2c.data_ptr(), s2c.data_ptr<float>(), seg, E, a.ptr(y), dt, P, H, I, 1, stream));
+  check(L.gb_moe_unpermute(a.ptr(y), dt, at_, tw.data_ptr<float>(), T, topk, H, out.data_ptr(), stream));
+  return out;
 }
 
 at::Tensor permute_rows(const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
@@ -1052,6 +1097,7 @@ PYBIND11_MODULE(_gb_torch, m) {
   m.def("linear_fp8_blocks", &linear_fp8_blocks, Free());
   m.def("gemm_fp8_blocks", &gemm_fp8_blocks, Free());
   m.def("gemm_fp8_blocks_grouped", &gemm_fp8_blocks_grouped, Free());
+  m.def("moe_fp8_blocks", &moe_fp8_blocks, Free());
   m.def("moe_sort", &moe_sort, Free());
   m.def("moe_permute", &moe_permute, Free());
   m.def("moe_unpermute", &moe_unpermute, Free());

@@ -629,7 +629,7 @@ def moe_gemv_sorted(x_sorted: torch.Tensor, w: PackedWeight, offsets: torch.Tens
 
 # ------------------------------------------------------------------ block-scaled E4M3
 # Weights [N, K] float8_e4m3fn with one fp32 scale per 128 x 128 block, activations [M, K] with one per 1 x 128
-# block; the last blocks may be short.  Compiled host path: csrc/gb_torch.cpp.
+# block; the last blocks may be short.  Inference only: results carry no gradient.  Compiled host path: csrc/gb_torch.cpp.
 FP8_BLOCK = 128
 
 
@@ -703,3 +703,14 @@ def moe_swiglu_fp8(h: torch.Tensor, offsets: torch.Tensor | None = None, scale_r
     """:func:`fp8_quantize_blocks` of silu(gate) * up, taken in fp32, over rows h [P, 2 I] = [gate | up]: (q [P, I], scale).
     ``offsets``: rows past offsets[-1] are left unset."""
     return nat.host("routed SwiGLU and block quantiser").moe_swiglu_fp8(h, offsets, _rule(scale_rule))
+
+
+def moe_fp8_blocks(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
+                   topk_weights: torch.Tensor, topk_ids: torch.Tensor, *, expert_base: int = 0,
+                   scale_rule: str = "recip") -> torch.Tensor:
+    """A routed SwiGLU layer in block-scaled E4M3, one host call: :func:`moe_sort`, :func:`moe_permute_fp8`, the gate and up
+    projections [E, 2 inter, hidden] grouped, :func:`moe_swiglu_fp8`, the down projection [E, hidden, inter] grouped,
+    :func:`moe_unpermute` with the router's weights.  ``x`` [..., hidden] bf16, fp16 or fp32; rows between the projections
+    and the result have its type."""
+    return nat.host("routed block-scaled layer").moe_fp8_blocks(x, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_base,
+                                                                _rule(scale_rule))

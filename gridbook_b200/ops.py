@@ -370,6 +370,32 @@ def _(qw_flat, lut_f32, scale, row0, nrows, K, k_bits, type_size):
     return qw_flat.new_empty((nrows, K), dtype=torch.bfloat16)
 
 
+# --------------------------------------------------------------------------- block-scaled E4M3
+@torch.library.custom_op("prismaquant::fp8_blocks_linear", mutates_args=())
+def fp8_blocks_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    """kernels.linear_fp8_blocks as an opaque operator (no counterpart in the reference, whose source-FP8 lane
+    multiplies bf16 activations, gridbook/fp8_source_w8a16.py)."""
+    return kernels.linear_fp8_blocks(x, weight, weight_scale, scale_rule=ACT_SCALE_RULE)
+
+
+@fp8_blocks_linear.register_fake
+def _(x, weight, weight_scale):
+    return torch.empty((*x.shape[:-1], weight.shape[0]), dtype=x.dtype, device=x.device)
+
+
+@torch.library.custom_op("prismaquant::fp8_blocks_moe", mutates_args=())
+def fp8_blocks_moe(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
+                   topk_weights: torch.Tensor, topk_ids: torch.Tensor, expert_base: int) -> torch.Tensor:
+    """kernels.moe_fp8_blocks as an opaque operator."""
+    return kernels.moe_fp8_blocks(x, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_base=int(expert_base),
+                                  scale_rule=ACT_SCALE_RULE)
+
+
+@fp8_blocks_moe.register_fake
+def _(x, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_base):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 # --------------------------------------------------------------------------- layer registry
 # Weak, monotonic integer indirection so the two whole-dispatch ops stay opaque to Dynamo
 # (gridbook/ops.py:686-728).

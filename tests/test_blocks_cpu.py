@@ -126,3 +126,36 @@ def test_rounding_of_the_plain_form_is_the_formats():
     mid = (grid[1:] + grid[:-1]) / 2
     v = torch.cat([grid, mid, mid + 1e-4, mid - 1e-4])
     assert torch.equal(e4m3_round(v), v.float().to(E4M3).double())
+
+
+def test_layers_refuse_what_does_not_fit():
+    from gridbook_b200.block_fp8 import BlockFP8Linear, BlockFP8MoE
+    w, s = torch.zeros(200, 272, dtype=E4M3), torch.ones(2, 3)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        BlockFP8Linear(200, 64)
+    lin = BlockFP8Linear(272, 200)
+    with pytest.raises(RuntimeError, match="before load"):
+        lin(torch.zeros(1, 272))
+    for a, b in ((w.float(), s), (w[:128], s), (w, s[:1]), (w, s.int())):
+        with pytest.raises(ValueError):
+            lin.load(a, b, "cpu")
+    for args in ((4, 250, 128), (4, 256, 100), (0, 256, 128), (1025, 256, 128)):
+        with pytest.raises(ValueError):
+            BlockFP8MoE(*args)
+    moe = BlockFP8MoE(2, 256, 128)
+    w13, s13, w2, s2 = torch.zeros(2, 256, 256, dtype=E4M3), torch.ones(2, 2, 2), torch.zeros(2, 256, 128, dtype=E4M3), torch.ones(2, 2, 1)
+    for args in ((w13[:1], s13, w2, s2), (w13, s13[:, :1], w2, s2), (w13, s13, w2.half(), s2), (w13, s13, w2, s2[..., :0])):
+        with pytest.raises(ValueError):
+            moe.load(*args, "cpu")
+
+
+def test_operators_trace_without_running():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from gridbook_b200 import ops  # noqa: F401
+    with FakeTensorMode():
+        x = torch.empty(3, 5, 256, dtype=torch.bfloat16)
+        y = torch.ops.prismaquant.fp8_blocks_linear(x, torch.empty(200, 256, dtype=E4M3), torch.empty(2, 2))
+        assert y.shape == (3, 5, 200) and y.dtype is torch.bfloat16
+        z = torch.ops.prismaquant.fp8_blocks_moe(x, torch.empty(2, 256, 256, dtype=E4M3), torch.empty(2, 2, 2), torch.empty(2, 256, 128, dtype=E4M3),
+                                                 torch.empty(2, 2, 1), torch.empty(15, 2), torch.empty(15, 2, dtype=torch.int32), 0)
+        assert z.shape == x.shape
