@@ -6,10 +6,15 @@
 // kind::f8f6f4) and the blocks are added in fp32 registers: every block has an accumulator of its own in tensor memory, a ring
 // of them, and the read-out warps turn each into one multiply-add per element while the next blocks are multiplied.
 //
-// Two kernels.  gemm_blocks_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x 256 or 128 features, activations on
-// the M side, so that a thread holds one row and its scale is one number per block.  gemm_blocks_rows_kernel: few rows; the
-// WEIGHTS are the M side (128 features a CTA, one scale per block for the whole tile), the rows the N side in steps of
-// sixteen, K sliced over a thread-block cluster where there are fewer tiles than SMs.
+// Two kernels.  gemm_blocks_tile_kernel: activations on the M side, so that a thread holds one row and its scale is one number per
+// block; tiles of 128 rows x 256 features on single CTAs (K sliced over a thread-block cluster where there are fewer tiles
+// than SMs; grouped), or of 256 x 256 on CTA pairs (cta_group::2).  gemm_blocks_rows_kernel: few rows; the WEIGHTS are the M side
+// (128 features a CTA, one scale per block for the whole tile), the rows the N side in steps of sixteen, K sliced alike.
+//
+// What bounds them.  Tiles: the tensor cores take 392 ns a slab of 256 x 256 x 128 with nothing to wait for (3.1 PFLOP/s); the
+// multiply-adds of the read-out (two warps of a scheduler, 256 clocks of its 700 a slab) and the power cap leave 2.3 - 2.5.  Rows: the
+// bytes of the weights, up to some 64 rows; from there on the shared memory, through which every warp gets the rows' scales
+// at 128 bytes a clock beside the operands.
 #include "gb_blocks.cuh"
 
 #include <cuda.h>
@@ -21,6 +26,7 @@ namespace {
 constexpr int kSlab = 128;                           // columns of a block = bytes of K of a stage (one swizzle span)
 constexpr int kBM = 128;                             // rows of an operand tile of a CTA on the M side
 constexpr int kMaxGroups = 1024;                     // experts of one grouped launch
+constexpr int kMaxSlices = 8;                        // of K, over a thread-block cluster
 constexpr int kSegBytes = 2 * (kMaxGroups + 1) * 4 + 8;
 
 struct BlocksParams {
@@ -134,9 +140,21 @@ GB_DEVINL void commit_to(uint32_t bar) {
   else
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-GB_DEVINL void commit_pair(uint32_t bar, uint32_t to_peer) {
-  commit_to<2>(bar);
-  commit_to<2>(bar + to_peer);
+// To the barrier of every CTA that works on the tile.
+template <int kCtas>
+GB_DEVINL void commit_all(uint32_t bar, uint32_t to_peer) {
+  commit_to<kCtas>(bar);
+  if (kCtas == 2) commit_to<2>(bar + to_peer);
+}
+template <int kCtas>
+GB_DEVINL void tmem_alloc(uint32_t slot, uint32_t cols) {
+  if (kCtas == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
 }
 GB_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
@@ -227,49 +245,54 @@ GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, i
   if (lane == 31) base_s[p.E] = incl;
 }
 
-// ======================================== CTA pairs ========================================================
-constexpr int kPairM = 256;                          // rows of a pair's tile
+// ======================================== CTA pairs, and single CTAs ========================================================
 constexpr int kEpiWarps = 8;                         // two per lane quarter, half of the columns each
 constexpr int kOutChunk = 2048;                      // 32 rows x 32 16-bit columns on their way out
 constexpr int kPairThreads = 32 * (kEpiWarps + 4);     // three warpgroups, the last two warps idle
 // A thread of the read-out holds 128 sums and has 64 more on their way; 168 registers a thread at launch.
-constexpr int kReadRegs = 224, kOtherRegs = 56;
-static_assert(256 * kReadRegs + 128 * kOtherRegs <= 384 * 168, "a register split draws on what the block was launched with");
+// (What spills is a scale on its way, and the wait for it: 333 rows of 5120 x 17408 in single CTAs 45 us with 224 of them.)
+template <int kCtas>
+struct Registers {
+  static constexpr int kRead = kCtas == 2 ? 224 : 232, kOther = kCtas == 2 ? 56 : 40;
+  static_assert(256 * kRead + 128 * kOther <= 384 * 168, "a register split draws on what the block was launched with");
+};
 constexpr int kTmemCols = 512;
 constexpr int kBN = 256, kPart = 128, kParts = 2;    // features of a tile, of a part: one block of features, an accumulator
 constexpr int kAccs = kTmemCols / kPart;
 constexpr int kGroupM = 16;                          // row tiles walked together before the next columns (see gb_gemm_pair.cu)
 
-template <bool kGrouped>
-struct Pair {
-  static constexpr int kABytes = kBM * kSlab, kBBytes = kBN / 2 * kSlab, kStageBytes = kABytes + kBBytes;
+template <int kCtas, bool kGrouped>
+struct Tile {
+  static constexpr int kM = kBM * kCtas;               // rows of a tile
+  static constexpr int kABytes = kBM * kSlab, kBBytes = kBN / kCtas * kSlab, kStageBytes = kABytes + kBBytes;
   static constexpr int kChunks = kGrouped ? 1 : 2;     // on their way out, of a warp
   static constexpr int kOutBytes = kEpiWarps * kChunks * kOutChunk + (kGrouped ? kSegBytes : 0);
   // an even number: each of the two MMA issuers meets every phase of the stages that it waits for
   static constexpr int kStages = (227 * 1024 - 2048 - kOutBytes) / kStageBytes / 2 * 2;
   static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 2048;
+  static_assert(kStages >= 4, "the sums of a sliced K lie over four stages");
 };
 
-// The tiles of a pair: first, first + stride, ...
-template <bool kGrouped>
-struct PairTiles {
+// The tiles of a pair or CTA: first, first + stride, ...
+template <int kM, bool kGrouped>
+struct TileWalk {
   int tile, stride, e = 0;
   int m0 = 0, n0 = 0, w0 = 0, end = 0;               // first row, first feature, first weight row, end of the rows that count
-  GB_DEVINL PairTiles(int first, int stride_) : tile(first - stride_), stride(stride_) {}
+  GB_DEVINL TileWalk(int first, int stride_) : tile(first - stride_), stride(stride_) {}
   GB_DEVINL bool next(const BlocksParams& p, int total, const int* seg_s, const int* base_s) {
     tile += stride;
     if (tile >= total) return false;
     if (kGrouped) {                                  // features fastest: a row tile's columns run together
       const int gp = tile / p.n_tiles, nt = tile - gp * p.n_tiles;
       while (base_s[e + 1] <= gp) ++e;               // experts without rows are stepped over
-      m0 = seg_s[e] + (gp - base_s[e]) * kPairM;
+      m0 = seg_s[e] + (gp - base_s[e]) * kM;
       end = seg_s[e + 1];
       n0 = nt * kBN;
       w0 = e * (int)p.N + n0;
     } else {
       const int per = kGroupM * p.n_tiles, g = tile / per, in = tile - g * per;
       const int rows = min(kGroupM, p.m_tiles - g * kGroupM);
-      m0 = (g * kGroupM + in % rows) * kPairM;
+      m0 = (g * kGroupM + in % rows) * kM;
       n0 = in / rows * kBN;
       w0 = n0;
       end = (int)p.M;
@@ -289,11 +312,11 @@ GB_DEVINL void read64(uint32_t at, uint32_t (&v)[2][32]) {
   tmem_wait_ld(v[1]);
 }
 
-template <bool kGrouped>
+template <int kCtas, bool kGrouped>
 __global__ void __launch_bounds__(kPairThreads, 1)
-gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
+gemm_blocks_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
                         const __grid_constant__ BlocksParams p) {
-  using S = Pair<kGrouped>;
+  using S = Tile<kCtas, kGrouped>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
@@ -310,8 +333,8 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   int* base_s = seg_s + kMaxGroups + 1;
 
   const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-  uint32_t rank;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  uint32_t rank = 0;                                       // of the pair
+  if constexpr (kCtas == 2) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   gb_pdl_launch_dependents();
   {                                                        // a barrier of each kind per thread
     const uint32_t i = threadIdx.x;
@@ -321,45 +344,51 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     if (i < kAccs) {
       bar_init(acc_full + 8 * i, 1);
-      bar_init(acc_empty + 8 * i, kEpiWarps);
+      bar_init(acc_empty + 8 * i, 4 * kCtas);
     }
     if (i == 0) *abort_flag = 0;
     gb_fence_barrier_init();
   }
-  if (warp == kEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"((uint32_t)kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
+  if (warp == kEpiWarps + 1) tmem_alloc<kCtas>(slot, kTmemCols);
   gb_pdl_wait();
-  if (kGrouped && warp == kEpiWarps) load_segments(p, kPairM, seg_s, base_s);
+  if (kGrouped && warp == kEpiWarps) load_segments(p, S::kM, seg_s, base_s);
   tmem_fence_before();
   __syncthreads();
-  gb_cluster_sync();                                                     // both CTAs' barriers exist
+  if constexpr (kCtas == 2) gb_cluster_sync();                           // both CTAs' barriers exist
   tmem_fence_after();
   const uint32_t tmem_base = *slot_ptr;
   const int total = kGrouped ? base_s[p.E] * p.n_tiles : p.m_tiles * p.n_tiles;
-  const int stride = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
+  const int stride = (int)gridDim.x / kCtas, first = (int)blockIdx.x / kCtas;
+  // K slices, of single CTAs: a tile for every cluster along y
+  const int slice = kCtas == 1 ? (int)blockIdx.y : 0, k_begin = kCtas == 1 ? slice * p.per_slice : 0;
+  const int k_end = kCtas == 1 ? min(p.kb, k_begin + p.per_slice) : p.kb;
 
   if (warp == kEpiWarps) {
     // ------------------------------- producer (each CTA) -------------------------------
-    fewer_registers<kOtherRegs>();
-    const uint32_t full_pair = (uint32_t)uniform((int)leader_addr(full_bar));
+    fewer_registers<Registers<kCtas>::kOther>();
+    const uint32_t full_pair = kCtas == 2 ? (uint32_t)uniform((int)leader_addr(full_bar)) : full_bar;
     const int me = uniform((int)rank);
     const bool one = gb_elect_one();
     int s = 0;
     uint32_t ph = 1;
     bool ok = true;
-    for (PairTiles<kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+    for (TileWalk<S::kM, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
       const int m0 = uniform(T.m0) + me * kBM, w0 = uniform(T.w0) + me * (kPart / 2);
-      for (int kt = 0; kt < p.kb; ++kt) {
+      for (int kt = k_begin; kt < k_end; ++kt) {
         ok = warp_wait<kTensorMemory>(empty_bar + 8 * s, ph, abort_flag, p.status, 91);
         if (!ok) break;
         if (one) {
           const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
-          if (me == 0) expect_tx(full_bar + 8 * s, 2 * S::kStageBytes);
-          tma_load_pair(st, &map_a, kt * kSlab, m0, full_pair + 8 * s);
-          tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);                          // half of a part's
-          tma_load_pair(st + S::kABytes + S::kBBytes / 2, &map_b, kt * kSlab, w0 + kPart, full_pair + 8 * s);  // features each
+          if (me == 0) expect_tx(full_bar + 8 * s, kCtas * S::kStageBytes);
+          if constexpr (kCtas == 2) {
+            tma_load_pair(st, &map_a, kt * kSlab, m0, full_pair + 8 * s);
+            tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);                            // half of a part's
+            tma_load_pair(st + S::kABytes + S::kBBytes / 2, &map_b, kt * kSlab, w0 + kPart, full_pair + 8 * s);    // features each
+          } else {
+            tma_load_2d(st, &map_a, kt * kSlab, m0, full_pair + 8 * s);
+            tma_load_2d(st + S::kABytes, &map_b, kt * kSlab, w0, full_pair + 8 * s);
+            tma_load_2d(st + S::kABytes + S::kBBytes / 2, &map_b, kt * kSlab, w0 + kPart, full_pair + 8 * s);
+          }
         }
         __syncwarp();
         if (++s == kStages) { s = 0; ph ^= 1; }
@@ -368,14 +397,16 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   } else if (warp == kEpiWarps + 1 || warp == kEpiWarps + 2) {
     // ------ MMA issuers (the leader's): the waits, MMAs and commits of a slab take one some 700 clocks, so two share the slabs
     // in turn; every slab has accumulators of its own, so that their order does not matter ------
-    fewer_registers<kOtherRegs>();
+    fewer_registers<Registers<kCtas>::kOther>();
     if (uniform((int)rank) == 0) {
-      uint32_t to_peer;                                      // distance of the peer's barriers
-      asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
-      to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
+      uint32_t to_peer = 0;                                  // distance of the peer's barriers
+      if constexpr (kCtas == 2) {
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
+        to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
+      }
       const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
       const int tiles = uniform(total > first ? (total - first + stride - 1) / stride : 0), turn = warp - kEpiWarps - 1;
-      const int64_t slabs = (int64_t)tiles * p.kb;
+      const int64_t slabs = (int64_t)tiles * (k_end - k_begin);
       const bool one = gb_elect_one();
       int s = turn % kStages;
       uint32_t ph = turn >= kStages ? 1 : 0, acc_ph = 1;
@@ -395,9 +426,9 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
           if (one) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)                      // 32 columns of K per instruction
-              mma<2>(tmem + (uint32_t)(buf * kPart), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), p.idesc, k > 0);
-            commit_pair(acc_full + 8 * buf, to_peer);
-            if (h == kParts - 1) commit_pair(empty_bar + 8 * s, to_peer);
+              mma<kCtas>(tmem + (uint32_t)(buf * kPart), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), p.idesc, k > 0);
+            commit_all<kCtas>(acc_full + 8 * buf, to_peer);
+            if (h == kParts - 1) commit_all<kCtas>(empty_bar + 8 * s, to_peer);
           }
           __syncwarp();
         }
@@ -408,8 +439,8 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
   } else if (warp < kEpiWarps) {
     // ------------------------------- read-out (each CTA) --------------------------------
-    more_registers<kReadRegs>();
-    const uint32_t acc_empty_pair = leader_addr(acc_empty);
+    more_registers<Registers<kCtas>::kRead>();
+    const uint32_t acc_empty_pair = kCtas == 2 ? leader_addr(acc_empty) : acc_empty;
     // Four warps for each part, one per lane quarter: while one of a scheduler's two adds, the other waits or loads.  (All
     // eight on half of every part wait together and then add together.)
     constexpr int kOuts = kPart / 32;
@@ -419,7 +450,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     int buf = part, flip = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (PairTiles<kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
+    for (TileWalk<S::kM, kGrouped> T(first, stride); ok && T.next(p, total, seg_s, base_s);) {
       const int row0 = T.m0 + (int)rank * kBM + quarter * 32, row = row0 + lane, n0 = T.n0 + c_lo;
       const bool row_ok = row < T.end;
       const float* as = row_ok ? p.a_scale + (int64_t)row * p.kb : nullptr;
@@ -428,16 +459,16 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       float acc[kPart];
 #pragma unroll
       for (int c = 0; c < kPart; ++c) acc[c] = 0.0f;
-      float4 as4 = scales4(as, 0, p.kb, p.vec4), bs4 = scales4(bs, 0, p.kb, p.vec4);
-      for (int kt0 = 0; ok && kt0 < p.kb; kt0 += 4) {
+      float4 as4 = scales4(as, k_begin, p.kb, p.vec4), bs4 = scales4(bs, k_begin, p.kb, p.vec4);
+      for (int kt0 = k_begin; ok && kt0 < k_end; kt0 += 4) {
         const float4 sc = make_float4(as4.x * bs4.x, as4.y * bs4.y, as4.z * bs4.z, as4.w * bs4.w);
-        if (kt0 + 4 < p.kb) {                                // the next four blocks' while these are added
+        if (kt0 + 4 < k_end) {                               // the next four blocks' while these are added
           as4 = scales4(as, kt0 + 4, p.kb, p.vec4);
           bs4 = scales4(bs, kt0 + 4, p.kb, p.vec4);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (!ok || kt0 + j >= p.kb) break;
+          if (!ok || kt0 + j >= k_end) break;
           const float scale = pick(sc, j);
           ok = warp_wait<kTensorMemory>(acc_full + 8 * buf, ph, abort_flag, p.status, 94);
           if (!ok) break;
@@ -449,11 +480,64 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
           read64(at + (uint32_t)(buf * kPart + 64), v);
           tmem_fence_before();
           __syncwarp();
-          arrive_cluster(acc_empty_pair + 8 * buf, lane == 0);
+          if constexpr (kCtas == 2) arrive_cluster(acc_empty_pair + 8 * buf, lane == 0);
+          else if (lane == 0) arrive(acc_empty_pair + 8 * buf);
           buf += kParts;
           if (buf >= kAccs) { buf -= kAccs; ph ^= 1; }
 #pragma unroll
           for (int c = 0; c < 64; ++c) add_scaled(acc[64 + c], v[c >> 5][c & 31], scale);
+        }
+      }
+      if constexpr (kCtas == 1 && !kGrouped) {
+        if (p.slices > 1) {
+          // Every CTA of the cluster has finished its MMAs, and with them its loads: the sums go into the shared memory of the CTA
+          // that owns the features, [slice][own feature][row], over the ring, and it adds them in the order of K.
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+          const bool live = !*abort_flag;
+          const int own = (16 + p.slices - 1) / p.slices, r = quarter * 32 + lane;       // sixteens of features
+          gb_cluster_sync();
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < kPart / 16; ++i) {
+              const int c0 = part * (kPart / 16) + i, to = c0 / own;
+              uint32_t dst;
+              asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                           : "=r"(dst) : "r"(ring + (uint32_t)((slice * own + c0 - to * own) * 16 * kBM + r) * 4u), "r"(to));
+#pragma unroll
+              for (int c = 0; c < 16; ++c)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + (uint32_t)c * kBM * 4u), "f"(acc[16 * i + c]) : "memory");
+            }
+          }
+          gb_cluster_sync();                                 // the last access to another CTA's memory lies in front of it
+          if (live) {
+            for (int i = part; i < own && slice * own + i < 16; i += 2) {
+              float sum[16] = {};
+              for (int q = 0; q < p.slices; ++q) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                  float v;
+                  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(ring + (uint32_t)(((q * own + i) * 16 + c) * kBM + r) * 4u) : "memory");
+                  sum[c] += v;
+                }
+              }
+              const int f = T.n0 + (slice * own + i) * 16;
+              const int64_t d = (int64_t)row * p.N + f;
+              if (!row_ok || f >= p.N) continue;
+              if (p.out16 && p.out != GB_DTYPE_FP32) {
+#pragma unroll
+                for (int c = 0; c < 16; c += 8)
+                  if (f + c < p.N)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.D) + d + c) =
+                        make_uint4(pack2(sum[c], sum[c + 1], p.out), pack2(sum[c + 2], sum[c + 3], p.out), pack2(sum[c + 4], sum[c + 5], p.out),
+                                   pack2(sum[c + 6], sum[c + 7], p.out));
+              } else {
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                  if (f + c < p.N) store1(p.D, d + c, sum[c], p.out);
+              }
+            }
+          }
+          break;                                             // one tile a cluster
         }
       }
       if (!ok) break;
@@ -503,19 +587,27 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
-    fewer_registers<kOtherRegs>();
+    fewer_registers<Registers<kCtas>::kOther>();
+  }
+  if (kCtas == 1 && !kGrouped && p.slices > 1 && warp >= kEpiWarps) {       // the read-out's meetings with the other slices
+    gb_cluster_sync();
+    gb_cluster_sync();
   }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
   if (*abort_flag) __nanosleep(1000000);                   // loads and MMAs still in flight end before the memory goes
-  gb_cluster_sync();                                       // the peer may still signal barriers here
-  if (warp == kEpiWarps + 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols) : "memory");
+  if constexpr (kCtas == 2) gb_cluster_sync();             // the peer may still signal barriers here
+  if (warp == kEpiWarps + 1) {
+    if constexpr (kCtas == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols) : "memory");
+  }
 }
 
 // ======================================== few rows =========================================================
-constexpr int kMaxStages = 12, kMaxSlices = 8;
+constexpr int kMaxStages = 12;
 constexpr int kScaleSlots = 4;                       // groups of four blocks whose scales are there ahead of their sums
 constexpr int kQuantWarps = 4, kQuantStages = 10, kScaleRing = 32;    // rows quantised here: warps that do, fewest stages, blocks whose scales are kept
 
@@ -571,8 +663,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     gb_fence_barrier_init();
   }
   if (warp == kRead + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gb_smem_u32(&slot_s)), "r"(S::kTmem) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc<1>(gb_smem_u32(&slot_s), S::kTmem);
   }
   // the sums of a sliced K have a place of their own: that the others have started is all that a CTA has to know, by the end
   if (p.slices > 1 && !p.overlay) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -962,13 +1053,14 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 
 // ======================================== host =============================================================
 std::mutex g_mutex;
-int g_pairs[64][2];                                        // pairs that run at once, per device and kernel (0: not asked)
+int g_pairs[64];                                           // pairs that run at once, per device (0: not asked)
 std::atomic<bool> g_ready[64];                             // shared-memory limits of the device's kernels are set
 
 int set_limits() {
 #define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
-  GB_ATTR(gemm_blocks_pair_kernel<false>, Pair<false>::kSmem);
-  GB_ATTR(gemm_blocks_pair_kernel<true>, Pair<true>::kSmem);
+  GB_ATTR((gemm_blocks_tile_kernel<2, false>), (Tile<2, false>::kSmem));
+  GB_ATTR((gemm_blocks_tile_kernel<1, false>), (Tile<1, false>::kSmem));
+  GB_ATTR((gemm_blocks_tile_kernel<1, true>), (Tile<1, true>::kSmem));
   GB_ATTR((gemm_blocks_rows_kernel<16, false, void>), kSmemMax);
   GB_ATTR((gemm_blocks_rows_kernel<32, false, void>), kSmemMax);
   GB_ATTR((gemm_blocks_rows_kernel<64, false, void>), kSmemMax);
@@ -996,40 +1088,52 @@ int ready() {
   return rc;
 }
 
-template <bool kGrouped>
 int resident_pairs() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   std::lock_guard<std::mutex> lock(g_mutex);
-  int& n = g_pairs[dev][kGrouped];
+  int& n = g_pairs[dev];
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * 256);
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = Pair<kGrouped>::kSmem;
+    cfg.dynamicSmemBytes = Tile<2, false>::kSmem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_blocks_pair_kernel<kGrouped>, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_blocks_tile_kernel<2, false>, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
   }
   return n;
 }
 
-template <bool kGrouped>
-int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
-  using S = Pair<kGrouped>;
-  const int pairs = resident_pairs<kGrouped>();
-  if (pairs <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+// Slices of K of a single CTA's tiles: as many as the SMs take, at least eight blocks each; slices start at multiples of four blocks
+// where rows of the scales are whole 16-byte pieces.
+struct Slices { int n, per; };
+Slices slices_of(int64_t tiles, int kb) {
+  static GbClusters clusters;
+  int want = 1;
+  for (int n = 2; n <= kMaxSlices && tiles * n <= gb_sm_count() && n * 8 <= kb; ++n)
+    if (tiles <= clusters.ask((const void*)gemm_blocks_tile_kernel<1, false>, kPairThreads, Tile<1, false>::kSmem, n)) want = n;
+  int per = (kb + want - 1) / want;
+  if (kb % 4 == 0) per = (per + 3) / 4 * 4;
+  return {(kb + per - 1) / per, per};
+}
+
+template <int kCtas, bool kGrouped>
+int run_tiles(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream_t stream) {
+  using S = Tile<kCtas, kGrouped>;
+  const int most = kCtas == 2 ? resident_pairs() : gb_sm_count();
+  if (most <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
   p.n_tiles = (int)((p.N + kBN - 1) / kBN);
-  p.m_tiles = (int)((p.M + kPairM - 1) / kPairM);
-  p.idesc = (1u << 4) | ((uint32_t)(kPart >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24);
+  p.m_tiles = (int)((p.M + S::kM - 1) / S::kM);
+  p.idesc = (1u << 4) | ((uint32_t)(kPart >> 3) << 17) | ((uint32_t)(S::kM >> 4) << 24);
   p.out_tma = p.N % 8 == 0 && p.out != GB_DTYPE_FP32;
   CUtensorMap map_a, map_b, map_d = {};
   int rc = gb_tensor_map_operand(&map_a, A, p.M, K, 1, kBM);
   if (rc != GB_OK) return rc;
-  rc = gb_tensor_map_operand(&map_b, W, (kGrouped ? p.E : 1) * p.N, K, 1, kPart / 2);
+  rc = gb_tensor_map_operand(&map_b, W, (kGrouped ? p.E : 1) * p.N, K, 1, kPart / kCtas);
   if (rc != GB_OK) return rc;
   if (p.out_tma) {
     rc = gb_tensor_map_out(&map_d, p.D, p.M, p.N);
@@ -1037,20 +1141,30 @@ int run_pair(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   }
   const int64_t tiles = (int64_t)(p.m_tiles + (kGrouped ? p.E : 0)) * p.n_tiles;      // grouped: at least as many as the routing can make
   GB_REQUIRE(tiles < (1ll << 31), "too many output tiles");
+  Slices slices = {1, p.kb};
+  if (kCtas == 1 && !kGrouped) slices = slices_of(tiles, p.kb);
+  p.slices = slices.n;
+  p.per_slice = slices.per;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+  cfg.gridDim = dim3((unsigned)(kCtas * (tiles < most ? tiles : most)), (unsigned)p.slices);
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (kCtas == 2 || p.slices > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = kCtas; attr[n].val.clusterDim.y = (unsigned)p.slices; attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (gb_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = n;
   gb_count_launch();
-  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_pair_kernel<kGrouped>, map_a, map_b, map_d, p));
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_blocks_tile_kernel<kCtas, kGrouped>, map_a, map_b, map_d, p));
   return GB_OK;
 }
 
@@ -1154,12 +1268,17 @@ BlocksParams params(const float* as, const float* bs, void* D, int out, int64_t 
   return p;
 }
 
-// Where the rows kernel is the faster one: up to 128 rows, and past them where its tiles are one wave (the pairs' tiles, a
-// quarter as many, leave more of the GPU idle).  us, pairs / rows kernel: 100 rows of 4096 x 4096 20.0 / 12.3, 128 of 5120 x 17408
-// 61.5 / 28.7, of 34816 x 5120 46.5 / 42.1, 160 of 5120 x 17408 61.5 / 49.4, 333 of 2048 x 5120 22.6 / 16.4, of 5120 x 17408 62.8 / 59.4; but 200 of
-// 34816 x 5120 48.2 / 72.2, 512 of 5120 x 5120 24.4 / 40.3.
-bool few_rows(int64_t M, int64_t N) {
-  return M <= 128 || ((M + 127) / 128) * ((N + kBM - 1) / kBM) <= gb_sm_count();
+// Which kernel a dense product takes; us.
+//   rows kernel / single CTAs: 64 rows of 5120 x 17408 23.0 / 28.7, 100 of 4096 x 4096 12.3 / 12.9, 128 of 34816 x 5120 42.0 / 36.9, 160 of 2048 x 8192
+//     14.4 / 18.5 (eight slices of K, whose sums cost more the larger the tiles), of 5120 x 17408 49.2 / 34.9, 333 of 2048 x 5120 16.4 / 16.4,
+//     of 5120 x 17408 59.4 / 43.0.
+//   pairs / single CTAs: 333 rows of 5120 x 17408 62.8 / 43.0, 512 of 5120 x 5120 24.4 / 24.6, 700 of 4096 x 4096 21.7 / 20.9, 256 of 34816 x 5120 49.6 / 52,
+//     8192 of 34816 x 5120 over two seconds, where the power cap rules, 1407 / 1465: a pair fetches its features once for both.
+enum Route { kRowsRoute, kCtaRoute, kPairRoute };
+Route route_of(int64_t M, int64_t N) {
+  const int64_t sms = gb_sm_count(), n_tiles = (N + kBN - 1) / kBN, tiles = (M + kBM - 1) / kBM * n_tiles;
+  if (M <= 64 || (M <= kBM && 2 * n_tiles < sms) || 6 * tiles < sms) return kRowsRoute;
+  return tiles <= sms ? kCtaRoute : kPairRoute;
 }
 
 }  // namespace
@@ -1171,8 +1290,9 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
   const int rc = check_blocks(A, a_scale, W, w_scale, D, out, M, N, K, 1);
   if (rc != GB_OK || M == 0) return rc;
   const BlocksParams p = params(a_scale, w_scale, D, out, M, N, K, beside);
-  if (few_rows(M, N)) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
-  return run_pair<false>(A, W, K, p, (cudaStream_t)stream);
+  const Route route = route_of(M, N);
+  if (route == kRowsRoute) return run_few<false>(A, W, K, p, M, (cudaStream_t)stream);
+  return route == kCtaRoute ? run_tiles<1, false>(A, W, K, p, (cudaStream_t)stream) : run_tiles<2, false>(A, W, K, p, (cudaStream_t)stream);
 }
 
 // us, two launches / one: 1 row of 34816 x 5120 34.9 / 32.9, 4 rows 35.7 / 33.7, 8 rows 36.7 / 43.0; 4 rows of 4096 x 4096 10.3 / 8.4, 16 rows
@@ -1207,11 +1327,12 @@ int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const void* 
   BlocksParams p = params(a_scale, w_scale, D, out, P, N, K, beside);
   p.seg = seg_offsets;
   p.E = (int)E;
-  // us, pairs / rows kernel, 128 experts of 1536 x 2048: 69 rows an expert on average 113 / 80, 96 116 / 91, 128 119 / 122, 256 165 / 198;
-  // 32 of 4096 x 7168: 100 240 / 187, 150 243 / 303.  A pass holds twice the average where that is at most 128.
+  // us, rows kernel / tiles of 128 rows, 128 experts of 1536 x 2048: 32 rows an expert on average 71.7 / 79.5, 64 77.9 / 83.4, 96 90.4 / 86.5,
+  // 128 122 / 100, 256 198 / 148 (pairs' tiles of 256 rows 116, 119 and 164); 32 of 4096 x 7168: 100 185 / 173.  A pass of the
+  // rows kernel holds twice the average where that is at most 128.
   const int64_t mean = P / E;
-  if (mean <= 112) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
-  return run_pair<true>(A, W, K, p, (cudaStream_t)stream);
+  if (mean <= 72) return run_few<true>(A, W, K, p, 2 * mean, (cudaStream_t)stream);
+  return run_tiles<1, true>(A, W, K, p, (cudaStream_t)stream);
 }
 
 }  // extern "C"
