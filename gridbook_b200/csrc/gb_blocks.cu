@@ -73,6 +73,8 @@ GB_DEVINL void store8(uint8_t* row, int64_t c, int64_t K, uint2 q) {
   }
 }
 
+GB_DEVINL bool in_rows(int64_t at, int64_t rows) { return (uint64_t)at < (uint64_t)rows; }
+
 struct QuantizeParams {
   const void* x;
   int64_t ld, rows, K;        // of the result; a swiglu row is [gate | up]
@@ -141,7 +143,7 @@ quantize_blocks_kernel(const __grid_constant__ QuantizeParams p) {
       for (int s = 0; s < p.topk; ++s) {   // the same for all sixteen lanes
         int64_t to = __shfl_sync(0xffffffffu, to_lane, s & 15, 16);
         if (s >= 16) to = row[i] < rows ? p.place[row[i] * p.topk + s] : -1;
-        if (to < 0) continue;
+        if (!in_rows(to, p.rows * p.topk)) continue;
         store8<kVec>(p.q + to * p.K, c, p.K, q);
         if (lane == 0) p.scale[to * p.blocks + block[i]] = scale;
       }
@@ -151,7 +153,7 @@ quantize_blocks_kernel(const __grid_constant__ QuantizeParams p) {
     }
   }
   if constexpr (kSource == kSorted) {      // rows that no pair has read zero
-    const int64_t pairs = p.rows * p.topk, first = *p.live, left = (pairs - first) * p.blocks;
+    const int64_t pairs = p.rows * p.topk, first = max(*p.live, 0), left = (pairs - first) * p.blocks;
     for (int64_t u = (int64_t)blockIdx.x * kHalfWarps + half; u < left; u += (int64_t)gridDim.x * kHalfWarps) {
       const int64_t to = first + u / p.blocks, b = u % p.blocks;
       store8<kVec>(p.q + to * p.K, b * kBlock + lane * 8, p.K, make_uint2(0u, 0u));
@@ -356,6 +358,8 @@ int launch_sort(const void* ids, int P, int E, int64_t base, int32_t* counts, in
 // ---- tokens into expert order and back ---------------------------------------------------------------------
 // A CTA holds blockDim.y tokens, blockDim.x lanes walk a row in vectors of V.  All three are bound by memory.
 
+// Places and counts come from a sort of the same pairs; whatever they say, no row outside of [0, pairs) is touched.
+
 // rows[place[t, s]] = x[t]: a token's row is read once and written for each of its experts; rows that no pair has
 // become zero.
 template <typename V>
@@ -371,11 +375,11 @@ permute_kernel(const uint8_t* __restrict__ x, int64_t pitch, const int32_t* __re
       const V v = from[c];
       for (int s = 0; s < topk; ++s) {
         const int64_t to = place[t * topk + s];
-        if (to >= 0) reinterpret_cast<V*>(rows + to * row_bytes)[c] = v;
+        if (in_rows(to, T * topk)) reinterpret_cast<V*>(rows + to * row_bytes)[c] = v;
       }
     }
   }
-  for (int64_t j = *live + t; j < T * topk; j += (int64_t)gridDim.x * blockDim.y) {
+  for (int64_t j = max(*live, 0) + t; j < T * topk; j += (int64_t)gridDim.x * blockDim.y) {
     V* to = reinterpret_cast<V*>(rows + j * row_bytes);
     for (int c = threadIdx.x; c < vecs; c += blockDim.x) to[c] = V{};
   }
@@ -416,6 +420,7 @@ unpermute_kernel(const typename T::word* __restrict__ y, const int32_t* __restri
 #pragma unroll
       for (int j = 0; j < kInFlight; ++j) {
         at[j] = s0 + j < topk ? place[t * topk + s0 + j] : -1;
+        if (!in_rows(at[j], tokens * topk)) at[j] = -1;
         weight[j] = w && s0 + j < topk ? w[t * topk + s0 + j] : 1.0f;
       }
 #pragma unroll
@@ -456,6 +461,7 @@ unpermute_grad_kernel(const typename T::word* __restrict__ d_out, const typename
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       at[j] = mine && s0 + j < topk ? (int64_t)place[t * topk + s0 + j] : -1;
+      if (!in_rows(at[j], tokens * topk)) at[j] = -1;
       weight[j] = at[j] >= 0 ? w[t * topk + s0 + j] : 0.0f;
       dot[j] = 0.0f;
     }
@@ -501,7 +507,7 @@ unpermute_grad_kernel(const typename T::word* __restrict__ d_out, const typename
     }
   }
   if (d_y) {
-    for (int64_t j = *live + t; j < tokens * topk; j += (int64_t)gridDim.x * blockDim.y) {
+    for (int64_t j = max(*live, 0) + t; j < tokens * topk; j += (int64_t)gridDim.x * blockDim.y) {
       typename P::raw* to = reinterpret_cast<typename P::raw*>(d_y + j * H);
       for (int c = threadIdx.x; c < vecs; c += blockDim.x) to[c] = typename P::raw{};
     }

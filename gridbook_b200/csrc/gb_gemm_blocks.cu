@@ -229,7 +229,8 @@ GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, i
   int tiles = 0;
 #pragma unroll 8
   for (int e = e0; e < e1; ++e) {
-    const int lo = p.seg[e], hi = p.seg[e + 1];
+    // within the rows there are, whatever the offsets say
+    const int lo = min(max(p.seg[e], 0), (int)p.M), hi = min(max(p.seg[e + 1], lo), (int)p.M);
     seg_s[e] = lo;
     base_s[e] = tiles;
     tiles += (hi - lo + tile_rows - 1) / tile_rows;

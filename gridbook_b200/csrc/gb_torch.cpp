@@ -862,12 +862,13 @@ at::Tensor gemm_fp8_blocks_grouped(const at::Tensor& a, const at::Tensor& a_scal
 }
 
 // ------------------------------------------------------------------ tokens sorted by expert and back
-int64_t check_ids(const at::Tensor& topk_ids, int64_t E) {
+int64_t check_ids(const at::Tensor& topk_ids, int64_t E, int64_t base) {
   need_cuda(topk_ids);
   need(topk_ids.dim() == 2, "expert ids of shape [tokens, top-k] expected");
   need(!topk_ids.is_floating_point() && !topk_ids.is_complex() && topk_ids.scalar_type() != at::kBool, "expert ids are whole numbers");
   const int64_t topk = topk_ids.size(1), P = topk_ids.size(0) * topk;
   need(E >= 1 && E <= 4096 && topk >= 1 && P < (1ll << 30), "1 to 4096 experts, at least one a token and fewer than 2^30 pairs expected");
+  need(base >= 0 && base < (1ll << 30), "expert_base outside [0, 2^30)");
   return P;
 }
 
@@ -889,7 +890,7 @@ void sort_pairs(const at::Tensor& topk_ids, int64_t E, int64_t base, int32_t* co
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& topk_ids, int64_t E, int64_t base) {
-  const int64_t P = check_ids(topk_ids, E);
+  const int64_t P = check_ids(topk_ids, E, base);
   const c10::cuda::CUDAGuard guard(topk_ids.device());
   const auto opt = topk_ids.options().dtype(at::kInt);
   if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
@@ -936,7 +937,7 @@ at::Tensor moe_fp8_blocks(const at::Tensor& x, const at::Tensor& w13, const at::
   need_operand(w2, s2, 3, "w2", true);
   const int64_t E = w13.size(0), H = w13.size(2), I = w2.size(2);
   need(w2.size(0) == E && w2.size(1) == H && w13.size(1) == 2 * I, "w13 [E, 2 inter, hidden] and w2 [E, hidden, inter] expected");
-  const int64_t P = check_ids(topk_ids, E), T = topk_ids.size(0), topk = topk_ids.size(1);
+  const int64_t P = check_ids(topk_ids, E, base), T = topk_ids.size(0), topk = topk_ids.size(1);
   need(x.dim() >= 1 && x.size(-1) == H && x.numel() == T * H, std::to_string(T) + " tokens of " + std::to_string(H) + " values expected");
   need(topk_weights.is_floating_point() && topk_weights.numel() == P, "one router weight for each of " + std::to_string(P) + " pairs expected");
   const c10::cuda::CUDAGuard guard(x.device());

@@ -659,7 +659,8 @@ def gemm_fp8_blocks_grouped(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Ten
                             offsets: torch.Tensor, *, out: torch.Tensor | None = None,
                             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """:func:`gemm_fp8_blocks` over expert segments: rows ``offsets[e]:offsets[e+1]`` of ``a`` [P, K] times ``b[e]`` of [E, N, K]
-    with ``b_scale`` [E, ceil(N/128), ceil(K/128)], up to 1024 experts.  Rows past ``offsets[E]`` are left unwritten."""
+    with ``b_scale`` [E, ceil(N/128), ceil(K/128)], up to 1024 experts.  Rows past ``offsets[E]`` are left unwritten;
+    offsets outside of the rows are taken as the nearest row."""
     return nat.host("grouped block-scaled GEMM").gemm_fp8_blocks_grouped(a, a_scale, b, b_scale, offsets, out, out_dtype)
 
 
@@ -676,7 +677,8 @@ class MoESort:
 
 def moe_sort(topk_ids: torch.Tensor, E: int, *, expert_base: int = 0) -> MoESort:
     """Sorts the pairs of ``topk_ids`` [T, top-k] by expert, on the device and without a host read.  The ``E`` experts held
-    here are the global ids [expert_base, expert_base + E); others, -1 among them, are dropped."""
+    here are the global ids [expert_base, expert_base + E); others, -1 among them, are dropped.  What reads a sort treats
+    places that are no row as dropped."""
     counts, offsets, order, place = nat.host("MoE routing").moe_sort(topk_ids, E, expert_base)
     return MoESort(counts, offsets, order, place, topk_ids.shape[1])
 

@@ -447,7 +447,7 @@ GB_API int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_
  * inner sums in fp32 on the tensor cores, the outer in fp32 registers, one rounding to `out` (GB_DTYPE_*).
  * K a multiple of 16, operands and D 16-byte aligned.  Grouped: A [P, K] rows sorted by expert (expert e
  * owns seg_offsets[e] .. seg_offsets[e + 1]), W [E, N, K], w_scale [E, ceil(N/128), ceil(K/128)], E <= 1024;
- * rows of D from seg_offsets[E] on are left as they are.
+ * rows of D from seg_offsets[E] on are left as they are.  Offsets are taken within [0, P].
  * beside: W, its scales and seg_offsets are not written by the launch right ahead on the stream, and that
  * launch lets this one start only behind its own wait (the quantisers above do): W is then fetched while
  * that launch still runs.  0 is always right. */
@@ -464,7 +464,8 @@ GB_API int gb_gemm_fp8_blocks_grouped(const void* A, const float* a_scale, const
 /* ---- tokens sorted by expert and back -------------------------------------------- */
 /* gb_moe_sort: gb_moe_route_inv without weights in one launch of one cluster, ids int32 or int64 (id_bytes), for up
  * to 65536 pairs and 1024 experts (gb_moe_sort_applies; GB_EUNSUPPORTED past them: use gb_moe_route_inv).
- * place [T * topk] and *live = offsets[E] from either.
+ * place [T * topk] and *live = offsets[E] from either; the entries below touch no row outside of [0, T * topk),
+ * a place that is none counts as dropped.
  * gb_moe_permute: rows[place[p]] = x[p / topk], x [T, H] with rows `ld` elements of elem_bytes (2 or 4)
  * apart; rows from *live on become zero.
  * gb_moe_unpermute: out[t] = sum over slots of weights[p] * y[place[p]] (weights NULL: ones; dropped pairs

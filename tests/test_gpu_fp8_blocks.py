@@ -305,3 +305,80 @@ def test_weights_written_right_before_the_call(dev):
         q, sq = kernels.fp8_quantize_blocks(x)
         assert torch.equal(kernels.gemm_fp8_blocks(q, sq, w, s), want[i % 2])
     _status()
+
+
+# ------------------------------------------------------------------ offsets outside the rows, and past 32 bits
+@pytest.mark.parametrize("P,E", [(200, 4), (1000, 2)])                  # few and many rows an expert: both kernels
+def test_segments_are_taken_within_the_rows(dev, P, E):
+    from gridbook_b200 import kernels
+    g = _gen(dev, P)
+    N, K = 264, 272
+    a, sa = B.rows(P, K, g, dev)
+    w, sw = B.weights((E, N, K), g, dev)
+    inside = torch.tensor([0] * E + [P], dtype=torch.int32, device=dev)
+    outside = torch.tensor([-5] + [0] * (E - 1) + [P + 1000], dtype=torch.int32, device=dev)
+    want = kernels.gemm_fp8_blocks_grouped(a, sa, w, sw, inside)
+    assert torch.equal(kernels.gemm_fp8_blocks_grouped(a, sa, w, sw, outside), want)
+    B.assert_product(want, B.dequant_rows(a, sa), B.dequant_weight(w[-1], sw[-1]), "last expert")
+    _status()
+
+
+def test_rows_past_two_gigabytes(dev):
+    """More than 2^31 values of x, of q and of the product; the last rows are looked at."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, 21)
+    M, K = 140000, 16384
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=dev)
+    x[-3:] = torch.randn(3, K, generator=g, device=dev).to(torch.bfloat16)
+    q, s = kernels.fp8_quantize_blocks(x)
+    few, fs = kernels.fp8_quantize_blocks(x[-3:])
+    assert torch.equal(q[-3:].view(torch.uint8), few.view(torch.uint8)) and torch.equal(s[-3:], fs)
+    assert not bool(q[-100:-3].view(torch.uint8).any())
+    del q, s
+    w, sw = B.weights((64, K), g, dev)
+    y = kernels.linear_fp8_blocks(x, w, sw)
+    B.assert_product(y[-3:], B.dequant_rows(few, fs), B.dequant_weight(w, sw), "last rows")
+    assert not bool(y[-100:-3].any())
+    del x, y
+    a, sa = B.rows(70000, 16, g, dev)
+    w, sw = B.weights((32768, 16), g, dev)
+    y = kernels.gemm_fp8_blocks(a, sa, w, sw)
+    assert y.numel() > 2 ** 31
+    B.assert_product(y[-3:], B.dequant_rows(a[-3:], sa[-3:]), B.dequant_weight(w, sw), "last rows of a large product")
+    _status()
+
+
+def test_weights_past_four_gigabytes(dev):
+    from gridbook_b200 import kernels
+    g = _gen(dev, 22)
+    E, N, K = 257, 4096, 4096
+    w = torch.zeros(E, N, K, dtype=torch.float8_e4m3fn, device=dev)
+    sw = torch.ones(E, N // 128, K // 128, device=dev)
+    one, s1 = B.weights((N, K), g, dev)
+    w[-1].view(torch.uint8).copy_(one.view(torch.uint8))
+    sw[-1] = s1
+    for P in (6, 257 * 80):
+        a, sa = B.rows(P, K, g, dev)
+        offsets = torch.zeros(E + 1, dtype=torch.int32, device=dev)
+        offsets[-1] = P
+        y = kernels.gemm_fp8_blocks_grouped(a, sa, w, sw, offsets)
+        B.assert_product(y[-6:], B.dequant_rows(a[-6:], sa[-6:]), B.dequant_weight(one, s1), f"{P} rows")
+    _status()
+
+
+def test_more_slots_than_half_a_warp(dev):
+    """A token's row written to twenty places."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, 23)
+    T, topk, K, E = 37, 20, 272, 64
+    ids = torch.stack([torch.randperm(E, generator=g, device=dev)[:topk] for _ in range(T)]).to(torch.int32)
+    ids[::3, 17] = -1
+    x = torch.randn(T, K, generator=g, device=dev).to(torch.bfloat16)
+    r = kernels.moe_sort(ids, E)
+    q, s = kernels.moe_permute_fp8(x, r)
+    fq, fs = kernels.fp8_quantize_blocks(x)
+    live = int(r.offsets[-1])
+    token = (r.order[:live] // topk).long()
+    assert torch.equal(q[:live].view(torch.uint8), fq.view(torch.uint8)[token]) and torch.equal(s[:live], fs[token])
+    assert not bool(q[live:].view(torch.uint8).any()) and not bool(s[live:].any())
+    _status()

@@ -224,3 +224,77 @@ def test_streams_and_graphs(dev):
         torch.cuda.synchronize()
         for p, q in zip(res, eager[k]):
             assert torch.equal(p, q)
+
+
+def test_expert_base_is_not_negative(dev):
+    from gridbook_b200 import kernels
+    for T in (4, 70000):                                                # both sorts
+        ids = torch.full((T, 1), -1, dtype=torch.int64, device=dev)
+        for base in (-3, 1 << 30):
+            with pytest.raises(RuntimeError, match="expert_base"):
+                kernels.moe_sort(ids, 8, expert_base=base)
+        assert int(kernels.moe_sort(ids, 8).offsets[-1]) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_places_outside_the_rows_count_nothing(dev, dtype):
+    """A sort put together by hand: places that are no row are treated as dropped pairs, a negative count as none."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, 31)
+    T, topk, H = 6, 2, 40
+    x = torch.randn(T, H, generator=g, device=dev).to(dtype)
+    place = torch.tensor([0, -1, 3, 12, 1, -7, 2 ** 31 - 1, 2, 4, 13, 5, -2 ** 31], dtype=torch.int32, device=dev)
+    r = kernels.MoESort(None, torch.tensor([0, -9], dtype=torch.int32, device=dev), None, place, topk)
+    good = [(p // topk, at) for p, at in enumerate(place.tolist()) if 0 <= at < T * topk]
+    want = torch.zeros(T * topk, H, device=dev, dtype=dtype)
+    for t, at in good:
+        want[at] = x[t]
+    none = kernels.MoESort(None, torch.tensor([0, T * topk], dtype=torch.int32, device=dev), None, place, topk)
+    rows = kernels.moe_permute(x, none)
+    for t, at in good:
+        assert torch.equal(rows[at], x[t])
+    q, s = kernels.moe_permute_fp8(x, none)
+    fq, fs = kernels.fp8_quantize_blocks(x)
+    for t, at in good:
+        assert torch.equal(q[at].view(torch.uint8), fq[t].view(torch.uint8)) and torch.equal(s[at], fs[t])
+    y = want.clone().requires_grad_()
+    w = torch.ones(T, topk, device=dev, requires_grad=True)
+    out = kernels.moe_unpermute(y, none, w)
+    ref = torch.zeros(T, H, device=dev, dtype=torch.float64)
+    for t, at in good:
+        ref[t] += want[at].double()
+    assert bool(((out.double() - ref).abs() <= B.HALF[dtype] * ref.abs() + 1e-6).all())
+    out.sum().backward()
+    for t, at in good:
+        assert torch.equal(y.grad[at], torch.ones_like(y.grad[at]))
+    hit = torch.zeros(T * topk, dtype=torch.bool, device=dev)
+    hit[[p for p, at in enumerate(place.tolist()) if 0 <= at < T * topk]] = True
+    assert not bool(w.grad.reshape(-1)[~hit].any())
+    kernels.moe_permute(x, r)                                           # rows from a negative count on: all of them become zero or a token's
+    torch.cuda.synchronize()
+
+
+def test_rows_past_two_gigabytes(dev):
+    from gridbook_b200 import kernels
+    g = _gen(dev, 32)
+    T, topk, H, E = 40000, 8, 7168, 16
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device=dev)
+    x[-2:] = torch.randn(2, H, generator=g, device=dev).to(torch.bfloat16)
+    ids = torch.zeros(T, topk, dtype=torch.int32, device=dev)
+    ids[-2:] = E - 1                                                    # their rows come last
+    r = kernels.moe_sort(ids, E)
+    rows = kernels.moe_permute(x, r)
+    assert rows.numel() > 2 ** 31
+    assert torch.equal(rows[-2 * topk:], x[-2:].repeat_interleave(topk, 0))
+    w = torch.full((T, topk), 0.125, device=dev)
+    out = kernels.moe_unpermute(rows, r, w)
+    assert torch.equal(out[-2:], x[-2:]) and not bool(out[-100:-2].any())
+    y, wg = rows.requires_grad_(), w.requires_grad_()
+    dy, dw = torch.autograd.grad(kernels.moe_unpermute(y, r, wg), [y, wg], x)
+    assert torch.equal(dy[-2 * topk:], (x[-2:].float() * 0.125).to(torch.bfloat16).repeat_interleave(topk, 0))
+    sq = x[-2:].double().square().sum(-1, keepdim=True)
+    assert bool(((dw[-2:].double() - sq).abs() <= H * 2.0 ** -24 * sq).all())
+    q, s = kernels.moe_permute_fp8(x, r)
+    fq, fs = kernels.fp8_quantize_blocks(x[-2:])
+    assert torch.equal(q[-2 * topk:].view(torch.uint8), fq.view(torch.uint8).repeat_interleave(topk, 0))
+    assert torch.equal(s[-2 * topk:], fs.repeat_interleave(topk, 0))
