@@ -47,6 +47,7 @@ struct BlocksParams {
   // rows kernel
   int rows_per_pass, passes, per_slice, slices, stages;
   int overlay, sums_at;      // sums of a sliced K lie over the ring, or that far behind its start
+  int pitch;                 // rows of a slice's sums in a CTA
   // rows quantised by the kernel itself: M of them, ld elements apart
   const void* x;
   int64_t ld, K;
@@ -632,6 +633,7 @@ gemm_blocks_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
 
 // ======================================== few rows =========================================================
 constexpr int kMaxStages = 12;
+constexpr int kFewStages = 8;                        // of CTAs with one tile and up to sixteen rows
 constexpr int kScaleSlots = 4;                       // groups of four blocks whose scales are there ahead of their sums
 constexpr int kQuantWarps = 4, kQuantStages = 10, kScaleRing = 32;    // rows quantised here: warps that do, fewest stages, blocks whose scales are kept
 
@@ -840,6 +842,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
           // The stage is free once the MMAs that read it last are done.  A barrier's parity tells a phase from the next one only:
           // this wait's phase cannot be over, for its MMAs need the block that is written below, and the phase before the last is,
           // for the warp has waited, a step or two ago, for a slab at most `stages` before this one (steps of no more than four slabs).
+          // With eight stages and one tile a CTA the eight lanes that wait come to their stages in turn and meet every phase.
           const bool there = !live || try_wait<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u);
           if (!__all_sync(0xffffffffu, there)) {
             if (!there) wait_slow<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u, &abort_s, p.status, 98);
@@ -1013,7 +1016,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   }
 
   if (p.slices > 1) {
-    // Sums into the shared memory of the CTA that owns the row, [slice][own row][feature]; where that lies over the operand
+    // Sums into the shared memory of the CTA that owns the row, [slice][own row][feature] (never more than the product's rows); where that lies over the operand
     // ring, every CTA of the cluster has finished its MMAs first, and with them its loads.  Rows are owned in sixteens.
     const bool live = warp < kRead && !abort_s && first < total;
     const int rows = live ? last.rows : 0, cols = (rows + 15) / 16 * 16;
@@ -1034,7 +1037,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         const int to = r0 / own, off = r0 - to * own;
         uint32_t dst;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                     : "=r"(dst) : "r"(sums + (uint32_t)((slice * own + off) * kBM + feature) * 4u), "r"(to));
+                     : "=r"(dst) : "r"(sums + (uint32_t)((slice * p.pitch + off) * kBM + feature) * 4u), "r"(to));
 #pragma unroll
         for (int c = 0; c < 16; ++c)
           if (r0 + c < rows)
@@ -1050,7 +1053,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         for (int q = 0; q < p.slices; ++q) {
           float v[4];
           asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(sums + (uint32_t)((q * own + r) * kBM + f) * 4u));
+                       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(sums + (uint32_t)((q * p.pitch + r) * kBM + f) * 4u));
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] += v[i];
         }
@@ -1219,11 +1222,16 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   constexpr int kFixed = 1024 + (S::kQuantize ? kScaleRing : 4 * kScaleSlots) * kR * 4 + (kGrouped ? kSegBytes : 0);
   // the sums take up to 64 KB: of their own where that leaves enough stages
   constexpr int kLeast = S::kQuantize ? kQuantStages : 8;
-  const int own = (kR / 16 + p.slices - 1) / p.slices * 16, sums = p.slices > 1 ? p.slices * own * kBM * 4 : 0;
+  const int own = (kR / 16 + p.slices - 1) / p.slices * 16;
+  p.pitch = p.M < own ? (int)p.M : own;
+  const int sums = p.slices > 1 ? p.slices * p.pitch * kBM * 4 : 0;
   p.overlay = (kSmemMax - kFixed - sums) / S::kStageBytes < kLeast;
   p.stages = (kSmemMax - kFixed - (p.overlay ? 0 : sums)) / S::kStageBytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   p.stages &= ~1;
+  // One tile a CTA and few rows: eight stages do, and more in flight at the start cost (one row of 5120 x 8192 10.5 us with ten, 9.9 with
+  // eight, 10.6 with twelve and 11.8 with four; 16 rows 10.9 and 10.7).
+  if (kR == 16 && !kGrouped && (p.slices > 1 || most <= sms) && p.stages > kFewStages) p.stages = kFewStages;
   static_assert(!S::kQuantize || (kSmemMax - kFixed) / S::kStageBytes >= kLeast, "the quantising warps count on so many stages");
   p.sums_at = kFixed - 1024 + p.stages * S::kStageBytes;
   p.idesc = 1u << 4;

@@ -382,3 +382,21 @@ def test_more_slots_than_half_a_warp(dev):
     assert torch.equal(q[:live].view(torch.uint8), fq.view(torch.uint8)[token]) and torch.equal(s[:live], fs[token])
     assert not bool(q[live:].view(torch.uint8).any()) and not bool(s[live:].any())
     _status()
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 9, 16])
+@pytest.mark.parametrize("N,K", [(128, 9008), (300, 17408), (5120, 17408), (20000, 1040)])
+def test_linear_more_blocks_than_stages(dev, M, N, K):
+    """Rings that are gone round several times, with one tile a CTA and with several."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, M + N + K)
+    w, sw = B.weights((N, K), g, dev)
+    x = torch.randn(M, K, generator=g, device=dev).to(torch.bfloat16)
+    q, s = kernels.fp8_quantize_blocks(x)
+    want = kernels.gemm_fp8_blocks(q, s, w, sw, out_dtype=torch.float32)
+    B.assert_product(want, B.dequant_rows(q, s), B.dequant_weight(w, sw), "product")
+    y = kernels.linear_fp8_blocks(x, w, sw, out_dtype=torch.float32)
+    B.assert_product(y, B.dequant_rows(q, s), B.dequant_weight(w, sw), "linear")
+    for _ in range(20):
+        assert torch.equal(kernels.linear_fp8_blocks(x, w, sw, out_dtype=torch.float32), y)
+    _status()
