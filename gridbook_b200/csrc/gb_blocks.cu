@@ -164,18 +164,15 @@ quantize_blocks_kernel(const __grid_constant__ QuantizeParams p) {
 
 template <typename T, Source kSource>
 int launch_quantize(const QuantizeParams& p, bool vec, cudaStream_t stream) {
-  // one block each for less than a wave of them, two from there on (8192 rows of 5120 bf16: 32.3 us, 31.2, four 32.9); one where every
-  // block is written several times (4096 tokens x 8 x 2048 columns: 23 us, four 27)
-  const int64_t few = 8ll * gb_sm_count() * kHalfWarps;
-  const int per = kSource != kSorted && p.units > few ? 2 : 1;
+  // one block each for less than a wave of them, two from there on (8192 rows of 5120 bf16: 32.3 us, 31.2, four 32.9); where every
+  // block is written several times, from two waves on (one, two, four: 512 tokens x 8 of 7168 columns 10.8 us, 11.6, 13.6; 4096 of
+  // 2048 21.4, 20.5, 22.2; 2048 of 7168 35.4, 33.9, 37.8)
+  const int64_t few = (kSource == kSorted ? 16ll : 8ll) * gb_sm_count() * kHalfWarps;
+  const int per = p.units > few ? 2 : 1;
   const dim3 grid((unsigned)((p.units + per * kHalfWarps - 1) / (per * kHalfWarps)));
 #define GB_Q(v, n) GB_CUDA_OK(gb_launch(quantize_blocks_kernel<T, kSource, v, n>, grid, dim3(kThreads), 0, stream, p))
-  if constexpr (kSource == kSorted) {
-    if (vec) GB_Q(true, 1); else GB_Q(false, 1);
-  } else {
-    if (vec) { if (per == 2) GB_Q(true, 2); else GB_Q(true, 1); }
-    else { if (per == 2) GB_Q(false, 2); else GB_Q(false, 1); }
-  }
+  if (vec) { if (per == 2) GB_Q(true, 2); else GB_Q(true, 1); }
+  else { if (per == 2) GB_Q(false, 2); else GB_Q(false, 1); }
 #undef GB_Q
   return GB_OK;
 }

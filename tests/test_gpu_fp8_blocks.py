@@ -400,3 +400,23 @@ def test_linear_more_blocks_than_stages(dev, M, N, K):
     for _ in range(20):
         assert torch.equal(kernels.linear_fp8_blocks(x, w, sw, out_dtype=torch.float32), y)
     _status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K", [(2500, 2048), (1300, 4990)])
+def test_many_tokens_into_expert_order(dev, dtype, T, K):
+    """Enough blocks that a half warp takes two, in rows of whole and of ragged blocks."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, T)
+    topk, E = 3, 24
+    ids = torch.rand(T, E + 4, generator=g, device=dev).topk(topk, -1)[1]
+    x = torch.randn(T, K, generator=g, device=dev).to(dtype)
+    r = kernels.moe_sort(ids, E, expert_base=2)
+    q, s = kernels.moe_permute_fp8(x, r)
+    fq, fs = kernels.fp8_quantize_blocks(x)
+    live = int(r.offsets[-1])
+    token = (r.order[:live] // topk).long()
+    assert 0 < live < T * topk
+    assert torch.equal(q[:live].view(torch.uint8), fq.view(torch.uint8)[token]) and torch.equal(s[:live], fs[token])
+    assert not bool(q[live:].view(torch.uint8).any()) and not bool(s[live:].any())
+    _status()
