@@ -898,8 +898,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Te
   const c10::cuda::CUDAGuard guard(topk_ids.device());
   const auto opt = topk_ids.options().dtype(at::kInt);
   if (P == 0) return {at::zeros({E}, opt), at::zeros({E + 1}, opt), at::empty({0}, opt), at::empty({0}, opt)};
-  at::Tensor counts = fresh({E}, at::kInt, topk_ids), offsets = fresh({E + 1}, at::kInt, topk_ids), order = fresh({P}, at::kInt, topk_ids),
-             place = fresh({P}, at::kInt, topk_ids);
+  // four tensors in one allocation, each from a 256-byte boundary on (four allocations: 1.6 us of host time more, of 7.0)
+  const int64_t e0 = (E + 63) / 64 * 64, e1 = (E + 1 + 63) / 64 * 64, p0 = (P + 63) / 64 * 64;
+  const at::Tensor all = fresh({e0 + e1 + p0 + P}, at::kInt, topk_ids);
+  const auto part = [&](int64_t first, int64_t n) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(first);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+  };
+  at::Tensor counts = part(0, E), offsets = part(e0, E + 1), order = part(e0 + e1, P), place = part(e0 + e1 + p0, P);
   sort_pairs(topk_ids, E, base, counts.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), order.data_ptr<int32_t>(), place.data_ptr<int32_t>(),
              c10::cuda::getCurrentCUDAStream().stream());
   return {counts, offsets, order, place};
