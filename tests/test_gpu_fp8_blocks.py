@@ -420,3 +420,22 @@ def test_many_tokens_into_expert_order(dev, dtype, T, K):
     assert torch.equal(q[:live].view(torch.uint8), fq.view(torch.uint8)[token]) and torch.equal(s[:live], fs[token])
     assert not bool(q[live:].view(torch.uint8).any()) and not bool(s[live:].any())
     _status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N", [(1300, 4099), (1300, 4098), (1300, 4100), (1300, 4104), (300, 1003), (300, 1004), (300, 1006), (300, 1016), (2500, 1030)])
+def test_product_rows_of_every_alignment(dev, dtype, M, N):
+    """Rows of D that are whole 16-byte pieces, words, single values: on pairs, single CTAs and slices of K; nothing beside them is written."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, M + N)
+    a, sa = B.rows(M, 1040, g, dev)
+    w, sw = B.weights((N, 1040), g, dev)
+    y = kernels.gemm_fp8_blocks(a, sa, w, sw, out_dtype=dtype)
+    B.assert_product(y, B.dequant_rows(a, sa), B.dequant_weight(w, sw), f"{M}x{N}")
+    counts = [M // 2 - 7, 0, M - M // 2 - 4]                            # eleven rows behind the last segment
+    offsets = torch.tensor([0, counts[0], counts[0], sum(counts)], dtype=torch.int32, device=dev)
+    out = torch.full((M, N), 77.0, dtype=dtype, device=dev)
+    kernels.gemm_fp8_blocks_grouped(a, sa, w.unsqueeze(0).repeat(3, 1, 1), sw.unsqueeze(0).repeat(3, 1, 1), offsets, out=out)
+    B.assert_product(out[:M - 11], B.dequant_rows(a[:M - 11], sa[:M - 11]), B.dequant_weight(w, sw), f"grouped {M}x{N}")
+    assert bool((out[M - 11:] == 77.0).all())
+    _status()
