@@ -16,6 +16,7 @@
 // bytes of the weights, up to some 64 rows; from there on the shared memory, through which every warp gets the rows' scales
 // at 128 bytes a clock beside the operands.
 #include "gb_blocks.cuh"
+#include "gb_row_ring.cuh"
 
 #include <cuda.h>
 #include <atomic>
@@ -696,8 +697,11 @@ gemm_blocks_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
 // ======================================== few rows =========================================================
 constexpr int kMaxStages = 12;
 constexpr int kFewStages = 8;                        // of CTAs with one tile and up to sixteen rows
+static_assert(kFewStages % 2 == 0 && gb_row_ring::kStages % 2 == 0, "each of the two MMA issuers meets every phase of its stages");
 constexpr int kScaleSlots = 4;                       // groups of four blocks whose scales are there ahead of their sums
-constexpr int kQuantWarps = 4, kQuantStages = 10, kScaleRing = 32;    // rows quantised here: warps that do, fewest stages, blocks whose scales are kept
+constexpr int kQuantWarps = 4, kQuantMaxRows = 4, kScaleRing = 32;    // rows quantised here: warps that do, most rows, blocks whose scales are kept
+static_assert(gb_row_ring::kSlabsAStep * kQuantMaxRows <= 4 * kQuantWarps, "a group of eight lanes for each block of a step");
+static_assert(kScaleRing >= gb_row_ring::kStages + 8 + 4, "see the read-out: stages and accumulators, and some");
 
 // In: the type of rows that the kernel quantises itself, or void: A is E4M3 with its scales.
 template <int kR, typename In = void>
@@ -867,66 +871,66 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     }
   } else if (kQuantize && warp >= kRead + 3) {
     // ------- rows -> E4M3 in the operand's place, their scales times the tile's: eight lanes take a row's block, sixteen columns
-    // each; items (block, row) in that order, up to sixteen a step, loaded two steps ahead -------
+    // each, four slabs a step, loaded two steps ahead, over the ends of tiles too -------
     if constexpr (kQuantize) {
       constexpr int kPieces = sizeof(typename In::word);       // of sixteen bytes, in sixteen columns
-      const int mine = (warp - kRead - 3) * 4 + (lane >> 3), c = lane & 7, rows = (int)p.M, step = min(4 * kQuantWarps, 4 * rows);
-      const uint32_t total_items = (uint32_t)k_n * (uint32_t)rows;
-      struct Raw { uint4 v[kPieces]; float bs; int kt, row; };
-      int before = 0;                                      // slabs of the items before this one
-      bool ok = true;
-      for (int item = first; ok && item < total; item += stride) {
-        const Item t = item_at(item, 0);
-        const float* bs = p.b_scale + (int64_t)(t.n0 / kSlab) * p.kb;
-        auto load = [&](uint32_t i, Raw& r) {
-          const bool live = mine < step && i < total_items;
-          r.kt = live ? (int)(i / (uint32_t)rows) : -1;
-          r.row = live ? (int)(i - (uint32_t)r.kt * (uint32_t)rows) : 0;
-          const int64_t col = (int64_t)(k_begin + r.kt) * kSlab + c * 16;
-          const uint4* at = reinterpret_cast<const uint4*>(static_cast<const typename In::word*>(p.x) + r.row * p.ld + col);
+      const int group = (warp - kRead - 3) * 4 + (lane >> 3), c = lane & 7, rows = (int)p.M;
+      const int row = gb_row_ring::row(group, rows), slabs = (total > first ? (total - first + stride - 1) / stride : 0) * k_n;
+      const typename In::word* x = static_cast<const typename In::word*>(p.x) + row * p.ld + (int64_t)k_begin * kSlab + c * 16;
+      const int64_t width = p.K - (int64_t)k_begin * kSlab - c * 16;
+      struct Raw { uint4 v[kPieces]; float bs; };
+      // where the loads are: a slab, the tile of features that it belongs to (there is one pass of rows), its block within the tile
+      int ahead = gb_row_ring::works(group, rows) ? gb_row_ring::first_slab(group, rows) : slabs, item = first, kt = ahead;
+      auto load = [&](Raw& r) {
+        const bool live = ahead < slabs;
+        if (live)
+          for (; kt >= k_n; kt -= k_n) item += stride;
+        const uint4* at = reinterpret_cast<const uint4*>(x + (int64_t)kt * kSlab);
 #pragma unroll
-          for (int q = 0; q < kPieces; ++q) r.v[q] = live && col < p.K ? at[q] : make_uint4(0u, 0u, 0u, 0u);
-          r.bs = live ? bs[k_begin + r.kt] : 0.0f;
-        };
-        Raw cur, next;
-        load((uint32_t)mine, cur);
-        load((uint32_t)(mine + step), next);
-        for (uint32_t i0 = 0; i0 < total_items; i0 += (uint32_t)step) {
-          Raw after;
-          load(i0 + (uint32_t)(mine + 2 * step), after);
-          float v[16], scale;
-          uint32_t q[4];
-#pragma unroll
-          for (int k = 0; k < kPieces; ++k) gb_blocks::unpack16<In>(cur.v[k], v + k * (16 / kPieces));
-          gb_blocks::quantize_block<16, 8>(v, p.scale_rule, scale, q);
-          const bool live = cur.kt >= 0;
-          const int n = before + cur.kt, turn = n / p.stages, s = n - turn * p.stages;
-          // The stage is free once the MMAs that read it last are done.  A barrier's parity tells a phase from the next one only:
-          // this wait's phase cannot be over, for its MMAs need the block that is written below, and the phase before the last is,
-          // for the warp has waited, a step or two ago, for a slab at most `stages` before this one (steps of no more than four slabs).
-          // With eight stages and one tile a CTA the eight lanes that wait come to their stages in turn and meet every phase.
-          const bool there = !live || try_wait<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u);
-          if (!__all_sync(0xffffffffu, there)) {
-            if (!there) wait_slow<kOfCta>(empty_bar + 8 * s, (uint32_t)(turn & 1) ^ 1u, &abort_s, p.status, 98);
-            ok = !__any_sync(0xffffffffu, abort_s != 0);
-            if (!ok) break;
-          }
-          if (live) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                         ::"r"(ring + (uint32_t)s * S::kStageBytes + kBM * kSlab + (uint32_t)(cur.row * kSlab + ((c ^ (cur.row & 7)) * 16))), "r"(q[0]),
-                           "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
-            if (c == 0) scale_s[(n % kScaleRing) * kR + cur.row] = scale * cur.bs;
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (live && c == 0) {
-            arrive(full_bar + 8 * s);
-            arrive(sc_full + 8 * (n % kScaleRing));
-          }
-          cur = next;
-          next = after;
+        for (int q = 0; q < kPieces; ++q) r.v[q] = live && (int64_t)kt * kSlab < width ? at[q] : make_uint4(0u, 0u, 0u, 0u);
+        r.bs = live ? p.b_scale[(int64_t)item * p.kb + k_begin + kt] : 0.0f;
+        if (live) {
+          ahead += gb_row_ring::kSlabsAStep;
+          kt += gb_row_ring::kSlabsAStep;
         }
-        before += k_n;
+      };
+      int n = ahead;                                         // the slab that is written
+      Raw cur, next;
+      load(cur);
+      load(next);
+      bool ok = true;
+      for (int n0 = 0; n0 < slabs; n0 += gb_row_ring::kSlabsAStep, n += gb_row_ring::kSlabsAStep) {
+        Raw after;
+        load(after);
+        float v[16], scale;
+        uint32_t q[4];
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) gb_blocks::unpack16<In>(cur.v[k], v + k * (16 / kPieces));
+        gb_blocks::quantize_block<16, 8>(v, p.scale_rule, scale, q);
+        const bool live = n < slabs;
+        const int s = n % gb_row_ring::kStages;
+        // The stage is free once the MMAs that read it last are done; this group has waited for every phase of the stage before.
+        const uint32_t parity = (uint32_t)(n / gb_row_ring::kStages & 1) ^ 1u;
+        const bool there = !live || try_wait<kOfCta>(empty_bar + 8 * s, parity);
+        if (!__all_sync(0xffffffffu, there)) {
+          if (!there) wait_slow<kOfCta>(empty_bar + 8 * s, parity, &abort_s, p.status, 98);
+          ok = !__any_sync(0xffffffffu, abort_s != 0);
+          if (!ok) break;
+        }
+        if (live) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(ring + (uint32_t)s * S::kStageBytes + kBM * kSlab + (uint32_t)(row * kSlab + ((c ^ (row & 7)) * 16))), "r"(q[0]), "r"(q[1]),
+                         "r"(q[2]), "r"(q[3]) : "memory");
+          if (c == 0) scale_s[(n % kScaleRing) * kR + row] = scale * cur.bs;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (live && c == 0) {
+          arrive(full_bar + 8 * s);
+          arrive(sc_full + 8 * (n % kScaleRing));
+        }
+        cur = next;
+        next = after;
       }
     }
   } else if (warp == kRead + 3) {
@@ -1014,7 +1018,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         if (++buf == kAccs) { buf = 0; ph ^= 1; }
         if (kQuantize) {
           // no arrival: an entry is written again 32 slabs on, behind a stage that was freed by MMAs whose accumulators this
-          // warp had released long after (stages + accumulators <= 20 slabs)
+          // warp had released long after (stages + accumulators = 16 slabs)
           if (++slot == kScaleRing) { slot = 0; sc_ph ^= 1; }
         } else if ((kt & 3) == 3 || kt + 1 == k_n) {
           __syncwarp();
@@ -1283,7 +1287,7 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   p.slices = (p.kb + p.per_slice - 1) / p.per_slice;
   constexpr int kFixed = 1024 + (S::kQuantize ? kScaleRing : 4 * kScaleSlots) * kR * 4 + (kGrouped ? kSegBytes : 0);
   // the sums take up to 64 KB: of their own where that leaves enough stages
-  constexpr int kLeast = S::kQuantize ? kQuantStages : 8;
+  constexpr int kLeast = 8;
   const int own = (kR / 16 + p.slices - 1) / p.slices * 16;
   p.pitch = p.M < own ? (int)p.M : own;
   const int sums = p.slices > 1 ? p.slices * p.pitch * kBM * 4 : 0;
@@ -1294,7 +1298,9 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   // One tile a CTA and few rows: eight stages do, and more in flight at the start cost (one row of 5120 x 8192 10.5 us with ten, 9.9 with
   // eight, 10.6 with twelve and 11.8 with four; 16 rows 10.9 and 10.7).
   if (kR == 16 && !kGrouped && (p.slices > 1 || most <= sms) && p.stages > kFewStages) p.stages = kFewStages;
-  static_assert(!S::kQuantize || (kSmemMax - kFixed) / S::kStageBytes >= kLeast, "the quantising warps count on so many stages");
+  if (S::kQuantize) p.stages = gb_row_ring::kStages;
+  static_assert(!S::kQuantize || (kSmemMax - kFixed - kMaxSlices * kQuantMaxRows * kBM * 4) / S::kStageBytes >= gb_row_ring::kStages,
+                "so many stages, and the sums of a sliced K beside them");
   p.sums_at = kFixed - 1024 + p.stages * S::kStageBytes;
   p.idesc = 1u << 4;
   CUtensorMap map_w, map_x = {};
@@ -1391,7 +1397,6 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
 
 // us, two launches / one: 1 row of 34816 x 5120 34.9 / 32.9, 4 rows 35.7 / 33.7, 8 rows 36.7 / 43.0; 4 rows of 4096 x 4096 10.3 / 8.4, 16 rows
 // 10.3 / 12.3: every CTA quantises all rows, four blocks at a time and warp.
-static constexpr int64_t kQuantMaxRows = 4;
 
 int gb_linear_fp8_blocks(const void* x, int dtype, int64_t ld, int scale_rule, const void* W, const float* w_scale, void* D, int out, int64_t M, int64_t N,
                          int64_t K, void* stream) {
