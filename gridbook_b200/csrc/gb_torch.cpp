@@ -997,8 +997,14 @@ at::Tensor unpermute_rows(const at::Tensor& y, const at::Tensor& place, const at
   return out;
 }
 
-void first_derivatives_only() {
+// Tangents of forward-mode differentiation would be dropped without a word: nodes of the graph give the backward pass alone.
+void no_tangents(std::initializer_list<const at::Tensor*> all) {
+  for (const at::Tensor* t : all) GB_NEED(!t->defined() || !t->_fw_grad(0).defined(), "the sorted rows have no forward-mode derivatives");
+}
+
+void first_derivatives_only(const at::Tensor& grad) {
   GB_NEED(!at::GradMode::is_enabled(), "the sorted rows' gradients have no derivatives of their own (create_graph)");
+  no_tangents({&grad});
 }
 
 using torch::autograd::SavedVariable;
@@ -1022,7 +1028,7 @@ struct PermuteBackward : SortedBackward {
   PermuteBackward(const at::Tensor& x, const at::Tensor& place_, const at::Tensor& offsets_, int64_t topk_)
       : SortedBackward(place_, offsets_, topk_), shape(x.sizes().vec()) {}
   variable_list apply(variable_list&& grads) override {
-    first_derivatives_only();
+    first_derivatives_only(grads[0]);
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {at::Tensor()};
     return {unpermute_rows(grads[0], place.unpack(), offsets.unpack(), topk, at::Tensor()).view(shape)};
@@ -1032,7 +1038,7 @@ struct PermuteBackward : SortedBackward {
 struct SumBackward : SortedBackward {                              // of moe_unpermute without weights
   using SortedBackward::SortedBackward;
   variable_list apply(variable_list&& grads) override {
-    first_derivatives_only();
+    first_derivatives_only(grads[0]);
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {at::Tensor()};
     return {permute_rows(grads[0], place.unpack(), offsets.unpack(), topk)};
@@ -1053,7 +1059,7 @@ struct UnpermuteBackward : SortedBackward {
     y.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    first_derivatives_only();
+    first_derivatives_only(grads[0]);
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
     const at::Tensor places = place.unpack(), offs = offsets.unpack(), weights = w.unpack(), g = grads[0].contiguous();
@@ -1081,6 +1087,7 @@ std::shared_ptr<N> node_of(torch::autograd::edge_list&& edges, Args&&... args) {
 }
 
 at::Tensor moe_permute(const at::Tensor& x, const at::Tensor& place, const at::Tensor& offsets, int64_t topk) {
+  no_tangents({&x});
   need_cuda(x);
   dtype_code(x.scalar_type(), "moe_permute");
   if (!(at::GradMode::is_enabled() && x.requires_grad())) return permute_rows(x, place, offsets, topk);
@@ -1095,6 +1102,8 @@ at::Tensor moe_permute(const at::Tensor& x, const at::Tensor& place, const at::T
 }
 
 at::Tensor moe_unpermute(const at::Tensor& y, const at::Tensor& place, const at::Tensor& offsets, int64_t topk, const Opt& weights) {
+  no_tangents({&y});
+  if (weights.has_value()) no_tangents({&*weights});
   need_cuda(y);
   dtype_code(y.scalar_type(), "moe_unpermute");
   at::Tensor w;
