@@ -69,6 +69,12 @@ GB_DEVINL uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+// The sum rounded down, and so -0 where it is exactly zero.
+GB_DEVINL uint64_t fma_down_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
 GB_DEVINL float max_nan(float a, float b) {
   float r;
@@ -92,14 +98,16 @@ GB_DEVINL void quantize_block(const float (&v)[kN], int scale_rule, float& scale
 #pragma unroll
     for (int i = 0; i < kN / 2; ++i) h[i] = gb_cvt_e4m3x2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale));
   } else {
-    // gb_div of two values at a time
+    // gb_div of two values at a time.  The remainder is exact, so that its rounding says one thing only, the sign of a remainder of zero: with
+    // -0 the correction leaves a quotient of -0 what it is, where +0 would make it +0.  (It is not exact next to the least fp32
+    // values, whose quotients are far below E4M3's least.)
     const float rinv = __frcp_rn(scale);
     const uint64_t r2 = pack_f32x2(rinv, rinv), d2 = pack_f32x2(-scale, -scale);
 #pragma unroll
     for (int i = 0; i < kN / 2; ++i) {
       const uint64_t v2 = pack_f32x2(v[2 * i], v[2 * i + 1]);
       uint64_t t = mul_f32x2(v2, r2);
-      t = fma_f32x2(fma_f32x2(t, d2, v2), r2, t);
+      t = fma_f32x2(fma_down_f32x2(t, d2, v2), r2, t);
       float lo, hi;
       asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(t));
       h[i] = gb_cvt_e4m3x2(lo, hi);
