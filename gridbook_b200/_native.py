@@ -28,7 +28,7 @@ REQUIRED_SYMBOLS = (
     "gb_moe_mlp_pairs_workspace_bytes", "gb_moe_mlp_pairs",
     "gb_expand_fp8_bf16", "gb_fp8_quantize_rows", "gb_gemm_tn", "gb_gemm_tn_grouped", "gb_moe_gather_rows", "gb_moe_swiglu_rows", "gb_moe_gemv_sorted",
     "gb_moe_route_inv", "gb_moe_fp4_pass_rows", "gb_moe_fp4_operand_bytes", "gb_moe_fp4_rows", "gb_moe_fp4_swiglu_rows", "gb_moe_gemv_fp4", "gb_moe_gemm_fp4",
-    "gb_fp8_quantize_blocks", "gb_moe_swiglu_fp8", "gb_moe_permute_fp8", "gb_gemm_fp8_blocks", "gb_gemm_fp8_blocks_grouped", "gb_linear_fp8_blocks",
+    "gb_fp8_quantize_blocks", "gb_moe_swiglu_fp8", "gb_moe_permute_fp8", "gb_gemm_fp8_blocks", "gb_gemm_fp8_blocks_grouped", "gb_linear_fp8_blocks", "gb_gemm_fp8_blocks_kernel",
     "gb_moe_sort", "gb_moe_sort_applies", "gb_moe_permute", "gb_moe_unpermute", "gb_moe_unpermute_grad",
     "gb_peer_alloc", "gb_peer_free", "gb_peer_export", "gb_peer_open", "gb_peer_close",
     "gb_peer_allgather", "gb_peer_allgather_ll", "gb_peer_barrier", "gb_launch_count", "gb_gemv_allgather", "gb_moe_combine_peer",
@@ -160,6 +160,7 @@ def _declare(lib) -> None:
     lib.gb_moe_swiglu_fp8.argtypes = [vp, i32, i64, vp, i64, i64, i32, vp, vp, vp]
     lib.gb_moe_permute_fp8.argtypes = [vp, i32, i64, vp, vp, i64, i64, i64, i32, vp, vp, vp]
     lib.gb_gemm_fp8_blocks.argtypes = [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, vp]
+    lib.gb_gemm_fp8_blocks_kernel.argtypes = [i64, i64, i64, ctypes.POINTER(i32)]
     lib.gb_linear_fp8_blocks.argtypes = [vp, i32, i64, i32, vp, vp, vp, i32, i64, i64, i64, vp]
     lib.gb_gemm_fp8_blocks_grouped.argtypes = [vp, vp, vp, vp, vp, i64, vp, i32, i64, i64, i64, i32, vp]
     lib.gb_moe_sort_applies.argtypes = [i64, i64]

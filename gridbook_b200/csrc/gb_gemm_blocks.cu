@@ -1395,6 +1395,15 @@ int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const
   return route == kCtaRoute ? run_tiles<1, false>(A, W, K, p, (cudaStream_t)stream) : run_tiles<2, false>(A, W, K, p, (cudaStream_t)stream);
 }
 
+// The kernel that gb_gemm_fp8_blocks launches, and its slices of K where those are told.
+int gb_gemm_fp8_blocks_kernel(int64_t M, int64_t N, int64_t K, int32_t* slices) {
+  if (slices) *slices = 1;
+  const Route route = route_of(M, N);
+  if (route == kCtaRoute && slices && ready() == GB_OK)
+    *slices = slices_of((M + kBM - 1) / kBM * ((N + kBN - 1) / kBN), (int)((K + kSlab - 1) / kSlab)).n;
+  return route;
+}
+
 // us, two launches / one: 1 row of 34816 x 5120 34.9 / 32.9, 4 rows 35.7 / 33.7, 8 rows 36.7 / 43.0; 4 rows of 4096 x 4096 10.3 / 8.4, 16 rows
 // 10.3 / 12.3: every CTA quantises all rows, four blocks at a time and warp.
 

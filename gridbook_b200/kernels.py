@@ -648,6 +648,13 @@ def gemm_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
     return nat.host("block-scaled GEMM").gemm_fp8_blocks(a, a_scale, b, b_scale, out_dtype)
 
 
+def gemm_fp8_blocks_kernel(M: int, N: int, K: int) -> tuple[str, int]:
+    """The kernel that :func:`gemm_fp8_blocks` launches for a product, and over how many slices its tiles split K."""
+    slices = ctypes.c_int32()
+    route = nat.load("block-scaled GEMM").gb_gemm_fp8_blocks_kernel(M, N, K, ctypes.byref(slices))
+    return ("gemm_blocks_rows_kernel", "gemm_blocks_tile_kernel<1>", "gemm_blocks_tile_kernel<2>")[route], slices.value
+
+
 def linear_fp8_blocks(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *, out_dtype: torch.dtype | None = None,
                       scale_rule: str = "recip") -> torch.Tensor:
     """y[..., N] = quantised(x)[..., K] . (weight * weight_scale)^T: :func:`fp8_quantize_blocks` and

@@ -453,6 +453,8 @@ GB_API int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_
  * that launch still runs.  0 is always right. */
 GB_API int gb_gemm_fp8_blocks(const void* A, const float* a_scale, const void* W, const float* w_scale, void* D, int out,
                               int64_t M, int64_t N, int64_t K, int beside, void* stream);
+/* Which kernel that is: 0 few rows, 1 tiles on single CTAs (*slices, if not null: over how many K is split), 2 tiles on pairs. */
+GB_API int gb_gemm_fp8_blocks_kernel(int64_t M, int64_t N, int64_t K, int32_t* slices);
 /* gb_fp8_quantize_blocks and gb_gemm_fp8_blocks of up to 4 rows in one launch, the same values; x 16-byte aligned, rows
  * whole 16-byte pieces apart (GB_EUNSUPPORTED otherwise: call the two). */
 GB_API int gb_linear_fp8_blocks(const void* x, int dtype, int64_t ld, int scale_rule, const void* W, const float* w_scale, void* D,
