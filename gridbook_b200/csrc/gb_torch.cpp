@@ -876,6 +876,12 @@ int64_t check_ids(const at::Tensor& topk_ids, int64_t E, int64_t base) {
   return P;
 }
 
+// A weight for each pair, in the pairs' order: [.., top-k], or flat.  As many in another shape (slots first) are other pairs' weights.
+void need_weights(const at::Tensor& w, int64_t P, int64_t topk) {
+  GB_NEED(w.is_floating_point() && w.numel() == P, "one router weight for each of " + std::to_string(P) + " pairs expected");
+  GB_NEED(w.dim() == 1 || w.size(-1) == topk || w.size(-1) == 1, "router weights of shape [tokens, " + std::to_string(topk) + "] expected");
+}
+
 void sort_pairs(const at::Tensor& topk_ids, int64_t E, int64_t base, int32_t* counts, int32_t* offsets, int32_t* order, int32_t* place, void* stream) {
   const int64_t T = topk_ids.size(0), topk = topk_ids.size(1), P = T * topk;
   const bool wide = topk_ids.scalar_type() == at::kLong;
@@ -951,7 +957,7 @@ at::Tensor moe_fp8_blocks(const at::Tensor& x, const at::Tensor& w13, const at::
   GB_NEED(w2.size(0) == E && w2.size(1) == H && w13.size(1) == 2 * I, "w13 [E, 2 inter, hidden] and w2 [E, hidden, inter] expected");
   const int64_t P = check_ids(topk_ids, E, base), T = topk_ids.size(0), topk = topk_ids.size(1);
   GB_NEED(x.dim() >= 1 && x.size(-1) == H && x.numel() == T * H, std::to_string(T) + " tokens of " + std::to_string(H) + " values expected");
-  GB_NEED(topk_weights.is_floating_point() && topk_weights.numel() == P, "one router weight for each of " + std::to_string(P) + " pairs expected");
+  need_weights(topk_weights, P, topk);
   const c10::cuda::CUDAGuard guard(x.device());
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   at::Tensor out = fresh(x.sizes(), x.scalar_type(), x);
@@ -1103,13 +1109,15 @@ at::Tensor moe_permute(const at::Tensor& x, const at::Tensor& place, const at::T
 
 at::Tensor moe_unpermute(const at::Tensor& y, const at::Tensor& place, const at::Tensor& offsets, int64_t topk, const Opt& weights) {
   no_tangents({&y});
-  if (weights.has_value()) no_tangents({&*weights});
+  if (weights.has_value() && weights->defined()) {
+    no_tangents({&*weights});
+    need_weights(*weights, place.numel(), topk);
+  }
   need_cuda(y);
   dtype_code(y.scalar_type(), "moe_unpermute");
   at::Tensor w;
   if (weights.has_value() && weights->defined()) {
     same_device(y, {&*weights});
-    GB_NEED(weights->is_floating_point() && weights->numel() == place.numel(), "one weight for each of " + std::to_string(place.numel()) + " pairs expected");
     w = weights->to(at::kFloat).contiguous();
   }
   if (!(at::GradMode::is_enabled() && (y.requires_grad() || (w.defined() && w.requires_grad())))) return unpermute_rows(y, place, offsets, topk, w);
