@@ -12,7 +12,7 @@
 // (128 features a CTA, one scale per block for the whole tile), the rows the N side in steps of sixteen, K sliced alike.
 //
 // What bounds them.  Tiles: the tensor cores take 392 ns a slab of 256 x 256 x 128 with nothing to wait for (3.1 PFLOP/s); the
-// multiply-adds of the read-out (two warps of a scheduler, 256 clocks of its 700 a slab) and the power cap leave 2.3 - 2.5.  Rows: the
+// multiply-adds of the read-out (two warps of a scheduler, 256 clocks of its 700 a slab) and the power cap leave 2.4 in a graph and 2.1 over seconds.  Rows: the
 // bytes of the weights, up to some 64 rows; from there on the shared memory, through which every warp gets the rows' scales
 // at 128 bytes a clock beside the operands.
 #include "gb_blocks.cuh"
@@ -1404,8 +1404,9 @@ int gb_gemm_fp8_blocks_kernel(int64_t M, int64_t N, int64_t K, int32_t* slices) 
   return route;
 }
 
-// us, two launches / one: 1 row of 34816 x 5120 34.9 / 32.9, 4 rows 35.7 / 33.7, 8 rows 36.7 / 43.0; 4 rows of 4096 x 4096 10.3 / 8.4, 16 rows
-// 10.3 / 12.3: every CTA quantises all rows, four blocks at a time and warp.
+// us in a graph of many layers, two launches / one: 1 row of 34816 x 5120 30.8 / 28.9, 4 rows 30.7 / 29.1; 1 row of 4096 x 4096 7.9 / 6.1, 4 rows
+// 8.1 / 6.2.  Not more rows: every CTA quantises all of them (when one launch took them, 8 rows of 34816 x 5120 36.7 / 43.0, 16 rows of 4096 x 4096
+// 10.3 / 12.3).
 
 int gb_linear_fp8_blocks(const void* x, int dtype, int64_t ld, int scale_rule, const void* W, const float* w_scale, void* D, int out, int64_t M, int64_t N,
                          int64_t K, void* stream) {

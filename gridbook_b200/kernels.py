@@ -692,13 +692,14 @@ def moe_sort(topk_ids: torch.Tensor, E: int, *, expert_base: int = 0) -> MoESort
 
 def moe_permute(x: torch.Tensor, s: MoESort) -> torch.Tensor:
     """Token rows [T, H] (bf16, fp16 or fp32) in expert order: out[j] = x[order[j] // top-k], zero past offsets[E].
-    Differentiable in ``x``."""
+    Differentiable in ``x``, by backward passes alone."""
     return nat.host("routed row permutation").moe_permute(x, s.place, s.offsets, s.topk)
 
 
 def moe_unpermute(y: torch.Tensor, s: MoESort, weights: torch.Tensor | None = None) -> torch.Tensor:
     """Sorted rows back to their tokens: out[t] = sum over slots of weights[t, slot] * y[place[t, slot]], in fp32 and slot order,
-    rounded once; dropped pairs count nothing, ``weights`` None: ones.  Differentiable in ``y`` and ``weights``."""
+    rounded once; dropped pairs count nothing, ``weights`` ([.., top-k] or flat) None: ones.  Differentiable in ``y`` and
+    ``weights``, by backward passes alone."""
     return nat.host("routed row combination").moe_unpermute(y, s.place, s.offsets, s.topk, weights)
 
 
