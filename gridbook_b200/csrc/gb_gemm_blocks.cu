@@ -42,6 +42,7 @@ struct BlocksParams {
   int out_tma, out16;        // 16-bit rows of D that TMA takes; rows of D are whole 16-byte pieces
   const int32_t* seg;        // [E + 1], or null
   int E;
+  int most_row_tiles;        // grouped: of offsets that rise
   int beside;                // W, its scales and seg are not written by the launch ahead: read before it has finished
   uint32_t idesc;            // without M and N
   int* status;
@@ -265,7 +266,9 @@ GB_DEVINL void stage_piece(uint32_t chunk, int q, uint32_t a, uint32_t b, uint32
 }
 
 // Segment starts and the number of row tiles in front of each expert, into shared memory, by one warp: a lane takes consecutive
-// experts, so that their loads are in flight together.
+// experts, so that their loads are in flight together.  Offsets that fall and rise again make segments that overlap and more tiles: a lane's
+// stop at kManyTiles, which rising offsets never have, so that the sum fits, and row_tiles takes no more than those can have.
+constexpr int kManyTiles = 1 << 25;
 GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, int* base_s) {
   const int lane = threadIdx.x & 31, per = (p.E + 31) / 32, e0 = lane * per, e1 = min(p.E, e0 + per);
   int tiles = 0;
@@ -275,9 +278,10 @@ GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, i
     const int lo = min(max(p.seg[e], 0), (int)p.M), hi = min(max(p.seg[e + 1], lo), (int)p.M);
     seg_s[e] = lo;
     base_s[e] = tiles;
-    tiles += (hi - lo + tile_rows - 1) / tile_rows;
+    tiles += (hi - lo + tile_rows - 1) / tile_rows;        // below 2^28: 32 experts of fewer than 2^30 rows in tiles of 128, or of a few rows in smaller ones
     if (e == p.E - 1) seg_s[p.E] = hi;
   }
+  tiles = min(tiles, kManyTiles);
   int incl = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -287,6 +291,7 @@ GB_DEVINL void load_segments(const BlocksParams& p, int tile_rows, int* seg_s, i
   for (int e = e0; e < e1; ++e) base_s[e] += incl - tiles;
   if (lane == 31) base_s[p.E] = incl;
 }
+GB_DEVINL int row_tiles(const BlocksParams& p, const int* base_s) { return min(base_s[p.E], p.most_row_tiles); }
 
 // The expert whose row tiles hold tile `gp`: e or a later one; those without rows are stepped over, 32 at a time.  By a whole warp. (One
 // at a time, a load from shared memory each: 12.4 us instead of 10.0 for one token of eight of 128 experts, 39 instead of 12.4 of 1024.)
@@ -412,7 +417,7 @@ gemm_blocks_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   if constexpr (kCtas == 2) gb_cluster_sync();                           // both CTAs' barriers exist
   tmem_fence_after();
   const uint32_t tmem_base = *slot_ptr;
-  const int total = kGrouped ? base_s[p.E] * p.n_tiles : p.m_tiles * p.n_tiles;
+  const int total = kGrouped ? row_tiles(p, base_s) * p.n_tiles : p.m_tiles * p.n_tiles;
   const int stride = (int)gridDim.x / kCtas, first = (int)blockIdx.x / kCtas;
   // K slices, of single CTAs: a tile for every cluster along y
   const int slice = kCtas == 1 ? (int)blockIdx.y : 0, k_begin = kCtas == 1 ? slice * p.per_slice : 0;
@@ -766,7 +771,7 @@ gemm_blocks_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   tmem_fence_after();
   const uint32_t tmem = (uint32_t)uniform((int)slot_s);
   // sliced: one item per cluster; otherwise the CTA walks items
-  const int total = kGrouped ? base_s[p.E] * p.n_tiles : p.passes * p.n_tiles;
+  const int total = kGrouped ? row_tiles(p, base_s) * p.n_tiles : p.passes * p.n_tiles;
   const int slice = (int)blockIdx.y, k_begin = slice * p.per_slice, k_end = min(p.kb, k_begin + p.per_slice), k_n = k_end - k_begin;
   const int first = (int)blockIdx.x, stride = (int)gridDim.x;
 
@@ -1232,7 +1237,8 @@ int run_tiles(const void* A, const void* W, int64_t K, BlocksParams p, cudaStrea
     rc = gb_tensor_map_out(&map_d, p.D, p.M, p.N);
     if (rc != GB_OK) return rc;
   }
-  const int64_t tiles = (int64_t)(p.m_tiles + (kGrouped ? p.E : 0)) * p.n_tiles;      // grouped: at least as many as the routing can make
+  p.most_row_tiles = (int)(p.M / S::kM + (p.M < p.E ? p.M : p.E));
+  const int64_t tiles = (int64_t)(kGrouped ? p.most_row_tiles : p.m_tiles) * p.n_tiles;
   GB_REQUIRE(tiles < (1ll << 31), "too many output tiles");
   Slices slices = {1, p.kb};
   if (kCtas == 1 && !kGrouped) slices = slices_of(tiles, p.kb);
@@ -1269,8 +1275,8 @@ int run_rows(const void* A, const void* W, int64_t K, BlocksParams p, cudaStream
   p.n_tiles = (int)((p.N + kBM - 1) / kBM);
   int64_t most;                                            // items there can be
   if (kGrouped) {
-    const int64_t hit = p.M < p.E ? p.M : p.E;
-    most = (p.M / kR + hit) * p.n_tiles;
+    p.most_row_tiles = (int)(p.M / kR + (p.M < p.E ? p.M : p.E));
+    most = (int64_t)p.most_row_tiles * p.n_tiles;
   } else {
     p.passes = (int)((p.M + kR - 1) / kR);
     p.rows_per_pass = (int)(((p.M + p.passes - 1) / p.passes + 15) / 16 * 16);

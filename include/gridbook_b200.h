@@ -447,7 +447,8 @@ GB_API int gb_moe_permute_fp8(const void* x, int dtype, int64_t ld, const int32_
  * inner sums in fp32 on the tensor cores, the outer in fp32 registers, one rounding to `out` (GB_DTYPE_*).
  * K a multiple of 16, operands and D 16-byte aligned.  Grouped: A [P, K] rows sorted by expert (expert e
  * owns seg_offsets[e] .. seg_offsets[e + 1]), W [E, N, K], w_scale [E, ceil(N/128), ceil(K/128)], E <= 1024;
- * rows of D from seg_offsets[E] on are left as they are.  Offsets are taken within [0, P].
+ * rows of D from seg_offsets[E] on are left as they are.  Offsets are taken within [0, P].  Where they fall,
+ * segments overlap: which of them writes a row, or none, is open, nothing else is touched.
  * beside: W, its scales and seg_offsets are not written by the launch right ahead on the stream, and that
  * launch lets this one start only behind its own wait (the quantisers above do): W is then fetched while
  * that launch still runs.  0 is always right. */
