@@ -30,6 +30,9 @@ REQUIRED_SYMBOLS = (
     "gb_moe_route_inv", "gb_moe_fp4_pass_rows", "gb_moe_fp4_operand_bytes", "gb_moe_fp4_rows", "gb_moe_fp4_swiglu_rows", "gb_moe_gemv_fp4", "gb_moe_gemm_fp4",
     "gb_fp8_quantize_blocks", "gb_moe_swiglu_fp8", "gb_moe_permute_fp8", "gb_gemm_fp8_blocks", "gb_gemm_fp8_blocks_grouped", "gb_linear_fp8_blocks", "gb_gemm_fp8_blocks_kernel",
     "gb_moe_sort", "gb_moe_sort_applies", "gb_moe_permute", "gb_moe_unpermute", "gb_moe_unpermute_grad",
+    "gb_moe_topk", "gb_moe_topk_grad", "gb_moe_balance_workspace_bytes", "gb_moe_balance", "gb_moe_balance_grad",
+    "gb_residual_norm", "gb_residual_norm_fp8", "gb_residual_norm_grad_workspace_bytes", "gb_residual_norm_grad",
+    "gb_linear_act", "gb_linear_act_grad_workspace_bytes", "gb_linear_act_grad",
     "gb_peer_alloc", "gb_peer_free", "gb_peer_export", "gb_peer_open", "gb_peer_close",
     "gb_peer_allgather", "gb_peer_allgather_ll", "gb_peer_barrier", "gb_launch_count", "gb_gemv_allgather", "gb_moe_combine_peer",
 )
@@ -41,6 +44,7 @@ MODE_PRODUCT, MODE_SIGNED, MODE_FULL = 0, 1, 2
 SCALE_NONE, SCALE_V1, SCALE_V2 = 0, 1, 2
 SCALE_RULE_RECIP, SCALE_RULE_DIV = 0, 1
 ACT_NONE, ACT_FP4_GROUP16, ACT_FP8_TOKEN = 0, 1, 2
+EPI_NONE, EPI_RELU, EPI_GELU, EPI_GELU_TANH, EPI_SILU = 0, 1, 2, 3, 4
 
 
 class NativeKernelUnavailableError(RuntimeError):
@@ -86,6 +90,20 @@ class GbGatherLayout(ctypes.Structure):
 
 class GbPeerRows(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p * 8), ("rows_per_rank", ctypes.c_int64)]
+
+
+class GbResidualNorm(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int64), ("H", ctypes.c_int64),
+                *((name, ctypes.c_void_p) for name in ("y", "r", "gate", "w", "pw")),
+                *((name, ctypes.c_int64) for name in ("y_ld", "r_ld", "gate_ld", "gate_rows")),
+                *((name, ctypes.c_int32) for name in ("dtype", "stream_dtype", "w_dtype", "pw_dtype")),
+                *((name, ctypes.c_float) for name in ("residual_scale", "branch_scale", "eps", "weight_offset"))]
+
+
+class GbResidualNormGrads(ctypes.Structure):
+    _fields_ = [*((name, ctypes.c_void_p) for name in ("stream", "rstd", "post_rstd", "d_h", "d_stream")),
+                ("d_h_ld", ctypes.c_int64), ("d_stream_ld", ctypes.c_int64),
+                *((name, ctypes.c_void_p) for name in ("d_y", "d_r", "d_w", "d_pw", "d_gate"))]
 
 
 _LOCK = threading.Lock()
@@ -168,6 +186,23 @@ def _declare(lib) -> None:
     lib.gb_moe_permute.argtypes = [vp, i64, i64, vp, vp, i64, i64, i64, vp, vp]
     lib.gb_moe_unpermute.argtypes = [vp, i32, vp, vp, i64, i64, i64, vp, vp]
     lib.gb_moe_unpermute_grad.argtypes = [vp, vp, i32, vp, vp, vp, i64, i64, i64, vp, vp, vp]
+    f32 = ctypes.c_float
+    lib.gb_moe_topk.argtypes = [vp, i32, i64, i64, i64, i64, i32, i32, f32, vp, vp, vp]
+    lib.gb_moe_topk_grad.argtypes = [vp, i32, i64, vp, vp, i64, i64, i64, i32, i32, f32, vp, vp]
+    lib.gb_moe_balance_workspace_bytes.argtypes = [i64, i64]
+    lib.gb_moe_balance_workspace_bytes.restype = i64
+    lib.gb_moe_balance.argtypes = [vp, i32, i64, vp, i32, vp, i64, i64, i64, f32, f32, vp, vp, vp, vp, i64, vp]
+    lib.gb_moe_balance_grad.argtypes = [vp, i32, i64, vp, vp, vp, i64, i64, f32, f32, vp, vp]
+    norm, grads = ctypes.POINTER(GbResidualNorm), ctypes.POINTER(GbResidualNormGrads)
+    lib.gb_residual_norm.argtypes = [norm, vp, vp, vp, vp, vp]
+    lib.gb_residual_norm_fp8.argtypes = [norm, i32, vp, vp, vp, vp]
+    lib.gb_residual_norm_grad_workspace_bytes.argtypes = [norm, grads]
+    lib.gb_residual_norm_grad_workspace_bytes.restype = i64
+    lib.gb_residual_norm_grad.argtypes = [norm, grads, vp, i64, vp]
+    lib.gb_linear_act.argtypes = [vp, i64, vp, vp, vp, i64, i32, i64, i64, i64, i32, vp, vp, vp]
+    lib.gb_linear_act_grad_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32, i32, i32]
+    lib.gb_linear_act_grad_workspace_bytes.restype = i64
+    lib.gb_linear_act_grad.argtypes = [vp, i64, vp, vp, i64, vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp]
     lib.gb_launch_count.restype = i64
     lib.gb_peer_alloc.argtypes = [i64, ctypes.POINTER(vp)]
     lib.gb_peer_free.argtypes = [vp]

@@ -85,6 +85,11 @@ unsigned long long gb_wait_limit_ns();
 // Swizzled (128-byte) operand map over a row-major [rows, K] matrix of 2- or 1-byte elements:
 // box = 128 bytes of K x box_rows rows, rows past the end read zero.
 int gb_tensor_map_operand(void* map_out, const void* base, int64_t rows, int64_t K, int elem_bytes, int box_rows);
+// Row-major 16-bit matrix with rows `ld` elements apart (a multiple of eight) in boxes of box_cols x box_rows with the 128- or 64-byte
+// swizzle, zeros outside of it.
+int gb_tensor_map_rows16(void* map_out, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_cols, int box_rows, int swizzle_bytes);
+// out[c] = sum of part[s][c] over the shares, in a fixed order, as GB_DTYPE_* (gb_norm.cu).
+int gb_join_columns(const float* part, int64_t shares, int64_t columns, void* out, int dtype, cudaStream_t stream);
 // Row-major bf16 output [M, N] in boxes of 32 x 32 with the 64-byte swizzle (N a multiple of 8).
 int gb_tensor_map_out(void* map_out, void* base, int64_t M, int64_t N);
 // Activation operand of the grouped GEMM (gb_moe_gemm_fp4): tiles of 64 rows, [tile][64 code rows of q, 64 of the

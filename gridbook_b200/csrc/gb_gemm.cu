@@ -446,6 +446,13 @@ int gb_tensor_map_out(void* map_out, void* base, int64_t M, int64_t N) {
                      CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
+// 16-bit rows `ld` elements apart, in swizzled boxes.
+int gb_tensor_map_rows16(void* map_out, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_cols, int box_rows, int swizzle_bytes) {
+  return encode_rows(map_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, const_cast<void*>(base), (uint64_t)cols, (uint64_t)rows, (uint64_t)ld * 2,
+                     (uint32_t)box_cols, (uint32_t)box_rows, swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                     swizzle_bytes == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE);
+}
+
 int gb_prepare_gemm() {
   GB_CUDA_OK(cudaFuncSetAttribute((const void*)gemm_tn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   kGemmSmem + kGroupSmem));

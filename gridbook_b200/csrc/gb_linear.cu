@@ -1,0 +1,1105 @@
+// 16-bit linears with their epilogue, and the products of their backward pass.
+//
+//     z = X W^T + bias,   Y = act(z) + R        X [M, K], W [N, K], bias [N], R and Y [M, N], bf16 or fp16, sums in fp32
+//     dz = dY act'(z),  dX = dz W,  dW = dz^T X,  dbias = sum over rows of dz,  dR = dY
+//
+// Everything behind the product happens on the accumulators in fp32 before the one rounding to the output's type.  For the backward
+// pass the forward pass also stores z, rounded to the output's type: act' is taken at the rounded z, which adds half a step of it
+// times act'' to dz, less than dz's own rounding for the tensor cores does.
+//
+// Two kernels, as the other prefill GEMMs have them:
+//   linear_pair_kernel   256 x 256, 192 or 128 tiles on CTA pairs (cta_group::2), two accumulators, so that a tile's epilogue runs under
+//                        the next tile's MMAs.  The residual's tile comes by TMA into the buffers that the output leaves from, while
+//                        the MMAs run.
+//   linear_rows_kernel   128 weight rows times up to 256 activation rows on one CTA, K sliced over a cluster: few rows, narrow layers.
+// The backward products read the same matrices where they lie, along their other axis: an operand whose rows run along the
+// contraction is the tensor core's MN-major form, tiles of 64 columns x 64 rows with the 128-byte swizzle, so that nothing
+// is transposed in memory.  dW's contraction runs over M: where its tiles are fewer than the pairs, M is split and the slices' fp32 sums
+// are added by a second launch in their order.
+#include "gb_blocks.cuh"
+
+#include <cuda.h>
+#include <atomic>
+#include <mutex>
+
+namespace {
+
+using namespace gb_blocks;
+
+constexpr int kSlab = 64;                            // contraction elements of a stage: 128 bytes
+constexpr int kSlabBytes = 128;
+constexpr int kBM = 128;                             // rows of D that a CTA has
+constexpr int kEpiWarps = 8;
+constexpr uint32_t kTmemCols = 512;
+
+// ------------------------------------------------------------------------------------------------ waits, loads, MMAs
+template <bool kOfPair>
+GB_DEVINL bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  if (kOfPair)
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// A bounded wait that remembers a timeout for the rest of the CTA: later waits return at once.
+template <bool kOfPair>
+__device__ __noinline__ void wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 0; !*abort_flag; ++spin) {
+    if (try_wait<kOfPair>(bar, parity)) return;
+    if ((spin & 255u) == 255u) {
+      const uint64_t now = gb_globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 2000000000ull) { *abort_flag = 1; atomicExch(status, code); }
+    }
+  }
+}
+// By a whole warp that goes on together; false: given up.
+template <bool kOfPair = false>
+GB_DEVINL bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, try_wait<kOfPair>(bar, parity))) return true;
+  wait_slow<kOfPair>(bar, parity, abort_flag, status, code);
+  return !__any_sync(0xffffffffu, *abort_flag != 0);
+}
+GB_DEVINL int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+GB_DEVINL void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+GB_DEVINL void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+GB_DEVINL uint32_t leader_addr(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+// What the pair of arrive and wait hands over is tensor memory alone, ordered by its own fences: the arrive may be relaxed.
+GB_DEVINL void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+GB_DEVINL void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+// Into this CTA's shared memory, reported to a barrier of the pair.
+GB_DEVINL void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+GB_DEVINL void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(src) : "memory");
+}
+// An operand in shared memory, 128-byte swizzle.  K-major: rows of 128 bytes along the contraction, sixteen elements of it 32 bytes on.
+// MN-major: 64 x 64 tiles of 8 KiB, their rows along M or N; sixteen rows of the contraction 2048 bytes on.
+template <bool kMn>
+GB_DEVINL uint64_t desc_of(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (kMn ? (uint64_t)(8192u >> 4) << 16 : 0ull) | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <bool kMn>
+constexpr uint64_t kStep = kMn ? 2048 >> 4 : 32 >> 4;
+template <int kCtas>
+GB_DEVINL void mma_16bit(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
+  if (kCtas == 2)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+template <int kCtas>
+GB_DEVINL void commit_to(uint32_t bar) {
+  if (kCtas == 2) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+GB_DEVINL void tmem_ld32(uint32_t taddr, float (&f)[32]) {
+  uint32_t v[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+}
+GB_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr));
+}
+
+// ------------------------------------------------------------------------------------------------ elements
+GB_DEVINL float to_f(uint32_t half_word, int fp16) {
+  return fp16 ? __half2float(__ushort_as_half((uint16_t)half_word)) : gb_bf16_bits_to_f32(half_word & 0xFFFFu);
+}
+GB_DEVINL uint32_t pack2(float a, float b, int fp16) {
+  if (!fp16) return gb_pack_bf16x2(a, b);
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+GB_DEVINL uint16_t pack1(float a, int fp16) { return fp16 ? __half_as_ushort(__float2half_rn(a)) : (uint16_t)gb_f32_to_bf16_bits(a); }
+// v / (1 + e^-t): sigmoid-weighted; both functions are off by a few units in the last place of fp32, far below the output's.
+GB_DEVINL float weighted(float v, float t) { return __fdividef(v, 1.0f + __expf(-t)); }
+constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.044715f;      // 2 sqrt(2 / pi): (1 + tanh(u)) / 2 is the sigmoid of 2 u
+
+template <int kN>
+GB_DEVINL void activate(float (&v)[kN], int act) {
+  switch (act) {
+    case GB_EPI_RELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+      break;
+    case GB_EPI_GELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
+      break;
+    case GB_EPI_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = weighted(v[i], kTanhA * fmaf(kTanhB * v[i] * v[i], v[i], v[i]));
+      break;
+    case GB_EPI_SILU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = weighted(v[i], v[i]);
+      break;
+    default: break;
+  }
+}
+GB_DEVINL float slope(float z, int act) {
+  switch (act) {
+    case GB_EPI_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case GB_EPI_GELU: return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    case GB_EPI_GELU_TANH: {
+      const float c = fminf(fmaxf(z, -16.0f), 16.0f), s = 1.0f / (1.0f + expf(-kTanhA * fmaf(kTanhB * c * c, c, c)));   // constant past these
+      return z != z ? z : fmaf(kTanhA * c * s * (1.0f - s), fmaf(3.0f * kTanhB * c, c, 1.0f), s);
+    }
+    case GB_EPI_SILU: {
+      const float s = 1.0f / (1.0f + expf(-z));
+      return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    default: return 1.0f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ CTA pairs
+enum Major { kForward = 0, kRowsGrad = 1, kWeightGrad = 2 };   // which operands are MN-major: none, B, both
+enum Epilogue { kPlain = 0, kResidual = 1, kKeepZ = 2 };       // kKeepZ: z is stored too, with or without a residual
+
+constexpr int kPairM = 256;
+constexpr int kChunk = 2048;                         // 32 rows x 32 columns on their way out
+constexpr int kGroupM = 16;                          // row tiles walked together before the next columns
+
+template <Major kMajor, int kBN, int kEpi>
+struct Shape {
+  static constexpr bool kAmn = kMajor == kWeightGrad, kBmn = kMajor != kForward;
+  static constexpr int kABytes = kBM * kSlabBytes, kBBytes = kBN / 2 * kSlabBytes, kStageBytes = kABytes + kBBytes;
+  static constexpr int kCols = kBN / 2, kChunks = kCols / 32;                       // of an epilogue warp
+  static constexpr int kOut = kEpi == kPlain ? 2 : kChunks, kZ = kEpi == kKeepZ ? 2 : 0;
+  static constexpr int kOutBytes = kEpiWarps * (kOut + kZ) * kChunk;
+  static constexpr int kFixed = 1024 + kEpiWarps * kCols * 4 + 512;                 // alignment, bias, barriers
+  static constexpr int kFit = (227 * 1024 - kFixed - kOutBytes) / kStageBytes, kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + kFixed;
+};
+
+struct LinearParams {
+  int64_t M, N;                // of D
+  int k_tiles, m_tiles, n_tiles, slices, per_slice;
+  uint32_t idesc;
+  int fp16, act, tma;          // tma: rows of D, z and the residual come in whole 16-byte pieces
+  const uint16_t *bias, *r;
+  int64_t r_ld;
+  uint16_t *d, *z;
+  float* sums;                 // [slice][M][N] where slices > 1
+  int* status;
+  // few rows
+  int rows_per_pass, box_rows, stages;
+};
+
+GB_DEVINL void tile_at(const LinearParams& p, int tile, int& mt, int& nt) {
+  const int per = kGroupM * p.n_tiles, g = tile / per, in = tile - g * per;
+  const int rows = min(kGroupM, p.m_tiles - g * kGroupM);
+  mt = g * kGroupM + in % rows;
+  nt = in / rows;
+}
+
+constexpr int kPairThreads = 32 * (kEpiWarps + 2);
+
+template <Major kMajor, int kBN, int kEpi>
+__global__ void __launch_bounds__(kPairThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
+                   const __grid_constant__ CUtensorMap map_z, const __grid_constant__ CUtensorMap map_r, const __grid_constant__ LinearParams p) {
+  using S = Shape<kMajor, kBN, kEpi>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
+  uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
+  const uint32_t out_ring = ring + kStages * S::kStageBytes;             // per epilogue warp
+  const uint32_t bias_at = out_ring + S::kOutBytes;                      // [warp][columns] fp32
+  const uint32_t full_bar = bias_at + kEpiWarps * S::kCols * 4;          // leader: both CTAs' operand tiles have landed
+  const uint32_t empty_bar = full_bar + 8 * kStages;                     // the MMAs that read the stage are done
+  const uint32_t acc_full = empty_bar + 8 * kStages;                     // [2] accumulator complete
+  const uint32_t acc_empty = acc_full + 16;                              // [2] leader: drained by both CTAs
+  const uint32_t r_full = acc_empty + 16;                                // [epilogue warp] its part of the residual has landed
+  const uint32_t slot = r_full + 8 * kEpiWarps;
+  volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(ring_ptr + (slot - ring));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  gb_pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(full_bar + 8 * s, 1);
+      bar_init(empty_bar + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      bar_init(acc_full + 8 * b, 1);
+      bar_init(acc_empty + 8 * b, 2 * kEpiWarps);
+    }
+    for (int w = 0; w < kEpiWarps; ++w) bar_init(r_full + 8 * w, 1);
+    *abort_flag = 0;
+    gb_fence_barrier_init();
+  }
+  if (warp == kEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  gb_cluster_sync();                                                     // both CTAs' barriers exist
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *slot_ptr;
+  gb_pdl_wait();
+
+  const int per_tile = p.m_tiles * p.n_tiles, total_tiles = per_tile * p.slices;
+  const int stride = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
+
+  if (warp == kEpiWarps) {
+    // ------------------------------- producer (each CTA) -------------------------------
+    const uint32_t full_pair = (uint32_t)uniform((int)leader_addr(full_bar));
+    const int me = uniform((int)rank);
+    const bool one = gb_elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int tile = first; ok && tile < total_tiles; tile += stride) {
+      const int slice = tile / per_tile;
+      int mt, nt;
+      tile_at(p, tile - slice * per_tile, mt, nt);
+      const int m0 = uniform(mt * kPairM) + me * kBM, n0 = uniform(nt * kBN) + me * (kBN / 2);
+      const int k_end = min(p.k_tiles, (slice + 1) * p.per_slice);
+      for (int kt = slice * p.per_slice; kt < k_end; ++kt) {
+        ok = warp_wait<true>(empty_bar + 8 * s, ph, abort_flag, p.status, 101);
+        if (!ok) break;
+        if (one) {
+          const uint32_t st = ring + (uint32_t)s * S::kStageBytes, bar = full_pair + 8 * s;
+          if (me == 0) expect_tx(full_bar + 8 * s, 2 * S::kStageBytes);
+          if (S::kAmn) {
+#pragma unroll
+            for (int i = 0; i < kBM / 64; ++i) tma_load_pair(st + 8192 * i, &map_a, m0 + 64 * i, kt * kSlab, bar);
+          } else {
+            tma_load_pair(st, &map_a, kt * kSlab, m0, bar);
+          }
+          if (S::kBmn) {
+#pragma unroll
+            for (int i = 0; i < kBN / 128; ++i) tma_load_pair(st + S::kABytes + 8192 * i, &map_b, n0 + 64 * i, kt * kSlab, bar);
+          } else {
+            tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, n0, bar);
+          }
+        }
+        __syncwarp();
+        if (++s == kStages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // --------------------------- MMA issuer (the leader's) ------------------------------
+    if (uniform((int)rank) == 0) {
+      uint32_t to_peer;                                      // distance of the peer's barriers
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
+      to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
+      const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
+      const bool one = gb_elect_one();
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total_tiles; tile += stride, ++it) {
+        const int buf = it & 1, slice = tile / per_tile, k_begin = slice * p.per_slice, k_end = min(p.k_tiles, k_begin + p.per_slice);
+        ok = warp_wait<true>(acc_empty + 8 * buf, ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, p.status, 102);   // its last tile is drained
+        if (!ok) break;
+        const uint32_t acc = tmem + (buf ? 256u : 0u);
+        for (int kt = k_begin; kt < k_end; ++kt) {
+          ok = warp_wait(full_bar + 8 * s, ph, abort_flag, p.status, 103);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
+          const uint64_t da = desc_of<S::kAmn>(st), db = desc_of<S::kBmn>(st + S::kABytes);
+          if (one) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_16bit<2>(acc, da + kStep<S::kAmn> * k, db + kStep<S::kBmn> * k, p.idesc, kt > k_begin || k > 0);
+            commit_to<2>(empty_bar + 8 * s);
+            commit_to<2>(empty_bar + to_peer + 8 * s);
+          }
+          __syncwarp();
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+        if (ok && one) {
+          commit_to<2>(acc_full + 8 * buf);
+          commit_to<2>(acc_full + to_peer + 8 * buf);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------- epilogue (each CTA) --------------------------------
+    // Lane = row, 32 columns at a time, out through shared memory (64-byte swizzle), a TMA store each.
+    const uint32_t acc_empty_pair = leader_addr(acc_empty);
+    const int quarter = warp & 3, c_lo = (warp >> 2) * S::kCols;
+    const uint32_t out = out_ring + (uint32_t)warp * (S::kOut + S::kZ) * kChunk, z_out = out + S::kOut * kChunk;
+    const uint32_t bias_s = bias_at + (uint32_t)warp * S::kCols * 4, r_bar = r_full + 8 * warp;
+    const bool staged = p.tma && p.slices == 1, residual = kEpi != kPlain && p.r != nullptr;
+    const auto fetch_residual = [&](int tile) {              // a tile's part, by lane 0
+      int mt, nt;
+      tile_at(p, tile, mt, nt);
+      expect_tx(r_bar, S::kChunks * kChunk);
+      for (int c = 0; c < S::kChunks; ++c)
+        tma_load_2d(out + c * kChunk, &map_r, nt * kBN + c_lo + 32 * c, mt * kPairM + (int)rank * kBM + quarter * 32, r_bar);
+    };
+    if (residual && staged && lane == 0 && first < total_tiles) fetch_residual(first);
+    int it = 0, flip = 0;
+    for (int tile = first; tile < total_tiles; tile += stride, ++it) {
+      const int slice = tile / per_tile, buf = it & 1;
+      int mt, nt;
+      tile_at(p, tile - slice * per_tile, mt, nt);
+      const int n0 = nt * kBN + c_lo, row0 = mt * kPairM + (int)rank * kBM + quarter * 32, row = row0 + lane;
+      if (kMajor == kForward) {                              // the columns' biases, zeros past the last
+        __syncwarp();
+        for (int c = lane; c < S::kCols; c += 32) {
+          const float b = p.bias && n0 + c < p.N ? to_f(p.bias[n0 + c], p.fp16) : 0.0f;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_s + 4u * c), "f"(b) : "memory");
+        }
+        __syncwarp();
+      }
+      if (!warp_wait<true>(acc_full + 8 * buf, (uint32_t)(it >> 1) & 1, abort_flag, p.status, 104)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (residual && staged && !warp_wait(r_bar, (uint32_t)it & 1, abort_flag, p.status, 105)) break;
+      const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (buf ? 256u : 0u) + (uint32_t)c_lo;
+#pragma unroll 1
+      for (int c = 0; c < S::kChunks; ++c) {
+        float v[32];
+        tmem_ld32(at + 32u * c, v);
+        if (c == S::kChunks - 1) {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_cluster(acc_empty_pair + 8 * buf);
+        }
+        const int col = n0 + 32 * c;
+        if (kMajor != kForward && p.slices > 1) {
+          float* to = p.sums + ((int64_t)slice * p.M + row) * p.N + col;
+          if (row < p.M) {
+            if (p.N % 4 == 0) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                if (col + i < p.N) *reinterpret_cast<float4*>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col + i < p.N) to[i] = v[i];
+            }
+          }
+          continue;
+        }
+        if (kMajor == kForward) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float b[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3]) : "r"(bias_s + 128u * c + 4u * i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] += b[j];
+          }
+        }
+        const uint32_t row_at = (uint32_t)lane * 64u, swz = (uint32_t)((lane >> 1) & 3);
+        const auto put = [&](uint32_t dst, const float (&f)[32]) {     // eight rows touch eight bank groups
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)), "r"(pack2(f[8 * q], f[8 * q + 1], p.fp16)),
+                           "r"(pack2(f[8 * q + 2], f[8 * q + 3], p.fp16)), "r"(pack2(f[8 * q + 4], f[8 * q + 5], p.fp16)),
+                           "r"(pack2(f[8 * q + 6], f[8 * q + 7], p.fp16)) : "memory");
+        };
+        const auto send = [&](const CUtensorMap* map, uint32_t src) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && row0 < p.M && col < p.N) tma_store_2d(map, col, row0, src);   // what sticks out is not written
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        };
+        if (staged) {
+          uint32_t dst = out + (uint32_t)c * kChunk;
+          if (kEpi == kPlain) {
+            dst = out + (uint32_t)flip * kChunk;             // in turn across tiles: their chunks may be odd in number
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          } else if (kEpi == kKeepZ) {                       // the z before last, and with it the y before that, have left their buffers
+            asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
+          }
+          __syncwarp();
+          if (kEpi == kKeepZ) {
+            put(z_out + (uint32_t)flip * kChunk, v);
+            send(&map_z, z_out + (uint32_t)flip * kChunk);
+          }
+          flip ^= 1;
+          activate(v, p.act);
+          if (residual) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[8 * q + 2 * j] += to_f(w[j] & 0xFFFFu, p.fp16);
+                v[8 * q + 2 * j + 1] += to_f(w[j] >> 16, p.fp16);
+              }
+            }
+          }
+          put(dst, v);
+          send(&map_d, dst);
+        } else if (row < p.M) {
+          if (kEpi == kKeepZ) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (col + i < p.N) p.z[(int64_t)row * p.N + col + i] = pack1(v[i], p.fp16);
+          }
+          activate(v, p.act);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col + i < p.N)
+              p.d[(int64_t)row * p.N + col + i] = pack1(residual ? v[i] + to_f(p.r[(int64_t)row * p.r_ld + col + i], p.fp16) : v[i], p.fp16);
+        }
+      }
+      if (residual && staged && tile + stride < total_tiles) {           // the next tile's residual, once the output has left its buffers
+        if (lane == 0) {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          fetch_residual(tile + stride);
+        }
+        __syncwarp();
+      }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*abort_flag) __nanosleep(1000000);                   // loads and MMAs still in flight end before the memory goes
+  gb_cluster_sync();                                       // the peer may still signal barriers here
+  if (warp == kEpiWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// D[m, n] = sum over k of X[m, k] W[n, k]; kWmn: W's rows run along n (the rows' gradient, whose contraction is over the layer's
+// outputs).
+constexpr int kMaxRows = 256, kMaxStages = 8, kMaxSlices = 8;
+constexpr int kRowsSmem = 224 * 1024;
+constexpr int kRowsThreads = 32 * (kEpiWarps + 2);
+
+template <bool kWmn>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+linear_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_s[kMaxStages], empty_s[kMaxStages], acc_s;
+  __shared__ uint32_t slot_s;
+  __shared__ volatile int abort_s;
+  const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of a cluster
+  const uint32_t full_bar = gb_smem_u32(full_s), empty_bar = gb_smem_u32(empty_s), acc_bar = gb_smem_u32(&acc_s);
+  const uint32_t x_bytes = (uint32_t)p.box_rows * kSlabBytes, stage_bytes = kBM * kSlabBytes + x_bytes;
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int pass = (int)blockIdx.x / p.n_tiles, tile = (int)blockIdx.x - pass * p.n_tiles, slice = (int)blockIdx.y;
+  const int n0 = tile * kBM, m0 = pass * p.rows_per_pass;
+  const int rows = (int)min((int64_t)p.rows_per_pass, p.M - m0), cols = (rows + 15) / 16 * 16;
+  const int k_begin = slice * p.per_slice, k_end = min(p.k_tiles, k_begin + p.per_slice);
+
+  gb_pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      gb_mbar_init(&full_s[s], 1);
+      gb_mbar_init(&empty_s[s], 1);
+    }
+    gb_mbar_init(&acc_s, 1);
+    abort_s = 0;
+    gb_fence_barrier_init();
+  }
+  if (warp == kEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gb_smem_u32(&slot_s)), "r"(kTmemCols / 2) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, slot_s, 0);
+  gb_pdl_wait();
+
+  if (warp == kEpiWarps) {
+    // ------------------------------- producer -----------------------------------
+    const bool one = gb_elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    for (int kt = k_begin; kt < k_end; ++kt) {
+      if (!warp_wait(empty_bar + 8 * s, ph, &abort_s, p.status, 111)) break;
+      if (one) {
+        const uint32_t st = ring + (uint32_t)s * stage_bytes, bar = full_bar + 8 * s;
+        expect_tx(bar, stage_bytes);
+        if (kWmn) {
+#pragma unroll
+          for (int i = 0; i < kBM / 64; ++i) tma_load_2d(st + 8192 * i, &map_w, n0 + 64 * i, kt * kSlab, bar);
+        } else {
+          tma_load_2d(st, &map_w, kt * kSlab, n0, bar);
+        }
+        tma_load_2d(st + kBM * kSlabBytes, &map_x, kt * kSlab, m0, bar);
+      }
+      __syncwarp();
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // ------------------------------- MMA issuer ---------------------------------
+    const bool one = gb_elect_one();
+    const uint32_t idesc = p.idesc | (uint32_t)(cols >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int kt = k_begin; kt < k_end; ++kt) {
+      ok = warp_wait(full_bar + 8 * s, ph, &abort_s, p.status, 112);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (one) {
+        const uint32_t st = ring + (uint32_t)s * stage_bytes;
+        const uint64_t dw = desc_of<kWmn>(st), dx = desc_of<false>(st + kBM * kSlabBytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_16bit<1>(tmem, dw + kStep<kWmn> * k, dx + kStep<false> * k, idesc, kt > k_begin || k > 0);
+        commit_to<1>(empty_bar + 8 * s);
+      }
+      __syncwarp();
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+    if (ok && one) commit_to<1>(acc_bar);
+    __syncwarp();
+  } else {
+    if (!warp_wait(acc_bar, 0, &abort_s, p.status, 113)) abort_s = 1;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // All eight warps see the same flag behind it: the wait may run out in one and end in another, and they meet at barriers below.
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+  }
+
+  // Sums into the shared memory of the CTA that owns the activation row, [slice][own row][feature], over the operand ring: every CTA of
+  // the cluster has finished its MMAs, and with them its loads.  Rows are owned in sixteens.
+  const bool live = warp < kEpiWarps && !abort_s;
+  const int quarter = warp & 3, feature = quarter * 32 + lane;
+  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+  const int own = (cols / 16 + p.slices - 1) / p.slices * 16;
+  if (p.slices > 1) gb_cluster_sync();
+  if (live) {
+    for (int c = (warp >> 2) * 16; c < cols; c += 32) {
+      uint32_t v[16];
+      tmem_ld16(acc + (uint32_t)c, v);
+      const int to = c / own, at = c - to * own;
+      uint32_t dst = ring + (uint32_t)((slice * own + at) * kBM + feature) * 4u;
+      if (p.slices > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(dst), "r"(to));
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (p.slices > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)                         // rows past the last are sums of zeros
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + (uint32_t)i * kBM * 4u), "r"(v[i]) : "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + (uint32_t)i * kBM * 4u), "r"(v[i]) : "memory");
+      }
+    }
+  }
+  if (p.slices > 1) gb_cluster_sync();                       // the last access to another CTA's memory lies in front of it
+  else __syncthreads();
+  if (live) {
+    const int f = lane * 4, left = (int)min((int64_t)kBM, p.N - n0) - f;
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = p.bias && i < left ? to_f(p.bias[n0 + f + i], p.fp16) : 0.0f;
+    const int last = min(own, rows - slice * own);
+    for (int r = warp; r < last; r += kEpiWarps) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = 0.0f;
+#pragma unroll 4
+      for (int q = 0; q < p.slices; ++q) {
+        float u[4];
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(u[0]), "=f"(u[1]), "=f"(u[2]), "=f"(u[3]) : "r"(ring + (uint32_t)((q * own + r) * kBM + f) * 4u));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += u[i];
+      }
+      if (left <= 0) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += bias[i];
+      const int64_t m = m0 + slice * own + r, at = m * p.N + n0 + f;
+      if (p.tma) {
+        if (p.z) *reinterpret_cast<uint2*>(p.z + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
+        activate(v, p.act);
+        if (p.r) {
+          const uint2 w = *reinterpret_cast<const uint2*>(p.r + m * p.r_ld + n0 + f);
+          v[0] += to_f(w.x & 0xFFFFu, p.fp16); v[1] += to_f(w.x >> 16, p.fp16);
+          v[2] += to_f(w.y & 0xFFFFu, p.fp16); v[3] += to_f(w.y >> 16, p.fp16);
+        }
+        *reinterpret_cast<uint2*>(p.d + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
+      } else {
+        if (p.z) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < left) p.z[at + i] = pack1(v[i], p.fp16);
+        }
+        activate(v, p.act);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < left) p.d[at + i] = pack1(p.r ? v[i] + to_f(p.r[m * p.r_ld + n0 + f + i], p.fp16) : v[i], p.fp16);
+      }
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (abort_s) __nanosleep(1000000);                       // loads and MMAs still in flight end before the memory goes
+  if (warp == kEpiWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols / 2) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ elementwise parts of the backward pass
+struct DzParams {
+  const uint16_t *dy, *z;
+  uint16_t* dz;               // or null: only the column sums
+  int64_t M, N, dy_ld, dz_ld;
+  int fp16, act;
+  float* part;                // [blocks along M][N] column sums, or null
+};
+constexpr int kDzThreads = 256, kDzCols = 256;
+
+// A warp takes a row of 256 columns, a lane eight of them; a block's warps add their column sums up in their order.
+template <bool kVec>
+__global__ void __launch_bounds__(kDzThreads)
+linear_dz_kernel(const __grid_constant__ DzParams p) {
+  __shared__ float s[kDzThreads / 32][kDzCols];
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * kDzCols + lane * 8;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+  for (int64_t m = (int64_t)blockIdx.y * (kDzThreads / 32) + warp; m < p.M; m += (int64_t)gridDim.y * (kDzThreads / 32)) {
+    const uint16_t *dy = p.dy + m * p.dy_ld + c, *z = p.z ? p.z + m * p.N + c : nullptr;
+    uint32_t g[4] = {}, w[4] = {};
+    if (kVec) {
+      if (c < p.N) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(dy));
+        g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+        if (z) { const uint4 b = __ldg(reinterpret_cast<const uint4*>(z)); w[0] = b.x; w[1] = b.y; w[2] = b.z; w[3] = b.w; }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < p.N) {
+          g[i >> 1] |= (uint32_t)dy[i] << (16 * (i & 1));
+          if (z) w[i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
+        }
+    }
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      d[i] = to_f(g[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16);
+      if (z) d[i] *= slope(to_f(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16), p.act);
+      acc[i] += d[i];
+    }
+    if (p.dz) {
+      uint16_t* to = p.dz + m * p.dz_ld + c;
+      if (kVec) {
+        if (c < p.N)
+          *reinterpret_cast<uint4*>(to) = make_uint4(pack2(d[0], d[1], p.fp16), pack2(d[2], d[3], p.fp16), pack2(d[4], d[5], p.fp16), pack2(d[6], d[7], p.fp16));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < p.N) to[i] = pack1(d[i], p.fp16);
+      }
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[warp][lane * 8 + i] = acc[i];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.x * kDzCols + threadIdx.x;
+  if (col >= p.N) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kDzThreads / 32; ++w) sum += s[w][threadIdx.x];
+  p.part[(int64_t)blockIdx.y * p.N + col] = sum;
+}
+
+// The slices' sums, four values a thread.
+__global__ void __launch_bounds__(256)
+linear_slices_kernel(const float* sums, int64_t values, int slices, uint16_t* d, int fp16) {
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= values) return;
+  if (values % 4 == 0) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < slices; ++s) {
+      const float4 u = *reinterpret_cast<const float4*>(sums + s * values + at);
+      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
+    *reinterpret_cast<uint2*>(d + at) = make_uint2(pack2(v.x, v.y, fp16), pack2(v.z, v.w, fp16));
+  } else {
+    for (int i = 0; i < 4 && at + i < values; ++i) {
+      float v = 0.0f;
+      for (int s = 0; s < slices; ++s) v += sums[s * values + at + i];
+      d[at + i] = pack1(v, fp16);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+std::mutex g_mutex;
+int g_pairs[64];                                             // pairs that run at once, per device (0: not asked)
+std::atomic<bool> g_ready[64];
+GbClusters g_clusters;
+
+int set_limits() {
+#define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+#define GB_PAIR(M, N, E) GB_ATTR((linear_pair_kernel<M, N, E>), (Shape<M, N, E>::kSmem))
+  GB_PAIR(kForward, 256, kPlain);
+  GB_PAIR(kForward, 256, kResidual);
+  GB_PAIR(kForward, 256, kKeepZ);
+  GB_PAIR(kForward, 192, kPlain);
+  GB_PAIR(kForward, 192, kResidual);
+  GB_PAIR(kForward, 192, kKeepZ);
+  GB_PAIR(kRowsGrad, 256, kPlain);
+  GB_PAIR(kRowsGrad, 128, kPlain);
+  GB_PAIR(kWeightGrad, 256, kPlain);
+  GB_PAIR(kWeightGrad, 128, kPlain);
+  GB_ATTR(linear_rows_kernel<false>, kRowsSmem);
+  GB_ATTR(linear_rows_kernel<true>, kRowsSmem);
+#undef GB_PAIR
+#undef GB_ATTR
+  return GB_OK;
+}
+
+// Once per device: the kernels' shared memory, and how many pairs run at once.
+int ready(int* pairs) {
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  GB_REQUIRE(dev >= 0 && dev < 64, "device %d out of range", dev);
+  if (!g_ready[dev].load(std::memory_order_acquire)) {
+    if (gb_sm_count() <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+    std::lock_guard<std::mutex> lock(g_mutex);
+    const int rc = set_limits();
+    if (rc != GB_OK) return rc;
+    using S = Shape<kForward, 256, kPlain>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * 256);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    GB_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, linear_pair_kernel<kForward, 256, kPlain>, &cfg));
+    GB_REQUIRE(n > 0, "no CTA pair runs on this device");
+    g_pairs[dev] = n;
+    g_ready[dev].store(true, std::memory_order_release);
+  }
+  *pairs = g_pairs[dev];
+  return GB_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Operand maps: K-major [rows, contraction] in boxes of 64 x box_rows, MN-major [contraction, columns] in boxes of 64 x 64.
+int operand(CUtensorMap* map, const void* base, int64_t rows, int64_t inner, int64_t ld, int box_rows) {
+  return gb_tensor_map_rows16(map, base, inner, rows, ld, kSlab, box_rows, 128);
+}
+int tile_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld) { return gb_tensor_map_rows16(map, base, cols, rows, ld, 32, 32, 64); }
+
+struct Mats {
+  const void *a, *b;
+  int64_t a_ld, b_ld, K;       // K: the contraction
+};
+
+template <Major kMajor, int kBN, int kEpi>
+int run_pair(const Mats& m, LinearParams p, int pairs, cudaStream_t stream) {
+  using S = Shape<kMajor, kBN, kEpi>;
+  p.k_tiles = (int)ceil_div(m.K, kSlab);
+  p.m_tiles = (int)ceil_div(p.M, kPairM);
+  p.n_tiles = (int)ceil_div(p.N, kBN);
+  p.per_slice = (int)ceil_div(p.k_tiles, p.slices);
+  p.slices = (int)ceil_div(p.k_tiles, p.per_slice);
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles * p.slices;
+  GB_REQUIRE(tiles < (1ll << 30), "too many output tiles");
+  p.idesc |= ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24) | (S::kAmn ? 1u << 15 : 0u) | (S::kBmn ? 1u << 16 : 0u);
+  CUtensorMap map_a, map_b, map_d = {}, map_z = {}, map_r = {};
+  int rc = S::kAmn ? operand(&map_a, m.a, m.K, p.M, m.a_ld, kSlab) : operand(&map_a, m.a, p.M, m.K, m.a_ld, kBM);
+  if (rc != GB_OK) return rc;
+  rc = S::kBmn ? operand(&map_b, m.b, m.K, p.N, m.b_ld, kSlab) : operand(&map_b, m.b, p.N, m.K, m.b_ld, kBN / 2);
+  if (rc != GB_OK) return rc;
+  if (p.tma && p.slices == 1) {
+    rc = tile_map(&map_d, p.d, p.M, p.N, p.N);
+    if (rc == GB_OK && kEpi == kKeepZ) rc = tile_map(&map_z, p.z, p.M, p.N, p.N);
+    if (rc == GB_OK && kEpi != kPlain && p.r) rc = tile_map(&map_r, p.r, p.M, p.N, p.r_ld);
+    if (rc != GB_OK) return rc;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
+  gb_count_launch();
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, linear_pair_kernel<kMajor, kBN, kEpi>, map_a, map_b, map_d, map_z, map_r, p));
+  return GB_OK;
+}
+
+// Rows of a pass: all of them, else 192 or 256, whichever leaves fewer passes, then fewer empty rows.
+int pass_rows(int64_t M) {
+  if (M <= kMaxRows) return (int)M;
+  return ceil_div(M, 192) == ceil_div(M, 256) ? 192 : 256;
+}
+struct Split { int rows, slices, per_slice; int64_t tiles; };
+// K slices of the few-rows kernel: as many as the SMs take, at least four slabs each, no more than four past 64 rows.
+Split split_of(int64_t M, int64_t N, int64_t k_tiles) {
+  Split s;
+  s.rows = pass_rows(M);
+  s.tiles = ceil_div(N, kBM) * ceil_div(M, s.rows);
+  const int64_t sms = gb_sm_count();
+  int want = 1;
+  for (int n = 2; n <= (s.rows <= 64 ? kMaxSlices : 4) && s.tiles * n <= sms && n * 4 <= k_tiles; ++n)
+    if (s.tiles <= g_clusters.ask((const void*)linear_rows_kernel<false>, kRowsThreads, kRowsSmem, n)) want = n;
+  s.per_slice = (int)ceil_div(k_tiles, want);
+  s.slices = (int)ceil_div(k_tiles, s.per_slice);
+  return s;
+}
+// Where the few-rows kernel is the faster one: the rule of the other 16-bit GEMM (gb_gemm_rows_applies).
+bool rows_apply(int64_t M, int64_t N, int64_t k_tiles) {
+  if (M <= 192) return true;
+  if (M > 1024) return false;
+  const Split s = split_of(M, N, k_tiles);
+  return s.tiles <= gb_sm_count() && s.per_slice <= 64;
+}
+
+template <bool kWmn>
+int run_rows(const Mats& m, LinearParams p, cudaStream_t stream) {   // a: activation rows, b: weights
+  p.k_tiles = (int)ceil_div(m.K, kSlab);
+  const Split split = split_of(p.M, p.N, p.k_tiles);
+  GB_REQUIRE(split.tiles < (1ll << 31), "too many output tiles");
+  p.rows_per_pass = split.rows;
+  p.box_rows = (int)ceil_div(split.rows, 16) * 16;
+  p.n_tiles = (int)ceil_div(p.N, kBM);
+  p.per_slice = split.per_slice;
+  p.slices = split.slices;
+  p.idesc |= kWmn ? 1u << 15 : 0u;
+  const int stage = kBM * kSlabBytes + p.box_rows * kSlabBytes;
+  p.stages = (kRowsSmem - 1024) / stage;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  int bytes = p.stages * stage;
+  const int sums = (int)ceil_div(p.box_rows / 16, p.slices) * 16 * p.slices * kBM * 4;
+  if (bytes < sums) bytes = sums;
+  CUtensorMap map_w, map_x;
+  int rc = kWmn ? operand(&map_w, m.b, m.K, p.N, m.b_ld, kSlab) : operand(&map_w, m.b, p.N, m.K, m.b_ld, kBM);
+  if (rc != GB_OK) return rc;
+  rc = operand(&map_x, m.a, p.M, m.K, m.a_ld, p.box_rows);
+  if (rc != GB_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)split.tiles, (unsigned)p.slices);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = (size_t)bytes + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (gb_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.slices > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1; attr[n].val.clusterDim.y = (unsigned)p.slices; attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  gb_count_launch();
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, linear_rows_kernel<kWmn>, map_w, map_x, p));
+  return GB_OK;
+}
+
+LinearParams params_of(int64_t M, int64_t N, int dtype, void* d) {
+  LinearParams p = {};
+  p.M = M; p.N = N;
+  p.slices = 1;
+  p.fp16 = dtype == GB_DTYPE_FP16;
+  p.idesc = (1u << 4) | (p.fp16 ? 0u : (1u << 7) | (1u << 10));
+  p.tma = N % 8 == 0;
+  p.d = static_cast<uint16_t*>(d);
+  p.status = gb_status_word();
+  return p;
+}
+
+// Width of a tile: 256 columns, or `narrow` where that saves more of the last wave than its extra operand traffic costs.
+bool narrower(int64_t M, int64_t N, int narrow, int64_t pairs) {
+  const int64_t mt = ceil_div(M, kPairM);
+  return ceil_div(mt * ceil_div(N, narrow), pairs) * narrow * 21 < ceil_div(mt * ceil_div(N, 256), pairs) * 256 * 20;
+}
+
+int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
+  GB_REQUIRE(dtype == GB_DTYPE_BF16 || dtype == GB_DTYPE_FP16, "bf16 or fp16 expected");
+  GB_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "bad shape M=%lld N=%lld K=%lld", (long long)M,
+             (long long)N, (long long)K);
+  GB_REQUIRE(K % 8 == 0, "K=%lld: rows are fetched in 16-byte pieces, a multiple of 8 is needed", (long long)K);
+  return GB_OK;
+}
+bool aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// The backward pass's plan: where the pieces of the workspace lie, and over how many slices dW's contraction is split.
+struct GradPlan {
+  bool own_dz;                 // dz is a matrix of its own
+  int64_t dz_ld, dz_at, part_at, sums_at, bytes;
+  int part_rows, slices, narrow;
+};
+GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool products, bool bias, bool weight, bool dy_whole) {
+  GradPlan g = {};
+  auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
+  g.dz_ld = ceil_div(N, 8) * 8;
+  g.own_dz = products && (act != GB_EPI_NONE || N % 8 != 0 || !dy_whole);
+  int64_t at = 0;
+  g.dz_at = at;
+  if (g.own_dz) at += up(M * g.dz_ld * 2);
+  const int64_t sms = gb_sm_count() > 0 ? gb_sm_count() : 148;
+  // about eight blocks an SM; a block's warps walk at least two rows each
+  int64_t rows = ceil_div(sms * 8, ceil_div(N, kDzCols));
+  if (rows > ceil_div(M, 16)) rows = ceil_div(M, 16);
+  g.part_rows = (int)(rows < 1 ? 1 : rows > 512 ? 512 : rows);
+  g.part_at = at;
+  if (bias) at += up((int64_t)g.part_rows * N * 4);
+  g.sums_at = at;
+  g.slices = 1;
+  if (weight) {
+    const int64_t pairs = sms / 2, k_tiles = ceil_div(M, kSlab);
+    g.narrow = narrower(N, K, 128, pairs);
+    const int64_t tiles = ceil_div(N, kPairM) * ceil_div(K, g.narrow ? 128 : 256);
+    // as many slices as the pairs take at once, of at least eight slabs
+    while (g.slices < 16 && tiles * (g.slices + 1) <= pairs && (g.slices + 1) * 8 <= k_tiles) ++g.slices;
+    if (g.slices > 1) at += up((int64_t)g.slices * N * K * 4);
+  }
+  g.bytes = at;
+  return g;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, const void* r, int64_t r_ld, int dtype, int64_t M, int64_t N, int64_t K, int act,
+                  void* y, void* z, void* stream) {
+  int rc = check_shape(M, N, K, dtype);
+  if (rc != GB_OK) return rc;
+  GB_REQUIRE(x && w && y, "null pointer argument");
+  GB_REQUIRE(act >= GB_EPI_NONE && act <= GB_EPI_SILU, "unknown activation %d", act);
+  GB_REQUIRE(aligned(x) && aligned(w) && aligned(y) && aligned(z) && x_ld >= K && x_ld % 8 == 0, "operands must be rows of whole 16-byte pieces");
+  GB_REQUIRE(!r || r_ld >= N, "residual rows that do not overlap expected");
+  int pairs = 0;
+  rc = ready(&pairs);
+  if (rc != GB_OK) return rc;
+  LinearParams p = params_of(M, N, dtype, y);
+  p.act = act;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.r = static_cast<const uint16_t*>(r);
+  p.r_ld = r_ld;
+  p.z = static_cast<uint16_t*>(z);
+  if (r && (!aligned(r) || r_ld % 8 != 0)) p.tma = 0;
+  const Mats m = {x, w, x_ld, K, K};
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (rows_apply(M, N, ceil_div(K, kSlab))) return run_rows<false>(m, p, st);
+  if (narrower(M, N, 192, pairs))
+    return z ? run_pair<kForward, 192, kKeepZ>(m, p, pairs, st) : r ? run_pair<kForward, 192, kResidual>(m, p, pairs, st) : run_pair<kForward, 192, kPlain>(m, p, pairs, st);
+  return z ? run_pair<kForward, 256, kKeepZ>(m, p, pairs, st) : r ? run_pair<kForward, 256, kResidual>(m, p, pairs, st) : run_pair<kForward, 256, kPlain>(m, p, pairs, st);
+}
+
+int64_t gb_linear_act_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int rows, int weight, int bias, int dy_whole) {
+  return M < 1 || N < 1 || K < 1 ? 0 : grad_plan(M, N, K, act, rows || weight, bias != 0, weight != 0, dy_whole != 0).bytes;
+}
+
+int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void* x, int64_t x_ld, const void* w, int dtype, int64_t M, int64_t N, int64_t K, int act,
+                       void* dx, void* dw, void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_shape(M, N, K, dtype);
+  if (rc != GB_OK) return rc;
+  GB_REQUIRE(act >= GB_EPI_NONE && act <= GB_EPI_SILU, "unknown activation %d", act);
+  GB_REQUIRE(dy && (act == GB_EPI_NONE || z) && (!dx || w) && (!dw || x), "null pointer argument");
+  GB_REQUIRE(dy_ld >= N && (!dw || (x_ld >= K && x_ld % 8 == 0)), "rows that do not overlap expected");
+  GB_REQUIRE(aligned(w) && aligned(x) && aligned(z) && aligned(dx) && aligned(dw), "operands must be rows of whole 16-byte pieces");
+  int pairs = 0;
+  rc = ready(&pairs);
+  if (rc != GB_OK) return rc;
+  const bool dy_whole = aligned(dy) && dy_ld % 8 == 0;
+  const GradPlan g = grad_plan(M, N, K, act, dx || dw, dbias != nullptr, dw != nullptr, dy_whole);
+  if (workspace_bytes < g.bytes || (g.bytes > 0 && !workspace))
+    return gb_fail(GB_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)g.bytes);
+  GB_REQUIRE(aligned(workspace), "the workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const void* dz = dy;
+  int64_t dz_ld = dy_ld;
+  if (g.own_dz || dbias) {
+    DzParams d = {};
+    d.dy = static_cast<const uint16_t*>(dy);
+    d.z = act == GB_EPI_NONE ? nullptr : static_cast<const uint16_t*>(z);
+    d.dz = g.own_dz ? reinterpret_cast<uint16_t*>(ws + g.dz_at) : nullptr;
+    d.M = M; d.N = N; d.dy_ld = dy_ld; d.dz_ld = g.dz_ld;
+    d.fp16 = dtype == GB_DTYPE_FP16; d.act = act;
+    d.part = dbias ? reinterpret_cast<float*>(ws + g.part_at) : nullptr;
+    const dim3 grid((unsigned)ceil_div(N, kDzCols), (unsigned)g.part_rows);
+    if (N % 8 == 0 && dy_whole) GB_CUDA_OK(gb_launch(linear_dz_kernel<true>, grid, dim3(kDzThreads), 0, st, d));
+    else GB_CUDA_OK(gb_launch(linear_dz_kernel<false>, grid, dim3(kDzThreads), 0, st, d));
+    if (g.own_dz) { dz = ws + g.dz_at; dz_ld = g.dz_ld; }
+    if (dbias) {
+      rc = gb_join_columns(d.part, g.part_rows, N, dbias, dtype, st);
+      if (rc != GB_OK) return rc;
+    }
+  }
+  if (dx) {                                                  // [M, K], the contraction over N
+    const LinearParams p = params_of(M, K, dtype, dx);
+    const Mats m = {dz, w, dz_ld, K, N};
+    if (rows_apply(M, K, ceil_div(N, kSlab))) rc = run_rows<true>(m, p, st);
+    else rc = narrower(M, K, 128, pairs) ? run_pair<kRowsGrad, 128, kPlain>(m, p, pairs, st) : run_pair<kRowsGrad, 256, kPlain>(m, p, pairs, st);
+    if (rc != GB_OK) return rc;
+  }
+  if (dw) {                                                  // [N, K], the contraction over M
+    LinearParams p = params_of(N, K, dtype, dw);
+    const Mats m = {dz, x, dz_ld, x_ld, M};
+    const int64_t k_tiles = ceil_div(M, kSlab);
+    p.slices = (int)ceil_div(k_tiles, ceil_div(k_tiles, g.slices));      // none of them empty
+    p.sums = reinterpret_cast<float*>(ws + g.sums_at);
+    rc = g.narrow ? run_pair<kWeightGrad, 128, kPlain>(m, p, pairs, st) : run_pair<kWeightGrad, 256, kPlain>(m, p, pairs, st);
+    if (rc != GB_OK) return rc;
+    if (p.slices > 1)
+      GB_CUDA_OK(gb_launch(linear_slices_kernel, dim3((unsigned)ceil_div(N * K, 1024)), dim3(256), 0, st, p.sums, N * K, p.slices, p.d, p.fp16));
+  }
+  return GB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,804 @@
+// The norms behind and in front of a block, with the block's gate and the residual stream between them, and their gradients.
+//
+// For a row y that a block gives and the row r of the stream, H values each,
+//     u = y, or y_hat (o + pw) with y_hat = y / sqrt(mean y^2 + eps)         the norm behind the block
+//     x = a r + b g u                                                        the stream, stored in its own type
+//     h = x_hat (o + w)        with x_hat = x / sqrt(mean x^2 + eps)         the norm in front of the next block
+// g a gate for each channel, row or group of rows, or 1; o 0, or 1 for weights kept around zero.  h is taken from x as it is stored,
+// so that it is the norm of what is returned; in E4M3 blocks (one scale per 128 columns) from x before its rounding.
+// With gradients dh and ds of h and x,
+//     dx = ds + (dh (o + w) - x_hat mean(dh (o + w) x_hat)) / rms x,      dr = a dx,      dw = sum over rows of dh x_hat
+//     du = b g dx,   dg = sum over its rows of b u dx,   dpw = sum over rows of du y_hat
+//     dy = du, or (du (o + pw) - y_hat mean(du (o + pw) y_hat)) / rms y
+//
+// Bound by memory: a row is read and written once, and used in registers and shared memory in between.  Blocks stay and walk the
+// rows; whole rows come by bulk copies into a ring that is some rows ahead, so that loads go on through the sums over a row.
+// A thread has the same eight (or sixteen) columns of every row: the weights' gradients add up in its registers, and a second launch
+// adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value.
+#include "gb_blocks.cuh"
+
+namespace {
+
+using namespace gb_blocks;
+
+constexpr uint32_t kAll = 0xFFFFFFFFu;
+constexpr int kMostStages = 8;
+constexpr int kRingMax = 208 * 1024;
+
+struct NormParams {
+  int64_t T, H;
+  const void *y, *r, *gate, *w, *pw;
+  int64_t y_ld, r_ld, gate_ld, gate_rows;                // rows that share a row of the gate
+  int w_type, pw_type;                                   // GB_DTYPE_*
+  float a, b, eps, offset;
+  float inv_h;
+  void *h, *s;                                           // out; backward: s is in
+  float *rstd, *post_rstd;                               // out or null; backward: in
+  uint8_t* q;
+  float* scale;
+  int scale_rule;
+  int stages;
+  uint32_t stage_bytes;
+  uint32_t in_at[5];                                     // where a stage holds the arrays of a row; ~0u: not read
+  int* status;
+  // backward
+  const void *dh, *ds;
+  int64_t dh_ld, ds_ld;
+  void *dy, *dr, *dg;                                    // dg: where every row has a gate of its own
+  float *part_w, *part_pw, *part_g;                      // [blocks][H]
+  int per_gate;                                          // blocks that work on the rows of one gate row
+  float* means;                                          // [T], value by value: mean(dh (o + w) x_hat)
+};
+
+GB_DEVINL float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+// Sum over the block's threads, in the same order each time.  `turn` changes the buffer from call to call: one barrier is enough.
+GB_DEVINL float block_sum(float v, float (*red)[32], int& turn) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  float* to = red[turn & 1];
+  ++turn;
+  if (lane == 0) to[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? to[lane] : 0.0f);
+}
+GB_DEVINL float value_of(const void* p, int type, int64_t c) {
+  if (type == GB_DTYPE_BF16) return to_f32<Bf16>(__ldg(static_cast<const uint16_t*>(p) + c));
+  if (type == GB_DTYPE_FP16) return to_f32<Fp16>(__ldg(static_cast<const uint16_t*>(p) + c));
+  return __ldg(static_cast<const float*>(p) + c);
+}
+
+// Eight values from a column on.
+template <typename T>
+GB_DEVINL void load8(const typename T::word* p, float (&v)[8]) {
+  unpack16<T>(*reinterpret_cast<const uint4*>(p), v);
+  if constexpr (sizeof(typename T::word) == 4) unpack16<T>(*reinterpret_cast<const uint4*>(p + 4), v + 4);
+}
+template <typename T>
+GB_DEVINL void store8(typename T::word* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = pack16<T>(v);
+  if constexpr (sizeof(typename T::word) == 4) *reinterpret_cast<uint4*>(p + 4) = pack16<T>(v + 4);
+}
+GB_DEVINL void weights8(const void* p, int type, int64_t c, float offset, float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 1.0f;
+    return;
+  }
+  if (type == GB_DTYPE_BF16) load8<Bf16>(static_cast<const uint16_t*>(p) + c, v);
+  else if (type == GB_DTYPE_FP16) load8<Fp16>(static_cast<const uint16_t*>(p) + c, v);
+  else load8<Fp32>(static_cast<const uint32_t*>(p) + c, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += offset;
+}
+template <typename R>
+GB_DEVINL float as_stored(float v) { return to_f32<R>(from_f32<R>(v)); }
+
+// The ring of rows.  A wait that runs out is remembered with the step it belongs to: the block leaves together behind that step's
+// barrier, however far its fastest thread has come.
+struct Ring {
+  uint64_t* full;
+  volatile int* gave_up;
+  int stages;
+  GB_DEVINL void wait(int i, int* status, int code) const {
+    if (!gb_mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u)) {
+      atomicMin((int*)gave_up, i);
+      atomicExch(status, code);
+    }
+  }
+};
+
+template <typename T, typename R, int kV, int kThreads, bool kFp8>
+__global__ void __launch_bounds__(kThreads)
+norm_rows_kernel(const __grid_constant__ NormParams p) {
+  using word = typename T::word;
+  using rword = typename R::word;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kMostStages];
+  __shared__ float red[2][32];
+  __shared__ int gave_up;
+  const int tid = threadIdx.x;
+  const int64_t step = gridDim.x;
+  gb_pdl_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
+    gave_up = 0x7FFFFFFF;
+    gb_fence_barrier_init();
+  }
+  __syncthreads();
+  gb_pdl_wait();
+  const uint32_t y_bytes = (uint32_t)(p.H * sizeof(word)), r_bytes = (uint32_t)(p.H * sizeof(rword));
+  auto fetch = [&](int64_t t, int s) {
+    uint8_t* st = ring + (size_t)s * p.stage_bytes;
+    const bool gate = p.in_at[2] != ~0u;
+    gb_mbar_expect_tx(&full[s], y_bytes + r_bytes + (gate ? y_bytes : 0u));
+    gb_bulk_g2s(st + p.in_at[0], static_cast<const word*>(p.y) + t * p.y_ld, y_bytes, &full[s]);
+    gb_bulk_g2s(st + p.in_at[1], static_cast<const rword*>(p.r) + t * p.r_ld, r_bytes, &full[s]);
+    if (gate) gb_bulk_g2s(st + p.in_at[2], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
+  };
+  if (tid == 0)
+    for (int s = 0; s < p.stages; ++s)
+      if (blockIdx.x + s * step < p.T) fetch(blockIdx.x + s * step, s);
+  const Ring wheel{full, &gave_up, p.stages};
+  int turn = 0, i = 0;
+  for (int64_t t = blockIdx.x; t < p.T; t += step, ++i) {
+    const int s = i % p.stages;
+    const uint8_t* st = ring + (size_t)s * p.stage_bytes;
+    wheel.wait(i, p.status, 91);
+    float x[kV][8], rp = 1.0f, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+      if (c < p.H) {
+        load8<T>(reinterpret_cast<const word*>(st + p.in_at[0]) + c, x[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(x[k][j], x[k][j], sum);
+      }
+    }
+    if (p.pw) rp = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+      if (c < p.H) {
+        float v[8];
+        if (p.pw) {
+          weights8(p.pw, p.pw_type, c, p.offset, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[k][j] *= rp * v[j];
+        }
+        if (p.gate) {
+          if (p.in_at[2] != ~0u) load8<T>(reinterpret_cast<const word*>(st + p.in_at[2]) + c, v);
+          else load8<T>(static_cast<const word*>(p.gate) + t / p.gate_rows * p.gate_ld + c, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[k][j] *= v[j];
+        }
+        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[1]) + c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[k][j] = fmaf(p.b, x[k][j], p.a * v[j]);
+          if (!kFp8) x[k][j] = as_stored<R>(x[k][j]);
+          sum = fmaf(x[k][j], x[k][j], sum);
+        }
+        store8<R>(static_cast<rword*>(p.s) + t * p.H + c, x[k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+      }
+    }
+    const float rs = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
+    if (gave_up <= i) break;
+    if (tid == 0) {                                      // every thread has taken what it needs of the stage
+      if (t + p.stages * step < p.T) fetch(t + p.stages * step, s);
+      if (p.rstd) p.rstd[t] = rs;
+      if (p.post_rstd) p.post_rstd[t] = rp;
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+      float v[8];
+      if (c < p.H) {
+        weights8(p.w, p.w_type, c, p.offset, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= x[k][j] * rs;
+        if (!kFp8) store8<T>(static_cast<word*>(p.h) + t * p.H + c, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      }
+      if constexpr (kFp8) {                              // sixteen neighbours have a block
+        float scale;
+        uint32_t q[2];
+        quantize_block<8, 16>(v, p.scale_rule, scale, q);
+        if (c < p.H) {
+          *reinterpret_cast<uint2*>(p.q + t * p.H + c) = make_uint2(q[0], q[1]);
+          if ((tid & 15) == 0) p.scale[t * ((p.H + kBlock - 1) / kBlock) + c / kBlock] = scale;
+        }
+      }
+    }
+  }
+  if (gave_up != 0x7FFFFFFF) __nanosleep(1000000);       // copies still in flight end before the memory goes
+}
+
+template <typename T, typename R, int kV, int kThreads>
+__global__ void __launch_bounds__(kThreads)
+norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
+  using word = typename T::word;
+  using rword = typename R::word;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kMostStages];
+  __shared__ float red[2][32];
+  __shared__ int gave_up;
+  const int tid = threadIdx.x;
+  gb_pdl_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
+    gave_up = 0x7FFFFFFF;
+    gb_fence_barrier_init();
+  }
+  __syncthreads();
+  gb_pdl_wait();
+  const int64_t rows = p.per_gate == 0 ? p.T : p.gate_rows;          // of the block's share: all, or those of a gate row
+  const int64_t first = p.per_gate == 0 ? 0 : blockIdx.x / p.per_gate * p.gate_rows;
+  const int64_t begin = p.per_gate == 0 ? blockIdx.x : blockIdx.x % p.per_gate, step = p.per_gate == 0 ? gridDim.x : p.per_gate;
+  const uint32_t y_bytes = (uint32_t)(p.H * sizeof(word)), r_bytes = (uint32_t)(p.H * sizeof(rword));
+  auto fetch = [&](int64_t t, int s) {
+    uint8_t* st = ring + (size_t)s * p.stage_bytes;
+    gb_mbar_expect_tx(&full[s], p.stage_bytes);
+    gb_bulk_g2s(st + p.in_at[0], static_cast<const rword*>(p.s) + t * p.H, r_bytes, &full[s]);
+    if (p.in_at[1] != ~0u) gb_bulk_g2s(st + p.in_at[1], static_cast<const word*>(p.dh) + t * p.dh_ld, y_bytes, &full[s]);
+    if (p.in_at[2] != ~0u) gb_bulk_g2s(st + p.in_at[2], static_cast<const rword*>(p.ds) + t * p.ds_ld, r_bytes, &full[s]);
+    if (p.in_at[3] != ~0u) gb_bulk_g2s(st + p.in_at[3], static_cast<const word*>(p.y) + t * p.y_ld, y_bytes, &full[s]);
+    if (p.in_at[4] != ~0u) gb_bulk_g2s(st + p.in_at[4], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
+  };
+  if (tid == 0)
+    for (int s = 0; s < p.stages; ++s)
+      if (begin + s * step < rows) fetch(first + begin + s * step, s);
+  const Ring wheel{full, &gave_up, p.stages};
+  float acc_w[kV][8], acc_pw[kV][8], acc_g[kV][8];
+#pragma unroll
+  for (int k = 0; k < kV; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc_w[k][j] = acc_pw[k][j] = acc_g[k][j] = 0.0f;
+  int turn = 0, i = 0;
+  for (int64_t n = begin; n < rows; n += step, ++i) {
+    const int64_t t = first + n;
+    const int s = i % p.stages;
+    const uint8_t* st = ring + (size_t)s * p.stage_bytes;
+    const float rs = __ldg(p.rstd + t), rp = p.pw ? __ldg(p.post_rstd + t) : 1.0f;
+    wheel.wait(i, p.status, 92);
+    float d[kV][8], m1 = 0.0f, m2 = 0.0f;                // d: dh (o + w), dx, du (o + pw) in turn
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[k][j] = 0.0f;
+      if (c < p.H && p.dh) {
+        float x[8], w[8];
+        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[0]) + c, x);
+        load8<T>(reinterpret_cast<const word*>(st + p.in_at[1]) + c, d[k]);
+        weights8(p.w, p.w_type, c, p.offset, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xh = x[j] * rs;
+          acc_w[k][j] = fmaf(d[k][j], xh, acc_w[k][j]);
+          d[k][j] *= w[j];
+          m1 = fmaf(d[k][j], xh, m1);
+        }
+      }
+    }
+    m1 = block_sum(m1, red, turn) * p.inv_h;
+    uint4 y_raw[kV][sizeof(word) / 2];
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+      if (c < p.H) {
+        float x[8], v[8];
+        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[0]) + c, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[k][j] = rs * fmaf(-x[j] * rs, m1, d[k][j]);
+        if (p.ds) {
+          load8<R>(reinterpret_cast<const rword*>(st + p.in_at[2]) + c, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[k][j] += v[j];
+        }
+        if (p.dr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = p.a * d[k][j];
+          store8<R>(static_cast<rword*>(p.dr) + t * p.H + c, v);
+        }
+        float u[8], w[8];                                // y_hat (or y), o + pw
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = w[j] = 1.0f;
+        if (p.in_at[3] != ~0u) {
+          const word* y = reinterpret_cast<const word*>(st + p.in_at[3]) + c;
+#pragma unroll
+          for (int q = 0; q < (int)sizeof(word) / 2; ++q) y_raw[k][q] = reinterpret_cast<const uint4*>(y)[q];
+          load8<T>(y, u);
+        }
+        if (p.pw) {
+          weights8(p.pw, p.pw_type, c, p.offset, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] *= rp;
+        }
+        float g[8];
+        if (p.gate) {
+          if (p.in_at[4] != ~0u) load8<T>(reinterpret_cast<const word*>(st + p.in_at[4]) + c, g);
+          else load8<T>(static_cast<const word*>(p.gate) + t / p.gate_rows * p.gate_ld + c, g);
+          float dg[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            dg[j] = p.b * d[k][j] * (u[j] * w[j]);
+            acc_g[k][j] += dg[j];
+            g[j] *= p.b;
+          }
+          if (p.dg) store8<T>(static_cast<word*>(p.dg) + t * p.H + c, dg);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = p.b;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float du = g[j] * d[k][j];
+          acc_pw[k][j] = fmaf(du, u[j], acc_pw[k][j]);
+          d[k][j] = du * w[j];
+          m2 = fmaf(d[k][j], u[j], m2);
+        }
+      }
+    }
+    m2 = block_sum(m2, red, turn) * p.inv_h;
+    if (gave_up <= i) break;
+    if (tid == 0 && n + p.stages * step < rows) fetch(t + p.stages * step, s);
+    if (p.dy) {
+#pragma unroll
+      for (int k = 0; k < kV; ++k) {
+        const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+        if (c < p.H) {
+          if (p.pw) {
+            float y[8];
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(word) / 2; ++q) unpack16<T>(y_raw[k][q], y + q * (16 / sizeof(word)));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[k][j] = rp * fmaf(-y[j] * rp, m2, d[k][j]);
+          }
+          store8<T>(static_cast<word*>(p.dy) + t * p.H + c, d[k]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kV; ++k) {
+    const int64_t c = ((int64_t)k * blockDim.x + tid) * 8, at = (int64_t)blockIdx.x * p.H + c;
+    if (c < p.H) {
+      if (p.part_w) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_w) + at, acc_w[k]);
+      if (p.part_pw) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_pw) + at, acc_pw[k]);
+      if (p.part_g) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + at, acc_g[k]);
+    }
+  }
+  if (gave_up != 0x7FFFFFFF) __nanosleep(1000000);
+}
+
+// ------------------------------------------------------------------------------------------------ value by value
+constexpr int kAnyThreads = 256;
+
+template <typename T, typename R>
+struct Values {
+  const NormParams& p;
+  int64_t t;
+  GB_DEVINL float y(int64_t c) const { return to_f32<T>(static_cast<const typename T::word*>(p.y)[t * p.y_ld + c]); }
+  GB_DEVINL float gate(int64_t c) const {
+    return p.gate ? to_f32<T>(static_cast<const typename T::word*>(p.gate)[t / p.gate_rows * p.gate_ld + c]) : 1.0f;
+  }
+  GB_DEVINL float w(int64_t c) const { return p.w ? value_of(p.w, p.w_type, c) + p.offset : 1.0f; }
+  GB_DEVINL float pw(int64_t c) const { return p.pw ? value_of(p.pw, p.pw_type, c) + p.offset : 1.0f; }
+  GB_DEVINL float x(int64_t c, float rp) const {
+    const float u = p.pw ? y(c) * (rp * pw(c)) : y(c);
+    return fmaf(p.b, u * gate(c), p.a * to_f32<R>(static_cast<const typename R::word*>(p.r)[t * p.r_ld + c]));
+  }
+  // backward: p.s holds the stream
+  GB_DEVINL float x_hat(int64_t c, float rs) const { return to_f32<R>(static_cast<const typename R::word*>(p.s)[t * p.H + c]) * rs; }
+  GB_DEVINL float dh(int64_t c) const { return p.dh ? to_f32<T>(static_cast<const typename T::word*>(p.dh)[t * p.dh_ld + c]) : 0.0f; }
+  GB_DEVINL float dx(int64_t c, float rs, float m1) const {
+    const float d = rs * fmaf(-x_hat(c, rs), m1, dh(c) * w(c));
+    return p.ds ? d + to_f32<R>(static_cast<const typename R::word*>(p.ds)[t * p.ds_ld + c]) : d;
+  }
+};
+
+template <typename T, typename R, bool kFp8>
+__global__ void __launch_bounds__(kAnyThreads)
+norm_any_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float red[2][32];
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  int turn = 0;
+  const Values<T, R> v{p, (int64_t)blockIdx.x};
+  float rp = 1.0f, sum = 0.0f;
+  if (p.pw) {
+    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) sum = fmaf(v.y(c), v.y(c), sum);
+    rp = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
+  }
+  sum = 0.0f;
+  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
+    float x = v.x(c, rp);
+    static_cast<typename R::word*>(p.s)[v.t * p.H + c] = from_f32<R>(x);
+    if (!kFp8) x = as_stored<R>(x);
+    sum = fmaf(x, x, sum);
+  }
+  const float rs = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
+  if (threadIdx.x == 0) {
+    if (p.rstd) p.rstd[v.t] = rs;
+    if (p.post_rstd) p.post_rstd[v.t] = rp;
+  }
+  if constexpr (!kFp8) {
+    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads)
+      static_cast<typename T::word*>(p.h)[v.t * p.H + c] = from_f32<T>(as_stored<R>(v.x(c, rp)) * rs * v.w(c));
+  } else {
+    const int64_t blocks = (p.H + kBlock - 1) / kBlock;
+    for (int64_t b0 = 0; b0 < blocks; b0 += kAnyThreads / 16) {
+      const int64_t b = b0 + threadIdx.x / 16, c = b * kBlock + (threadIdx.x & 15) * 8;
+      float h[8], scale;
+      uint32_t q[2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = c + j < p.H ? v.x(c + j, rp) * rs * v.w(c + j) : 0.0f;
+      quantize_block<8, 16>(h, p.scale_rule, scale, q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < p.H) p.q[v.t * p.H + c + j] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
+      if (b < blocks && (threadIdx.x & 15) == 0) p.scale[v.t * blocks + b] = scale;
+    }
+  }
+}
+
+template <typename T, typename R>
+__global__ void __launch_bounds__(kAnyThreads)
+norm_any_grad_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float red[2][32];
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  int turn = 0;
+  const Values<T, R> v{p, (int64_t)blockIdx.x};
+  const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
+  float m1 = 0.0f, m2 = 0.0f;
+  if (p.dh)
+    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) m1 = fmaf(v.dh(c) * v.w(c), v.x_hat(c, rs), m1);
+  m1 = block_sum(m1, red, turn) * p.inv_h;
+  if (threadIdx.x == 0) p.means[v.t] = m1;
+  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
+    const float dx = v.dx(c, rs, m1);
+    if (p.dr) static_cast<typename R::word*>(p.dr)[v.t * p.H + c] = from_f32<R>(p.a * dx);
+    if (p.dg) static_cast<typename T::word*>(p.dg)[v.t * p.H + c] = from_f32<T>(p.b * dx * (v.y(c) * (rp * v.pw(c))));
+    if (p.pw) m2 = fmaf(p.b * v.gate(c) * dx * v.pw(c), v.y(c) * rp, m2);
+    else if (p.dy) static_cast<typename T::word*>(p.dy)[v.t * p.H + c] = from_f32<T>(p.b * v.gate(c) * dx);
+  }
+  if (!p.pw || !p.dy) return;
+  m2 = block_sum(m2, red, turn) * p.inv_h;
+  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
+    const float du = p.b * v.gate(c) * v.dx(c, rs, m1);
+    static_cast<typename T::word*>(p.dy)[v.t * p.H + c] = from_f32<T>(rp * fmaf(-v.y(c) * rp, m2, du * v.pw(c)));
+  }
+}
+
+// The weights' gradients over a block's share of the rows; a thread has a column.
+template <typename T, typename R>
+__global__ void __launch_bounds__(kAnyThreads)
+norm_any_columns_kernel(const __grid_constant__ NormParams p, int64_t column_blocks) {
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  const int64_t share = blockIdx.x / column_blocks, c = (blockIdx.x - share * column_blocks) * kAnyThreads + threadIdx.x;
+  if (c >= p.H) return;
+  const int64_t shares = gridDim.x / column_blocks;
+  const int64_t rows = p.per_gate == 0 ? p.T : p.gate_rows, first = p.per_gate == 0 ? 0 : share / p.per_gate * p.gate_rows;
+  const int64_t begin = p.per_gate == 0 ? share : share % p.per_gate, step = p.per_gate == 0 ? shares : p.per_gate;
+  float w = 0.0f, pw = 0.0f, g = 0.0f;
+  for (int64_t n = begin; n < rows; n += step) {
+    const Values<T, R> v{p, first + n};
+    const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
+    w = fmaf(v.dh(c), v.x_hat(c, rs), w);
+    if (p.part_pw || p.part_g) {
+      const float dx = v.dx(c, rs, p.means[v.t]), y_hat = v.y(c) * rp;
+      pw = fmaf(p.b * v.gate(c) * dx, y_hat, pw);
+      g = fmaf(p.b * dx, y_hat * v.pw(c), g);
+    }
+  }
+  const int64_t at = share * p.H + c;
+  if (p.part_w) p.part_w[at] = w;
+  if (p.part_pw) p.part_pw[at] = pw;
+  if (p.part_g) p.part_g[at] = g;
+}
+
+// The shares' sums: a block adds up 32 columns of one result, warp w every 32nd share.
+struct JoinParams {
+  const float* part[3];       // w, pw, gate: shares of H sums each
+  void* out[3];
+  int type[3];
+  int64_t H, shares, gates;   // shares in all, gate rows
+  int64_t column_blocks;
+};
+constexpr int kJoinThreads = 1024;
+
+__global__ void __launch_bounds__(kJoinThreads)
+norm_join_kernel(const __grid_constant__ JoinParams p) {
+  __shared__ float s[32][33];
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  const int64_t job = blockIdx.x / p.column_blocks, col = (blockIdx.x - job * p.column_blocks) * 32 + (threadIdx.x & 31);
+  int which = 2;
+  int64_t gate = job;                                    // jobs: the weights that are asked for, then the gate's rows
+  for (int k = 0; k < 2; ++k)
+    if (p.part[k]) {
+      if (gate == 0) { which = k; break; }
+      --gate;
+    }
+  const int64_t n = which == 2 ? p.shares / p.gates : p.shares;
+  const float* from = p.part[which] + (which == 2 ? gate * n * p.H : 0);
+  float sum = 0.0f;
+  if (col < p.H)
+    for (int64_t i = threadIdx.x >> 5; i < n; i += 32) sum += from[i * p.H + col];
+  s[threadIdx.x & 31][threadIdx.x >> 5] = sum;
+  __syncthreads();
+  const int c = threadIdx.x >> 5;
+  sum = warp_sum(s[c][threadIdx.x & 31]);
+  const int64_t at = (blockIdx.x - job * p.column_blocks) * 32 + c;
+  if ((threadIdx.x & 31) != 0 || at >= p.H) return;
+  const int64_t to = which == 2 ? gate * p.H + at : at;
+  if (p.type[which] == GB_DTYPE_BF16) static_cast<uint16_t*>(p.out[which])[to] = from_f32<Bf16>(sum);
+  else if (p.type[which] == GB_DTYPE_FP16) static_cast<uint16_t*>(p.out[which])[to] = from_f32<Fp16>(sum);
+  else static_cast<float*>(p.out[which])[to] = sum;
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int size_of(int type) { return type == GB_DTYPE_FP32 ? 4 : 2; }
+
+// Threads of a block, eight (kV = 1) or sixteen columns each; 0: rows too long.
+struct Width { int v, threads, most; };
+Width width_of(int64_t H) {
+  if (H <= 2048) return {1, (int)((H + 255) / 256 * 32), 256};
+  if (H <= 16384) return {2, (int)((H + 511) / 512 * 32), H <= 8192 ? 512 : 1024};
+  return {0, 0, 0};
+}
+
+bool whole(const void* p, int64_t ld, int size) { return !p || (((uintptr_t)p & 15u) == 0 && ld * size % 16 == 0); }
+
+int check_args(const gb_residual_norm_args* a) {
+  GB_REQUIRE(a != nullptr, "null arguments");
+  GB_REQUIRE(a->dtype >= GB_DTYPE_BF16 && a->dtype <= GB_DTYPE_FP32, "unknown element type %d", a->dtype);
+  GB_REQUIRE(a->stream_dtype == a->dtype || a->stream_dtype == GB_DTYPE_FP32, "the stream has the rows' type or fp32");
+  GB_REQUIRE(a->T >= 0 && a->T < (1ll << 31) && a->H >= 1 && a->H < (1ll << 31), "bad shape T=%lld H=%lld", (long long)a->T, (long long)a->H);
+  for (int t : {a->w ? a->w_dtype : 0, a->pw ? a->pw_dtype : 0}) GB_REQUIRE(t >= GB_DTYPE_BF16 && t <= GB_DTYPE_FP32, "unknown weight type %d", t);
+  GB_REQUIRE(!a->gate || (a->gate_rows >= 1 && a->T % a->gate_rows == 0), "gate rows of %lld rows each do not make up %lld", (long long)a->gate_rows, (long long)a->T);
+  GB_REQUIRE(a->y_ld >= a->H && a->r_ld >= a->H && (!a->gate || a->gate_ld >= a->H), "rows that do not overlap expected");
+  return GB_OK;
+}
+
+NormParams params_of(const gb_residual_norm_args* a) {
+  NormParams p = {};
+  p.T = a->T; p.H = a->H;
+  p.y = a->y; p.r = a->r; p.gate = a->gate; p.w = a->w; p.pw = a->pw;
+  p.y_ld = a->y_ld; p.r_ld = a->r_ld; p.gate_ld = a->gate_ld; p.gate_rows = a->gate ? a->gate_rows : 1;
+  p.w_type = a->w_dtype; p.pw_type = a->pw_dtype;
+  p.a = a->residual_scale; p.b = a->branch_scale; p.eps = a->eps; p.offset = a->weight_offset;
+  p.inv_h = (float)(1.0 / (double)a->H);
+  p.status = gb_status_word();
+  for (uint32_t& at : p.in_at) at = ~0u;
+  return p;
+}
+
+// Blocks an SM, and stages of their rings: about 1024 threads, rows ahead for each of them.
+struct Plan { int per_sm, stages; };
+Plan plan_of(int threads, uint32_t stage_bytes) {
+  int per_sm = 1024 / threads;
+  if (per_sm < 1) per_sm = 1;
+  if (per_sm > 16) per_sm = 16;
+  while (per_sm > 1 && (uint32_t)kRingMax / per_sm < 2 * stage_bytes + 1024) --per_sm;
+  int stages = (int)(((uint32_t)kRingMax / per_sm - 1024) / stage_bytes);
+  return {per_sm, stages > 4 ? 4 : stages};
+}
+
+template <typename Go>
+int with_types(int dtype, int stream_dtype, Go go) {
+  if (dtype == GB_DTYPE_BF16) return stream_dtype == GB_DTYPE_FP32 ? go(Bf16(), Fp32()) : go(Bf16(), Bf16());
+  if (dtype == GB_DTYPE_FP16) return stream_dtype == GB_DTYPE_FP32 ? go(Fp16(), Fp32()) : go(Fp16(), Fp16());
+  return go(Fp32(), Fp32());
+}
+template <typename Go>
+int with_width(const Width& w, Go go) {
+  using std::integral_constant;
+  if (w.v == 1) return go(integral_constant<int, 1>(), integral_constant<int, 256>());
+  if (w.most == 512) return go(integral_constant<int, 2>(), integral_constant<int, 512>());
+  return go(integral_constant<int, 2>(), integral_constant<int, 1024>());
+}
+
+template <typename K, typename... Args>
+int launch_ring(K kernel, int blocks, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+  if (smem > 40 * 1024) GB_CUDA_OK(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMax));
+  GB_CUDA_OK(gb_launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), smem, stream, args...));
+  return GB_OK;
+}
+
+template <bool kFp8>
+int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
+  const int sms = gb_sm_count();
+  if (sms <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+  const int size = size_of(a->dtype), rsize = size_of(a->stream_dtype);
+  const Width width = width_of(a->H);
+  const bool full = a->gate && a->gate_rows == 1 && a->T > 1;
+  p.in_at[0] = 0;
+  p.in_at[1] = (uint32_t)(a->H * size);
+  if (full) p.in_at[2] = (uint32_t)(a->H * (size + rsize));
+  p.stage_bytes = (uint32_t)(a->H * (size * (full ? 2 : 1) + rsize));
+  const bool vec = width.v > 0 && a->H % 8 == 0 && whole(a->y, a->y_ld, size) && whole(a->r, a->r_ld, rsize) && whole(a->gate, a->gate_ld, size) &&
+                   whole(a->w, 0, 1) && whole(a->pw, 0, 1) && whole(p.h, 0, 1) && whole(p.s, 0, 1) && whole(p.q, 0, 1) &&
+                   p.stage_bytes <= (uint32_t)kRingMax - 1024;
+  return with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
+    using T = decltype(t);
+    using R = decltype(r);
+    if (!vec) {
+      GB_CUDA_OK(gb_launch(norm_any_kernel<T, R, kFp8>, dim3((unsigned)a->T), dim3(kAnyThreads), 0, stream, p));
+      return GB_OK;
+    }
+    return with_width(width, [&](auto v, auto most) -> int {
+      const Plan plan = plan_of(width.threads, p.stage_bytes);
+      p.stages = plan.stages;
+      const int64_t blocks = a->T < (int64_t)sms * plan.per_sm ? a->T : (int64_t)sms * plan.per_sm;
+      return launch_ring(norm_rows_kernel<T, R, decltype(v)::value, decltype(most)::value, kFp8>, (int)blocks, width.threads,
+                         (size_t)p.stages * p.stage_bytes, stream, p);
+    });
+  });
+}
+
+// How the rows are shared out for the backward pass: `blocks` shares, `per_gate` of them for the rows of a gate row (0: no sums of its gate).
+struct Shares { int64_t blocks; int per_gate; int64_t gates; };
+Shares shares_of(const gb_residual_norm_args* a, bool gate_sums, int64_t target) {
+  if (!gate_sums) return {a->T < target ? a->T : target, 0, 1};
+  const int64_t gates = a->T / a->gate_rows;
+  int64_t per = target / gates;
+  per = per < 1 ? 1 : per > a->gate_rows ? a->gate_rows : per;
+  return {gates * per, (int)per, gates};
+}
+
+struct GradPlan {
+  bool vec, gate_sums, gate_rows;
+  Width width;
+  Plan plan;
+  Shares shares;
+  uint32_t at[5], stage_bytes;
+  int64_t w_at, pw_at, g_at, means_at, bytes;
+};
+GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads* g) {
+  GradPlan r = {};
+  const int size = size_of(a->dtype), rsize = size_of(a->stream_dtype);
+  r.gate_rows = a->gate && a->gate_rows == 1 && a->T > 1;
+  r.gate_sums = a->gate && g->d_gate && !r.gate_rows;
+  r.width = width_of(a->H);
+  uint32_t at = 0;
+  auto place = [&](bool read, int bytes) {
+    const uint32_t here = read ? at : ~0u;
+    if (read) at += (uint32_t)(a->H * bytes);
+    return here;
+  };
+  const bool need_y = a->pw || (a->gate && g->d_gate);
+  r.vec = r.width.v > 0 && a->H % 8 == 0;
+  if (r.vec) {
+    r.at[0] = place(true, rsize);
+    r.at[1] = place(g->d_h != nullptr, size);
+    r.at[2] = place(g->d_stream != nullptr, rsize);
+    r.at[3] = place(need_y, size);
+    r.at[4] = place(r.gate_rows, size);
+    r.stage_bytes = at;
+    r.vec = at <= (uint32_t)kRingMax - 1024 && whole(a->y, a->y_ld, size) && whole(a->gate, a->gate_ld, size) && whole(a->w, 0, 1) && whole(a->pw, 0, 1) &&
+            whole(g->stream, 0, 1) && whole(g->d_h, g->d_h_ld, size) && whole(g->d_stream, g->d_stream_ld, rsize) && whole(g->d_y, 0, 1) &&
+            whole(g->d_r, 0, 1) && whole(g->d_gate, 0, 1);
+  }
+  if (r.vec) r.plan = plan_of(r.width.threads, r.stage_bytes);
+  const int64_t sms = gb_sm_count();
+  r.shares = shares_of(a, r.gate_sums, r.vec ? sms * r.plan.per_sm : 64);
+  auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
+  const int64_t sums = up(r.shares.blocks * a->H * 4);
+  r.pw_at = g->d_w ? sums : 0;
+  r.g_at = r.pw_at + (g->d_pw ? sums : 0);
+  r.means_at = r.g_at + (r.gate_sums ? sums : 0);
+  r.bytes = r.means_at + (r.vec ? 0 : up(a->T * 4));
+  return r;
+}
+
+int launch_join(JoinParams j, int64_t jobs, cudaStream_t stream) {
+  j.column_blocks = (j.H + 31) / 32;
+  GB_REQUIRE(jobs * j.column_blocks < (1ll << 31), "too many gate rows");
+  GB_CUDA_OK(gb_launch(norm_join_kernel, dim3((unsigned)(jobs * j.column_blocks)), dim3(kJoinThreads), 0, stream, j));
+  return GB_OK;
+}
+
+}  // namespace
+
+int gb_join_columns(const float* part, int64_t shares, int64_t columns, void* out, int dtype, cudaStream_t stream) {
+  JoinParams j = {};
+  j.part[0] = part; j.out[0] = out; j.type[0] = dtype;
+  j.H = columns; j.shares = shares; j.gates = 1;
+  return launch_join(j, 1, stream);
+}
+
+extern "C" {
+
+int gb_residual_norm(const gb_residual_norm_args* a, void* h, void* stream_out, float* rstd, float* post_rstd, void* stream) {
+  const int rc = check_args(a);
+  if (rc != GB_OK) return rc;
+  if (a->T == 0) return GB_OK;
+  GB_REQUIRE(a->y && a->r && h && stream_out, "null pointer argument");
+  NormParams p = params_of(a);
+  p.h = h; p.s = stream_out; p.rstd = rstd; p.post_rstd = a->pw ? post_rstd : nullptr;
+  return forward<false>(a, p, (cudaStream_t)stream);
+}
+
+int gb_residual_norm_fp8(const gb_residual_norm_args* a, int scale_rule, void* q, float* scale, void* stream_out, void* stream) {
+  const int rc = check_args(a);
+  if (rc != GB_OK) return rc;
+  if (a->T == 0) return GB_OK;
+  GB_REQUIRE(a->y && a->r && q && scale && stream_out, "null pointer argument");
+  GB_REQUIRE(scale_rule == GB_SCALE_RULE_RECIP || scale_rule == GB_SCALE_RULE_DIV, "unknown scale rule %d", scale_rule);
+  NormParams p = params_of(a);
+  p.q = static_cast<uint8_t*>(q); p.scale = scale; p.s = stream_out; p.scale_rule = scale_rule;
+  return forward<true>(a, p, (cudaStream_t)stream);
+}
+
+int64_t gb_residual_norm_grad_workspace_bytes(const gb_residual_norm_args* a, const gb_residual_norm_grads* g) {
+  return !a || !g || a->T < 1 || a->H < 1 ? 0 : grad_plan(a, g).bytes;
+}
+
+int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm_grads* g, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_args(a);
+  if (rc != GB_OK) return rc;
+  GB_REQUIRE(g != nullptr, "null arguments");
+  if (a->T == 0) return GB_OK;
+  GB_REQUIRE(g->stream && g->rstd && (!a->pw || (g->post_rstd && a->y)) && (!a->gate || a->y), "null pointer argument");
+  GB_REQUIRE((!g->d_h || g->d_h_ld >= a->H) && (!g->d_stream || g->d_stream_ld >= a->H), "rows that do not overlap expected");
+  GB_REQUIRE((!g->d_w || a->w) && (!g->d_pw || a->pw) && (!g->d_gate || a->gate), "a gradient of what there is not");
+  if (gb_sm_count() <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
+  const GradPlan plan = grad_plan(a, g);
+  if (workspace_bytes < plan.bytes || (plan.bytes > 0 && !workspace))
+    return gb_fail(GB_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)plan.bytes);
+  GB_REQUIRE(((uintptr_t)workspace & 15u) == 0, "the workspace must be 16-byte aligned");
+  NormParams p = params_of(a);
+  p.s = const_cast<void*>(g->stream);
+  p.rstd = const_cast<float*>(g->rstd); p.post_rstd = const_cast<float*>(g->post_rstd);
+  p.dh = g->d_h; p.ds = g->d_stream; p.dh_ld = g->d_h_ld; p.ds_ld = g->d_stream_ld;
+  p.dy = g->d_y; p.dr = g->d_r; p.dg = plan.gate_rows ? g->d_gate : nullptr;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part_w = g->d_w ? reinterpret_cast<float*>(ws + plan.w_at) : nullptr;
+  p.part_pw = g->d_pw ? reinterpret_cast<float*>(ws + plan.pw_at) : nullptr;
+  p.part_g = plan.gate_sums ? reinterpret_cast<float*>(ws + plan.g_at) : nullptr;
+  p.means = plan.vec ? nullptr : reinterpret_cast<float*>(ws + plan.means_at);
+  p.per_gate = plan.shares.per_gate;
+  const bool sums = p.part_w || p.part_pw || p.part_g;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rc2 = with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
+    using T = decltype(t);
+    using R = decltype(r);
+    if (!plan.vec) {
+      GB_CUDA_OK(gb_launch(norm_any_grad_kernel<T, R>, dim3((unsigned)a->T), dim3(kAnyThreads), 0, st, p));
+      if (!sums) return GB_OK;
+      const int64_t column_blocks = (a->H + kAnyThreads - 1) / kAnyThreads, blocks = column_blocks * plan.shares.blocks;
+      GB_REQUIRE(blocks < (1ll << 31), "too many gate rows");
+      GB_CUDA_OK(gb_launch(norm_any_columns_kernel<T, R>, dim3((unsigned)blocks), dim3(kAnyThreads), 0, st, p, column_blocks));
+      return GB_OK;
+    }
+    for (int k = 0; k < 5; ++k) p.in_at[k] = plan.at[k];
+    p.stage_bytes = plan.stage_bytes;
+    p.stages = plan.plan.stages;
+    return with_width(plan.width, [&](auto v, auto most) -> int {
+      return launch_ring(norm_rows_grad_kernel<T, R, decltype(v)::value, decltype(most)::value>, (int)plan.shares.blocks, plan.width.threads,
+                         (size_t)p.stages * p.stage_bytes, st, p);
+    });
+  });
+  if (rc2 != GB_OK || !sums) return rc2;
+  JoinParams j = {};
+  j.part[0] = p.part_w; j.part[1] = p.part_pw; j.part[2] = p.part_g;
+  j.out[0] = g->d_w; j.out[1] = g->d_pw; j.out[2] = g->d_gate;
+  j.type[0] = a->w_dtype; j.type[1] = a->pw_dtype; j.type[2] = a->dtype;
+  j.H = a->H; j.shares = plan.shares.blocks; j.gates = plan.shares.gates;
+  return launch_join(j, (p.part_w ? 1 : 0) + (p.part_pw ? 1 : 0) + (p.part_g ? j.gates : 0), st);
+}
+
+}  // extern "C"

@@ -48,7 +48,10 @@ namespace {
   F(gb_moe_mlp_pairs_workspace_bytes) F(gb_moe_combine) F(gb_gemv_hinted) F(gb_scales_e4m3) F(gb_moe_route_inv) \
   F(gb_moe_fp4_pass_rows) F(gb_moe_fp4_operand_bytes) F(gb_moe_fp4_rows) F(gb_moe_fp4_swiglu_rows) \
   F(gb_moe_gemv_fp4) F(gb_moe_gemm_fp4) F(gb_fp8_quantize_blocks) F(gb_moe_swiglu_fp8) F(gb_moe_permute_fp8) \
-  F(gb_gemm_fp8_blocks) F(gb_gemm_fp8_blocks_grouped) F(gb_linear_fp8_blocks) F(gb_moe_sort) F(gb_moe_sort_applies) F(gb_moe_permute) F(gb_moe_unpermute) F(gb_moe_unpermute_grad)
+  F(gb_gemm_fp8_blocks) F(gb_gemm_fp8_blocks_grouped) F(gb_linear_fp8_blocks) F(gb_moe_sort) F(gb_moe_sort_applies) F(gb_moe_permute) F(gb_moe_unpermute) F(gb_moe_unpermute_grad) \
+  F(gb_moe_topk) F(gb_moe_topk_grad) F(gb_moe_balance_workspace_bytes) F(gb_moe_balance) F(gb_moe_balance_grad) \
+  F(gb_residual_norm) F(gb_residual_norm_fp8) F(gb_residual_norm_grad_workspace_bytes) F(gb_residual_norm_grad) \
+  F(gb_linear_act) F(gb_linear_act_grad_workspace_bytes) F(gb_linear_act_grad)
 
 struct Lib {
 #define GB_FN(name) decltype(&::name) name = nullptr;
@@ -1004,13 +1007,13 @@ at::Tensor unpermute_rows(const at::Tensor& y, const at::Tensor& place, const at
 }
 
 // Tangents of forward-mode differentiation would be dropped without a word: nodes of the graph give the backward pass alone.
-void no_tangents(std::initializer_list<const at::Tensor*> all) {
-  for (const at::Tensor* t : all) GB_NEED(!t->defined() || !t->_fw_grad(0).defined(), "the sorted rows have no forward-mode derivatives");
+void no_tangents(std::initializer_list<const at::Tensor*> all, const char* what = "the sorted rows") {
+  for (const at::Tensor* t : all) GB_NEED(!t->defined() || !t->_fw_grad(0).defined(), std::string(what) + " have no forward-mode derivatives");
 }
 
-void first_derivatives_only(const at::Tensor& grad) {
-  GB_NEED(!at::GradMode::is_enabled(), "the sorted rows' gradients have no derivatives of their own (create_graph)");
-  no_tangents({&grad});
+void first_derivatives_only(const at::Tensor& grad, const char* what = "the sorted rows") {
+  GB_NEED(!at::GradMode::is_enabled(), std::string(what) + "' gradients have no derivatives of their own (create_graph)");
+  no_tangents({&grad}, what);
 }
 
 using torch::autograd::SavedVariable;
@@ -1133,6 +1136,433 @@ at::Tensor moe_unpermute(const at::Tensor& y, const at::Tensor& place, const at:
   return out;
 }
 
+// ------------------------------------------------------------------ the router
+at::Tensor given(const Opt& t) { return t.has_value() ? *t : at::Tensor(); }
+bool wants_grad(std::initializer_list<const at::Tensor*> all) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : all)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+void* current_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+// Logits [tokens, experts] as the kernels take them.
+int logits_code(const at::Tensor& logits, const char* what) {
+  need_cuda(logits);
+  GB_NEED(logits.dim() == 2 && logits.size(1) >= 1, std::string(what) + ": logits of shape [tokens, experts] expected");
+  GB_NEED(logits.size(1) <= 4096, std::string(what) + ": at most 4096 experts, got " + std::to_string(logits.size(1)));
+  return dtype_code(logits.scalar_type(), what);
+}
+// Their rows for a [T, E] that may be empty.
+struct LogitRows {
+  at::Tensor t;
+  int64_t T, E, ld;
+  explicit LogitRows(const at::Tensor& x) : T(x.size(0)), E(x.size(1)) {
+    const bool rows = x.stride(1) == 1 && x.stride(0) >= E;
+    t = rows ? x : x.contiguous();
+    ld = rows && T > 0 ? x.stride(0) : E;
+  }
+};
+
+constexpr const char* kRouter = "the router's weights";
+
+struct TopkBackward : torch::autograd::Node {
+  SavedVariable logits, ids;
+  int sigmoid, renormalize;
+  double scale;
+  TopkBackward(const at::Tensor& logits_, int sigmoid_, int renormalize_, double scale_)
+      : logits(logits_, false), sigmoid(sigmoid_), renormalize(renormalize_), scale(scale_) {}
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data();
+    ids.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    first_derivatives_only(grads[0], kRouter);
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {at::Tensor()};
+    const at::Tensor l = logits.unpack(), chosen = ids.unpack(), g = grads[0].contiguous();
+    const c10::cuda::CUDAGuard guard(l.device());
+    const LogitRows r(l);
+    at::Tensor d = fresh({r.T, r.E}, l.scalar_type(), l);
+    check(L.gb_moe_topk_grad(r.t.data_ptr(), dtype_code(l.scalar_type(), "moe_topk"), r.ld, chosen.data_ptr<int32_t>(), g.data_ptr<float>(), r.T, r.E,
+                             chosen.size(1), sigmoid, renormalize, (float)scale, d.data_ptr(), current_stream()));
+    return {d};
+  }
+};
+
+Two moe_topk(const at::Tensor& logits, int64_t topk, const std::string& score, bool renormalize, double scale) {
+  const int dt = logits_code(logits, "moe_topk");
+  no_tangents({&logits}, kRouter);
+  GB_NEED(score == "softmax" || score == "sigmoid", "moe_topk: score \"softmax\" or \"sigmoid\" expected, got \"" + score + "\"");
+  GB_NEED(topk >= 1 && topk <= 32 && topk <= logits.size(1), "moe_topk: top-" + std::to_string(topk) + " of " + std::to_string(logits.size(1)) +
+                                                                " experts: 1 to 32, and no more than there are, expected");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int sigmoid = score == "sigmoid";
+  std::shared_ptr<TopkBackward> node;
+  if (wants_grad({&logits})) node = node_of<TopkBackward>(torch::autograd::collect_next_edges(logits), logits, sigmoid, (int)renormalize, scale);
+  at::Tensor weights, ids;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const LogitRows r(logits);
+    weights = fresh({r.T, topk}, at::kFloat, logits);
+    ids = fresh({r.T, topk}, at::kInt, logits);
+    check(L.gb_moe_topk(r.t.data_ptr(), dt, r.ld, r.T, r.E, topk, sigmoid, renormalize, (float)scale, weights.data_ptr<float>(), ids.data_ptr<int32_t>(),
+                        current_stream()));
+  }
+  if (node) {
+    torch::autograd::set_history(weights, node);
+    node->ids = SavedVariable(ids, false);
+  }
+  return {weights, ids};
+}
+
+constexpr const char* kBalance = "the balance loss";
+
+struct BalanceBackward : torch::autograd::Node {
+  SavedVariable logits, mask, stats;
+  double coef, z_coef;
+  BalanceBackward(const at::Tensor& logits_, const at::Tensor& mask_, double coef_, double z_coef_)
+      : logits(logits_, false), mask(mask_, false), coef(coef_), z_coef(z_coef_) {}
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data();
+    mask.reset_data();
+    stats.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    first_derivatives_only(grads[0], kBalance);
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {at::Tensor()};
+    const at::Tensor l = logits.unpack(), m = mask.unpack(), s = stats.unpack(), g = grads[0];
+    const c10::cuda::CUDAGuard guard(l.device());
+    const LogitRows r(l);
+    at::Tensor d = fresh({r.T, r.E}, l.scalar_type(), l);
+    check(L.gb_moe_balance_grad(r.t.data_ptr(), dtype_code(l.scalar_type(), "moe_balance_loss"), r.ld,
+                                m.defined() ? static_cast<const uint8_t*>(m.data_ptr()) : nullptr, s.data_ptr<float>(), g.data_ptr<float>(), r.T, r.E,
+                                (float)coef, (float)z_coef, d.data_ptr(), current_stream()));
+    return {d};
+  }
+};
+
+Two moe_balance_loss(const at::Tensor& logits, const at::Tensor& ids, double coef, double z_coef, const Opt& mask_) {
+  const int dt = logits_code(logits, "moe_balance_loss");
+  no_tangents({&logits}, kBalance);
+  at::Tensor mask = given(mask_);
+  same_device(logits, {&ids});
+  GB_NEED(ids.dim() == 2 && ids.size(0) == logits.size(0) && ids.size(1) >= 1, "moe_balance_loss: expert ids of shape [tokens, top-k] expected");
+  GB_NEED(!ids.is_floating_point() && !ids.is_complex() && ids.scalar_type() != at::kBool, "expert ids are whole numbers");
+  GB_NEED(ids.numel() < (1ll << 31), "moe_balance_loss: fewer than 2^31 pairs expected");
+  if (mask.defined()) {
+    same_device(logits, {&mask});
+    GB_NEED(mask.scalar_type() == at::kBool && mask.dim() == 1 && mask.size(0) == logits.size(0), "moe_balance_loss: mask: one truth value a token expected");
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t T = logits.size(0), E = logits.size(1);
+  std::shared_ptr<BalanceBackward> node;
+  at::Tensor loss, counts, stats;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    if (mask.defined()) mask = mask.contiguous();
+    if (wants_grad({&logits})) node = node_of<BalanceBackward>(torch::autograd::collect_next_edges(logits), logits, mask, coef, z_coef);
+    if (T == 0) {
+      loss = at::zeros({}, logits.options().dtype(at::kFloat));
+      counts = at::zeros({E}, logits.options().dtype(at::kInt));
+      stats = at::zeros({E + 1}, logits.options().dtype(at::kFloat));
+    } else {
+      const LogitRows r(logits);
+      const bool wide = ids.scalar_type() == at::kLong;
+      const at::Tensor pairs = (wide || ids.scalar_type() == at::kInt ? ids : ids.to(at::kInt)).contiguous();
+      loss = fresh({}, at::kFloat, logits);
+      counts = fresh({E}, at::kInt, logits);
+      stats = fresh({E + 1}, at::kFloat, logits);
+      Arena a;
+      const int ws = a.add(L.gb_moe_balance_workspace_bytes(T, E));
+      a.alloc(logits);
+      check(L.gb_moe_balance(r.t.data_ptr(), dt, r.ld, pairs.data_ptr(), wide ? 8 : 4, mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr()) : nullptr,
+                             T, E, ids.size(1), (float)coef, (float)z_coef, loss.data_ptr<float>(), counts.data_ptr<int32_t>(), stats.data_ptr<float>(),
+                             a.ptr(ws), a.total, current_stream()));
+    }
+  }
+  if (node) {
+    torch::autograd::set_history(loss, node);
+    node->stats = SavedVariable(stats, false);
+  }
+  return {loss, counts};
+}
+
+// ------------------------------------------------------------------ the norms behind and in front of a block
+constexpr const char* kNorms = "the residual norms";
+
+// How many rows share a row of the gate: one per channel, per row, or per group of rows that lie together (ones behind the leading
+// dimensions that it has in common with the rows).
+int64_t rows_of_gate(const at::Tensor& gate, const at::Tensor& y) {
+  const int64_t n = y.dim() - 1, lead = gate.dim() - 1;
+  GB_NEED(gate.dim() >= 1 && lead <= n && gate.size(-1) == y.size(-1), "gate: one value for each channel expected, shared by rows or not");
+  int64_t rows = 1;
+  bool shared = true;
+  for (int64_t i = n - 1; i >= 0; --i) {
+    const int64_t at_ = i - (n - lead), size = at_ >= 0 ? gate.size(at_) : 1;
+    if (shared && size == 1) { rows *= y.size(i); continue; }
+    shared = false;
+    GB_NEED(size == y.size(i), "gate: the rows that share it must lie together: the leading sizes of the rows, then ones, expected");
+  }
+  return rows;
+}
+
+struct NormCall {
+  gb_residual_norm_args a{};
+  at::Tensor y, r, gate, w, pw;
+  NormCall(const at::Tensor& y_, const at::Tensor& r_, const at::Tensor& w_, const at::Tensor& pw_, const at::Tensor& gate_, double rs, double bs, double eps,
+           double offset) {
+    need_cuda(y_);
+    a.dtype = dtype_code(y_.scalar_type(), "residual_norm");
+    same_device(y_, {&r_});
+    GB_NEED(r_.sizes() == y_.sizes(), "residual_norm: rows and residual of one shape expected");
+    GB_NEED(r_.scalar_type() == y_.scalar_type() || r_.scalar_type() == at::kFloat, "residual_norm: the residual has the rows' type or float32");
+    a.stream_dtype = dtype_code(r_.scalar_type(), "residual_norm");
+    GB_NEED(y_.dim() >= 1 && y_.size(-1) >= 1, "rows of at least one value expected");
+    a.H = y_.size(-1);
+    a.T = y_.numel() / a.H;
+    GB_NEED(a.T < (1ll << 31) && a.H < (1ll << 31), "residual_norm: too many rows or channels");
+    const auto weight = [&](const at::Tensor& t, at::Tensor& to, const void*& p, int32_t& code, const char* name) {
+      if (!t.defined()) return;
+      same_device(y_, {&t});
+      GB_NEED(t.dim() == 1 && t.size(0) == a.H, std::string(name) + ": one value for each of " + std::to_string(a.H) + " channels expected");
+      code = dtype_code(t.scalar_type(), name);
+      to = t.contiguous();
+      p = to.data_ptr();
+    };
+    weight(w_, w, a.w, a.w_dtype, "weight");
+    weight(pw_, pw, a.pw, a.pw_dtype, "post_weight");
+    a.gate_rows = 1;
+    if (gate_.defined()) {
+      same_device(y_, {&gate_});
+      GB_NEED(gate_.scalar_type() == y_.scalar_type(), "gate: the rows' type expected");
+      const int64_t rows = rows_of_gate(gate_, y_);
+      if (a.T > 0) {
+        const RowsOf g(gate_);
+        gate = g.t;
+        a.gate = gate.data_ptr();
+        a.gate_ld = g.ld;
+        a.gate_rows = rows;
+      }
+    }
+    a.y_ld = a.r_ld = a.H;
+    if (a.T > 0) {
+      const RowsOf yr(y_), rr(r_);
+      y = yr.t; r = rr.t;
+      a.y_ld = yr.ld; a.r_ld = rr.ld;
+      a.y = y.data_ptr(); a.r = r.data_ptr();
+    }
+    a.residual_scale = (float)rs; a.branch_scale = (float)bs; a.eps = (float)eps; a.weight_offset = (float)offset;
+  }
+};
+
+struct NormBackward : torch::autograd::Node {
+  SavedVariable y, w, pw, gate, stream, rstd, post_rstd;
+  double rs, bs, eps, offset;
+  at::ScalarType stream_type;
+  NormBackward(const at::Tensor& y_, const at::Tensor& w_, const at::Tensor& pw_, const at::Tensor& gate_, double rs_, double bs_, double eps_, double offset_)
+      : y(y_, false), w(w_, false), pw(pw_, false), gate(gate_, false), rs(rs_), bs(bs_), eps(eps_), offset(offset_) {}
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&y, &w, &pw, &gate, &stream, &rstd, &post_rstd}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    for (const at::Tensor& g : grads) first_derivatives_only(g, kNorms);
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(5);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const at::Tensor rows = y.unpack(), weight = w.unpack(), post = pw.unpack(), gates = gate.unpack(), s = stream.unpack();
+    const c10::cuda::CUDAGuard guard(rows.device());
+    const NormCall c(rows, s, weight, post, gates, rs, bs, eps, offset);      // the stream lies in the residual's place: its type alone counts
+    const auto like = [&](int i, const at::Tensor& t) {
+      if (t.defined() && task_should_compute_output(i)) out[i] = c.a.T > 0 ? fresh(t.sizes(), t.scalar_type(), t) : at::zeros(t.sizes(), t.options());
+    };
+    like(0, rows);
+    like(1, s);
+    like(2, weight);
+    like(3, post);
+    like(4, gates);
+    if (c.a.T == 0) return out;
+    gb_residual_norm_grads g{};
+    at::Tensor dh, ds;
+    if (grads[0].defined()) { const RowsOf r(grads[0]); dh = r.t; g.d_h = dh.data_ptr(); g.d_h_ld = r.ld; }
+    if (grads[1].defined()) { const RowsOf r(grads[1]); ds = r.t; g.d_stream = ds.data_ptr(); g.d_stream_ld = r.ld; }
+    const at::Tensor r1 = rstd.unpack(), r2 = post_rstd.unpack();
+    g.stream = s.data_ptr();
+    g.rstd = r1.data_ptr<float>();
+    g.post_rstd = r2.defined() ? r2.data_ptr<float>() : nullptr;
+    const auto ptr = [&](int i) { return out[i].defined() ? out[i].data_ptr() : nullptr; };
+    g.d_y = ptr(0); g.d_r = ptr(1); g.d_w = ptr(2); g.d_pw = ptr(3); g.d_gate = ptr(4);
+    Arena a;
+    const int ws = a.add(L.gb_residual_norm_grad_workspace_bytes(&c.a, &g));
+    a.alloc(rows);
+    check(L.gb_residual_norm_grad(&c.a, &g, a.ptr(ws), a.total, current_stream()));
+    return out;
+  }
+};
+
+Two residual_norm(const at::Tensor& y, const at::Tensor& r, const Opt& weight, const Opt& post_weight, const Opt& gate, double rs, double bs, double eps,
+                  double offset) {
+  const at::Tensor w = given(weight), pw = given(post_weight), g = given(gate);
+  no_tangents({&y, &r, &w, &pw, &g}, kNorms);
+  std::shared_ptr<NormBackward> node;
+  if (wants_grad({&y, &r, &w, &pw, &g}))
+    node = node_of<NormBackward>(torch::autograd::collect_next_edges(y, r, w, pw, g), y, w, pw, g, rs, bs, eps, offset);
+  at::Tensor h, stream, rstd, post_rstd;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    need_cuda(y);
+    const c10::cuda::CUDAGuard guard(y.device());
+    const NormCall c(y, r, w, pw, g, rs, bs, eps, offset);
+    h = fresh(y.sizes(), y.scalar_type(), y);
+    stream = fresh(y.sizes(), r.scalar_type(), y);
+    if (node) {
+      rstd = fresh({c.a.T}, at::kFloat, y);
+      if (pw.defined()) post_rstd = fresh({c.a.T}, at::kFloat, y);
+    }
+    check(L.gb_residual_norm(&c.a, h.data_ptr(), stream.data_ptr(), node ? rstd.data_ptr<float>() : nullptr,
+                             post_rstd.defined() ? post_rstd.data_ptr<float>() : nullptr, current_stream()));
+  }
+  if (node) {
+    node->stream = SavedVariable(stream.detach(), false);          // without the node that will hold it; changes in place are still seen
+    node->rstd = SavedVariable(rstd, false);
+    node->post_rstd = SavedVariable(post_rstd, false);
+    torch::autograd::set_history(h, node);
+    torch::autograd::set_history(stream, node);
+  }
+  return {h, stream};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm_fp8(const at::Tensor& y, const at::Tensor& r, const Opt& weight, const Opt& post_weight, const Opt& gate,
+                                                                 double rs, double bs, double eps, double offset, int rule) {
+  const at::Tensor w = given(weight), pw = given(post_weight), g = given(gate);
+  GB_NEED(!wants_grad({&y, &r, &w, &pw, &g}), "residual_norm_fp8 has no gradient: call it under no_grad, or residual_norm");
+  no_tangents({&y, &r, &w, &pw, &g}, kNorms);
+  need_cuda(y);
+  const c10::cuda::CUDAGuard guard(y.device());
+  const NormCall c(y, r, w, pw, g, rs, bs, eps, offset);
+  at::Tensor q = fresh(y.sizes(), at::kFloat8_e4m3fn, y), scale = fresh(with_last(y, blocks(c.a.H)), at::kFloat, y), stream = fresh(y.sizes(), r.scalar_type(), y);
+  check(L.gb_residual_norm_fp8(&c.a, rule, q.data_ptr(), scale.data_ptr<float>(), stream.data_ptr(), current_stream()));
+  return {q, scale, stream};
+}
+
+// ------------------------------------------------------------------ 16-bit linears with their epilogue
+constexpr const char* kLinears = "the 16-bit linears";
+
+int half_code(const at::Tensor& t) {
+  if (t.scalar_type() == at::kBFloat16) return GB_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return GB_DTYPE_FP16;
+  throw py::type_error("linear_act takes bfloat16 or float16");
+}
+
+// Rows that TMA can fetch: whole 16-byte pieces, copied where they are not.
+struct PieceRows {
+  at::Tensor t;
+  int64_t ld;
+  explicit PieceRows(const at::Tensor& x) {
+    const RowsOf r(x);
+    t = r.t; ld = r.ld;
+    if (ld % 8 != 0 || ((uintptr_t)t.data_ptr() & 15u) != 0) {
+      t = at::empty({r.M, r.K}, x.options(), at::MemoryFormat::Contiguous).copy_(x.reshape({r.M, r.K}));
+      ld = r.K;
+    }
+  }
+};
+
+struct LinearActBackward : torch::autograd::Node {
+  SavedVariable x, w, z;
+  int act;
+  bool bias, residual;
+  std::vector<int64_t> x_shape;
+  LinearActBackward(const at::Tensor& x_, const at::Tensor& w_, int act_, bool bias_, bool residual_)
+      : x(w_.requires_grad() ? x_ : at::Tensor(), false), w(w_, false), act(act_), bias(bias_), residual(residual_), x_shape(x_.sizes().vec()) {}
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&x, &w, &z}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    first_derivatives_only(grads[0], kLinears);
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    if (residual && task_should_compute_output(3)) out[3] = grads[0];
+    const at::Tensor weight = w.unpack(), rows = x.unpack(), kept = z.unpack();
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const int64_t N = weight.size(0), K = weight.size(1), M = grads[0].numel() / N;
+    const bool need_x = task_should_compute_output(0), need_w = rows.defined() && task_should_compute_output(1), need_b = bias && task_should_compute_output(2);
+    if (!need_x && !need_w && !need_b) return out;
+    if (M == 0) {
+      if (need_x) out[0] = at::zeros(x_shape, weight.options());
+      if (need_w) out[1] = at::zeros({N, K}, weight.options());
+      if (need_b) out[2] = at::zeros({N}, weight.options());
+      return out;
+    }
+    if (need_x) out[0] = fresh(x_shape, weight.scalar_type(), weight);
+    if (need_w) out[1] = fresh({N, K}, weight.scalar_type(), weight);
+    if (need_b) out[2] = fresh({N}, weight.scalar_type(), weight);
+    const RowsOf g(grads[0]);
+    const at::Tensor wc = need_x ? PieceRows(weight.contiguous()).t : weight;
+    at::Tensor xr;
+    int64_t x_ld = K;
+    if (need_w) { const PieceRows r(rows); xr = r.t; x_ld = r.ld; }
+    const bool whole = g.ld % 8 == 0 && ((uintptr_t)g.t.data_ptr() & 15u) == 0;
+    Arena a;
+    const int ws = a.add(L.gb_linear_act_grad_workspace_bytes(M, N, K, act, need_x, need_w, need_b, whole));
+    a.alloc(weight);
+    const auto ptr = [&](int i) { return out[i].defined() ? out[i].data_ptr() : nullptr; };
+    check(L.gb_linear_act_grad(g.t.data_ptr(), g.ld, kept.defined() ? kept.data_ptr() : nullptr, need_w ? xr.data_ptr() : nullptr, x_ld,
+                               need_x ? wc.data_ptr() : nullptr, half_code(weight), M, N, K, act, ptr(0), ptr(1), ptr(2), a.ptr(ws), a.total, current_stream()));
+    return out;
+  }
+};
+
+at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w, const Opt& bias, int act, const Opt& residual) {
+  const at::Tensor b = given(bias), r = given(residual);
+  no_tangents({&x, &w, &b, &r}, kLinears);
+  same_device(x, {&w});
+  const int dt = half_code(x);
+  GB_NEED(w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1, "linear_act: a weight [out, in] expected");
+  const int64_t N = w.size(0), K = w.size(1);
+  GB_NEED(x.dim() >= 1 && x.size(-1) == K, "linear_act: rows of " + std::to_string(K) + " values expected");
+  GB_NEED(K % 8 == 0, "linear_act: rows of " + std::to_string(K) + " values; they are fetched in 16-byte pieces, a multiple of 8 is needed");
+  GB_NEED(w.scalar_type() == x.scalar_type(), "linear_act: rows and weight of one type expected");
+  const std::vector<int64_t> shape = with_last(x, N);
+  if (b.defined()) {
+    same_device(x, {&b});
+    GB_NEED(b.scalar_type() == x.scalar_type() && b.dim() == 1 && b.size(0) == N, "linear_act: bias: " + std::to_string(N) + " values of the rows' type expected");
+  }
+  if (r.defined()) {
+    same_device(x, {&r});
+    GB_NEED(r.scalar_type() == x.scalar_type() && r.sizes() == at::IntArrayRef(shape), "linear_act: a residual of the result's shape and type expected");
+  }
+  std::shared_ptr<LinearActBackward> node;
+  if (wants_grad({&x, &w, &b, &r})) node = node_of<LinearActBackward>(torch::autograd::collect_next_edges(x, w, b, r), x, w, act, b.defined(), r.defined());
+  at::Tensor y, z;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(x.device());
+    y = fresh(shape, x.scalar_type(), x);
+    if (y.numel() > 0) {
+      const PieceRows xr(x);
+      const at::Tensor wc = PieceRows(w.contiguous()).t, bc = b.defined() ? b.contiguous() : b;
+      at::Tensor rt;
+      int64_t r_ld = N;
+      if (r.defined()) { const RowsOf rr(r); rt = rr.t; r_ld = rr.ld; }
+      if (node && act != GB_EPI_NONE && wants_grad({&x, &w, &b})) z = fresh({y.numel() / N, N}, x.scalar_type(), x);
+      check(L.gb_linear_act(xr.t.data_ptr(), xr.ld, wc.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, rt.defined() ? rt.data_ptr() : nullptr, r_ld, dt,
+                            y.numel() / N, N, K, act, y.data_ptr(), z.defined() ? z.data_ptr() : nullptr, current_stream()));
+    }
+  }
+  if (node) {
+    torch::autograd::set_history(y, node);
+    node->z = SavedVariable(z, false);
+  }
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gb_torch, m) {
@@ -1160,5 +1590,10 @@ PYBIND11_MODULE(_gb_torch, m) {
   m.def("moe_sort", &moe_sort, Free());
   m.def("moe_permute", &moe_permute, Free());
   m.def("moe_unpermute", &moe_unpermute, Free());
+  m.def("moe_topk", &moe_topk, Free());
+  m.def("moe_balance_loss", &moe_balance_loss, Free());
+  m.def("residual_norm", &residual_norm, Free());
+  m.def("residual_norm_fp8", &residual_norm_fp8, Free());
+  m.def("linear_act", &linear_act, Free());
   m.def("shared_row", &shared_row, py::arg("plans"), py::arg("x"), py::arg("rule"), py::arg("routes") = py::none());
 }

@@ -724,3 +724,62 @@ def moe_fp8_blocks(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, 
     and the result have its type."""
     return nat.host("routed block-scaled layer").moe_fp8_blocks(x, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_base,
                                                                 _rule(scale_rule))
+
+
+# ------------------------------------------------------------------ the router
+def moe_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", renormalize: bool = True, scale: float = 1.0):
+    """A token's experts: (weights [T, top-k] fp32, ids [T, top-k] int32) of the ``topk`` largest logits of each row [T, E] (bf16, fp16 or
+    fp32; E up to 4096, top-k up to 32), ties to the lowest expert, NaN above all.  An expert at -inf is never chosen; slots that find
+    none get id -1 and weight 0, which :func:`moe_sort` drops.  weights = scale * c, over the sum of the chosen c where ``renormalize``,
+    with c the softmax of the row or the sigmoid of the logits, in fp32 (chosen scores that are all zero give zero).  Differentiable in
+    ``logits``, by backward passes alone."""
+    return nat.host("router").moe_topk(logits, topk, score, renormalize, scale)
+
+
+def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, coef: float = 1e-2, z_coef: float = 0.0,
+                     mask: torch.Tensor | None = None):
+    """(loss, counts): the experts' balance loss, a fp32 scalar, and the int32 pairs of each of the E experts.  Over the n tokens that
+    count - those of ``mask`` [T] (bool, None: all) that have a logit above -inf -
+    loss = coef * E * sum_e f_e P_e + z_coef * mean(logsumexp^2), with f_e = counts_e / (n top-k) and P_e the mean of softmax(logits)_e: coef for a
+    routing that is even.  Ids outside of [0, E) are not counted; without tokens all is zero.  Differentiable in ``logits``, by
+    backward passes alone (the counts are constants)."""
+    return nat.host("balance loss").moe_balance_loss(logits, topk_ids, coef, z_coef, mask)
+
+
+# ------------------------------------------------------------------ the norms behind and in front of a block
+def residual_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, *, post_weight: torch.Tensor | None = None,
+                  gate: torch.Tensor | None = None, residual_scale: float = 1.0, branch_scale: float = 1.0, eps: float = 1e-6,
+                  weight_offset: float = 0.0):
+    """A block's output onto the residual stream and the next block's norm, one pass: (h, stream) with
+    stream = residual_scale * residual + branch_scale * gate * u, u = y or, with ``post_weight``, rms(y) * (weight_offset + post_weight);
+    h = rms(stream) * (weight_offset + weight), taken from the stream as it is stored.  rms(v) = v / sqrt(mean(v^2) + eps) over the last
+    dimension, in fp32.  ``y`` [.., H] bf16, fp16 or fp32, ``residual`` of its type or fp32 (h and stream have theirs); weights [H] of any of the
+    three; ``gate`` of y's type: [H], y's shape, or y's leading sizes followed by ones ([batch, 1, H]: one for each sequence).
+    Differentiable in all five, by backward passes alone; the stream is what the backward pass reads again."""
+    return nat.host("residual norm").residual_norm(y, residual, weight, post_weight, gate, residual_scale, branch_scale, eps, weight_offset)
+
+
+def residual_norm_fp8(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, *, post_weight: torch.Tensor | None = None,
+                      gate: torch.Tensor | None = None, residual_scale: float = 1.0, branch_scale: float = 1.0, eps: float = 1e-6,
+                      weight_offset: float = 0.0, scale_rule: str = "recip"):
+    """:func:`residual_norm` whose h goes straight into block-scaled layers: (q, scale, stream), q and scale as
+    :func:`fp8_quantize_blocks` gives them for h in fp32, h taken from the stream before its rounding.  Inference only: inputs that ask
+    for a gradient are refused."""
+    return nat.host("residual norm").residual_norm_fp8(y, residual, weight, post_weight, gate, residual_scale, branch_scale, eps, weight_offset,
+                                                       _rule(scale_rule))
+
+
+# ------------------------------------------------------------------ 16-bit linears with their epilogue
+_EPILOGUES = {None: nat.EPI_NONE, "none": nat.EPI_NONE, "relu": nat.EPI_RELU, "gelu": nat.EPI_GELU, "gelu_tanh": nat.EPI_GELU_TANH,
+              "silu": nat.EPI_SILU}
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x . weight^T + bias) + residual, one kernel: ``x`` [.., K] and ``weight`` [N, K] bf16 or fp16, ``bias`` [N] and ``residual`` [.., N] of
+    their type, sums and epilogue in fp32, one rounding.  ``activation``: None, "relu", "gelu" (by erf), "gelu_tanh" or "silu".  K is a
+    multiple of 8.  Differentiable in all four, by backward passes alone; with an activation the forward pass keeps its argument,
+    rounded to the type."""
+    if activation not in _EPILOGUES:
+        raise ValueError(f"linear_act: activation {activation!r}; None, relu, gelu, gelu_tanh or silu expected")
+    return nat.host("16-bit linear").linear_act(x, weight, bias, _EPILOGUES[activation], residual)

@@ -486,6 +486,70 @@ GB_API int gb_moe_unpermute_grad(const void* d_out, const void* y, int dtype, co
                                  const float* weights, int64_t T, int64_t topk, int64_t H, void* d_y, float* d_w,
                                  void* stream);
 
+/* ---- 16-bit linears with their epilogue ------------------------------------------ */
+/* gb_linear_act: z = X W^T + bias, Y = act(z) + R: X [M, K] with rows x_ld elements apart, W [N, K], bias [N] or NULL, R [M, N] with rows
+ * r_ld apart or NULL, Y [M, N], all bf16 or all fp16, sums and epilogue in fp32, one rounding.  K and x_ld are multiples of 8,
+ * operands 16-byte aligned.  z (NULL: not kept) is what gb_linear_act_grad takes, [M, N].
+ * gb_linear_act_grad: of dY (rows dy_ld apart), dX = dz W, dW = dz^T X, dbias = column sums of dz with dz = dY act'(z) rounded to
+ * the type (the column sums take it before); any of the three NULL.  The workspace's size depends on what is asked for and on
+ * dy_whole: dY 16-byte aligned and dy_ld a multiple of 8. */
+enum { GB_EPI_NONE = 0, GB_EPI_RELU = 1, GB_EPI_GELU = 2, GB_EPI_GELU_TANH = 3, GB_EPI_SILU = 4 };
+GB_API int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, const void* r, int64_t r_ld, int dtype,
+                         int64_t M, int64_t N, int64_t K, int act, void* y, void* z, void* stream);
+GB_API int64_t gb_linear_act_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int rows, int weight, int bias,
+                                                  int dy_whole);
+GB_API int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void* x, int64_t x_ld, const void* w,
+                              int dtype, int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* dbias,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- the router's choice and the experts' balance ----------------------------- */
+/* gb_moe_topk: of each row of logits [T, E] (dtype, rows `ld` elements apart; E <= 4096), the topk <= 32 largest, ties to
+ * the lowest expert, an expert at -inf never: ids [T, topk], -1 where no expert is left, and weights scale * c_j (over the
+ * sum of the chosen ones where renormalize), c the softmax or the sigmoid of the logits, 0 without an expert.
+ * gb_moe_topk_grad: d_logits [T, E] (dtype) of d_weights [T, topk].
+ * gb_moe_balance: loss = coef E sum_e f_e P_e + z_coef mean(z^2) over the n tokens that count (mask NULL: all, else those with a byte
+ * that is not 0; a token without a logit above -inf counts not), f_e = counts_e / (n topk), P_e the mean of the softmax, z the
+ * log of the sum of exponentials; ids of 4 or 8 bytes, those outside of [0, E) are not counted.  stats [E + 1] is what
+ * gb_moe_balance_grad needs of it: d_logits [T, E] = *d_loss * d loss / d logits, rows that do not count zero. */
+GB_API int gb_moe_topk(const void* logits, int dtype, int64_t ld, int64_t T, int64_t E, int64_t topk, int sigmoid,
+                       int renormalize, float scale, float* weights, int32_t* ids, void* stream);
+GB_API int gb_moe_topk_grad(const void* logits, int dtype, int64_t ld, const int32_t* ids, const float* d_weights, int64_t T,
+                            int64_t E, int64_t topk, int sigmoid, int renormalize, float scale, void* d_logits, void* stream);
+GB_API int64_t gb_moe_balance_workspace_bytes(int64_t T, int64_t E);
+GB_API int gb_moe_balance(const void* logits, int dtype, int64_t ld, const void* ids, int id_bytes, const uint8_t* mask,
+                          int64_t T, int64_t E, int64_t topk, float coef, float z_coef, float* loss, int32_t* counts,
+                          float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+GB_API int gb_moe_balance_grad(const void* logits, int dtype, int64_t ld, const uint8_t* mask, const float* stats,
+                               const float* d_loss, int64_t T, int64_t E, float coef, float z_coef, void* d_logits,
+                               void* stream);
+
+/* ---- the norms behind and in front of a block ---------------------------------- */
+/* u = y, or rms(y) * (weight_offset + pw); x = residual_scale * r + branch_scale * gate * u, stored as the stream;
+ * h = rms(x as stored) * (weight_offset + w), in E4M3 blocks of x before its rounding.  rms(v) = v / sqrt(mean v^2 + eps).
+ * y, gate and h have `dtype`, r and the stream `stream_dtype` (dtype or fp32); outputs are contiguous. */
+typedef struct gb_residual_norm_args {
+  int64_t T, H;
+  const void *y, *r;                    /* rows y_ld and r_ld elements apart */
+  const void *gate, *w, *pw;            /* NULL: ones; pw NULL: no norm behind the block */
+  int64_t y_ld, r_ld, gate_ld;
+  int64_t gate_rows;                    /* rows that share a row of the gate: T for one per channel, 1 for one per row */
+  int32_t dtype, stream_dtype, w_dtype, pw_dtype;
+  float residual_scale, branch_scale, eps, weight_offset;
+} gb_residual_norm_args;
+typedef struct gb_residual_norm_grads {
+  const void* stream;                   /* as stored */
+  const float *rstd, *post_rstd;        /* [T] of the forward pass; post_rstd with pw alone */
+  const void *d_h, *d_stream;           /* NULL: none */
+  int64_t d_h_ld, d_stream_ld;
+  void *d_y, *d_r, *d_w, *d_pw, *d_gate;  /* NULL: not asked for; types of what they are gradients of */
+} gb_residual_norm_grads;
+GB_API int gb_residual_norm(const gb_residual_norm_args* a, void* h, void* stream_out, float* rstd, float* post_rstd, void* stream);
+GB_API int gb_residual_norm_fp8(const gb_residual_norm_args* a, int scale_rule, void* q, float* scale, void* stream_out,
+                                void* stream);
+GB_API int64_t gb_residual_norm_grad_workspace_bytes(const gb_residual_norm_args* a, const gb_residual_norm_grads* g);
+GB_API int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm_grads* g, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 /* Kernel launches this library has issued in this process so far (launches recorded into a
  * CUDA graph count once, at capture).  No reference counterpart; used by the benchmark to
  * report how many of its own kernels a step runs. */
