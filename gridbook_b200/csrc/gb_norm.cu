@@ -71,29 +71,124 @@ GB_DEVINL float value_of(const void* p, int type, int64_t c) {
   return __ldg(static_cast<const float*>(p) + c);
 }
 
-// Eight values from a column on.
-template <typename T>
-GB_DEVINL void load8(const typename T::word* p, float (&v)[8]) {
-  unpack16<T>(*reinterpret_cast<const uint4*>(p), v);
-  if constexpr (sizeof(typename T::word) == 4) unpack16<T>(*reinterpret_cast<const uint4*>(p + 4), v + 4);
+// Eight columns of a row in fp32, as four pairs: products and sums go two at a time (a third fewer instructions, which the norms are
+// bound by next to memory).
+struct F8 { uint64_t v[4]; };
+GB_DEVINL uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
-template <typename T>
-GB_DEVINL void store8(typename T::word* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = pack16<T>(v);
-  if constexpr (sizeof(typename T::word) == 4) *reinterpret_cast<uint4*>(p + 4) = pack16<T>(v + 4);
-}
-GB_DEVINL void weights8(const void* p, int type, int64_t c, float offset, float (&v)[8]) {
-  if (!p) {
+GB_DEVINL uint64_t both(float v) { return pack_f32x2(v, v); }
+GB_DEVINL F8 all8(float v) { const uint64_t b = both(v); return {{b, b, b, b}}; }
+#define GB_EACH for (int i_ = 0; i_ < 4; ++i_)
+GB_DEVINL F8 operator*(const F8& a, const F8& b) {
+  F8 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 1.0f;
-    return;
+  GB_EACH r.v[i_] = mul_f32x2(a.v[i_], b.v[i_]);
+  return r;
+}
+GB_DEVINL F8 operator*(const F8& a, uint64_t b) { return a * F8{{b, b, b, b}}; }
+GB_DEVINL F8 operator+(const F8& a, const F8& b) {
+  F8 r;
+#pragma unroll
+  GB_EACH r.v[i_] = add_f32x2(a.v[i_], b.v[i_]);
+  return r;
+}
+GB_DEVINL F8 fma8(const F8& a, const F8& b, const F8& c) {
+  F8 r;
+#pragma unroll
+  GB_EACH r.v[i_] = fma_f32x2(a.v[i_], b.v[i_], c.v[i_]);
+  return r;
+}
+GB_DEVINL F8 fma8(const F8& a, uint64_t b, const F8& c) { return fma8(a, F8{{b, b, b, b}}, c); }
+GB_DEVINL void dot8(const F8& a, const F8& b, uint64_t& sum) {          // two sums: of the even columns and the odd ones
+#pragma unroll
+  GB_EACH sum = fma_f32x2(a.v[i_], b.v[i_], sum);
+}
+#undef GB_EACH
+GB_DEVINL float halves(uint64_t v) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+  return lo + hi;
+}
+GB_DEVINL uint64_t words(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+// As they lie in memory.
+template <typename T>
+struct Raw8 { uint4 q[sizeof(typename T::word) / 2]; };
+template <typename T>
+GB_DEVINL Raw8<T> raw8(const typename T::word* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(typename T::word) / 2; ++i) r.q[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T>
+GB_DEVINL F8 f8(const Raw8<T>& r) {
+  if constexpr (sizeof(typename T::word) == 4) return {{words(r.q[0].x, r.q[0].y), words(r.q[0].z, r.q[0].w), words(r.q[1].x, r.q[1].y), words(r.q[1].z, r.q[1].w)}};
+  else {
+    F8 f;
+    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, Bf16>) f.v[i] = words(w[i] << 16, w[i] & 0xFFFF0000u);
+      else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f.v[i] = pack_f32x2(h.x, h.y);
+      }
+    }
+    return f;
   }
-  if (type == GB_DTYPE_BF16) load8<Bf16>(static_cast<const uint16_t*>(p) + c, v);
-  else if (type == GB_DTYPE_FP16) load8<Fp16>(static_cast<const uint16_t*>(p) + c, v);
-  else load8<Fp32>(static_cast<const uint32_t*>(p) + c, v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += offset;
 }
+template <typename T>
+GB_DEVINL F8 load8(const typename T::word* p) { return f8<T>(raw8<T>(p)); }
+template <typename T>
+GB_DEVINL Raw8<T> rounded(const F8& f) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("mov.b64 {%0, %1}, %2;" : "=r"(w[2 * i]), "=r"(w[2 * i + 1]) : "l"(f.v[i]));
+  Raw8<T> r;
+  if constexpr (sizeof(typename T::word) == 4) {
+    r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.q[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float lo = __uint_as_float(w[2 * i]), hi = __uint_as_float(w[2 * i + 1]);
+      if constexpr (std::is_same_v<T, Bf16>) h[i] = gb_pack_bf16x2(lo, hi);
+      else { const __half2 v = __floats2half2_rn(lo, hi); h[i] = *reinterpret_cast<const uint32_t*>(&v); }
+    }
+    r.q[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  }
+  return r;
+}
+template <typename T>
+GB_DEVINL void store8(typename T::word* p, const Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(typename T::word) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.q[i];
+}
+template <typename T>
+GB_DEVINL void store8(typename T::word* p, const F8& f) { store8<T>(p, rounded<T>(f)); }
+// Weights of eight columns, o + w; kRaw: of the rows' own type.
+template <typename T, bool kRaw>
+struct Weights {
+  const void* p;
+  int type;
+  float offset;
+  GB_DEVINL F8 get(int c) const {
+    F8 v;
+    if (kRaw) v = load8<T>(static_cast<const typename T::word*>(p) + c);
+    else if (type == GB_DTYPE_BF16) v = load8<Bf16>(static_cast<const uint16_t*>(p) + c);
+    else if (type == GB_DTYPE_FP16) v = load8<Fp16>(static_cast<const uint16_t*>(p) + c);
+    else v = load8<Fp32>(static_cast<const uint32_t*>(p) + c);
+    return offset == 0.0f ? v : v + all8(offset);
+  }
+};
 template <typename R>
 GB_DEVINL float as_stored(float v) { return to_f32<R>(from_f32<R>(v)); }
 
@@ -103,16 +198,16 @@ struct Ring {
   uint64_t* full;
   volatile int* gave_up;
   int stages;
-  GB_DEVINL void wait(int i, int* status, int code) const {
-    if (!gb_mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u)) {
+  GB_DEVINL void wait(int i, int s, int* status, int code) const {     // step i, in stage s
+    if (!gb_mbar_wait(&full[s], (uint32_t)(i / stages) & 1u)) {
       atomicMin((int*)gave_up, i);
       atomicExch(status, code);
     }
   }
 };
 
-template <typename T, typename R, int kV, int kThreads, bool kFp8>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, typename R, int kV, int kThreads, bool kFp8, bool kRaw>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 norm_rows_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
   using rword = typename R::word;
@@ -120,8 +215,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
   __shared__ uint64_t full[kMostStages];
   __shared__ float red[2][32];
   __shared__ int gave_up;
-  const int tid = threadIdx.x;
-  const int64_t step = gridDim.x;
+  const int tid = threadIdx.x, H = (int)p.H, T_ = (int)p.T, step = (int)gridDim.x;
   gb_pdl_launch_dependents();
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
@@ -130,92 +224,81 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
   }
   __syncthreads();
   gb_pdl_wait();
-  const uint32_t y_bytes = (uint32_t)(p.H * sizeof(word)), r_bytes = (uint32_t)(p.H * sizeof(rword));
+  const uint32_t y_bytes = (uint32_t)(H * (int)sizeof(word)), r_bytes = (uint32_t)(H * (int)sizeof(rword));
+  const bool own_gate = p.in_at[2] != ~0u;               // every row has a gate of its own
   auto fetch = [&](int64_t t, int s) {
     uint8_t* st = ring + (size_t)s * p.stage_bytes;
-    const bool gate = p.in_at[2] != ~0u;
-    gb_mbar_expect_tx(&full[s], y_bytes + r_bytes + (gate ? y_bytes : 0u));
+    gb_mbar_expect_tx(&full[s], p.stage_bytes);
     gb_bulk_g2s(st + p.in_at[0], static_cast<const word*>(p.y) + t * p.y_ld, y_bytes, &full[s]);
     gb_bulk_g2s(st + p.in_at[1], static_cast<const rword*>(p.r) + t * p.r_ld, r_bytes, &full[s]);
-    if (gate) gb_bulk_g2s(st + p.in_at[2], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
+    if (own_gate) gb_bulk_g2s(st + p.in_at[2], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
   };
   if (tid == 0)
     for (int s = 0; s < p.stages; ++s)
-      if (blockIdx.x + s * step < p.T) fetch(blockIdx.x + s * step, s);
+      if ((int64_t)blockIdx.x + (int64_t)s * step < T_) fetch((int64_t)blockIdx.x + (int64_t)s * step, s);
+  const bool one_gate = p.gate && p.gate_rows == p.T;    // the same for all rows
+  const Weights<T, kRaw> w{p.w, p.w_type, p.offset}, pw{p.pw, p.pw_type, p.offset};
   const Ring wheel{full, &gave_up, p.stages};
-  int turn = 0, i = 0;
-  for (int64_t t = blockIdx.x; t < p.T; t += step, ++i) {
-    const int s = i % p.stages;
+  int turn = 0, i = 0, s = 0;
+  for (int64_t t = blockIdx.x; t < T_; t += step, ++i) {
     const uint8_t* st = ring + (size_t)s * p.stage_bytes;
-    wheel.wait(i, p.status, 91);
-    float x[kV][8], rp = 1.0f, sum = 0.0f;
+    wheel.wait(i, s, p.status, 91);
+    F8 x[kV];
+    float rp = 1.0f;
+    uint64_t sum = 0;
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
-      if (c < p.H) {
-        load8<T>(reinterpret_cast<const word*>(st + p.in_at[0]) + c, x[k]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(x[k][j], x[k][j], sum);
+      const int c = (k * (int)blockDim.x + tid) * 8;
+      x[k] = all8(0.0f);
+      if (c < H) {
+        x[k] = load8<T>(reinterpret_cast<const word*>(st + p.in_at[0]) + c);
+        dot8(x[k], x[k], sum);
       }
     }
-    if (p.pw) rp = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
-    sum = 0.0f;
+    if (p.pw) rp = rsqrtf(fmaf(block_sum(halves(sum), red, turn), p.inv_h, p.eps));
+    sum = 0;
+    const word* gate_row = static_cast<const word*>(p.gate);
+    if (gate_row && !one_gate && !own_gate) gate_row += (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
+    rword* out = static_cast<rword*>(p.s) + t * H;
+    const uint64_t scale_r = both(p.a), scale_u = both(p.b * rp);
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
-      if (c < p.H) {
-        float v[8];
-        if (p.pw) {
-          weights8(p.pw, p.pw_type, c, p.offset, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[k][j] *= rp * v[j];
-        }
-        if (p.gate) {
-          if (p.in_at[2] != ~0u) load8<T>(reinterpret_cast<const word*>(st + p.in_at[2]) + c, v);
-          else load8<T>(static_cast<const word*>(p.gate) + t / p.gate_rows * p.gate_ld + c, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[k][j] *= v[j];
-        }
-        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[1]) + c, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[k][j] = fmaf(p.b, x[k][j], p.a * v[j]);
-          if (!kFp8) x[k][j] = as_stored<R>(x[k][j]);
-          sum = fmaf(x[k][j], x[k][j], sum);
-        }
-        store8<R>(static_cast<rword*>(p.s) + t * p.H + c, x[k]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+      const int c = (k * (int)blockDim.x + tid) * 8;
+      if (c < H) {
+        if (p.pw) x[k] = x[k] * pw.get(c);
+        if (p.gate) x[k] = x[k] * load8<T>(own_gate ? reinterpret_cast<const word*>(st + p.in_at[2]) + c : gate_row + c);
+        x[k] = fma8(x[k], scale_u, load8<R>(reinterpret_cast<const rword*>(st + p.in_at[1]) + c) * scale_r);
+        const Raw8<R> kept = rounded<R>(x[k]);
+        store8<R>(out + c, kept);
+        if (!kFp8) x[k] = f8<R>(kept);
+        dot8(x[k], x[k], sum);
       }
     }
-    const float rs = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
+    const float rs = rsqrtf(fmaf(block_sum(halves(sum), red, turn), p.inv_h, p.eps));
     if (gave_up <= i) break;
     if (tid == 0) {                                      // every thread has taken what it needs of the stage
-      if (t + p.stages * step < p.T) fetch(t + p.stages * step, s);
+      if (t + (int64_t)p.stages * step < T_) fetch(t + (int64_t)p.stages * step, s);
       if (p.rstd) p.rstd[t] = rs;
       if (p.post_rstd) p.post_rstd[t] = rp;
     }
+    if (++s == p.stages) s = 0;
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
-      float v[8];
-      if (c < p.H) {
-        weights8(p.w, p.w_type, c, p.offset, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= x[k][j] * rs;
-        if (!kFp8) store8<T>(static_cast<word*>(p.h) + t * p.H + c, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      const int c = (k * (int)blockDim.x + tid) * 8;
+      x[k] = x[k] * both(rs);
+      if (c < H) {
+        if (p.w) x[k] = x[k] * w.get(c);
+        if (!kFp8) store8<T>(static_cast<word*>(p.h) + t * H + c, x[k]);
       }
       if constexpr (kFp8) {                              // sixteen neighbours have a block
-        float scale;
+        float scale, h[8];
         uint32_t q[2];
-        quantize_block<8, 16>(v, p.scale_rule, scale, q);
-        if (c < p.H) {
-          *reinterpret_cast<uint2*>(p.q + t * p.H + c) = make_uint2(q[0], q[1]);
-          if ((tid & 15) == 0) p.scale[t * ((p.H + kBlock - 1) / kBlock) + c / kBlock] = scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("mov.b64 {%0, %1}, %2;" : "=f"(h[2 * j]), "=f"(h[2 * j + 1]) : "l"(x[k].v[j]));
+        quantize_block<8, 16>(h, p.scale_rule, scale, q);
+        if (c < H) {
+          *reinterpret_cast<uint2*>(p.q + t * H + c) = make_uint2(q[0], q[1]);
+          if ((tid & 15) == 0) p.scale[t * ((H + kBlock - 1) / kBlock) + c / kBlock] = scale;
         }
       }
     }
@@ -223,16 +306,17 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
   if (gave_up != 0x7FFFFFFF) __nanosleep(1000000);       // copies still in flight end before the memory goes
 }
 
-template <typename T, typename R, int kV, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+// kR rows at a time between the barriers: they share what is unpacked of the weights.
+template <typename T, typename R, int kV, int kR, int kThreads, bool kRaw>
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 2 : 1)
 norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
   using rword = typename R::word;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMostStages];
-  __shared__ float red[2][32];
+  __shared__ float red[2][kR][32];
   __shared__ int gave_up;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, H = (int)p.H;
   gb_pdl_launch_dependents();
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
@@ -241,138 +325,156 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   }
   __syncthreads();
   gb_pdl_wait();
-  const int64_t rows = p.per_gate == 0 ? p.T : p.gate_rows;          // of the block's share: all, or those of a gate row
-  const int64_t first = p.per_gate == 0 ? 0 : blockIdx.x / p.per_gate * p.gate_rows;
-  const int64_t begin = p.per_gate == 0 ? blockIdx.x : blockIdx.x % p.per_gate, step = p.per_gate == 0 ? gridDim.x : p.per_gate;
-  const uint32_t y_bytes = (uint32_t)(p.H * sizeof(word)), r_bytes = (uint32_t)(p.H * sizeof(rword));
-  auto fetch = [&](int64_t t, int s) {
+  // the block's share of the rows, of all or of those of a gate row: first + begin, + step, ..
+  const int rows = p.per_gate == 0 ? (int)p.T : (int)p.gate_rows, first = p.per_gate == 0 ? 0 : (int)blockIdx.x / p.per_gate * rows;
+  const int begin = p.per_gate == 0 ? (int)blockIdx.x : (int)blockIdx.x % p.per_gate, step = p.per_gate == 0 ? (int)gridDim.x : p.per_gate;
+  const int mine = (rows - begin + step - 1) / step;
+  const uint32_t y_bytes = (uint32_t)(H * (int)sizeof(word)), r_bytes = (uint32_t)(H * (int)sizeof(rword));
+  const bool own_gate = p.in_at[4] != ~0u;               // every row has a gate of its own
+  auto fetch = [&](int n, int s) {                       // the n-th row of the share
+    const int64_t t = first + begin + (int64_t)n * step;
     uint8_t* st = ring + (size_t)s * p.stage_bytes;
     gb_mbar_expect_tx(&full[s], p.stage_bytes);
-    gb_bulk_g2s(st + p.in_at[0], static_cast<const rword*>(p.s) + t * p.H, r_bytes, &full[s]);
+    gb_bulk_g2s(st + p.in_at[0], static_cast<const rword*>(p.s) + t * H, r_bytes, &full[s]);
     if (p.in_at[1] != ~0u) gb_bulk_g2s(st + p.in_at[1], static_cast<const word*>(p.dh) + t * p.dh_ld, y_bytes, &full[s]);
     if (p.in_at[2] != ~0u) gb_bulk_g2s(st + p.in_at[2], static_cast<const rword*>(p.ds) + t * p.ds_ld, r_bytes, &full[s]);
     if (p.in_at[3] != ~0u) gb_bulk_g2s(st + p.in_at[3], static_cast<const word*>(p.y) + t * p.y_ld, y_bytes, &full[s]);
-    if (p.in_at[4] != ~0u) gb_bulk_g2s(st + p.in_at[4], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
+    if (own_gate) gb_bulk_g2s(st + p.in_at[4], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
   };
   if (tid == 0)
     for (int s = 0; s < p.stages; ++s)
-      if (begin + s * step < rows) fetch(first + begin + s * step, s);
+      if (s < mine) fetch(s, s);
+  const Weights<T, kRaw> w_of{p.w, p.w_type, p.offset}, pw_of{p.pw, p.pw_type, p.offset};
+  const word* gate_row = static_cast<const word*>(p.gate);
+  if (gate_row && p.per_gate != 0) gate_row += (int64_t)(first / rows) * p.gate_ld;
+  const bool many_gates = p.gate && !own_gate && p.per_gate == 0 && p.gate_rows != p.T;   // a gate without a gradient
   const Ring wheel{full, &gave_up, p.stages};
-  float acc_w[kV][8], acc_pw[kV][8], acc_g[kV][8];
+  F8 acc_w[kV], acc_pw[kV], acc_g[kV];
 #pragma unroll
-  for (int k = 0; k < kV; ++k)
+  for (int k = 0; k < kV; ++k) acc_w[k] = acc_pw[k] = acc_g[k] = all8(0.0f);
+  // sums over the block of a value for each row, in the same order each time
+  int turn = 0;
+  const auto sums = [&](float (&m)[kR]) {
+    const int warp = tid >> 5, lane = tid & 31, warps = (int)blockDim.x >> 5;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc_w[k][j] = acc_pw[k][j] = acc_g[k][j] = 0.0f;
-  int turn = 0, i = 0;
-  for (int64_t n = begin; n < rows; n += step, ++i) {
-    const int64_t t = first + n;
-    const int s = i % p.stages;
-    const uint8_t* st = ring + (size_t)s * p.stage_bytes;
-    const float rs = __ldg(p.rstd + t), rp = p.pw ? __ldg(p.post_rstd + t) : 1.0f;
-    wheel.wait(i, p.status, 92);
-    float d[kV][8], m1 = 0.0f, m2 = 0.0f;                // d: dh (o + w), dx, du (o + pw) in turn
+    for (int q = 0; q < kR; ++q) {
+      m[q] = warp_sum(m[q]);
+      if (lane == 0) red[turn][q][warp] = m[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kR; ++q) m[q] = warp_sum(lane < warps ? red[turn][q][lane] : 0.0f) * p.inv_h;
+    turn ^= 1;
+  };
+  int s = 0;
+  for (int n = 0; n < mine; n += kR) {
+    const uint8_t* st[kR];
+    int64_t t[kR];
+    bool on[kR];
+    float rs[kR], rp[kR], m1[kR], m2[kR];
+    F8 d[kR][kV];                                        // dh (o + w), dx, du (o + pw) in turn
+#pragma unroll
+    for (int q = 0; q < kR; ++q) {
+      const int sq = s + q < p.stages ? s + q : s + q - p.stages;
+      st[q] = ring + (size_t)sq * p.stage_bytes;
+      on[q] = n + q < mine;
+      t[q] = first + begin + (int64_t)(n + q) * step;
+      rs[q] = on[q] ? __ldg(p.rstd + t[q]) : 0.0f;
+      rp[q] = on[q] && p.pw ? __ldg(p.post_rstd + t[q]) : 1.0f;
+      if (on[q]) wheel.wait(n + q, sq, p.status, 92);
+    }
+    uint64_t sum[kR];
+#pragma unroll
+    for (int q = 0; q < kR; ++q) sum[q] = 0;
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
+      const int c = (k * (int)blockDim.x + tid) * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[k][j] = 0.0f;
-      if (c < p.H && p.dh) {
-        float x[8], w[8];
-        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[0]) + c, x);
-        load8<T>(reinterpret_cast<const word*>(st + p.in_at[1]) + c, d[k]);
-        weights8(p.w, p.w_type, c, p.offset, w);
+      for (int q = 0; q < kR; ++q) d[q][k] = all8(0.0f);
+      if (c < H && p.dh) {
+        const F8 w = p.w ? w_of.get(c) : all8(1.0f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float xh = x[j] * rs;
-          acc_w[k][j] = fmaf(d[k][j], xh, acc_w[k][j]);
-          d[k][j] *= w[j];
-          m1 = fmaf(d[k][j], xh, m1);
+        for (int q = 0; q < kR; ++q) {
+          if (!on[q]) continue;
+          const F8 xh = load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[0]) + c) * both(rs[q]);
+          d[q][k] = load8<T>(reinterpret_cast<const word*>(st[q] + p.in_at[1]) + c);
+          acc_w[k] = fma8(d[q][k], xh, acc_w[k]);
+          d[q][k] = d[q][k] * w;
+          dot8(d[q][k], xh, sum[q]);
         }
       }
     }
-    m1 = block_sum(m1, red, turn) * p.inv_h;
-    uint4 y_raw[kV][sizeof(word) / 2];
+#pragma unroll
+    for (int q = 0; q < kR; ++q) { m1[q] = halves(sum[q]); sum[q] = 0; }
+    sums(m1);
+    Raw8<T> y_raw[kR][kV];
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
-      if (c < p.H) {
-        float x[8], v[8];
-        load8<R>(reinterpret_cast<const rword*>(st + p.in_at[0]) + c, x);
+      const int c = (k * (int)blockDim.x + tid) * 8;
+      if (c < H) {
+        const F8 w = p.pw ? pw_of.get(c) : all8(1.0f);
+        F8 g = all8(1.0f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[k][j] = rs * fmaf(-x[j] * rs, m1, d[k][j]);
-        if (p.ds) {
-          load8<R>(reinterpret_cast<const rword*>(st + p.in_at[2]) + c, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[k][j] += v[j];
-        }
-        if (p.dr) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = p.a * d[k][j];
-          store8<R>(static_cast<rword*>(p.dr) + t * p.H + c, v);
-        }
-        float u[8], w[8];                                // y_hat (or y), o + pw
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = w[j] = 1.0f;
-        if (p.in_at[3] != ~0u) {
-          const word* y = reinterpret_cast<const word*>(st + p.in_at[3]) + c;
-#pragma unroll
-          for (int q = 0; q < (int)sizeof(word) / 2; ++q) y_raw[k][q] = reinterpret_cast<const uint4*>(y)[q];
-          load8<T>(y, u);
-        }
-        if (p.pw) {
-          weights8(p.pw, p.pw_type, c, p.offset, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) u[j] *= rp;
-        }
-        float g[8];
-        if (p.gate) {
-          if (p.in_at[4] != ~0u) load8<T>(reinterpret_cast<const word*>(st + p.in_at[4]) + c, g);
-          else load8<T>(static_cast<const word*>(p.gate) + t / p.gate_rows * p.gate_ld + c, g);
-          float dg[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dg[j] = p.b * d[k][j] * (u[j] * w[j]);
-            acc_g[k][j] += dg[j];
-            g[j] *= p.b;
+        for (int q = 0; q < kR; ++q) {
+          if (!on[q]) continue;
+          F8& e = d[q][k];
+          // dx; e is not scaled by 1 / rms yet
+          e = fma8(load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[0]) + c), both(-rs[q] * m1[q]), e);
+          e = p.ds ? fma8(e, both(rs[q]), load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[2]) + c)) : e * both(rs[q]);
+          if (p.dr) store8<R>(static_cast<rword*>(p.dr) + t[q] * H + c, e * both(p.a));
+          F8 v = all8(0.0f);                             // y_hat, or y
+          if (p.in_at[3] != ~0u) {
+            y_raw[q][k] = raw8<T>(reinterpret_cast<const word*>(st[q] + p.in_at[3]) + c);
+            v = f8<T>(y_raw[q][k]);
+            if (p.pw) v = v * both(rp[q]);
           }
-          if (p.dg) store8<T>(static_cast<word*>(p.dg) + t * p.H + c, dg);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[j] = p.b;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float du = g[j] * d[k][j];
-          acc_pw[k][j] = fmaf(du, u[j], acc_pw[k][j]);
-          d[k][j] = du * w[j];
-          m2 = fmaf(d[k][j], u[j], m2);
+          e = e * both(p.b);
+          if (p.gate) {
+            if (q == 0 || own_gate || many_gates) {
+              const word* from = own_gate ? reinterpret_cast<const word*>(st[q] + p.in_at[4]) : gate_row;
+              if (many_gates) from += (int64_t)((uint32_t)t[q] / (uint32_t)p.gate_rows) * p.gate_ld;
+              g = load8<T>(from + c);
+            }
+            const F8 u = v * w;
+            if (p.dg) store8<T>(static_cast<word*>(p.dg) + t[q] * H + c, e * u);
+            else if (p.part_g) acc_g[k] = fma8(e, u, acc_g[k]);
+            e = e * g;
+          }
+          if (p.pw) {
+            acc_pw[k] = fma8(e, v, acc_pw[k]);
+            e = e * w;
+            dot8(e, v, sum[q]);
+          }
         }
       }
     }
-    m2 = block_sum(m2, red, turn) * p.inv_h;
-    if (gave_up <= i) break;
-    if (tid == 0 && n + p.stages * step < rows) fetch(t + p.stages * step, s);
+#pragma unroll
+    for (int q = 0; q < kR; ++q) m2[q] = halves(sum[q]);
+    sums(m2);
+    if (gave_up <= n + kR - 1) break;
+#pragma unroll
+    for (int q = 0; q < kR; ++q) {
+      if (tid == 0 && n + q + p.stages < mine) fetch(n + q + p.stages, s);
+      if (++s == p.stages) s = 0;
+    }
     if (p.dy) {
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
-        const int64_t c = ((int64_t)k * blockDim.x + tid) * 8;
-        if (c < p.H) {
-          if (p.pw) {
-            float y[8];
+        const int c = (k * (int)blockDim.x + tid) * 8;
 #pragma unroll
-            for (int q = 0; q < (int)sizeof(word) / 2; ++q) unpack16<T>(y_raw[k][q], y + q * (16 / sizeof(word)));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) d[k][j] = rp * fmaf(-y[j] * rp, m2, d[k][j]);
-          }
-          store8<T>(static_cast<word*>(p.dy) + t * p.H + c, d[k]);
+        for (int q = 0; q < kR; ++q) {
+          if (c >= H || !on[q]) continue;
+          if (p.pw) d[q][k] = fma8(f8<T>(y_raw[q][k]), both(-rp[q] * m2[q]), d[q][k]) * both(rp[q]);
+          store8<T>(static_cast<word*>(p.dy) + t[q] * H + c, d[q][k]);
         }
       }
     }
   }
 #pragma unroll
   for (int k = 0; k < kV; ++k) {
-    const int64_t c = ((int64_t)k * blockDim.x + tid) * 8, at = (int64_t)blockIdx.x * p.H + c;
-    if (c < p.H) {
+    const int c = (k * (int)blockDim.x + tid) * 8;
+    const int64_t at = (int64_t)blockIdx.x * H + c;
+    if (c < H) {
       if (p.part_w) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_w) + at, acc_w[k]);
       if (p.part_pw) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_pw) + at, acc_pw[k]);
       if (p.part_g) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + at, acc_g[k]);
@@ -560,6 +662,16 @@ Width width_of(int64_t H) {
   return {0, 0, 0};
 }
 
+// For the backward pass: eight columns keep 24 sums in registers, and two rows at a time need 96 of them.
+Width grad_width_of(int64_t H) {
+  const int threads = (int)((H + 255) / 256 * 32);
+  if (H <= 2048) return {1, threads, 256};
+  if (H <= 5120) return {1, threads, 640};
+  if (H <= 8192) return {1, threads, 1024};
+  if (H <= 16384) return {2, (int)((H + 511) / 512 * 32), 1024};
+  return {0, 0, 0};
+}
+
 bool whole(const void* p, int64_t ld, int size) { return !p || (((uintptr_t)p & 15u) == 0 && ld * size % 16 == 0); }
 
 int check_args(const gb_residual_norm_args* a) {
@@ -586,15 +698,15 @@ NormParams params_of(const gb_residual_norm_args* a) {
   return p;
 }
 
-// Blocks an SM, and stages of their rings: about 1024 threads, rows ahead for each of them.
+// Blocks an SM, and stages of their rings: as many threads as the registers give, rows ahead for each of them.
 struct Plan { int per_sm, stages; };
-Plan plan_of(int threads, uint32_t stage_bytes) {
-  int per_sm = 1024 / threads;
+Plan plan_of(int threads, int most_threads, uint32_t stage_bytes) {
+  int per_sm = most_threads / threads;
   if (per_sm < 1) per_sm = 1;
   if (per_sm > 16) per_sm = 16;
   while (per_sm > 1 && (uint32_t)kRingMax / per_sm < 2 * stage_bytes + 1024) --per_sm;
   int stages = (int)(((uint32_t)kRingMax / per_sm - 1024) / stage_bytes);
-  return {per_sm, stages > 4 ? 4 : stages};
+  return {per_sm, stages > kMostStages ? kMostStages : stages};
 }
 
 template <typename Go>
@@ -618,6 +730,9 @@ int launch_ring(K kernel, int blocks, int threads, size_t smem, cudaStream_t str
   return GB_OK;
 }
 
+// Whether the weights have the rows' type.
+bool own_type(const gb_residual_norm_args* a) { return (!a->w || a->w_dtype == a->dtype) && (!a->pw || a->pw_dtype == a->dtype); }
+
 template <bool kFp8>
 int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
   const int sms = gb_sm_count();
@@ -632,6 +747,7 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
   const bool vec = width.v > 0 && a->H % 8 == 0 && whole(a->y, a->y_ld, size) && whole(a->r, a->r_ld, rsize) && whole(a->gate, a->gate_ld, size) &&
                    whole(a->w, 0, 1) && whole(a->pw, 0, 1) && whole(p.h, 0, 1) && whole(p.s, 0, 1) && whole(p.q, 0, 1) &&
                    p.stage_bytes <= (uint32_t)kRingMax - 1024;
+  const bool raw = own_type(a);
   return with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
@@ -640,11 +756,13 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
       return GB_OK;
     }
     return with_width(width, [&](auto v, auto most) -> int {
-      const Plan plan = plan_of(width.threads, p.stage_bytes);
+      const Plan plan = plan_of(width.threads, 1024, p.stage_bytes);
       p.stages = plan.stages;
       const int64_t blocks = a->T < (int64_t)sms * plan.per_sm ? a->T : (int64_t)sms * plan.per_sm;
-      return launch_ring(norm_rows_kernel<T, R, decltype(v)::value, decltype(most)::value, kFp8>, (int)blocks, width.threads,
-                         (size_t)p.stages * p.stage_bytes, stream, p);
+      constexpr int kV = decltype(v)::value, kMost = decltype(most)::value;
+      const size_t smem = (size_t)p.stages * p.stage_bytes;
+      if (raw) return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, true>, (int)blocks, width.threads, smem, stream, p);
+      return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, false>, (int)blocks, width.threads, smem, stream, p);
     });
   });
 }
@@ -672,7 +790,7 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
   const int size = size_of(a->dtype), rsize = size_of(a->stream_dtype);
   r.gate_rows = a->gate && a->gate_rows == 1 && a->T > 1;
   r.gate_sums = a->gate && g->d_gate && !r.gate_rows;
-  r.width = width_of(a->H);
+  r.width = grad_width_of(a->H);
   uint32_t at = 0;
   auto place = [&](bool read, int bytes) {
     const uint32_t here = read ? at : ~0u;
@@ -692,7 +810,7 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
             whole(g->stream, 0, 1) && whole(g->d_h, g->d_h_ld, size) && whole(g->d_stream, g->d_stream_ld, rsize) && whole(g->d_y, 0, 1) &&
             whole(g->d_r, 0, 1) && whole(g->d_gate, 0, 1);
   }
-  if (r.vec) r.plan = plan_of(r.width.threads, r.stage_bytes);
+  if (r.vec) r.plan = plan_of(r.width.threads, r.width.most <= 256 ? 512 : 65536 / 96, r.stage_bytes);
   const int64_t sms = gb_sm_count();
   r.shares = shares_of(a, r.gate_sums, r.vec ? sms * r.plan.per_sm : 64);
   auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
@@ -773,6 +891,7 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   p.per_gate = plan.shares.per_gate;
   const bool sums = p.part_w || p.part_pw || p.part_g;
   const cudaStream_t st = (cudaStream_t)stream;
+  const bool raw = own_type(a);
   const int rc2 = with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
@@ -787,10 +906,20 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
     for (int k = 0; k < 5; ++k) p.in_at[k] = plan.at[k];
     p.stage_bytes = plan.stage_bytes;
     p.stages = plan.plan.stages;
-    return with_width(plan.width, [&](auto v, auto most) -> int {
-      return launch_ring(norm_rows_grad_kernel<T, R, decltype(v)::value, decltype(most)::value>, (int)plan.shares.blocks, plan.width.threads,
-                         (size_t)p.stages * p.stage_bytes, st, p);
-    });
+    const auto go = [&](auto v, auto r_, auto most) -> int {
+      constexpr int kV = decltype(v)::value, kR = decltype(r_)::value, kMost = decltype(most)::value;
+      const size_t smem = (size_t)p.stages * p.stage_bytes;
+      if (raw) return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, true>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
+      return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, false>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    if (plan.width.v == 2) return go(two, one, integral_constant<int, 1024>());
+    if (plan.width.most == 1024) return go(one, one, integral_constant<int, 1024>());
+    const bool pairs = p.stages >= 4;                    // two rows at hand, two on their way
+    if (plan.width.most == 640) return pairs ? go(one, two, integral_constant<int, 640>()) : go(one, one, integral_constant<int, 640>());
+    return pairs ? go(one, two, integral_constant<int, 256>()) : go(one, one, integral_constant<int, 256>());
   });
   if (rc2 != GB_OK || !sums) return rc2;
   JoinParams j = {};

@@ -55,33 +55,34 @@ def stream_of(y, r, pw, gate, offset=0.0):
     return A * r.double() + b, A * r.double().abs() + b.abs()
 
 
-def grads(s, y, w, pw, gate, dh, ds, offset=0.0):
+def grads(s, y, w, pw, gate, dh, ds, offset=0.0, scales=(A, BR), eps=EPS):
     """(gradients, what fp32 may be off by) in fp64, the stream as it is stored: of y, residual, weight, post weight, and of the gate for each row."""
     H = s.shape[-1]
+    res, br = scales
     s, y, dh, ds = (t.double() for t in (s, y, dh, ds))
     c = (depth(H) + 24) * U                               # of a sum over a row, and of the few products around it
-    rs = 1.0 / torch.sqrt(s.square().mean(-1, keepdim=True) + EPS)
+    rs = 1.0 / torch.sqrt(s.square().mean(-1, keepdim=True) + eps)
     xh = s * rs
     k = dh * (offset + w.double())
     m1, m1s = (k * xh).mean(-1, keepdim=True), (k * xh).abs().mean(-1, keepdim=True)
     dx = ds + rs * (k - xh * m1)
     e_dx = c * (ds.abs() + rs * (k.abs() + 2 * xh.abs() * m1s)) * 2
-    g = BR if gate is None else BR * gate.double()
+    g = br if gate is None else br * gate.double()
     ga = abs(g) if gate is None else g.abs()
     du, e_du = g * dx, ga * e_dx + 2 * U * (g * dx).abs()
     if pw is None:
         u, dy, e_dy, dpw, e_dpw = y, du, e_du, None, None
     else:
         p = offset + pw.double()
-        rp = 1.0 / torch.sqrt(y.square().mean(-1, keepdim=True) + EPS)
+        rp = 1.0 / torch.sqrt(y.square().mean(-1, keepdim=True) + eps)
         yh = y * rp
         u, t, e_t = yh * p, du * p, e_du * p.abs() + U * (du * p).abs()
         m2, m2s = (t * yh).mean(-1, keepdim=True), (t * yh).abs().mean(-1, keepdim=True)
         dy = rp * (t - yh * m2)
         e_dy = rp * (e_t + yh.abs() * (e_t * yh.abs()).mean(-1, keepdim=True)) + 2 * c * rp * (t.abs() + 2 * yh.abs() * m2s)
         dpw, e_dpw = du * yh, e_du * yh.abs() + 2 * c * (du * yh).abs()
-    dg, e_dg = BR * dx * u, BR * e_dx * u.abs() + 2 * c * (BR * dx * u).abs()
-    return {"y": (dy, e_dy), "r": (A * dx, A * e_dx + U * (A * dx).abs()), "w": (dh * xh, 2 * c * (dh * xh).abs()), "pw": (dpw, e_dpw), "g": (dg, e_dg)}
+    dg, e_dg = br * dx * u, br * e_dx * u.abs() + 2 * c * (br * dx * u).abs()
+    return {"y": (dy, e_dy), "r": (res * dx, res * e_dx + U * (res * dx).abs()), "w": (dh * xh, 2 * c * (dh * xh).abs()), "pw": (dpw, e_dpw), "g": (dg, e_dg)}
 
 
 def near(got, ref, err, name):
@@ -249,17 +250,20 @@ def test_strides_and_refusals(dev):
         y, r, gt = (cut(t) for t in base)
         for leaf in (y, r, gt):
             assert not leaf.is_contiguous()
-        got = kernels.residual_norm(y, r, w, post_weight=w, gate=gt)
-        want = kernels.residual_norm(y.contiguous(), r.contiguous(), w, post_weight=w, gate=gt.contiguous())
-        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        got = kernels.residual_norm(y, r, w, post_weight=w, gate=gt, residual_scale=A, branch_scale=BR, eps=EPS)
+        # rows that are no 16-byte pieces are added up in another order than contiguous ones: held to the formula, not to their bits
+        want, size = stream_of(y, r, w, gt)
+        near(got[1], want, (er(256) + 8 * U) * size, "stream")
+        ref = rms(got[1].double()) * w.double()
+        near(got[0], ref, (er(256) + 8 * U) * ref.abs(), "h")
         wide = torch.stack([w, w], 1)[:, 0]                                 # weights two apart
-        assert torch.equal(kernels.residual_norm(y, r, wide, post_weight=w, gate=gt)[0], want[0])
+        assert torch.equal(kernels.residual_norm(y, r, wide, post_weight=w, gate=gt, residual_scale=A, branch_scale=BR, eps=EPS)[0], got[0])
     # gradients that are broadcast numbers or lie elsewhere than on 16-byte pieces
     y = torch.randn(8, 256, generator=g, device=dev).to(BF).requires_grad_()
     h, s = kernels.residual_norm(y, base[0, :8, :256], w, post_weight=w)
-    d1, = torch.autograd.grad([h, s], [y], [torch.ones((), device=dev, dtype=BF).expand(8, 256), base[1, :8, 3:259]], retain_graph=True)
-    d2, = torch.autograd.grad([h, s], [y], [torch.ones(8, 256, device=dev, dtype=BF), base[1, :8, 3:259].contiguous()])
-    assert torch.equal(d1, d2)
+    one, ds = torch.ones((), device=dev, dtype=BF).expand(8, 256), base[1, :8, 3:259]
+    d1, = torch.autograd.grad([h, s], [y], [one, ds])
+    near(d1, *grads(s.detach(), y.detach(), w, w, None, one, ds, scales=(1.0, 1.0), eps=1e-6)["y"], "y")
     y, r = base[0, :, :256], base[1, :, :256]
     for call, kind in ((lambda: kernels.residual_norm(y, r[:4], w), RuntimeError), (lambda: kernels.residual_norm(y, r.half(), w), RuntimeError),
                        (lambda: kernels.residual_norm(y.double(), r.double()), TypeError), (lambda: kernels.residual_norm(y, r, w[:9]), RuntimeError),
