@@ -40,6 +40,7 @@ struct NormParams {
   int stages;
   uint32_t stage_bytes;
   uint32_t in_at[5];                                     // where a stage holds the arrays of a row; ~0u: not read
+  uint32_t w_at, pw_at, g_at;                            // behind the ring: the weights, and a gate that all rows of the block share
   int* status;
   // backward
   const void *dh, *ds;
@@ -174,21 +175,29 @@ GB_DEVINL void store8(typename T::word* p, const Raw8<T>& r) {
 }
 template <typename T>
 GB_DEVINL void store8(typename T::word* p, const F8& f) { store8<T>(p, rounded<T>(f)); }
-// Weights of eight columns, o + w; kRaw: of the rows' own type.
+// Weights of eight columns in shared memory, o + w; kRaw: of the rows' own type.
 template <typename T, bool kRaw>
 struct Weights {
-  const void* p;
+  const uint8_t* p;
   int type;
   float offset;
   GB_DEVINL F8 get(int c) const {
     F8 v;
-    if (kRaw) v = load8<T>(static_cast<const typename T::word*>(p) + c);
-    else if (type == GB_DTYPE_BF16) v = load8<Bf16>(static_cast<const uint16_t*>(p) + c);
-    else if (type == GB_DTYPE_FP16) v = load8<Fp16>(static_cast<const uint16_t*>(p) + c);
-    else v = load8<Fp32>(static_cast<const uint32_t*>(p) + c);
+    if (kRaw) v = load8<T>(reinterpret_cast<const typename T::word*>(p) + c);
+    else if (type == GB_DTYPE_BF16) v = load8<Bf16>(reinterpret_cast<const uint16_t*>(p) + c);
+    else if (type == GB_DTYPE_FP16) v = load8<Fp16>(reinterpret_cast<const uint16_t*>(p) + c);
+    else v = load8<Fp32>(reinterpret_cast<const uint32_t*>(p) + c);
     return offset == 0.0f ? v : v + all8(offset);
   }
 };
+// The weights' way there, by one thread; they are waited for like a row.
+GB_DEVINL void fetch_weights(const NormParams& p, uint8_t* smem, const void* gate, uint32_t gate_bytes, uint64_t* bar) {
+  const auto bytes = [&](int type) { return (uint32_t)(p.H * (type == GB_DTYPE_FP32 ? 4 : 2)); };
+  gb_mbar_expect_tx(bar, (p.w ? bytes(p.w_type) : 0u) + (p.pw ? bytes(p.pw_type) : 0u) + (p.g_at != ~0u ? gate_bytes : 0u));
+  if (p.w) gb_bulk_g2s(smem + p.w_at, p.w, bytes(p.w_type), bar);
+  if (p.pw) gb_bulk_g2s(smem + p.pw_at, p.pw, bytes(p.pw_type), bar);
+  if (p.g_at != ~0u) gb_bulk_g2s(smem + p.g_at, gate, gate_bytes, bar);
+}
 template <typename R>
 GB_DEVINL float as_stored(float v) { return to_f32<R>(from_f32<R>(v)); }
 
@@ -197,9 +206,8 @@ GB_DEVINL float as_stored(float v) { return to_f32<R>(from_f32<R>(v)); }
 struct Ring {
   uint64_t* full;
   volatile int* gave_up;
-  int stages;
-  GB_DEVINL void wait(int i, int s, int* status, int code) const {     // step i, in stage s
-    if (!gb_mbar_wait(&full[s], (uint32_t)(i / stages) & 1u)) {
+  GB_DEVINL void wait(int i, int s, uint32_t phase, int* status, int code) const {     // step i, in stage s
+    if (!gb_mbar_wait(&full[s], phase)) {
       atomicMin((int*)gave_up, i);
       atomicExch(status, code);
     }
@@ -212,13 +220,14 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
   using rword = typename R::word;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ uint64_t full[kMostStages];
+  __shared__ uint64_t full[kMostStages + 1];           // the last one: the weights
   __shared__ float red[2][32];
   __shared__ int gave_up;
   const int tid = threadIdx.x, H = (int)p.H, T_ = (int)p.T, step = (int)gridDim.x;
   gb_pdl_launch_dependents();
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
+    gb_mbar_init(&full[kMostStages], 1);
     gave_up = 0x7FFFFFFF;
     gb_fence_barrier_init();
   }
@@ -233,16 +242,20 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     gb_bulk_g2s(st + p.in_at[1], static_cast<const rword*>(p.r) + t * p.r_ld, r_bytes, &full[s]);
     if (own_gate) gb_bulk_g2s(st + p.in_at[2], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
   };
-  if (tid == 0)
-    for (int s = 0; s < p.stages; ++s)
+  if (tid == 0) {
+    fetch((int64_t)blockIdx.x, 0);                       // a block has a row at least
+    fetch_weights(p, ring, p.gate, y_bytes, &full[kMostStages]);
+    for (int s = 1; s < p.stages; ++s)
       if ((int64_t)blockIdx.x + (int64_t)s * step < T_) fetch((int64_t)blockIdx.x + (int64_t)s * step, s);
-  const bool one_gate = p.gate && p.gate_rows == p.T;    // the same for all rows
-  const Weights<T, kRaw> w{p.w, p.w_type, p.offset}, pw{p.pw, p.pw_type, p.offset};
-  const Ring wheel{full, &gave_up, p.stages};
+  }
+  const bool one_gate = p.g_at != ~0u;                   // the same for all rows
+  const Weights<T, kRaw> w{ring + p.w_at, p.w_type, p.offset}, pw{ring + p.pw_at, p.pw_type, p.offset};
+  const Ring wheel{full, &gave_up};
   int turn = 0, i = 0, s = 0;
+  uint32_t phase = 0;
   for (int64_t t = blockIdx.x; t < T_; t += step, ++i) {
     const uint8_t* st = ring + (size_t)s * p.stage_bytes;
-    wheel.wait(i, s, p.status, 91);
+    wheel.wait(i, s, phase, p.status, 91);
     F8 x[kV];
     float rp = 1.0f;
     uint64_t sum = 0;
@@ -257,8 +270,11 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     }
     if (p.pw) rp = rsqrtf(fmaf(block_sum(halves(sum), red, turn), p.inv_h, p.eps));
     sum = 0;
-    const word* gate_row = static_cast<const word*>(p.gate);
-    if (gate_row && !one_gate && !own_gate) gate_row += (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
+    if (i == 0) wheel.wait(0, kMostStages, 0, p.status, 91);
+    const word* gate_row = nullptr;
+    if (own_gate) gate_row = reinterpret_cast<const word*>(st + p.in_at[2]);
+    else if (one_gate) gate_row = reinterpret_cast<const word*>(ring + p.g_at);
+    else if (p.gate) gate_row = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
     rword* out = static_cast<rword*>(p.s) + t * H;
     const uint64_t scale_r = both(p.a), scale_u = both(p.b * rp);
 #pragma unroll
@@ -266,7 +282,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
       const int c = (k * (int)blockDim.x + tid) * 8;
       if (c < H) {
         if (p.pw) x[k] = x[k] * pw.get(c);
-        if (p.gate) x[k] = x[k] * load8<T>(own_gate ? reinterpret_cast<const word*>(st + p.in_at[2]) + c : gate_row + c);
+        if (p.gate) x[k] = x[k] * load8<T>(gate_row + c);
         x[k] = fma8(x[k], scale_u, load8<R>(reinterpret_cast<const rword*>(st + p.in_at[1]) + c) * scale_r);
         const Raw8<R> kept = rounded<R>(x[k]);
         store8<R>(out + c, kept);
@@ -281,7 +297,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
       if (p.rstd) p.rstd[t] = rs;
       if (p.post_rstd) p.post_rstd[t] = rp;
     }
-    if (++s == p.stages) s = 0;
+    if (++s == p.stages) { s = 0; phase ^= 1; }
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
       const int c = (k * (int)blockDim.x + tid) * 8;
@@ -313,13 +329,14 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
   using rword = typename R::word;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ uint64_t full[kMostStages];
+  __shared__ uint64_t full[kMostStages + 1];           // the last one: the weights
   __shared__ float red[2][kR][32];
   __shared__ int gave_up;
   const int tid = threadIdx.x, H = (int)p.H;
   gb_pdl_launch_dependents();
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) gb_mbar_init(&full[s], 1);
+    gb_mbar_init(&full[kMostStages], 1);
     gave_up = 0x7FFFFFFF;
     gb_fence_barrier_init();
   }
@@ -341,14 +358,16 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     if (p.in_at[3] != ~0u) gb_bulk_g2s(st + p.in_at[3], static_cast<const word*>(p.y) + t * p.y_ld, y_bytes, &full[s]);
     if (own_gate) gb_bulk_g2s(st + p.in_at[4], static_cast<const word*>(p.gate) + t * p.gate_ld, y_bytes, &full[s]);
   };
-  if (tid == 0)
-    for (int s = 0; s < p.stages; ++s)
+  if (tid == 0) {
+    if (mine > 0) fetch(0, 0);
+    fetch_weights(p, ring, static_cast<const word*>(p.gate) + (p.per_gate != 0 ? (int64_t)(first / rows) * p.gate_ld : 0), y_bytes, &full[kMostStages]);
+    for (int s = 1; s < p.stages; ++s)
       if (s < mine) fetch(s, s);
-  const Weights<T, kRaw> w_of{p.w, p.w_type, p.offset}, pw_of{p.pw, p.pw_type, p.offset};
-  const word* gate_row = static_cast<const word*>(p.gate);
-  if (gate_row && p.per_gate != 0) gate_row += (int64_t)(first / rows) * p.gate_ld;
-  const bool many_gates = p.gate && !own_gate && p.per_gate == 0 && p.gate_rows != p.T;   // a gate without a gradient
-  const Ring wheel{full, &gave_up, p.stages};
+  }
+  const Weights<T, kRaw> w_of{ring + p.w_at, p.w_type, p.offset}, pw_of{ring + p.pw_at, p.pw_type, p.offset};
+  const bool many_gates = p.gate && !own_gate && p.g_at == ~0u;      // a gate without a gradient
+  const Ring wheel{full, &gave_up};
+  wheel.wait(0, kMostStages, 0, p.status, 92);
   F8 acc_w[kV], acc_pw[kV], acc_g[kV];
 #pragma unroll
   for (int k = 0; k < kV; ++k) acc_w[k] = acc_pw[k] = acc_g[k] = all8(0.0f);
@@ -367,6 +386,17 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     turn ^= 1;
   };
   int s = 0;
+  uint32_t phase = 0;
+  float rs_next[kR], rp_next[kR];                        // of the rows to come
+  const auto norms = [&](int n) {
+#pragma unroll
+    for (int q = 0; q < kR; ++q) {
+      const int64_t t = first + begin + (int64_t)(n + q) * step;
+      rs_next[q] = n + q < mine ? __ldg(p.rstd + t) : 0.0f;
+      rp_next[q] = n + q < mine && p.pw ? __ldg(p.post_rstd + t) : 1.0f;
+    }
+  };
+  norms(0);
   for (int n = 0; n < mine; n += kR) {
     const uint8_t* st[kR];
     int64_t t[kR];
@@ -379,10 +409,11 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
       st[q] = ring + (size_t)sq * p.stage_bytes;
       on[q] = n + q < mine;
       t[q] = first + begin + (int64_t)(n + q) * step;
-      rs[q] = on[q] ? __ldg(p.rstd + t[q]) : 0.0f;
-      rp[q] = on[q] && p.pw ? __ldg(p.post_rstd + t[q]) : 1.0f;
-      if (on[q]) wheel.wait(n + q, sq, p.status, 92);
+      rs[q] = rs_next[q];
+      rp[q] = rp_next[q];
+      if (on[q]) wheel.wait(n + q, sq, phase ^ (s + q < p.stages ? 0u : 1u), p.status, 92);
     }
+    norms(n + kR);
     uint64_t sum[kR];
 #pragma unroll
     for (int q = 0; q < kR; ++q) sum[q] = 0;
@@ -431,8 +462,8 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
           e = e * both(p.b);
           if (p.gate) {
             if (q == 0 || own_gate || many_gates) {
-              const word* from = own_gate ? reinterpret_cast<const word*>(st[q] + p.in_at[4]) : gate_row;
-              if (many_gates) from += (int64_t)((uint32_t)t[q] / (uint32_t)p.gate_rows) * p.gate_ld;
+              const word* from = reinterpret_cast<const word*>(own_gate ? st[q] + p.in_at[4] : ring + p.g_at);
+              if (many_gates) from = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t[q] / (uint32_t)p.gate_rows) * p.gate_ld;
               g = load8<T>(from + c);
             }
             const F8 u = v * w;
@@ -455,7 +486,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
     for (int q = 0; q < kR; ++q) {
       if (tid == 0 && n + q + p.stages < mine) fetch(n + q + p.stages, s);
-      if (++s == p.stages) s = 0;
+      if (++s == p.stages) { s = 0; phase ^= 1; }
     }
     if (p.dy) {
 #pragma unroll
@@ -695,18 +726,35 @@ NormParams params_of(const gb_residual_norm_args* a) {
   p.inv_h = (float)(1.0 / (double)a->H);
   p.status = gb_status_word();
   for (uint32_t& at : p.in_at) at = ~0u;
+  p.w_at = p.pw_at = p.g_at = ~0u;
   return p;
 }
 
-// Blocks an SM, and stages of their rings: as many threads as the registers give, rows ahead for each of them.
+// Blocks an SM, as many as the registers give, and stages of their rings: two at least where there is room, behind `fixed` bytes.
 struct Plan { int per_sm, stages; };
-Plan plan_of(int threads, int most_threads, uint32_t stage_bytes) {
+Plan plan_of(int threads, int most_threads, int most_stages, uint32_t stage_bytes, uint32_t fixed) {
   int per_sm = most_threads / threads;
   if (per_sm < 1) per_sm = 1;
   if (per_sm > 16) per_sm = 16;
-  while (per_sm > 1 && (uint32_t)kRingMax / per_sm < 2 * stage_bytes + 1024) --per_sm;
-  int stages = (int)(((uint32_t)kRingMax / per_sm - 1024) / stage_bytes);
-  return {per_sm, stages > kMostStages ? kMostStages : stages};
+  while (per_sm > 1 && (uint32_t)kRingMax / per_sm < 2 * stage_bytes + fixed + 1024) --per_sm;
+  const int stages = (int)(((uint32_t)kRingMax / per_sm - 1024 - fixed) / stage_bytes);
+  return {per_sm, stages > most_stages ? most_stages : stages};
+}
+// Where the weights and a gate that a block's rows share lie behind the ring, from 0 on; their bytes.
+uint32_t place_weights(const gb_residual_norm_args* a, bool one_gate, uint32_t* w_at, uint32_t* pw_at, uint32_t* g_at) {
+  uint32_t at = 0;
+  const auto place = [&](bool there, int type, uint32_t* to) {
+    *to = there ? at : ~0u;
+    if (there) at += (uint32_t)(a->H * size_of(type));
+  };
+  place(a->w != nullptr, a->w_dtype, w_at);
+  place(a->pw != nullptr, a->pw_dtype, pw_at);
+  place(one_gate, a->dtype, g_at);
+  return at;
+}
+void behind_ring(NormParams& p, size_t ring) {
+  for (uint32_t* at : {&p.w_at, &p.pw_at, &p.g_at})
+    if (*at != ~0u) *at += (uint32_t)ring;
 }
 
 template <typename Go>
@@ -744,9 +792,10 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
   p.in_at[1] = (uint32_t)(a->H * size);
   if (full) p.in_at[2] = (uint32_t)(a->H * (size + rsize));
   p.stage_bytes = (uint32_t)(a->H * (size * (full ? 2 : 1) + rsize));
+  const uint32_t fixed = place_weights(a, a->gate && a->gate_rows == a->T && !full, &p.w_at, &p.pw_at, &p.g_at);
   const bool vec = width.v > 0 && a->H % 8 == 0 && whole(a->y, a->y_ld, size) && whole(a->r, a->r_ld, rsize) && whole(a->gate, a->gate_ld, size) &&
                    whole(a->w, 0, 1) && whole(a->pw, 0, 1) && whole(p.h, 0, 1) && whole(p.s, 0, 1) && whole(p.q, 0, 1) &&
-                   p.stage_bytes <= (uint32_t)kRingMax - 1024;
+                   p.stage_bytes + fixed <= (uint32_t)kRingMax - 1024;
   const bool raw = own_type(a);
   return with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
@@ -756,13 +805,15 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
       return GB_OK;
     }
     return with_width(width, [&](auto v, auto most) -> int {
-      const Plan plan = plan_of(width.threads, 1024, p.stage_bytes);
+      const Plan plan = plan_of(width.threads, 1024, 4, p.stage_bytes, fixed);
       p.stages = plan.stages;
       const int64_t blocks = a->T < (int64_t)sms * plan.per_sm ? a->T : (int64_t)sms * plan.per_sm;
       constexpr int kV = decltype(v)::value, kMost = decltype(most)::value;
-      const size_t smem = (size_t)p.stages * p.stage_bytes;
-      if (raw) return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, true>, (int)blocks, width.threads, smem, stream, p);
-      return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, false>, (int)blocks, width.threads, smem, stream, p);
+      NormParams q = p;
+      behind_ring(q, (size_t)p.stages * p.stage_bytes);
+      const size_t smem = (size_t)p.stages * p.stage_bytes + fixed;
+      if (raw) return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, true>, (int)blocks, width.threads, smem, stream, q);
+      return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, false>, (int)blocks, width.threads, smem, stream, q);
     });
   });
 }
@@ -782,7 +833,7 @@ struct GradPlan {
   Width width;
   Plan plan;
   Shares shares;
-  uint32_t at[5], stage_bytes;
+  uint32_t at[5], stage_bytes, weight_at[3], fixed;
   int64_t w_at, pw_at, g_at, means_at, bytes;
 };
 GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads* g) {
@@ -806,11 +857,12 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
     r.at[3] = place(need_y, size);
     r.at[4] = place(r.gate_rows, size);
     r.stage_bytes = at;
-    r.vec = at <= (uint32_t)kRingMax - 1024 && whole(a->y, a->y_ld, size) && whole(a->gate, a->gate_ld, size) && whole(a->w, 0, 1) && whole(a->pw, 0, 1) &&
+    r.fixed = place_weights(a, a->gate && !r.gate_rows && (r.gate_sums || a->gate_rows == a->T), &r.weight_at[0], &r.weight_at[1], &r.weight_at[2]);
+    r.vec = at + r.fixed <= (uint32_t)kRingMax - 1024 && whole(a->y, a->y_ld, size) && whole(a->gate, a->gate_ld, size) && whole(a->w, 0, 1) && whole(a->pw, 0, 1) &&
             whole(g->stream, 0, 1) && whole(g->d_h, g->d_h_ld, size) && whole(g->d_stream, g->d_stream_ld, rsize) && whole(g->d_y, 0, 1) &&
             whole(g->d_r, 0, 1) && whole(g->d_gate, 0, 1);
   }
-  if (r.vec) r.plan = plan_of(r.width.threads, r.width.most <= 256 ? 512 : 65536 / 96, r.stage_bytes);
+  if (r.vec) r.plan = plan_of(r.width.threads, r.width.most <= 256 ? 512 : 65536 / 96, kMostStages, r.stage_bytes, r.fixed);
   const int64_t sms = gb_sm_count();
   r.shares = shares_of(a, r.gate_sums, r.vec ? sms * r.plan.per_sm : 64);
   auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
@@ -906,9 +958,11 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
     for (int k = 0; k < 5; ++k) p.in_at[k] = plan.at[k];
     p.stage_bytes = plan.stage_bytes;
     p.stages = plan.plan.stages;
+    p.w_at = plan.weight_at[0]; p.pw_at = plan.weight_at[1]; p.g_at = plan.weight_at[2];
+    behind_ring(p, (size_t)p.stages * p.stage_bytes);
     const auto go = [&](auto v, auto r_, auto most) -> int {
       constexpr int kV = decltype(v)::value, kR = decltype(r_)::value, kMost = decltype(most)::value;
-      const size_t smem = (size_t)p.stages * p.stage_bytes;
+      const size_t smem = (size_t)p.stages * p.stage_bytes + plan.fixed;
       if (raw) return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, true>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
       return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, false>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
     };
