@@ -115,8 +115,7 @@ GB_DEVINL void commit_to(uint32_t bar) {
   if (kCtas == 2) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
   else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-GB_DEVINL void tmem_ld32(uint32_t taddr, float (&f)[32]) {
-  uint32_t v[32];
+GB_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -126,9 +125,6 @@ GB_DEVINL void tmem_ld32(uint32_t taddr, float (&f)[32]) {
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
 }
 GB_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -150,6 +146,15 @@ GB_DEVINL uint16_t pack1(float a, int fp16) { return fp16 ? __half_as_ushort(__f
 GB_DEVINL float weighted(float v, float t) { return __fdividef(v, 1.0f + __expf(-t)); }
 constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.044715f;      // 2 sqrt(2 / pi): (1 + tanh(u)) / 2 is the sigmoid of 2 u
 
+// 1 + erf(z / sqrt 2), and e^(-z^2 / 2) on the way: Abramowitz and Stegun's rational approximation 7.1.26 of erf, off by 1.5e-7 at most (a
+// sixteenth of half a step of fp16 next to one), a third of erff's instructions, and the exponential is what the slope needs too.
+GB_DEVINL float one_plus_erf(float z, float& bell) {
+  const float x = fabsf(z) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+  bell = __expf(-0.5f * z * z);
+  const float tail = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * bell;
+  return z < 0.0f ? tail : 2.0f - tail;                    // a NaN stays one
+}
+
 template <int kN>
 GB_DEVINL void activate(float (&v)[kN], int act) {
   switch (act) {
@@ -159,7 +164,10 @@ GB_DEVINL void activate(float (&v)[kN], int act) {
       break;
     case GB_EPI_GELU:
 #pragma unroll
-      for (int i = 0; i < kN; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
+      for (int i = 0; i < kN; ++i) {
+        float bell;
+        v[i] = 0.5f * v[i] * one_plus_erf(v[i], bell);
+      }
       break;
     case GB_EPI_GELU_TANH:
 #pragma unroll
@@ -172,25 +180,45 @@ GB_DEVINL void activate(float (&v)[kN], int act) {
     default: break;
   }
 }
-GB_DEVINL float slope(float z, int act) {
+// act' in place of its arguments.
+template <int kN>
+GB_DEVINL void slopes(float (&v)[kN], int act) {
   switch (act) {
-    case GB_EPI_RELU: return z > 0.0f ? 1.0f : 0.0f;
-    case GB_EPI_GELU: return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
-    case GB_EPI_GELU_TANH: {
-      const float c = fminf(fmaxf(z, -16.0f), 16.0f), s = 1.0f / (1.0f + expf(-kTanhA * fmaf(kTanhB * c * c, c, c)));   // constant past these
-      return z != z ? z : fmaf(kTanhA * c * s * (1.0f - s), fmaf(3.0f * kTanhB * c, c, 1.0f), s);
-    }
-    case GB_EPI_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      return s * fmaf(z, 1.0f - s, 1.0f);
-    }
-    default: return 1.0f;
+    case GB_EPI_RELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = v[i] > 0.0f ? 1.0f : 0.0f;
+      break;
+    case GB_EPI_GELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        float bell;
+        const float phi = 0.5f * one_plus_erf(v[i], bell);
+        v[i] = fabsf(v[i]) > 16.0f ? phi : fmaf(v[i] * 0.39894228040143268f, bell, phi);      // (an infinity times none)
+      }
+      break;
+    case GB_EPI_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float z = v[i], c = fminf(fmaxf(z, -16.0f), 16.0f), s = weighted(1.0f, kTanhA * fmaf(kTanhB * c * c, c, c));   // constant past these
+        v[i] = z != z ? z : fmaf(kTanhA * c * s * (1.0f - s), fmaf(3.0f * kTanhB * c, c, 1.0f), s);
+      }
+      break;
+    case GB_EPI_SILU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float s = weighted(1.0f, v[i]);
+        v[i] = s * fmaf(v[i], 1.0f - s, 1.0f);
+      }
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = 1.0f;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ CTA pairs
 enum Major { kForward = 0, kRowsGrad = 1, kWeightGrad = 2 };   // which operands are MN-major: none, B, both
-enum Epilogue { kPlain = 0, kResidual = 1, kKeepZ = 2 };       // kKeepZ: z is stored too, with or without a residual
+enum Epilogue { kPlain = 0, kResidual = 1, kKeepZ = 2, kBoth = 3 };   // kKeepZ: z is stored too
 
 constexpr int kPairM = 256;
 constexpr int kChunk = 2048;                         // 32 rows x 32 columns on their way out
@@ -201,9 +229,8 @@ struct Shape {
   static constexpr bool kAmn = kMajor == kWeightGrad, kBmn = kMajor != kForward;
   static constexpr int kABytes = kBM * kSlabBytes, kBBytes = kBN / 2 * kSlabBytes, kStageBytes = kABytes + kBBytes;
   static constexpr int kCols = kBN / 2, kChunks = kCols / 32;                       // of an epilogue warp
-  static constexpr int kOut = kEpi == kPlain ? 2 : kChunks, kZ = kEpi == kKeepZ ? 2 : 0;
-  static constexpr int kOutBytes = kEpiWarps * (kOut + kZ) * kChunk;
-  static constexpr int kFixed = 1024 + kEpiWarps * kCols * 4 + 512;                 // alignment, bias, barriers
+  static constexpr int kOutBytes = kEpiWarps * 2 * kChunk;
+  static constexpr int kFixed = 1024 + 512;                                         // alignment, barriers
   static constexpr int kFit = (227 * 1024 - kFixed - kOutBytes) / kStageBytes, kStages = kFit < 8 ? kFit : 8;
   static constexpr int kSmem = kStages * kStageBytes + kOutBytes + kFixed;
 };
@@ -234,20 +261,18 @@ constexpr int kPairThreads = 32 * (kEpiWarps + 2);
 template <Major kMajor, int kBN, int kEpi>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
-                   const __grid_constant__ CUtensorMap map_z, const __grid_constant__ CUtensorMap map_r, const __grid_constant__ LinearParams p) {
+                   const __grid_constant__ CUtensorMap map_z, const __grid_constant__ LinearParams p) {
   using S = Shape<kMajor, kBN, kEpi>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
   uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
   const uint32_t out_ring = ring + kStages * S::kStageBytes;             // per epilogue warp
-  const uint32_t bias_at = out_ring + S::kOutBytes;                      // [warp][columns] fp32
-  const uint32_t full_bar = bias_at + kEpiWarps * S::kCols * 4;          // leader: both CTAs' operand tiles have landed
+  const uint32_t full_bar = out_ring + S::kOutBytes;                     // leader: both CTAs' operand tiles have landed
   const uint32_t empty_bar = full_bar + 8 * kStages;                     // the MMAs that read the stage are done
   const uint32_t acc_full = empty_bar + 8 * kStages;                     // [2] accumulator complete
   const uint32_t acc_empty = acc_full + 16;                              // [2] leader: drained by both CTAs
-  const uint32_t r_full = acc_empty + 16;                                // [epilogue warp] its part of the residual has landed
-  const uint32_t slot = r_full + 8 * kEpiWarps;
+  const uint32_t slot = acc_empty + 16;
   volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(ring_ptr + (slot - ring));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
 
@@ -264,7 +289,6 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       bar_init(acc_full + 8 * b, 1);
       bar_init(acc_empty + 8 * b, 2 * kEpiWarps);
     }
-    for (int w = 0; w < kEpiWarps; ++w) bar_init(r_full + 8 * w, 1);
     *abort_flag = 0;
     gb_fence_barrier_init();
   }
@@ -359,46 +383,54 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
   } else {
     // ------------------------------- epilogue (each CTA) --------------------------------
-    // Lane = row, 32 columns at a time, out through shared memory (64-byte swizzle), a TMA store each.
+    // Lane = row, 32 columns at a time, out through shared memory (64-byte swizzle), a TMA store each; the next columns' sums and
+    // residuals are on their way meanwhile.  (Residuals by TMA into the buffers of the output, and buffers of z's own, took one or two
+    // of the six stages: 4096 x 8192 x 5120 with residual 263 us, keeping z 301.)
+    constexpr bool kRes = (kEpi & kResidual) != 0, kZ = (kEpi & kKeepZ) != 0;
     const uint32_t acc_empty_pair = leader_addr(acc_empty);
     const int quarter = warp & 3, c_lo = (warp >> 2) * S::kCols;
-    const uint32_t out = out_ring + (uint32_t)warp * (S::kOut + S::kZ) * kChunk, z_out = out + S::kOut * kChunk;
-    const uint32_t bias_s = bias_at + (uint32_t)warp * S::kCols * 4, r_bar = r_full + 8 * warp;
-    const bool staged = p.tma && p.slices == 1, residual = kEpi != kPlain && p.r != nullptr;
-    const auto fetch_residual = [&](int tile) {              // a tile's part, by lane 0
-      int mt, nt;
-      tile_at(p, tile, mt, nt);
-      expect_tx(r_bar, S::kChunks * kChunk);
-      for (int c = 0; c < S::kChunks; ++c)
-        tma_load_2d(out + c * kChunk, &map_r, nt * kBN + c_lo + 32 * c, mt * kPairM + (int)rank * kBM + quarter * 32, r_bar);
-    };
-    if (residual && staged && lane == 0 && first < total_tiles) fetch_residual(first);
+    const uint32_t out = out_ring + (uint32_t)warp * 2 * kChunk;
+    const uint32_t row_at = (uint32_t)lane * 64u, swz = (uint32_t)((lane >> 1) & 3);
+    const bool staged = p.tma && p.slices == 1;
     int it = 0, flip = 0;
     for (int tile = first; tile < total_tiles; tile += stride, ++it) {
       const int slice = tile / per_tile, buf = it & 1;
       int mt, nt;
       tile_at(p, tile - slice * per_tile, mt, nt);
       const int n0 = nt * kBN + c_lo, row0 = mt * kPairM + (int)rank * kBM + quarter * 32, row = row0 + lane;
-      if (kMajor == kForward) {                              // the columns' biases, zeros past the last
-        __syncwarp();
-        for (int c = lane; c < S::kCols; c += 32) {
-          const float b = p.bias && n0 + c < p.N ? to_f(p.bias[n0 + c], p.fp16) : 0.0f;
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_s + 4u * c), "f"(b) : "memory");
+      uint32_t bias[(S::kCols + 63) / 64];                          // columns 64 i + 2 lane and the next, zeros past the last
+      if (kMajor == kForward) {
+#pragma unroll
+        for (int i = 0; i < (S::kCols + 63) / 64; ++i) {
+          const int c = n0 + 64 * i + 2 * lane;
+          bias[i] = (p.bias && c < p.N ? (uint32_t)__ldg(p.bias + c) : 0u) | (p.bias && c + 1 < p.N ? (uint32_t)__ldg(p.bias + c + 1) << 16 : 0u);
         }
-        __syncwarp();
       }
+      uint4 rr[4];                                           // the row's residual, 32 columns
+      const auto fetch_residual = [&](int c) {
+        const uint16_t* from = p.r + (int64_t)row * p.r_ld + n0 + 32 * c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          rr[q] = staged && row < p.M && n0 + 32 * c + 8 * q < p.N ? __ldg(reinterpret_cast<const uint4*>(from) + q) : make_uint4(0u, 0u, 0u, 0u);
+      };
+      if (kRes) fetch_residual(0);
       if (!warp_wait<true>(acc_full + 8 * buf, (uint32_t)(it >> 1) & 1, abort_flag, p.status, 104)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (residual && staged && !warp_wait(r_bar, (uint32_t)it & 1, abort_flag, p.status, 105)) break;
       const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (buf ? 256u : 0u) + (uint32_t)c_lo;
-#pragma unroll 1
+      uint32_t raw[32];
+      tmem_ld32(at, raw);
+#pragma unroll
       for (int c = 0; c < S::kChunks; ++c) {
         float v[32];
-        tmem_ld32(at + 32u * c, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
         if (c == S::kChunks - 1) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) arrive_cluster(acc_empty_pair + 8 * buf);
+        } else {
+          tmem_ld32(at + 32u * (c + 1), raw);
         }
         const int col = n0 + 32 * c;
         if (kMajor != kForward && p.slices > 1) {
@@ -418,59 +450,46 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
         if (kMajor == kForward) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float b[4];
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3]) : "r"(bias_s + 128u * c + 4u * i));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i + j] += b[j];
+          for (int i = 0; i < 32; i += 2) {
+            const uint32_t b = __shfl_sync(0xffffffffu, bias[c / 2], 16 * (c & 1) + i / 2);
+            v[i] += to_f(b & 0xFFFFu, p.fp16);
+            v[i + 1] += to_f(b >> 16, p.fp16);
           }
         }
-        const uint32_t row_at = (uint32_t)lane * 64u, swz = (uint32_t)((lane >> 1) & 3);
-        const auto put = [&](uint32_t dst, const float (&f)[32]) {     // eight rows touch eight bank groups
+        const auto send = [&](const CUtensorMap* map) {      // v as it is now
+          const uint32_t dst = out + (uint32_t)flip * kChunk;            // in turn: the chunk before last has left its buffer
+          flip ^= 1;
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 4; ++q)                        // eight rows touch eight bank groups
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                         ::"r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)), "r"(pack2(f[8 * q], f[8 * q + 1], p.fp16)),
-                           "r"(pack2(f[8 * q + 2], f[8 * q + 3], p.fp16)), "r"(pack2(f[8 * q + 4], f[8 * q + 5], p.fp16)),
-                           "r"(pack2(f[8 * q + 6], f[8 * q + 7], p.fp16)) : "memory");
-        };
-        const auto send = [&](const CUtensorMap* map, uint32_t src) {
+                         ::"r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)), "r"(pack2(v[8 * q], v[8 * q + 1], p.fp16)),
+                           "r"(pack2(v[8 * q + 2], v[8 * q + 3], p.fp16)), "r"(pack2(v[8 * q + 4], v[8 * q + 5], p.fp16)),
+                           "r"(pack2(v[8 * q + 6], v[8 * q + 7], p.fp16)) : "memory");
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && row0 < p.M && col < p.N) tma_store_2d(map, col, row0, src);   // what sticks out is not written
+          if (lane == 0 && row0 < p.M && col < p.N) tma_store_2d(map, col, row0, dst);   // what sticks out is not written
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         };
         if (staged) {
-          uint32_t dst = out + (uint32_t)c * kChunk;
-          if (kEpi == kPlain) {
-            dst = out + (uint32_t)flip * kChunk;             // in turn across tiles: their chunks may be odd in number
-            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          } else if (kEpi == kKeepZ) {                       // the z before last, and with it the y before that, have left their buffers
-            asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
-          }
-          __syncwarp();
-          if (kEpi == kKeepZ) {
-            put(z_out + (uint32_t)flip * kChunk, v);
-            send(&map_z, z_out + (uint32_t)flip * kChunk);
-          }
-          flip ^= 1;
+          if (kZ) send(&map_z);
           activate(v, p.act);
-          if (residual) {
+          if (kRes) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)));
+              const uint32_t w[4] = {rr[q].x, rr[q].y, rr[q].z, rr[q].w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 v[8 * q + 2 * j] += to_f(w[j] & 0xFFFFu, p.fp16);
                 v[8 * q + 2 * j + 1] += to_f(w[j] >> 16, p.fp16);
               }
             }
+            if (c + 1 < S::kChunks) fetch_residual(c + 1);
           }
-          put(dst, v);
-          send(&map_d, dst);
+          send(&map_d);
         } else if (row < p.M) {
-          if (kEpi == kKeepZ) {
+          if (kZ) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (col + i < p.N) p.z[(int64_t)row * p.N + col + i] = pack1(v[i], p.fp16);
@@ -479,15 +498,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (col + i < p.N)
-              p.d[(int64_t)row * p.N + col + i] = pack1(residual ? v[i] + to_f(p.r[(int64_t)row * p.r_ld + col + i], p.fp16) : v[i], p.fp16);
+              p.d[(int64_t)row * p.N + col + i] = pack1(kRes ? v[i] + to_f(p.r[(int64_t)row * p.r_ld + col + i], p.fp16) : v[i], p.fp16);
         }
-      }
-      if (residual && staged && tile + stride < total_tiles) {           // the next tile's residual, once the output has left its buffers
-        if (lane == 0) {
-          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          fetch_residual(tile + stride);
-        }
-        __syncwarp();
       }
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -683,9 +695,9 @@ struct DzParams {
   int fp16, act;
   float* part;                // [blocks along M][N] column sums, or null
 };
-constexpr int kDzThreads = 256, kDzCols = 256;
+constexpr int kDzThreads = 256, kDzCols = 256, kDzRows = 4;
 
-// A warp takes a row of 256 columns, a lane eight of them; a block's warps add their column sums up in their order.
+// A warp takes four rows of 256 columns at a time, a lane eight columns; a block's warps add their column sums up in their order.
 template <bool kVec>
 __global__ void __launch_bounds__(kDzThreads)
 linear_dz_kernel(const __grid_constant__ DzParams p) {
@@ -697,39 +709,57 @@ linear_dz_kernel(const __grid_constant__ DzParams p) {
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-  for (int64_t m = (int64_t)blockIdx.y * (kDzThreads / 32) + warp; m < p.M; m += (int64_t)gridDim.y * (kDzThreads / 32)) {
-    const uint16_t *dy = p.dy + m * p.dy_ld + c, *z = p.z ? p.z + m * p.N + c : nullptr;
-    uint32_t g[4] = {}, w[4] = {};
-    if (kVec) {
-      if (c < p.N) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(dy));
-        g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
-        if (z) { const uint4 b = __ldg(reinterpret_cast<const uint4*>(z)); w[0] = b.x; w[1] = b.y; w[2] = b.z; w[3] = b.w; }
-      }
-    } else {
+  const int64_t step = (int64_t)gridDim.y * (kDzThreads / 32) * kDzRows;
+  for (int64_t m0 = ((int64_t)blockIdx.y * (kDzThreads / 32) + warp) * kDzRows; m0 < p.M; m0 += step) {
+    uint32_t g[kDzRows][4], w[kDzRows][4];                  // every row's bytes are on their way before the first is looked at
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < p.N) {
-          g[i >> 1] |= (uint32_t)dy[i] << (16 * (i & 1));
-          if (z) w[i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
-        }
-    }
-    float d[8];
+    for (int r = 0; r < kDzRows; ++r) {
+      const int64_t m = m0 + r;
+      const uint16_t *dy = p.dy + m * p.dy_ld + c, *z = p.z + m * p.N + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      d[i] = to_f(g[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16);
-      if (z) d[i] *= slope(to_f(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16), p.act);
-      acc[i] += d[i];
-    }
-    if (p.dz) {
-      uint16_t* to = p.dz + m * p.dz_ld + c;
+      for (int i = 0; i < 4; ++i) g[r][i] = w[r][i] = 0u;
+      if (m >= p.M) continue;
       if (kVec) {
-        if (c < p.N)
-          *reinterpret_cast<uint4*>(to) = make_uint4(pack2(d[0], d[1], p.fp16), pack2(d[2], d[3], p.fp16), pack2(d[4], d[5], p.fp16), pack2(d[6], d[7], p.fp16));
+        if (c < p.N) {
+          const uint4 a = __ldg(reinterpret_cast<const uint4*>(dy));
+          g[r][0] = a.x; g[r][1] = a.y; g[r][2] = a.z; g[r][3] = a.w;
+          if (p.z) { const uint4 b = __ldg(reinterpret_cast<const uint4*>(z)); w[r][0] = b.x; w[r][1] = b.y; w[r][2] = b.z; w[r][3] = b.w; }
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i < p.N) to[i] = pack1(d[i], p.fp16);
+          if (c + i < p.N) {
+            g[r][i >> 1] |= (uint32_t)dy[i] << (16 * (i & 1));
+            if (p.z) w[r][i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
+          }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kDzRows; ++r) {
+      if (m0 + r >= p.M) break;
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = to_f(g[r][i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16);
+      if (p.z) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(w[r][i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16);
+        slopes(f, p.act);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= f[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += d[i];
+      if (p.dz) {
+        uint16_t* to = p.dz + (m0 + r) * p.dz_ld + c;
+        if (kVec) {
+          if (c < p.N)
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack2(d[0], d[1], p.fp16), pack2(d[2], d[3], p.fp16), pack2(d[4], d[5], p.fp16), pack2(d[6], d[7], p.fp16));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < p.N) to[i] = pack1(d[i], p.fp16);
+        }
       }
     }
   }
@@ -780,9 +810,11 @@ int set_limits() {
   GB_PAIR(kForward, 256, kPlain);
   GB_PAIR(kForward, 256, kResidual);
   GB_PAIR(kForward, 256, kKeepZ);
+  GB_PAIR(kForward, 256, kBoth);
   GB_PAIR(kForward, 192, kPlain);
   GB_PAIR(kForward, 192, kResidual);
   GB_PAIR(kForward, 192, kKeepZ);
+  GB_PAIR(kForward, 192, kBoth);
   GB_PAIR(kRowsGrad, 256, kPlain);
   GB_PAIR(kRowsGrad, 128, kPlain);
   GB_PAIR(kWeightGrad, 256, kPlain);
@@ -848,15 +880,14 @@ int run_pair(const Mats& m, LinearParams p, int pairs, cudaStream_t stream) {
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles * p.slices;
   GB_REQUIRE(tiles < (1ll << 30), "too many output tiles");
   p.idesc |= ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kPairM >> 4) << 24) | (S::kAmn ? 1u << 15 : 0u) | (S::kBmn ? 1u << 16 : 0u);
-  CUtensorMap map_a, map_b, map_d = {}, map_z = {}, map_r = {};
+  CUtensorMap map_a, map_b, map_d = {}, map_z = {};
   int rc = S::kAmn ? operand(&map_a, m.a, m.K, p.M, m.a_ld, kSlab) : operand(&map_a, m.a, p.M, m.K, m.a_ld, kBM);
   if (rc != GB_OK) return rc;
   rc = S::kBmn ? operand(&map_b, m.b, m.K, p.N, m.b_ld, kSlab) : operand(&map_b, m.b, p.N, m.K, m.b_ld, kBN / 2);
   if (rc != GB_OK) return rc;
   if (p.tma && p.slices == 1) {
     rc = tile_map(&map_d, p.d, p.M, p.N, p.N);
-    if (rc == GB_OK && kEpi == kKeepZ) rc = tile_map(&map_z, p.z, p.M, p.N, p.N);
-    if (rc == GB_OK && kEpi != kPlain && p.r) rc = tile_map(&map_r, p.r, p.M, p.N, p.r_ld);
+    if (rc == GB_OK && (kEpi & kKeepZ)) rc = tile_map(&map_z, p.z, p.M, p.N, p.N);
     if (rc != GB_OK) return rc;
   }
   cudaLaunchConfig_t cfg = {};
@@ -872,7 +903,7 @@ int run_pair(const Mats& m, LinearParams p, int pairs, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = gb_pdl_enabled() ? 2 : 1;
   gb_count_launch();
-  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, linear_pair_kernel<kMajor, kBN, kEpi>, map_a, map_b, map_d, map_z, map_r, p));
+  GB_CUDA_OK(cudaLaunchKernelEx(&cfg, linear_pair_kernel<kMajor, kBN, kEpi>, map_a, map_b, map_d, map_z, p));
   return GB_OK;
 }
 
@@ -990,9 +1021,9 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool products, bool
   g.dz_at = at;
   if (g.own_dz) at += up(M * g.dz_ld * 2);
   const int64_t sms = gb_sm_count() > 0 ? gb_sm_count() : 148;
-  // about eight blocks an SM; a block's warps walk at least two rows each
+  // about eight blocks an SM; a block's warps take four rows each at least
   int64_t rows = ceil_div(sms * 8, ceil_div(N, kDzCols));
-  if (rows > ceil_div(M, 16)) rows = ceil_div(M, 16);
+  if (rows > ceil_div(M, 32)) rows = ceil_div(M, 32);
   g.part_rows = (int)(rows < 1 ? 1 : rows > 512 ? 512 : rows);
   g.part_at = at;
   if (bias) at += up((int64_t)g.part_rows * N * 4);
@@ -1035,9 +1066,12 @@ int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, 
   const Mats m = {x, w, x_ld, K, K};
   const cudaStream_t st = (cudaStream_t)stream;
   if (rows_apply(M, N, ceil_div(K, kSlab))) return run_rows<false>(m, p, st);
-  if (narrower(M, N, 192, pairs))
-    return z ? run_pair<kForward, 192, kKeepZ>(m, p, pairs, st) : r ? run_pair<kForward, 192, kResidual>(m, p, pairs, st) : run_pair<kForward, 192, kPlain>(m, p, pairs, st);
-  return z ? run_pair<kForward, 256, kKeepZ>(m, p, pairs, st) : r ? run_pair<kForward, 256, kResidual>(m, p, pairs, st) : run_pair<kForward, 256, kPlain>(m, p, pairs, st);
+  const auto go = [&](auto bn) -> int {
+    constexpr int kBN = decltype(bn)::value;
+    if (z) return r ? run_pair<kForward, kBN, kBoth>(m, p, pairs, st) : run_pair<kForward, kBN, kKeepZ>(m, p, pairs, st);
+    return r ? run_pair<kForward, kBN, kResidual>(m, p, pairs, st) : run_pair<kForward, kBN, kPlain>(m, p, pairs, st);
+  };
+  return narrower(M, N, 192, pairs) ? go(std::integral_constant<int, 192>()) : go(std::integral_constant<int, 256>());
 }
 
 int64_t gb_linear_act_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int rows, int weight, int bias, int dy_whole) {
