@@ -19,6 +19,7 @@
 #include "gb_blocks.cuh"
 
 #include <cuda.h>
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -69,9 +70,9 @@ GB_DEVINL void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.i
 GB_DEVINL void expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-GB_DEVINL uint32_t leader_addr(uint32_t addr) {
+GB_DEVINL uint32_t of_rank(uint32_t addr, uint32_t rank) {       // the same place in the shared memory of another CTA of the cluster
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
 // What the pair of arrive and wait hands over is tensor memory alone, ordered by its own fences: the arrive may be relaxed.
@@ -84,10 +85,10 @@ GB_DEVINL void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1,
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
 // Into this CTA's shared memory, reported to a barrier of the pair.
-GB_DEVINL void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+GB_DEVINL void tma_load_pair(uint32_t dst, uint64_t map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
 GB_DEVINL void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
@@ -224,15 +225,13 @@ constexpr int kPairM = 256;
 constexpr int kChunk = 2048;                         // 32 rows x 32 columns on their way out
 constexpr int kGroupM = 16;                          // row tiles walked together before the next columns
 
-template <Major kMajor, int kBN, int kEpi>
+constexpr int kOutBytes = kEpiWarps * 2 * kChunk, kPairFixed = 1024 + 512;        // alignment, barriers
+template <Major kMajor, int kBN>
 struct Shape {
   static constexpr bool kAmn = kMajor == kWeightGrad, kBmn = kMajor != kForward;
-  static constexpr int kABytes = kBM * kSlabBytes, kBBytes = kBN / 2 * kSlabBytes, kStageBytes = kABytes + kBBytes;
-  static constexpr int kCols = kBN / 2, kChunks = kCols / 32;                       // of an epilogue warp
-  static constexpr int kOutBytes = kEpiWarps * 2 * kChunk;
-  static constexpr int kFixed = 1024 + 512;                                         // alignment, barriers
-  static constexpr int kFit = (227 * 1024 - kFixed - kOutBytes) / kStageBytes, kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + kFixed;
+  static constexpr int kABytes = kBM * kSlabBytes, kBBytes = kBmn ? (kBN + 127) / 128 * 8192 : kBN / 2 * kSlabBytes, kStageBytes = kABytes + kBBytes;
+  static constexpr int kFit = (227 * 1024 - kPairFixed - kOutBytes) / kStageBytes, kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + kPairFixed;
 };
 
 struct LinearParams {
@@ -262,13 +261,14 @@ template <Major kMajor, int kBN, int kEpi>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
                    const __grid_constant__ CUtensorMap map_z, const __grid_constant__ LinearParams p) {
-  using S = Shape<kMajor, kBN, kEpi>;
+  using S = Shape<kMajor, kBN>;
+  constexpr bool kAmn = S::kAmn, kBmn = S::kBmn;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (gb_smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
   uint8_t* ring_ptr = smem_raw + (ring - gb_smem_u32(smem_raw));
-  const uint32_t out_ring = ring + kStages * S::kStageBytes;             // per epilogue warp
-  const uint32_t full_bar = out_ring + S::kOutBytes;                     // leader: both CTAs' operand tiles have landed
+  const uint32_t out_ring = ring + kStages * S::kStageBytes;            // two chunks per epilogue warp
+  const uint32_t full_bar = out_ring + kOutBytes;                     // leader: both CTAs' operand tiles have landed
   const uint32_t empty_bar = full_bar + 8 * kStages;                     // the MMAs that read the stage are done
   const uint32_t acc_full = empty_bar + 8 * kStages;                     // [2] accumulator complete
   const uint32_t acc_empty = acc_full + 16;                              // [2] leader: drained by both CTAs
@@ -303,76 +303,81 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const uint32_t tmem_base = *slot_ptr;
   gb_pdl_wait();
 
+  const int k_tiles = p.k_tiles, per_slice = p.per_slice;
   const int per_tile = p.m_tiles * p.n_tiles, total_tiles = per_tile * p.slices;
   const int stride = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
 
   if (warp == kEpiWarps) {
     // ------------------------------- producer (each CTA) -------------------------------
-    const uint32_t full_pair = (uint32_t)uniform((int)leader_addr(full_bar));
+    // What its loop and the issuer's need lies in registers or is known to the compiler: a stage costs each of them a wait, a vote and a
+    // copy or MMA issued at a time, and with widths, stages and addresses taken from the parameters the narrow tiles waited for them
+    // (512 x 4096 x 4096 in tiles of 128: 17.5 us, 18.5 so; stages of two slabs, fewer of them, 21.9).
+    const uint32_t full_pair = (uint32_t)uniform((int)of_rank(full_bar, 0));
     const int me = uniform((int)rank);
     const bool one = gb_elect_one();
-    int s = 0;
-    uint32_t ph = 1;
+    const uint64_t ma = reinterpret_cast<uint64_t>(&map_a), mb = reinterpret_cast<uint64_t>(&map_b);
+    uint32_t at = 0, bar = 0, ph = 1;                        // the stage's place in the ring, its barriers'
     bool ok = true;
     for (int tile = first; ok && tile < total_tiles; tile += stride) {
       const int slice = tile / per_tile;
       int mt, nt;
       tile_at(p, tile - slice * per_tile, mt, nt);
       const int m0 = uniform(mt * kPairM) + me * kBM, n0 = uniform(nt * kBN) + me * (kBN / 2);
-      const int k_end = min(p.k_tiles, (slice + 1) * p.per_slice);
-      for (int kt = slice * p.per_slice; kt < k_end; ++kt) {
-        ok = warp_wait<true>(empty_bar + 8 * s, ph, abort_flag, p.status, 101);
+      const int k_end = uniform(min(k_tiles, (slice + 1) * per_slice)) * kSlab;
+      for (int k = uniform(slice * per_slice) * kSlab; k < k_end; k += kSlab) {
+        ok = warp_wait<true>(empty_bar + bar, ph, abort_flag, p.status, 101);
         if (!ok) break;
         if (one) {
-          const uint32_t st = ring + (uint32_t)s * S::kStageBytes, bar = full_pair + 8 * s;
-          if (me == 0) expect_tx(full_bar + 8 * s, 2 * S::kStageBytes);
-          if (S::kAmn) {
+          const uint32_t sa = ring + at, sb = sa + S::kABytes, full = full_pair + bar;
+          if (me == 0) expect_tx(full_bar + bar, 2 * S::kStageBytes);
+          if (kAmn) {
 #pragma unroll
-            for (int i = 0; i < kBM / 64; ++i) tma_load_pair(st + 8192 * i, &map_a, m0 + 64 * i, kt * kSlab, bar);
+            for (int i = 0; i < kBM / 64; ++i) tma_load_pair(sa + 8192 * i, ma, m0 + 64 * i, k, full);
           } else {
-            tma_load_pair(st, &map_a, kt * kSlab, m0, bar);
+            tma_load_pair(sa, ma, k, m0, full);
           }
-          if (S::kBmn) {
+          if (kBmn) {
 #pragma unroll
-            for (int i = 0; i < kBN / 128; ++i) tma_load_pair(st + S::kABytes + 8192 * i, &map_b, n0 + 64 * i, kt * kSlab, bar);
+            for (int i = 0; i < S::kBBytes / 8192; ++i) tma_load_pair(sb + 8192 * i, mb, n0 + 64 * i, k, full);
           } else {
-            tma_load_pair(st + S::kABytes, &map_b, kt * kSlab, n0, bar);
+            tma_load_pair(sb, mb, k, n0, full);
           }
         }
         __syncwarp();
-        if (++s == kStages) { s = 0; ph ^= 1; }
+        at += S::kStageBytes;
+        bar += 8;
+        if (bar == 8 * kStages) { at = bar = 0; ph ^= 1; }
       }
     }
   } else if (warp == kEpiWarps + 1) {
     // --------------------------- MMA issuer (the leader's) ------------------------------
     if (uniform((int)rank) == 0) {
-      uint32_t to_peer;                                      // distance of the peer's barriers
-      asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(to_peer) : "r"(full_bar));
-      to_peer = (uint32_t)uniform((int)(to_peer - full_bar));
-      const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
+      const uint32_t to_peer = (uint32_t)uniform((int)(of_rank(full_bar, 1) - full_bar));   // distance of the peer's barriers
+      const uint32_t tmem = (uint32_t)uniform((int)tmem_base), idesc = p.idesc;
       const bool one = gb_elect_one();
-      int s = 0, it = 0;
-      uint32_t ph = 0;
+      int it = 0;
+      uint32_t at = 0, bar = 0, ph = 0;
       bool ok = true;
       for (int tile = first; ok && tile < total_tiles; tile += stride, ++it) {
-        const int buf = it & 1, slice = tile / per_tile, k_begin = slice * p.per_slice, k_end = min(p.k_tiles, k_begin + p.per_slice);
+        const int buf = it & 1, slice = tile / per_tile, stages = uniform(min(k_tiles, (slice + 1) * per_slice) - slice * per_slice);
         ok = warp_wait<true>(acc_empty + 8 * buf, ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, p.status, 102);   // its last tile is drained
         if (!ok) break;
         const uint32_t acc = tmem + (buf ? 256u : 0u);
-        for (int kt = k_begin; kt < k_end; ++kt) {
-          ok = warp_wait(full_bar + 8 * s, ph, abort_flag, p.status, 103);
+        for (int kt = 0; kt < stages; ++kt) {
+          ok = warp_wait(full_bar + bar, ph, abort_flag, p.status, 103);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t st = ring + (uint32_t)s * S::kStageBytes;
-          const uint64_t da = desc_of<S::kAmn>(st), db = desc_of<S::kBmn>(st + S::kABytes);
           if (one) {
+            const uint64_t da = desc_of<kAmn>(ring + at), db = desc_of<kBmn>(ring + at + S::kABytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_16bit<2>(acc, da + kStep<S::kAmn> * k, db + kStep<S::kBmn> * k, p.idesc, kt > k_begin || k > 0);
-            commit_to<2>(empty_bar + 8 * s);
-            commit_to<2>(empty_bar + to_peer + 8 * s);
+            for (int i = 0; i < 4; ++i) mma_16bit<2>(acc, da + kStep<kAmn> * i, db + kStep<kBmn> * i, idesc, kt > 0 || i > 0);
+            commit_to<2>(empty_bar + bar);
+            commit_to<2>(empty_bar + to_peer + bar);
           }
           __syncwarp();
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          at += S::kStageBytes;
+          bar += 8;
+          if (bar == 8 * kStages) { at = bar = 0; ph ^= 1; }
         }
         if (ok && one) {
           commit_to<2>(acc_full + 8 * buf);
@@ -387,8 +392,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     // residuals are on their way meanwhile.  (Residuals by TMA into the buffers of the output, and buffers of z's own, took one or two
     // of the six stages: 4096 x 8192 x 5120 with residual 263 us, keeping z 301.)
     constexpr bool kRes = (kEpi & kResidual) != 0, kZ = (kEpi & kKeepZ) != 0;
-    const uint32_t acc_empty_pair = leader_addr(acc_empty);
-    const int quarter = warp & 3, c_lo = (warp >> 2) * S::kCols;
+    const uint32_t acc_empty_pair = of_rank(acc_empty, 0);
+    constexpr int kChunks = kBN / 32, kHalf = (kChunks + 1) / 2;
+    const int mine = warp < 4 ? kHalf : kChunks - kHalf;                 // of the warp's columns
+    const int quarter = warp & 3, c_lo = warp < 4 ? 0 : 32 * kHalf;
     const uint32_t out = out_ring + (uint32_t)warp * 2 * kChunk;
     const uint32_t row_at = (uint32_t)lane * 64u, swz = (uint32_t)((lane >> 1) & 3);
     const bool staged = p.tma && p.slices == 1;
@@ -398,10 +405,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       int mt, nt;
       tile_at(p, tile - slice * per_tile, mt, nt);
       const int n0 = nt * kBN + c_lo, row0 = mt * kPairM + (int)rank * kBM + quarter * 32, row = row0 + lane;
-      uint32_t bias[(S::kCols + 63) / 64];                          // columns 64 i + 2 lane and the next, zeros past the last
+      uint32_t bias[2];                                      // of columns 64 i + 2 lane and the next, zeros past the last
       if (kMajor == kForward) {
 #pragma unroll
-        for (int i = 0; i < (S::kCols + 63) / 64; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const int c = n0 + 64 * i + 2 * lane;
           bias[i] = (p.bias && c < p.N ? (uint32_t)__ldg(p.bias + c) : 0u) | (p.bias && c + 1 < p.N ? (uint32_t)__ldg(p.bias + c + 1) << 16 : 0u);
         }
@@ -420,12 +427,13 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       uint32_t raw[32];
       tmem_ld32(at, raw);
 #pragma unroll
-      for (int c = 0; c < S::kChunks; ++c) {
+      for (int c = 0; c < kHalf; ++c) {
+        if (c >= mine) break;
         float v[32];
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-        if (c == S::kChunks - 1) {
+        if (c == mine - 1) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) arrive_cluster(acc_empty_pair + 8 * buf);
@@ -485,7 +493,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 v[8 * q + 2 * j + 1] += to_f(w[j] >> 16, p.fp16);
               }
             }
-            if (c + 1 < S::kChunks) fetch_residual(c + 1);
+            if (c + 1 < mine) fetch_residual(c + 1);
           }
           send(&map_d);
         } else if (row < p.M) {
@@ -519,6 +527,33 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 constexpr int kMaxRows = 256, kMaxStages = 8, kMaxSlices = 8;
 constexpr int kRowsSmem = 224 * 1024;
 constexpr int kRowsThreads = 32 * (kEpiWarps + 2);
+
+// The epilogue of four neighbouring outputs of a row; `left` of them and what lies behind them are inside.
+GB_DEVINL void finish4(const LinearParams& p, float (&v)[4], const float (&bias)[4], int64_t m, int n, int left) {
+  const int64_t at = m * p.N + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] += bias[i];
+  if (p.tma) {
+    if (p.z) *reinterpret_cast<uint2*>(p.z + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
+    activate(v, p.act);
+    if (p.r) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p.r + m * p.r_ld + n);
+      v[0] += to_f(w.x & 0xFFFFu, p.fp16); v[1] += to_f(w.x >> 16, p.fp16);
+      v[2] += to_f(w.y & 0xFFFFu, p.fp16); v[3] += to_f(w.y >> 16, p.fp16);
+    }
+    *reinterpret_cast<uint2*>(p.d + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
+  } else {
+    if (p.z) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) p.z[at + i] = pack1(v[i], p.fp16);
+    }
+    activate(v, p.act);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p.d[at + i] = pack1(p.r ? v[i] + to_f(p.r[m * p.r_ld + n + i], p.fp16) : v[i], p.fp16);
+  }
+}
 
 template <bool kWmn>
 __global__ void __launch_bounds__(kRowsThreads, 1)
@@ -654,29 +689,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         for (int i = 0; i < 4; ++i) v[i] += u[i];
       }
       if (left <= 0) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += bias[i];
-      const int64_t m = m0 + slice * own + r, at = m * p.N + n0 + f;
-      if (p.tma) {
-        if (p.z) *reinterpret_cast<uint2*>(p.z + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
-        activate(v, p.act);
-        if (p.r) {
-          const uint2 w = *reinterpret_cast<const uint2*>(p.r + m * p.r_ld + n0 + f);
-          v[0] += to_f(w.x & 0xFFFFu, p.fp16); v[1] += to_f(w.x >> 16, p.fp16);
-          v[2] += to_f(w.y & 0xFFFFu, p.fp16); v[3] += to_f(w.y >> 16, p.fp16);
-        }
-        *reinterpret_cast<uint2*>(p.d + at) = make_uint2(pack2(v[0], v[1], p.fp16), pack2(v[2], v[3], p.fp16));
-      } else {
-        if (p.z) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < left) p.z[at + i] = pack1(v[i], p.fp16);
-        }
-        activate(v, p.act);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < left) p.d[at + i] = pack1(p.r ? v[i] + to_f(p.r[m * p.r_ld + n0 + f + i], p.fp16) : v[i], p.fp16);
-      }
+      finish4(p, v, bias, (int64_t)m0 + slice * own + r, n0 + f, left);
     }
   }
   __syncwarp();
@@ -775,27 +788,28 @@ linear_dz_kernel(const __grid_constant__ DzParams p) {
   p.part[(int64_t)blockIdx.y * p.N + col] = sum;
 }
 
-// The slices' sums, four values a thread.
+// The slices' sums, in their order, and the epilogue behind them; a thread has four neighbours of a row.
 __global__ void __launch_bounds__(256)
-linear_slices_kernel(const float* sums, int64_t values, int slices, uint16_t* d, int fp16) {
+linear_join_kernel(const __grid_constant__ LinearParams p) {
   gb_pdl_launch_dependents();
   gb_pdl_wait();
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= values) return;
-  if (values % 4 == 0) {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = 0; s < slices; ++s) {
-      const float4 u = *reinterpret_cast<const float4*>(sums + s * values + at);
-      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-    }
-    *reinterpret_cast<uint2*>(d + at) = make_uint2(pack2(v.x, v.y, fp16), pack2(v.z, v.w, fp16));
-  } else {
-    for (int i = 0; i < 4 && at + i < values; ++i) {
-      float v = 0.0f;
-      for (int s = 0; s < slices; ++s) v += sums[s * values + at + i];
-      d[at + i] = pack1(v, fp16);
+  const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, m = blockIdx.y, at = m * p.N + n, values = p.M * p.N;
+  if (n >= p.N) return;
+  const int left = (int)min((int64_t)4, p.N - n);
+  float v[4] = {}, bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = p.bias && i < left ? to_f(p.bias[n + i], p.fp16) : 0.0f;
+  for (int s = 0; s < p.slices; ++s) {
+    if (p.N % 4 == 0) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p.sums + s * values + at));
+      v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) v[i] += p.sums[s * values + at + i];
     }
   }
+  finish4(p, v, bias, m, (int)n, left);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -806,19 +820,20 @@ GbClusters g_clusters;
 
 int set_limits() {
 #define GB_ATTR(k, bytes) GB_CUDA_OK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
-#define GB_PAIR(M, N, E) GB_ATTR((linear_pair_kernel<M, N, E>), (Shape<M, N, E>::kSmem))
-  GB_PAIR(kForward, 256, kPlain);
-  GB_PAIR(kForward, 256, kResidual);
-  GB_PAIR(kForward, 256, kKeepZ);
-  GB_PAIR(kForward, 256, kBoth);
-  GB_PAIR(kForward, 192, kPlain);
-  GB_PAIR(kForward, 192, kResidual);
-  GB_PAIR(kForward, 192, kKeepZ);
-  GB_PAIR(kForward, 192, kBoth);
+#define GB_PAIR(M, N, E) GB_ATTR((linear_pair_kernel<M, N, E>), (Shape<M, N>::kSmem))
+#define GB_FORWARD(N) GB_PAIR(kForward, N, kPlain); GB_PAIR(kForward, N, kResidual); GB_PAIR(kForward, N, kKeepZ); GB_PAIR(kForward, N, kBoth)
+  GB_FORWARD(256);
+  GB_FORWARD(224);
+  GB_FORWARD(192);
+  GB_FORWARD(160);
+  GB_FORWARD(128);
   GB_PAIR(kRowsGrad, 256, kPlain);
+  GB_PAIR(kRowsGrad, 192, kPlain);
   GB_PAIR(kRowsGrad, 128, kPlain);
   GB_PAIR(kWeightGrad, 256, kPlain);
+  GB_PAIR(kWeightGrad, 192, kPlain);
   GB_PAIR(kWeightGrad, 128, kPlain);
+#undef GB_FORWARD
   GB_ATTR(linear_rows_kernel<false>, kRowsSmem);
   GB_ATTR(linear_rows_kernel<true>, kRowsSmem);
 #undef GB_PAIR
@@ -836,11 +851,10 @@ int ready(int* pairs) {
     std::lock_guard<std::mutex> lock(g_mutex);
     const int rc = set_limits();
     if (rc != GB_OK) return rc;
-    using S = Shape<kForward, 256, kPlain>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * 256);
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.dynamicSmemBytes = Shape<kForward, 256>::kSmem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -871,7 +885,7 @@ struct Mats {
 
 template <Major kMajor, int kBN, int kEpi>
 int run_pair(const Mats& m, LinearParams p, int pairs, cudaStream_t stream) {
-  using S = Shape<kMajor, kBN, kEpi>;
+  using S = Shape<kMajor, kBN>;
   p.k_tiles = (int)ceil_div(m.K, kSlab);
   p.m_tiles = (int)ceil_div(p.M, kPairM);
   p.n_tiles = (int)ceil_div(p.N, kBN);
@@ -926,12 +940,10 @@ Split split_of(int64_t M, int64_t N, int64_t k_tiles) {
   s.slices = (int)ceil_div(k_tiles, s.per_slice);
   return s;
 }
-// Where the few-rows kernel is the faster one: the rule of the other 16-bit GEMM (gb_gemm_rows_applies).
-bool rows_apply(int64_t M, int64_t N, int64_t k_tiles) {
-  if (M <= 192) return true;
-  if (M > 1024) return false;
-  const Split s = split_of(M, N, k_tiles);
-  return s.tiles <= gb_sm_count() && s.per_slice <= 64;
+int run_join(const LinearParams& p, cudaStream_t stream) {
+  GB_REQUIRE(p.M <= 65535, "too many rows of sliced sums");
+  GB_CUDA_OK(gb_launch(linear_join_kernel, dim3((unsigned)ceil_div(p.N, 1024), (unsigned)p.M), dim3(256), 0, stream, p));
+  return GB_OK;
 }
 
 template <bool kWmn>
@@ -991,10 +1003,66 @@ LinearParams params_of(int64_t M, int64_t N, int dtype, void* d) {
   return p;
 }
 
-// Width of a tile: 256 columns, or `narrow` where that saves more of the last wave than its extra operand traffic costs.
-bool narrower(int64_t M, int64_t N, int narrow, int64_t pairs) {
-  const int64_t mt = ceil_div(M, kPairM);
-  return ceil_div(mt * ceil_div(N, narrow), pairs) * narrow * 21 < ceil_div(mt * ceil_div(N, 256), pairs) * 256 * 20;
+// Which kernel a product takes, and how wide a pair's tiles are: what this estimate, in us, is least for.  A slab of a tile costs what its
+// MMAs take, 30% more than at full rate, or what the fetches of all CTAs that run with it take out of L2 at 14 TB/s; in front and
+// behind are the launch, the first fetches and the last tile's epilogue, and the slices' sums on their way to each other.  Measured (estimated), us, weights
+// from HBM, tiles of 128 / 160 / 192 / 256 columns / few-rows kernel:
+//   128 x 4096 x 4096    17.8 (17.8) / 20.3 / 22.5 / 27.5 (28.4) / 13.8 (13.3)
+//   256 x 4096 x 4096    17.8 / 20.2 / 22.4 / 27.6 / 19.0 (17.3)
+//   512 x 4096 x 4096    18.5 (19.4) / 20.3 / 23.5 / 28.5 (28.4) / 23.4
+//   1000 x 2048 x 2048   12.4 (12.2) / 14.2 / 15.5 / 18.1 (17.2) / 17.8
+//   333 x 5120 x 17408   97 / 65 (65) / 72 (77) / 92 (101) / 81 (77)
+//   700 x 4096 x 4096    29.3 / 32.4 / 23.7 / 29.9 / 36.5
+//   4096 x 8192 x 5120   273 / 254 / 249 / 225
+double slab_us(int64_t ctas, double bytes, double columns) { return std::max(columns * 2.0 / 1900.0 * 1.3, (double)ctas * bytes / 14e6); }
+double pair_us(int64_t M, int64_t N, int64_t k_tiles, int width, int64_t pairs) {
+  const int64_t tiles = ceil_div(M, kPairM) * ceil_div(N, width), full = tiles / pairs, rest = tiles - full * pairs;
+  const double bytes = kBM * kSlabBytes + width / 2 * kSlabBytes;
+  return 4.0 + width / 128.0 + (double)k_tiles * ((double)full * slab_us(2 * pairs, bytes, width) + (rest ? slab_us(2 * rest, bytes, width) : 0.0));
+}
+double rows_us(int64_t M, int64_t N, int64_t k_tiles) {
+  const Split s = split_of(M, N, k_tiles);
+  const int64_t sms = gb_sm_count(), ctas = s.tiles * s.slices, box = ceil_div(s.rows, 16) * 16;
+  return 4.5 + (s.slices > 1 ? 1.0 + 0.02 * s.rows : 0.01 * s.rows) +
+         (double)(ceil_div(ctas, sms) * s.per_slice) * slab_us(std::min(ctas, sms), kBM * kSlabBytes + (double)box * kSlabBytes, (double)box);
+}
+constexpr int kWidths[] = {256, 224, 192, 160, 128}, kGradWidths[] = {256, 192, 128};
+template <int kN>
+int width_of(const int (&widths)[kN], int64_t M, int64_t N, int64_t k_tiles, int64_t pairs, double* us = nullptr) {
+  int best = 0;
+  double least = 0.0;
+  for (int w : widths) {
+    const double t = pair_us(M, N, k_tiles, w, pairs);
+    if (best == 0 || t < least) { least = t; best = w; }
+  }
+  if (us) *us = least;
+  return best;
+}
+// Width of a pair's tiles; 0: the few-rows kernel.
+template <int kN>
+int route_of(const int (&widths)[kN], int64_t M, int64_t N, int64_t K, int pairs) {
+  const int64_t k_tiles = ceil_div(K, kSlab);
+  double us;
+  const int width = width_of(widths, M, N, k_tiles, pairs, &us);
+  return M <= 1024 && rows_us(M, N, k_tiles) < us ? 0 : width;
+}
+template <int kEpi>
+int run_forward(int width, const Mats& m, const LinearParams& p, int pairs, cudaStream_t st) {
+  switch (width) {
+    case 224: return run_pair<kForward, 224, kEpi>(m, p, pairs, st);
+    case 192: return run_pair<kForward, 192, kEpi>(m, p, pairs, st);
+    case 160: return run_pair<kForward, 160, kEpi>(m, p, pairs, st);
+    case 128: return run_pair<kForward, 128, kEpi>(m, p, pairs, st);
+    default: return run_pair<kForward, 256, kEpi>(m, p, pairs, st);
+  }
+}
+template <Major kMajor>
+int run_grad(int width, const Mats& m, const LinearParams& p, int pairs, cudaStream_t st) {
+  switch (width) {
+    case 192: return run_pair<kMajor, 192, kPlain>(m, p, pairs, st);
+    case 128: return run_pair<kMajor, 128, kPlain>(m, p, pairs, st);
+    default: return run_pair<kMajor, 256, kPlain>(m, p, pairs, st);
+  }
 }
 
 int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
@@ -1010,9 +1078,10 @@ bool aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 struct GradPlan {
   bool own_dz;                 // dz is a matrix of its own
   int64_t dz_ld, dz_at, part_at, sums_at, bytes;
-  int part_rows, slices, narrow;
+  int part_rows, slices, rows_width, width;                  // slices of dW, widths of dX's and dW's tiles
 };
-GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool products, bool bias, bool weight, bool dy_whole) {
+GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool rows_too, bool weight, bool bias, bool dy_whole, int pairs) {
+  const bool products = rows_too || weight;
   GradPlan g = {};
   auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
   g.dz_ld = ceil_div(N, 8) * 8;
@@ -1029,10 +1098,11 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool products, bool
   if (bias) at += up((int64_t)g.part_rows * N * 4);
   g.sums_at = at;
   g.slices = 1;
+  if (rows_too) g.rows_width = route_of(kGradWidths, M, K, N, pairs);
   if (weight) {
-    const int64_t pairs = sms / 2, k_tiles = ceil_div(M, kSlab);
-    g.narrow = narrower(N, K, 128, pairs);
-    const int64_t tiles = ceil_div(N, kPairM) * ceil_div(K, g.narrow ? 128 : 256);
+    const int64_t k_tiles = ceil_div(M, kSlab);
+    g.width = width_of(kGradWidths, N, K, k_tiles, pairs);
+    const int64_t tiles = ceil_div(N, kPairM) * ceil_div(K, g.width);
     // as many slices as the pairs take at once, of at least eight slabs
     while (g.slices < 16 && tiles * (g.slices + 1) <= pairs && (g.slices + 1) * 8 <= k_tiles) ++g.slices;
     if (g.slices > 1) at += up((int64_t)g.slices * N * K * 4);
@@ -1065,17 +1135,15 @@ int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, 
   if (r && (!aligned(r) || r_ld % 8 != 0)) p.tma = 0;
   const Mats m = {x, w, x_ld, K, K};
   const cudaStream_t st = (cudaStream_t)stream;
-  if (rows_apply(M, N, ceil_div(K, kSlab))) return run_rows<false>(m, p, st);
-  const auto go = [&](auto bn) -> int {
-    constexpr int kBN = decltype(bn)::value;
-    if (z) return r ? run_pair<kForward, kBN, kBoth>(m, p, pairs, st) : run_pair<kForward, kBN, kKeepZ>(m, p, pairs, st);
-    return r ? run_pair<kForward, kBN, kResidual>(m, p, pairs, st) : run_pair<kForward, kBN, kPlain>(m, p, pairs, st);
-  };
-  return narrower(M, N, 192, pairs) ? go(std::integral_constant<int, 192>()) : go(std::integral_constant<int, 256>());
+  const int width = route_of(kWidths, M, N, K, pairs);
+  if (width == 0) return run_rows<false>(m, p, st);
+  if (z) return r ? run_forward<kBoth>(width, m, p, pairs, st) : run_forward<kKeepZ>(width, m, p, pairs, st);
+  return r ? run_forward<kResidual>(width, m, p, pairs, st) : run_forward<kPlain>(width, m, p, pairs, st);
 }
 
 int64_t gb_linear_act_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int rows, int weight, int bias, int dy_whole) {
-  return M < 1 || N < 1 || K < 1 ? 0 : grad_plan(M, N, K, act, rows || weight, bias != 0, weight != 0, dy_whole != 0).bytes;
+  int pairs = 0;
+  return M < 1 || N < 1 || K < 1 || ready(&pairs) != GB_OK ? 0 : grad_plan(M, N, K, act, rows != 0, weight != 0, bias != 0, dy_whole != 0, pairs).bytes;
 }
 
 int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void* x, int64_t x_ld, const void* w, int dtype, int64_t M, int64_t N, int64_t K, int act,
@@ -1090,7 +1158,7 @@ int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void*
   rc = ready(&pairs);
   if (rc != GB_OK) return rc;
   const bool dy_whole = aligned(dy) && dy_ld % 8 == 0;
-  const GradPlan g = grad_plan(M, N, K, act, dx || dw, dbias != nullptr, dw != nullptr, dy_whole);
+  const GradPlan g = grad_plan(M, N, K, act, dx != nullptr, dw != nullptr, dbias != nullptr, dy_whole, pairs);
   if (workspace_bytes < g.bytes || (g.bytes > 0 && !workspace))
     return gb_fail(GB_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)g.bytes);
   GB_REQUIRE(aligned(workspace), "the workspace must be 16-byte aligned");
@@ -1118,8 +1186,7 @@ int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void*
   if (dx) {                                                  // [M, K], the contraction over N
     const LinearParams p = params_of(M, K, dtype, dx);
     const Mats m = {dz, w, dz_ld, K, N};
-    if (rows_apply(M, K, ceil_div(N, kSlab))) rc = run_rows<true>(m, p, st);
-    else rc = narrower(M, K, 128, pairs) ? run_pair<kRowsGrad, 128, kPlain>(m, p, pairs, st) : run_pair<kRowsGrad, 256, kPlain>(m, p, pairs, st);
+    rc = g.rows_width == 0 ? run_rows<true>(m, p, st) : run_grad<kRowsGrad>(g.rows_width, m, p, pairs, st);
     if (rc != GB_OK) return rc;
   }
   if (dw) {                                                  // [N, K], the contraction over M
@@ -1128,10 +1195,9 @@ int gb_linear_act_grad(const void* dy, int64_t dy_ld, const void* z, const void*
     const int64_t k_tiles = ceil_div(M, kSlab);
     p.slices = (int)ceil_div(k_tiles, ceil_div(k_tiles, g.slices));      // none of them empty
     p.sums = reinterpret_cast<float*>(ws + g.sums_at);
-    rc = g.narrow ? run_pair<kWeightGrad, 128, kPlain>(m, p, pairs, st) : run_pair<kWeightGrad, 256, kPlain>(m, p, pairs, st);
+    rc = run_grad<kWeightGrad>(g.width, m, p, pairs, st);
+    if (rc == GB_OK && p.slices > 1) rc = run_join(p, st);
     if (rc != GB_OK) return rc;
-    if (p.slices > 1)
-      GB_CUDA_OK(gb_launch(linear_slices_kernel, dim3((unsigned)ceil_div(N * K, 1024)), dim3(256), 0, st, p.sums, N * K, p.slices, p.d, p.fp16));
   }
   return GB_OK;
 }
