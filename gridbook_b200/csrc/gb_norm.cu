@@ -17,6 +17,8 @@
 // adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value.
 #include "gb_blocks.cuh"
 
+#include <atomic>
+
 namespace {
 
 using namespace gb_blocks;
@@ -175,7 +177,12 @@ GB_DEVINL void store8(typename T::word* p, const Raw8<T>& r) {
 }
 template <typename T>
 GB_DEVINL void store8(typename T::word* p, const F8& f) { store8<T>(p, rounded<T>(f)); }
-// Weights of eight columns in shared memory, o + w; kRaw: of the rows' own type.
+// What a launch has is known to the compiler in the forms that models have: rows of exactly kV x 8 columns a thread, weights of the rows'
+// own type with nothing added, all gradients there and asked for.  (Bounds, types and absent inputs looked at for every eight
+// columns were a third of the instructions: 8192 x 5120 bf16 forward 66 us, backward 116.)
+enum Form { kAny = 0, kPostGate = 1, kPost = 2, kPre = 3 };          // both norms with a gate that rows share, without a gate; the second norm alone
+
+// Weights of eight columns in shared memory, o + w; kRaw: of the rows' own type, o zero.
 template <typename T, bool kRaw>
 struct Weights {
   const uint8_t* p;
@@ -187,7 +194,7 @@ struct Weights {
     else if (type == GB_DTYPE_BF16) v = load8<Bf16>(reinterpret_cast<const uint16_t*>(p) + c);
     else if (type == GB_DTYPE_FP16) v = load8<Fp16>(reinterpret_cast<const uint16_t*>(p) + c);
     else v = load8<Fp32>(reinterpret_cast<const uint32_t*>(p) + c);
-    return offset == 0.0f ? v : v + all8(offset);
+    return kRaw || offset == 0.0f ? v : v + all8(offset);
   }
 };
 // The weights' way there, by one thread; they are waited for like a row.
@@ -214,7 +221,7 @@ struct Ring {
   }
 };
 
-template <typename T, typename R, int kV, int kThreads, bool kFp8, bool kRaw>
+template <typename T, typename R, int kV, int kThreads, bool kFp8, Form kForm>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 norm_rows_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
@@ -234,7 +241,9 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
   __syncthreads();
   gb_pdl_wait();
   const uint32_t y_bytes = (uint32_t)(H * (int)sizeof(word)), r_bytes = (uint32_t)(H * (int)sizeof(rword));
-  const bool own_gate = p.in_at[2] != ~0u;               // every row has a gate of its own
+  constexpr bool kKnown = kForm != kAny;
+  const bool has_w = kKnown || p.w, has_pw = kKnown ? kForm != kPre : p.pw != nullptr, has_gate = kKnown ? kForm == kPostGate : p.gate != nullptr;
+  const bool own_gate = !kKnown && p.in_at[2] != ~0u;    // every row has a gate of its own
   auto fetch = [&](int64_t t, int s) {
     uint8_t* st = ring + (size_t)s * p.stage_bytes;
     gb_mbar_expect_tx(&full[s], p.stage_bytes);
@@ -248,8 +257,8 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     for (int s = 1; s < p.stages; ++s)
       if ((int64_t)blockIdx.x + (int64_t)s * step < T_) fetch((int64_t)blockIdx.x + (int64_t)s * step, s);
   }
-  const bool one_gate = p.g_at != ~0u;                   // the same for all rows
-  const Weights<T, kRaw> w{ring + p.w_at, p.w_type, p.offset}, pw{ring + p.pw_at, p.pw_type, p.offset};
+  const bool one_gate = kKnown ? has_gate : p.g_at != ~0u;                   // the same for all rows
+  const Weights<T, kKnown> w{ring + p.w_at, p.w_type, p.offset}, pw{ring + p.pw_at, p.pw_type, p.offset};
   const Ring wheel{full, &gave_up};
   int turn = 0, i = 0, s = 0;
   uint32_t phase = 0;
@@ -263,26 +272,26 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     for (int k = 0; k < kV; ++k) {
       const int c = (k * (int)blockDim.x + tid) * 8;
       x[k] = all8(0.0f);
-      if (c < H) {
+      if (kKnown || c < H) {
         x[k] = load8<T>(reinterpret_cast<const word*>(st + p.in_at[0]) + c);
         dot8(x[k], x[k], sum);
       }
     }
-    if (p.pw) rp = rsqrtf(fmaf(block_sum(halves(sum), red, turn), p.inv_h, p.eps));
+    if (has_pw) rp = rsqrtf(fmaf(block_sum(halves(sum), red, turn), p.inv_h, p.eps));
     sum = 0;
     if (i == 0) wheel.wait(0, kMostStages, 0, p.status, 91);
     const word* gate_row = nullptr;
     if (own_gate) gate_row = reinterpret_cast<const word*>(st + p.in_at[2]);
     else if (one_gate) gate_row = reinterpret_cast<const word*>(ring + p.g_at);
-    else if (p.gate) gate_row = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
+    else if (has_gate) gate_row = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
     rword* out = static_cast<rword*>(p.s) + t * H;
     const uint64_t scale_r = both(p.a), scale_u = both(p.b * rp);
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
       const int c = (k * (int)blockDim.x + tid) * 8;
-      if (c < H) {
-        if (p.pw) x[k] = x[k] * pw.get(c);
-        if (p.gate) x[k] = x[k] * load8<T>(gate_row + c);
+      if (kKnown || c < H) {
+        if (has_pw) x[k] = x[k] * pw.get(c);
+        if (has_gate) x[k] = x[k] * load8<T>(gate_row + c);
         x[k] = fma8(x[k], scale_u, load8<R>(reinterpret_cast<const rword*>(st + p.in_at[1]) + c) * scale_r);
         const Raw8<R> kept = rounded<R>(x[k]);
         store8<R>(out + c, kept);
@@ -302,8 +311,8 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     for (int k = 0; k < kV; ++k) {
       const int c = (k * (int)blockDim.x + tid) * 8;
       x[k] = x[k] * both(rs);
-      if (c < H) {
-        if (p.w) x[k] = x[k] * w.get(c);
+      if (kKnown || c < H) {
+        if (has_w) x[k] = x[k] * w.get(c);
         if (!kFp8) store8<T>(static_cast<word*>(p.h) + t * H + c, x[k]);
       }
       if constexpr (kFp8) {                              // sixteen neighbours have a block
@@ -312,7 +321,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) asm("mov.b64 {%0, %1}, %2;" : "=f"(h[2 * j]), "=f"(h[2 * j + 1]) : "l"(x[k].v[j]));
         quantize_block<8, 16>(h, p.scale_rule, scale, q);
-        if (c < H) {
+        if (kKnown || c < H) {
           *reinterpret_cast<uint2*>(p.q + t * H + c) = make_uint2(q[0], q[1]);
           if ((tid & 15) == 0) p.scale[t * ((H + kBlock - 1) / kBlock) + c / kBlock] = scale;
         }
@@ -323,7 +332,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
 }
 
 // kR rows at a time between the barriers: they share what is unpacked of the weights.
-template <typename T, typename R, int kV, int kR, int kThreads, bool kRaw>
+template <typename T, typename R, int kV, int kR, int kThreads, Form kForm>
 __global__ void __launch_bounds__(kThreads, kThreads <= 256 ? 2 : 1)
 norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   using word = typename T::word;
@@ -347,7 +356,10 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   const int begin = p.per_gate == 0 ? (int)blockIdx.x : (int)blockIdx.x % p.per_gate, step = p.per_gate == 0 ? (int)gridDim.x : p.per_gate;
   const int mine = (rows - begin + step - 1) / step;
   const uint32_t y_bytes = (uint32_t)(H * (int)sizeof(word)), r_bytes = (uint32_t)(H * (int)sizeof(rword));
-  const bool own_gate = p.in_at[4] != ~0u;               // every row has a gate of its own
+  constexpr bool kKnown = kForm != kAny;
+  const bool has_w = kKnown || p.w, has_pw = kKnown ? kForm != kPre : p.pw != nullptr, has_gate = kKnown ? kForm == kPostGate : p.gate != nullptr;
+  const bool has_y = kKnown ? kForm != kPre : p.in_at[3] != ~0u, has_dh = kKnown || p.dh, has_ds = kKnown || p.ds;
+  const bool own_gate = !kKnown && p.in_at[4] != ~0u;    // every row has a gate of its own
   auto fetch = [&](int n, int s) {                       // the n-th row of the share
     const int64_t t = first + begin + (int64_t)n * step;
     uint8_t* st = ring + (size_t)s * p.stage_bytes;
@@ -364,8 +376,8 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     for (int s = 1; s < p.stages; ++s)
       if (s < mine) fetch(s, s);
   }
-  const Weights<T, kRaw> w_of{ring + p.w_at, p.w_type, p.offset}, pw_of{ring + p.pw_at, p.pw_type, p.offset};
-  const bool many_gates = p.gate && !own_gate && p.g_at == ~0u;      // a gate without a gradient
+  const Weights<T, kKnown> w_of{ring + p.w_at, p.w_type, p.offset}, pw_of{ring + p.pw_at, p.pw_type, p.offset};
+  const bool many_gates = !kKnown && p.gate && !own_gate && p.g_at == ~0u;      // a gate without a gradient
   const Ring wheel{full, &gave_up};
   wheel.wait(0, kMostStages, 0, p.status, 92);
   F8 acc_w[kV], acc_pw[kV], acc_g[kV];
@@ -393,7 +405,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     for (int q = 0; q < kR; ++q) {
       const int64_t t = first + begin + (int64_t)(n + q) * step;
       rs_next[q] = n + q < mine ? __ldg(p.rstd + t) : 0.0f;
-      rp_next[q] = n + q < mine && p.pw ? __ldg(p.post_rstd + t) : 1.0f;
+      rp_next[q] = n + q < mine && has_pw ? __ldg(p.post_rstd + t) : 1.0f;
     }
   };
   norms(0);
@@ -422,8 +434,8 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
       const int c = (k * (int)blockDim.x + tid) * 8;
 #pragma unroll
       for (int q = 0; q < kR; ++q) d[q][k] = all8(0.0f);
-      if (c < H && p.dh) {
-        const F8 w = p.w ? w_of.get(c) : all8(1.0f);
+      if ((kKnown || c < H) && has_dh) {
+        const F8 w = has_w ? w_of.get(c) : all8(1.0f);
 #pragma unroll
         for (int q = 0; q < kR; ++q) {
           if (!on[q]) continue;
@@ -442,8 +454,8 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
       const int c = (k * (int)blockDim.x + tid) * 8;
-      if (c < H) {
-        const F8 w = p.pw ? pw_of.get(c) : all8(1.0f);
+      if (kKnown || c < H) {
+        const F8 w = has_pw ? pw_of.get(c) : all8(1.0f);
         F8 g = all8(1.0f);
 #pragma unroll
         for (int q = 0; q < kR; ++q) {
@@ -451,27 +463,27 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
           F8& e = d[q][k];
           // dx; e is not scaled by 1 / rms yet
           e = fma8(load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[0]) + c), both(-rs[q] * m1[q]), e);
-          e = p.ds ? fma8(e, both(rs[q]), load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[2]) + c)) : e * both(rs[q]);
-          if (p.dr) store8<R>(static_cast<rword*>(p.dr) + t[q] * H + c, e * both(p.a));
+          e = has_ds ? fma8(e, both(rs[q]), load8<R>(reinterpret_cast<const rword*>(st[q] + p.in_at[2]) + c)) : e * both(rs[q]);
+          if (kKnown || p.dr) store8<R>(static_cast<rword*>(p.dr) + t[q] * H + c, e * both(p.a));
           F8 v = all8(0.0f);                             // y_hat, or y
-          if (p.in_at[3] != ~0u) {
+          if (has_y) {
             y_raw[q][k] = raw8<T>(reinterpret_cast<const word*>(st[q] + p.in_at[3]) + c);
             v = f8<T>(y_raw[q][k]);
-            if (p.pw) v = v * both(rp[q]);
+            if (has_pw) v = v * both(rp[q]);
           }
           e = e * both(p.b);
-          if (p.gate) {
+          if (has_gate) {
             if (q == 0 || own_gate || many_gates) {
               const word* from = reinterpret_cast<const word*>(own_gate ? st[q] + p.in_at[4] : ring + p.g_at);
               if (many_gates) from = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t[q] / (uint32_t)p.gate_rows) * p.gate_ld;
               g = load8<T>(from + c);
             }
             const F8 u = v * w;
-            if (p.dg) store8<T>(static_cast<word*>(p.dg) + t[q] * H + c, e * u);
-            else if (p.part_g) acc_g[k] = fma8(e, u, acc_g[k]);
+            if (!kKnown && p.dg) store8<T>(static_cast<word*>(p.dg) + t[q] * H + c, e * u);
+            else if (kKnown || p.part_g) acc_g[k] = fma8(e, u, acc_g[k]);
             e = e * g;
           }
-          if (p.pw) {
+          if (has_pw) {
             acc_pw[k] = fma8(e, v, acc_pw[k]);
             e = e * w;
             dot8(e, v, sum[q]);
@@ -488,14 +500,14 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
       if (tid == 0 && n + q + p.stages < mine) fetch(n + q + p.stages, s);
       if (++s == p.stages) { s = 0; phase ^= 1; }
     }
-    if (p.dy) {
+    if (kKnown || p.dy) {
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         const int c = (k * (int)blockDim.x + tid) * 8;
 #pragma unroll
         for (int q = 0; q < kR; ++q) {
-          if (c >= H || !on[q]) continue;
-          if (p.pw) d[q][k] = fma8(f8<T>(y_raw[q][k]), both(-rp[q] * m2[q]), d[q][k]) * both(rp[q]);
+          if ((!kKnown && c >= H) || !on[q]) continue;
+          if (has_pw) d[q][k] = fma8(f8<T>(y_raw[q][k]), both(-rp[q] * m2[q]), d[q][k]) * both(rp[q]);
           store8<T>(static_cast<word*>(p.dy) + t[q] * H + c, d[q][k]);
         }
       }
@@ -505,7 +517,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   for (int k = 0; k < kV; ++k) {
     const int c = (k * (int)blockDim.x + tid) * 8;
     const int64_t at = (int64_t)blockIdx.x * H + c;
-    if (c < H) {
+    if (kKnown || c < H) {
       if (p.part_w) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_w) + at, acc_w[k]);
       if (p.part_pw) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_pw) + at, acc_pw[k]);
       if (p.part_g) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + at, acc_g[k]);
@@ -771,15 +783,37 @@ int with_width(const Width& w, Go go) {
   return go(integral_constant<int, 2>(), integral_constant<int, 1024>());
 }
 
-template <typename K, typename... Args>
-int launch_ring(K kernel, int blocks, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
-  if (smem > 40 * 1024) GB_CUDA_OK(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMax));
-  GB_CUDA_OK(gb_launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), smem, stream, args...));
+// The kernel's shared memory is asked for once a device (half a microsecond a call).
+template <auto kKernel>
+int launch_ring(int blocks, int threads, size_t smem, cudaStream_t stream, const NormParams& p) {
+  static std::atomic<uint64_t> asked{0};
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  GB_REQUIRE(dev >= 0 && dev < 64, "device %d out of range", dev);
+  if (!(asked.load(std::memory_order_acquire) >> dev & 1u)) {
+    GB_CUDA_OK(cudaFuncSetAttribute((const void*)kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMax));
+    asked.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  GB_CUDA_OK(gb_launch(kKernel, dim3((unsigned)blocks), dim3((unsigned)threads), smem, stream, p));
   return GB_OK;
 }
 
-// Whether the weights have the rows' type.
-bool own_type(const gb_residual_norm_args* a) { return (!a->w || a->w_dtype == a->dtype) && (!a->pw || a->pw_dtype == a->dtype); }
+Form form_of(const gb_residual_norm_args* a, const Width& w) {
+  if (a->H != (int64_t)w.v * w.threads * 8 || !a->w || a->w_dtype != a->dtype || (a->pw && a->pw_dtype != a->dtype) || a->weight_offset != 0.0f) return kAny;
+  if (!a->gate) return a->pw ? kPost : kPre;
+  return a->pw && a->gate_rows == a->T ? kPostGate : kAny;
+}
+// go(form) for one that is known at compile time.
+template <typename Go>
+int with_form(Form f, Go go) {
+  using std::integral_constant;
+  switch (f) {
+    case kPostGate: return go(integral_constant<Form, kPostGate>());
+    case kPost: return go(integral_constant<Form, kPost>());
+    case kPre: return go(integral_constant<Form, kPre>());
+    default: return go(integral_constant<Form, kAny>());
+  }
+}
 
 template <bool kFp8>
 int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
@@ -796,7 +830,7 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
   const bool vec = width.v > 0 && a->H % 8 == 0 && whole(a->y, a->y_ld, size) && whole(a->r, a->r_ld, rsize) && whole(a->gate, a->gate_ld, size) &&
                    whole(a->w, 0, 1) && whole(a->pw, 0, 1) && whole(p.h, 0, 1) && whole(p.s, 0, 1) && whole(p.q, 0, 1) &&
                    p.stage_bytes + fixed <= (uint32_t)kRingMax - 1024;
-  const bool raw = own_type(a);
+  const Form form = form_of(a, width);
   return with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
@@ -812,8 +846,9 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
       NormParams q = p;
       behind_ring(q, (size_t)p.stages * p.stage_bytes);
       const size_t smem = (size_t)p.stages * p.stage_bytes + fixed;
-      if (raw) return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, true>, (int)blocks, width.threads, smem, stream, q);
-      return launch_ring(norm_rows_kernel<T, R, kV, kMost, kFp8, false>, (int)blocks, width.threads, smem, stream, q);
+      return with_form(form, [&](auto f) -> int {
+        return launch_ring<norm_rows_kernel<T, R, kV, kMost, kFp8, decltype(f)::value>>((int)blocks, width.threads, smem, stream, q);
+      });
     });
   });
 }
@@ -943,7 +978,9 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   p.per_gate = plan.shares.per_gate;
   const bool sums = p.part_w || p.part_pw || p.part_g;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool raw = own_type(a);
+  // all gradients there and asked for
+  const bool all = g->d_h && g->d_stream && g->d_y && g->d_r && g->d_w && (!a->pw || g->d_pw) && (!a->gate || g->d_gate);
+  const Form form = all ? form_of(a, plan.width) : kAny;
   const int rc2 = with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
@@ -963,8 +1000,9 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
     const auto go = [&](auto v, auto r_, auto most) -> int {
       constexpr int kV = decltype(v)::value, kR = decltype(r_)::value, kMost = decltype(most)::value;
       const size_t smem = (size_t)p.stages * p.stage_bytes + plan.fixed;
-      if (raw) return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, true>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
-      return launch_ring(norm_rows_grad_kernel<T, R, kV, kR, kMost, false>, (int)plan.shares.blocks, plan.width.threads, smem, st, p);
+      return with_form(form, [&](auto f) -> int {
+        return launch_ring<norm_rows_grad_kernel<T, R, kV, kR, kMost, decltype(f)::value>>((int)plan.shares.blocks, plan.width.threads, smem, st, p);
+      });
     };
     using std::integral_constant;
     const integral_constant<int, 1> one;

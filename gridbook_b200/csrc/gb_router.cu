@@ -30,9 +30,26 @@ GB_DEVINL float warp_sum(float v) {
   return v;
 }
 GB_DEVINL float warp_max(float v) {                        // a NaN wins
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(kAll));
+  return r;
+}
+// Two sums at once: after the first exchange the lower half warp adds up the one and the upper half the other.
+GB_DEVINL void warp_sums(float& a, float& b) {
+  const bool up = threadIdx.x & 16;
+  float v = (up ? b : a) + __shfl_xor_sync(kAll, up ? a : b, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kAll, v, o));
-  return v;
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  a = __shfl_sync(kAll, v, 0);
+  b = __shfl_sync(kAll, v, 16);
+}
+// e^(v - top) from v and -top log2 e: one rounding of the exponent, two units of the function.  (expf's ten instructions for each expert
+// were half of the loss's.)
+constexpr float kLog2e = 1.4426950408889634f;
+GB_DEVINL float exp_from(float v, float minus_top2) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(v, kLog2e, minus_top2)));
+  return r;
 }
 
 // Whole numbers in the order of the logits, zeros alike; 0: no expert or one at -inf, NaN on top.
@@ -67,14 +84,37 @@ struct Row {
       for (int j = 0; j < kV; ++j) v[i + j] = e < E ? to_f32<T>(w[j]) : otherwise;
     }
   }
+  // The same in two steps: on their way, and as fp32.
+  struct Raw { alignas(16) word w[kPer]; };
+  static GB_DEVINL Raw fetch(const word* row, int E, int lane) {
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < kPer; i += kV) {
+      const int e = expert(i, lane);
+      if (e >= E) continue;
+      if constexpr (kV == 1) r.w[i] = row[e];
+      else if constexpr (kV * sizeof(word) == 16) *reinterpret_cast<uint4*>(r.w + i) = __ldg(reinterpret_cast<const uint4*>(row + e));
+      else *reinterpret_cast<uint2*>(r.w + i) = __ldg(reinterpret_cast<const uint2*>(row + e));
+    }
+    return r;
+  }
+  static GB_DEVINL void unpack(const Raw& r, int E, int lane, float (&v)[kPer], float otherwise) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = expert(i, lane) < E ? to_f32<T>(r.w[i]) : otherwise;
+  }
   static GB_DEVINL void store(word* row, int E, int lane, const float (&v)[kPer]) {
 #pragma unroll
     for (int i = 0; i < kPer; i += kV) {
       const int e = expert(i, lane);
       if (e >= E) continue;
       alignas(16) word w[kV];
+      if constexpr (kV > 1 && std::is_same_v<T, Bf16>) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) w[j] = from_f32<T>(v[i + j]);
+        for (int j = 0; j < kV; j += 2) *reinterpret_cast<uint32_t*>(w + j) = gb_pack_bf16x2(v[i + j], v[i + j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kV; ++j) w[j] = from_f32<T>(v[i + j]);
+      }
       if constexpr (kV == 1) row[e] = w[0];
       else if constexpr (kV * sizeof(word) == 16) *reinterpret_cast<uint4*>(row + e) = *reinterpret_cast<uint4*>(w);
       else *reinterpret_cast<uint2*>(row + e) = *reinterpret_cast<uint2*>(w);
@@ -263,24 +303,47 @@ balance_kernel(const __grid_constant__ BalanceParams p) {
   int n = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.0f;
-  for (int64_t t = (int64_t)blockIdx.x * kGroups + group; t < p.T; t += (int64_t)p.blocks * kGroups) {
-    if (p.mask && !p.mask[t]) continue;
+  // the next token's logits and ids are on their way while this one's are looked at
+  const int64_t step = (int64_t)p.blocks * kGroups;
+  const auto row = [&](int64_t t) { return static_cast<const typename T::word*>(p.logits) + t * p.ld; };
+  const auto live = [&](int64_t t) { return t < p.T && (!p.mask || p.mask[t]); };
+  const auto id_of = [&](int64_t t, int j) -> int64_t {
+    return p.id_bytes == 8 ? static_cast<const int64_t*>(p.ids)[t * p.topk + j] : static_cast<const int32_t*>(p.ids)[t * p.topk + j];
+  };
+  int64_t t = (int64_t)blockIdx.x * kGroups + group;
+  bool on = live(t);
+  typename R::Raw next = {};
+  int64_t next_id = -1;
+  if (on) {
+    next = R::fetch(row(t), p.E, lane);
+    if (lane < p.topk) next_id = id_of(t, lane);
+  }
+  for (; t < p.T; t += step) {
     float v[kPer], top = -inf, total = 0.0f;
-    R::load(static_cast<const typename T::word*>(p.logits) + t * p.ld, p.E, lane, v, -inf);
+    const bool counts = on;
+    const int64_t id = next_id;
+    R::unpack(next, p.E, lane, v, -inf);
+    on = live(t + step);
+    if (on) {
+      next = R::fetch(row(t + step), p.E, lane);
+      if (lane < p.topk) next_id = id_of(t + step, lane);
+    }
+    if (!counts) continue;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) top = max_nan(top, v[i]);
     top = over_token<kGroup, true>(top, s_red);
     if (top == -inf) continue;                             // nothing to choose from
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { v[i] = expf(v[i] - top); total += v[i]; }
+    for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], -top * kLog2e); total += v[i]; }
     total = over_token<kGroup, false>(total, s_red);
     const float r = 1.0f / total, z = top + logf(total);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[i], r, acc[i]);
     z2 = fmaf(z, z, z2);
     ++n;
-    for (int j = lane; j < p.topk; j += kGroup) {
-      const int64_t e = p.id_bytes == 8 ? static_cast<const int64_t*>(p.ids)[t * p.topk + j] : static_cast<const int32_t*>(p.ids)[t * p.topk + j];
+    if (lane < p.topk && (uint64_t)id < (uint64_t)p.E) atomicAdd(&s_counts[id], 1);
+    for (int j = lane + kGroup; j < p.topk; j += kGroup) {
+      const int64_t e = id_of(t, j);
       if ((uint64_t)e < (uint64_t)p.E) atomicAdd(&s_counts[e], 1);
     }
   }
@@ -368,50 +431,62 @@ balance_join_kernel(const __grid_constant__ BalanceParams p) {
   }
 }
 
+// A group of threads takes one token behind the other, the next one's logits on their way; the experts' shares stay in its registers.
 template <typename T, int kPer, bool kVec, int kGroup>
-__global__ void __launch_bounds__((kGroup > 32 ? kGroup : 256))
+__global__ void __launch_bounds__(256)
 balance_grad_kernel(const __grid_constant__ BalanceParams p) {
-  constexpr int kThreads = kGroup > 32 ? kGroup : 256, kGroups = kThreads / kGroup;
+  constexpr int kGroups = 256 / kGroup;
   __shared__ float s_red[32];
   gb_pdl_launch_dependents();
   gb_pdl_wait();
   using R = Row<T, kPer, kVec, kGroup>;
   using word = typename T::word;
   const int group = threadIdx.x / kGroup, lane = threadIdx.x % kGroup;
-  const int64_t t = (int64_t)blockIdx.x * kGroups + group;
-  if (t >= p.T) return;
   const float inf = __int_as_float(0x7F800000);
-  float v[kPer], top = -inf, total = 0.0f;
-  const bool live = !p.mask || p.mask[t];
-  if (live) R::load(static_cast<const word*>(p.logits) + t * p.ld, p.E, lane, v, -inf);
-  else {
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  const auto live = [&](int64_t t) { return t < p.T && (!p.mask || p.mask[t]); };
+  const auto row = [&](int64_t t) { return static_cast<const word*>(p.logits) + t * p.ld; };
+  int64_t t = (int64_t)blockIdx.x * kGroups + group;
+  bool on = live(t);
+  typename R::Raw next = {};
+  if (on) next = R::fetch(row(t), p.E, lane);
+  float f[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = -inf;
+  for (int i = 0; i < kPer; ++i) {
+    const int e = R::expert(i, lane);
+    f[i] = e < p.E ? __ldg(p.stats + e) : 0.0f;
   }
+  const float scale = *p.d_loss / fmaxf(__ldg(p.stats + p.E), 1.0f), b = p.coef * (float)p.E;
+  for (; t < p.T; t += step) {
+    float v[kPer], top = -inf, total = 0.0f, dot = 0.0f;
+    const bool counts = on;
+    R::unpack(next, p.E, lane, v, -inf);
+    on = live(t + step);
+    if (on) next = R::fetch(row(t + step), p.E, lane);
+    if (counts) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) top = max_nan(top, v[i]);
-  top = over_token<kGroup, true>(top, s_red);
-  if (top == -inf) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = 0.0f;
-  } else {
-    float f[kPer], dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = R::expert(i, lane);
-      f[i] = e < p.E ? __ldg(p.stats + e) : 0.0f;
+      for (int i = 0; i < kPer; ++i) top = max_nan(top, v[i]);
+      top = over_token<kGroup, true>(top, s_red);
     }
+    if (top == -inf) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { v[i] = expf(v[i] - top); total += v[i]; dot = fmaf(v[i], f[i], dot); }
-    total = over_token<kGroup, false>(total, s_red);
-    dot = over_token<kGroup, false>(dot, s_red);
-    const float r = 1.0f / total, z = top + logf(total);
-    const float a = *p.d_loss / __ldg(p.stats + p.E) * r, b = p.coef * (float)p.E;
-    dot *= r;
+      for (int i = 0; i < kPer; ++i) v[i] = 0.0f;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = a * v[i] * fmaf(b, f[i] - dot, 2.0f * p.z_coef * z);
+      for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], -top * kLog2e); total += v[i]; dot = fmaf(v[i], f[i], dot); }
+      if constexpr (kGroup == 32) {
+        warp_sums(total, dot);
+      } else {
+        total = over_token<kGroup, false>(total, s_red);
+        dot = over_token<kGroup, false>(dot, s_red);
+      }
+      const float r = 1.0f / total, z = top + logf(total), a = scale * r;
+      dot *= r;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = a * v[i] * fmaf(b, f[i] - dot, 2.0f * p.z_coef * z);
+    }
+    R::store(static_cast<word*>(p.d_logits) + t * p.E, p.E, lane, v);
   }
-  R::store(static_cast<word*>(p.d_logits) + t * p.E, p.E, lane, v);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -557,9 +632,10 @@ int gb_moe_balance_grad(const void* logits, int dtype, int64_t ld, const uint8_t
   p.mask = mask; p.stats = const_cast<float*>(stats);
   p.coef = coef; p.z_coef = z_coef; p.d_loss = d_loss; p.d_logits = d_logits;
   return dispatch<256>(dtype, E, logits, ld, d_logits, E, [&](auto t, auto per, auto vec, auto group) -> int {
-    constexpr int kGroup = decltype(group)::value, kThreads = kGroup > 32 ? kGroup : 256, kGroups = kThreads / kGroup;
-    GB_CUDA_OK(gb_launch(balance_grad_kernel<decltype(t), decltype(per)::value, decltype(vec)::value, kGroup>, dim3((unsigned)((T + kGroups - 1) / kGroups)),
-                         dim3(kThreads), 0, (cudaStream_t)stream, p));
+    constexpr int kGroup = decltype(group)::value, kGroups = 256 / kGroup;
+    const int64_t blocks = (T + kGroups - 1) / kGroups, most = (int64_t)gb_sm_count() * 6;       // about what runs at once
+    GB_CUDA_OK(gb_launch(balance_grad_kernel<decltype(t), decltype(per)::value, decltype(vec)::value, kGroup>, dim3((unsigned)(blocks < most ? blocks : most)),
+                         dim3(256), 0, (cudaStream_t)stream, p));
     return GB_OK;
   });
 }

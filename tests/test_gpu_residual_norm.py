@@ -102,7 +102,7 @@ def summed(pair, T):
 def test_values_and_gradients(dev, dtype, stream, T, H):
     from gridbook_b200 import kernels
     g = _gen(dev, T * 7 + H)
-    for gate, post, offset in (("channel", True, 0.0), ("none", False, 0.0), ("full", True, 1.0), ("channel", False, 0.0), ("none", True, 1.0), ("full", False, 0.0)):
+    for gate, post, offset in (("channel", True, 0.0), ("none", False, 0.0), ("full", True, 1.0), ("channel", False, 0.0), ("none", True, 1.0), ("full", False, 0.0), ("none", True, 0.0)):
         y, r, w, pw, gt = _inputs(T, H, dtype, stream, gate, post, g, dev)
         leaves = {k: v.clone().requires_grad_() for k, v in dict(y=y, r=r, w=w, pw=pw, g=gt).items() if v is not None}
         h, s = kernels.residual_norm(leaves["y"], leaves["r"], leaves["w"], post_weight=leaves.get("pw"), gate=leaves.get("g"), residual_scale=A, branch_scale=BR,
