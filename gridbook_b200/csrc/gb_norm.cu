@@ -17,6 +17,7 @@
 // adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value.
 #include "gb_blocks.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace {
@@ -49,7 +50,8 @@ struct NormParams {
   int64_t dh_ld, ds_ld;
   void *dy, *dr, *dg;                                    // dg: where every row has a gate of its own
   float *part_w, *part_pw, *part_g;                      // [blocks][H]
-  int per_gate;                                          // blocks that work on the rows of one gate row
+  int per_gate;                                          // blocks that work on the rows of one gate row; 0: no sums for a gate
+  int gates;                                             // gate rows where there are more than blocks: a block takes every gridDim-th; else 0
   float* means;                                          // [T], value by value: mean(dh (o + w) x_hat)
 };
 
@@ -351,17 +353,22 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   }
   __syncthreads();
   gb_pdl_wait();
-  // the block's share of the rows, of all or of those of a gate row: first + begin, + step, ..
+  // the block's share of the rows, of all or of those of a gate row: first + begin, + step, ..; or all of those of some gate rows
   const int rows = p.per_gate == 0 ? (int)p.T : (int)p.gate_rows, first = p.per_gate == 0 ? 0 : (int)blockIdx.x / p.per_gate * rows;
   const int begin = p.per_gate == 0 ? (int)blockIdx.x : (int)blockIdx.x % p.per_gate, step = p.per_gate == 0 ? (int)gridDim.x : p.per_gate;
-  const int mine = (rows - begin + step - 1) / step;
+  const bool some_gates = kForm == kAny && p.gates != 0;
+  const int mine = some_gates ? (p.gates - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * rows : (rows - begin + step - 1) / step;
+  const auto row_at = [&](int n) -> int64_t {            // the n-th row of the share
+    if (some_gates) return (int64_t)((int)blockIdx.x + n / rows * (int)gridDim.x) * rows + n % rows;
+    return first + begin + (int64_t)n * step;
+  };
   const uint32_t y_bytes = (uint32_t)(H * (int)sizeof(word)), r_bytes = (uint32_t)(H * (int)sizeof(rword));
   constexpr bool kKnown = kForm != kAny;
   const bool has_w = kKnown || p.w, has_pw = kKnown ? kForm != kPre : p.pw != nullptr, has_gate = kKnown ? kForm == kPostGate : p.gate != nullptr;
   const bool has_y = kKnown ? kForm != kPre : p.in_at[3] != ~0u, has_dh = kKnown || p.dh, has_ds = kKnown || p.ds;
   const bool own_gate = !kKnown && p.in_at[4] != ~0u;    // every row has a gate of its own
-  auto fetch = [&](int n, int s) {                       // the n-th row of the share
-    const int64_t t = first + begin + (int64_t)n * step;
+  auto fetch = [&](int n, int s) {
+    const int64_t t = row_at(n);
     uint8_t* st = ring + (size_t)s * p.stage_bytes;
     gb_mbar_expect_tx(&full[s], p.stage_bytes);
     gb_bulk_g2s(st + p.in_at[0], static_cast<const rword*>(p.s) + t * H, r_bytes, &full[s]);
@@ -403,7 +410,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
   const auto norms = [&](int n) {
 #pragma unroll
     for (int q = 0; q < kR; ++q) {
-      const int64_t t = first + begin + (int64_t)(n + q) * step;
+      const int64_t t = row_at(n + q);
       rs_next[q] = n + q < mine ? __ldg(p.rstd + t) : 0.0f;
       rp_next[q] = n + q < mine && has_pw ? __ldg(p.post_rstd + t) : 1.0f;
     }
@@ -420,7 +427,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
       const int sq = s + q < p.stages ? s + q : s + q - p.stages;
       st[q] = ring + (size_t)sq * p.stage_bytes;
       on[q] = n + q < mine;
-      t[q] = first + begin + (int64_t)(n + q) * step;
+      t[q] = row_at(n + q);
       rs[q] = rs_next[q];
       rp[q] = rp_next[q];
       if (on[q]) wheel.wait(n + q, sq, phase ^ (s + q < p.stages ? 0u : 1u), p.status, 92);
@@ -512,6 +519,14 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
         }
       }
     }
+    if (some_gates && p.part_g && (n + kR) % rows == 0) {  // the last row of a gate row's (two rows at a time: they are even in number)
+#pragma unroll
+      for (int k = 0; k < kV; ++k) {
+        const int c = (k * (int)blockDim.x + tid) * 8;
+        if (c < H) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + t[kR - 1] / rows * H + c, acc_g[k]);
+        acc_g[k] = all8(0.0f);
+      }
+    }
   }
 #pragma unroll
   for (int k = 0; k < kV; ++k) {
@@ -520,7 +535,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     if (kKnown || c < H) {
       if (p.part_w) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_w) + at, acc_w[k]);
       if (p.part_pw) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_pw) + at, acc_pw[k]);
-      if (p.part_g) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + at, acc_g[k]);
+      if (p.part_g && !some_gates) store8<Fp32>(reinterpret_cast<uint32_t*>(p.part_g) + at, acc_g[k]);
     }
   }
   if (gave_up != 0x7FFFFFFF) __nanosleep(1000000);
@@ -635,23 +650,26 @@ norm_any_columns_kernel(const __grid_constant__ NormParams p, int64_t column_blo
   const int64_t share = blockIdx.x / column_blocks, c = (blockIdx.x - share * column_blocks) * kAnyThreads + threadIdx.x;
   if (c >= p.H) return;
   const int64_t shares = gridDim.x / column_blocks;
-  const int64_t rows = p.per_gate == 0 ? p.T : p.gate_rows, first = p.per_gate == 0 ? 0 : share / p.per_gate * p.gate_rows;
+  const int64_t rows = p.per_gate == 0 ? p.T : p.gate_rows;
   const int64_t begin = p.per_gate == 0 ? share : share % p.per_gate, step = p.per_gate == 0 ? shares : p.per_gate;
-  float w = 0.0f, pw = 0.0f, g = 0.0f;
-  for (int64_t n = begin; n < rows; n += step) {
-    const Values<T, R> v{p, first + n};
-    const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
-    w = fmaf(v.dh(c), v.x_hat(c, rs), w);
-    if (p.part_pw || p.part_g) {
-      const float dx = v.dx(c, rs, p.means[v.t]), y_hat = v.y(c) * rp;
-      pw = fmaf(p.b * v.gate(c) * dx, y_hat, pw);
-      g = fmaf(p.b * dx, y_hat * v.pw(c), g);
+  float w = 0.0f, pw = 0.0f;
+  for (int64_t gate = p.per_gate == 0 ? 0 : share / p.per_gate; gate < (p.gates != 0 ? p.gates : share + 1); gate += shares) {
+    float g = 0.0f;
+    for (int64_t n = begin; n < rows; n += step) {
+      const Values<T, R> v{p, gate * rows + n};
+      const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
+      w = fmaf(v.dh(c), v.x_hat(c, rs), w);
+      if (p.part_pw || p.part_g) {
+        const float dx = v.dx(c, rs, p.means[v.t]), y_hat = v.y(c) * rp;
+        pw = fmaf(p.b * v.gate(c) * dx, y_hat, pw);
+        g = fmaf(p.b * dx, y_hat * v.pw(c), g);
+      }
     }
+    if (p.part_g) p.part_g[(p.gates != 0 ? gate : share) * p.H + c] = g;
   }
   const int64_t at = share * p.H + c;
   if (p.part_w) p.part_w[at] = w;
   if (p.part_pw) p.part_pw[at] = pw;
-  if (p.part_g) p.part_g[at] = g;
 }
 
 // The shares' sums: a block adds up 32 columns of one result, warp w every 32nd share.
@@ -659,7 +677,7 @@ struct JoinParams {
   const float* part[3];       // w, pw, gate: shares of H sums each
   void* out[3];
   int type[3];
-  int64_t H, shares, gates;   // shares in all, gate rows
+  int64_t H, shares, gate_shares;   // shares in all, of a gate row
   int64_t column_blocks;
 };
 constexpr int kJoinThreads = 1024;
@@ -677,7 +695,7 @@ norm_join_kernel(const __grid_constant__ JoinParams p) {
       if (gate == 0) { which = k; break; }
       --gate;
     }
-  const int64_t n = which == 2 ? p.shares / p.gates : p.shares;
+  const int64_t n = which == 2 ? p.gate_shares : p.shares;
   const float* from = p.part[which] + (which == 2 ? gate * n * p.H : 0);
   float sum = 0.0f;
   if (col < p.H)
@@ -854,12 +872,15 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
 }
 
 // How the rows are shared out for the backward pass: `blocks` shares, `per_gate` of them for the rows of a gate row (0: no sums of its gate).
+// Gate rows that are more than the target are dealt out to that many blocks, one whole: sums of the weights' gradients are kept for a
+// block, not for a gate row.
 struct Shares { int64_t blocks; int per_gate; int64_t gates; };
 Shares shares_of(const gb_residual_norm_args* a, bool gate_sums, int64_t target) {
   if (!gate_sums) return {a->T < target ? a->T : target, 0, 1};
   const int64_t gates = a->T / a->gate_rows;
+  if (gates > target) return {target, 1, gates};
   int64_t per = target / gates;
-  per = per < 1 ? 1 : per > a->gate_rows ? a->gate_rows : per;
+  per = per > a->gate_rows ? a->gate_rows : per;
   return {gates * per, (int)per, gates};
 }
 
@@ -892,7 +913,9 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
     r.at[3] = place(need_y, size);
     r.at[4] = place(r.gate_rows, size);
     r.stage_bytes = at;
-    r.fixed = place_weights(a, a->gate && !r.gate_rows && (r.gate_sums || a->gate_rows == a->T), &r.weight_at[0], &r.weight_at[1], &r.weight_at[2]);
+    // a gate row of the block's own; there are more than one for a block only where they are more than its SM takes blocks
+    const bool one_gate = a->gate && !r.gate_rows && (a->gate_rows == a->T || (r.gate_sums && a->T / a->gate_rows <= gb_sm_count()));
+    r.fixed = place_weights(a, one_gate, &r.weight_at[0], &r.weight_at[1], &r.weight_at[2]);
     r.vec = at + r.fixed <= (uint32_t)kRingMax - 1024 && whole(a->y, a->y_ld, size) && whole(a->gate, a->gate_ld, size) && whole(a->w, 0, 1) && whole(a->pw, 0, 1) &&
             whole(g->stream, 0, 1) && whole(g->d_h, g->d_h_ld, size) && whole(g->d_stream, g->d_stream_ld, rsize) && whole(g->d_y, 0, 1) &&
             whole(g->d_r, 0, 1) && whole(g->d_gate, 0, 1);
@@ -904,7 +927,7 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
   const int64_t sums = up(r.shares.blocks * a->H * 4);
   r.pw_at = g->d_w ? sums : 0;
   r.g_at = r.pw_at + (g->d_pw ? sums : 0);
-  r.means_at = r.g_at + (r.gate_sums ? sums : 0);
+  r.means_at = r.g_at + (r.gate_sums ? up(std::max(r.shares.blocks, r.shares.gates) * a->H * 4) : 0);
   r.bytes = r.means_at + (r.vec ? 0 : up(a->T * 4));
   return r;
 }
@@ -921,7 +944,7 @@ int launch_join(JoinParams j, int64_t jobs, cudaStream_t stream) {
 int gb_join_columns(const float* part, int64_t shares, int64_t columns, void* out, int dtype, cudaStream_t stream) {
   JoinParams j = {};
   j.part[0] = part; j.out[0] = out; j.type[0] = dtype;
-  j.H = columns; j.shares = shares; j.gates = 1;
+  j.H = columns; j.shares = shares; j.gate_shares = shares;
   return launch_join(j, 1, stream);
 }
 
@@ -957,7 +980,7 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   if (rc != GB_OK) return rc;
   GB_REQUIRE(g != nullptr, "null arguments");
   if (a->T == 0) return GB_OK;
-  GB_REQUIRE(g->stream && g->rstd && (!a->pw || (g->post_rstd && a->y)) && (!a->gate || a->y), "null pointer argument");
+  GB_REQUIRE(g->stream && g->rstd && (!a->pw || (g->post_rstd && a->y)) && (!g->d_gate || a->y), "null pointer argument");
   GB_REQUIRE((!g->d_h || g->d_h_ld >= a->H) && (!g->d_stream || g->d_stream_ld >= a->H), "rows that do not overlap expected");
   GB_REQUIRE((!g->d_w || a->w) && (!g->d_pw || a->pw) && (!g->d_gate || a->gate), "a gradient of what there is not");
   if (gb_sm_count() <= 0) return gb_fail(GB_ECUDA, "no usable CUDA device: %s", gb_last_error());
@@ -976,11 +999,12 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   p.part_g = plan.gate_sums ? reinterpret_cast<float*>(ws + plan.g_at) : nullptr;
   p.means = plan.vec ? nullptr : reinterpret_cast<float*>(ws + plan.means_at);
   p.per_gate = plan.shares.per_gate;
+  p.gates = plan.shares.gates > plan.shares.blocks ? (int)plan.shares.gates : 0;
   const bool sums = p.part_w || p.part_pw || p.part_g;
   const cudaStream_t st = (cudaStream_t)stream;
   // all gradients there and asked for
   const bool all = g->d_h && g->d_stream && g->d_y && g->d_r && g->d_w && (!a->pw || g->d_pw) && (!a->gate || g->d_gate);
-  const Form form = all ? form_of(a, plan.width) : kAny;
+  const Form form = all && !p.gates ? form_of(a, plan.width) : kAny;
   const int rc2 = with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
@@ -1009,7 +1033,7 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
     const integral_constant<int, 2> two;
     if (plan.width.v == 2) return go(two, one, integral_constant<int, 1024>());
     if (plan.width.most == 1024) return go(one, one, integral_constant<int, 1024>());
-    const bool pairs = p.stages >= 4;                    // two rows at hand, two on their way
+    const bool pairs = p.stages >= 4 && !(p.gates && a->gate_rows % 2);   // two rows at hand, two on their way, both of one gate row
     if (plan.width.most == 640) return pairs ? go(one, two, integral_constant<int, 640>()) : go(one, one, integral_constant<int, 640>());
     return pairs ? go(one, two, integral_constant<int, 256>()) : go(one, one, integral_constant<int, 256>());
   });
@@ -1018,8 +1042,8 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   j.part[0] = p.part_w; j.part[1] = p.part_pw; j.part[2] = p.part_g;
   j.out[0] = g->d_w; j.out[1] = g->d_pw; j.out[2] = g->d_gate;
   j.type[0] = a->w_dtype; j.type[1] = a->pw_dtype; j.type[2] = a->dtype;
-  j.H = a->H; j.shares = plan.shares.blocks; j.gates = plan.shares.gates;
-  return launch_join(j, (p.part_w ? 1 : 0) + (p.part_pw ? 1 : 0) + (p.part_g ? j.gates : 0), st);
+  j.H = a->H; j.shares = plan.shares.blocks; j.gate_shares = plan.shares.per_gate;
+  return launch_join(j, (p.part_w ? 1 : 0) + (p.part_pw ? 1 : 0) + (p.part_g ? plan.shares.gates : 0), st);
 }
 
 }  // extern "C"

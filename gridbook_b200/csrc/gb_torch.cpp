@@ -1313,21 +1313,25 @@ int64_t rows_of_gate(const at::Tensor& gate, const at::Tensor& y) {
 struct NormCall {
   gb_residual_norm_args a{};
   at::Tensor y, r, gate, w, pw;
-  NormCall(const at::Tensor& y_, const at::Tensor& r_, const at::Tensor& w_, const at::Tensor& pw_, const at::Tensor& gate_, double rs, double bs, double eps,
-           double offset) {
-    need_cuda(y_);
-    a.dtype = dtype_code(y_.scalar_type(), "residual_norm");
-    same_device(y_, {&r_});
-    GB_NEED(r_.sizes() == y_.sizes(), "residual_norm: rows and residual of one shape expected");
-    GB_NEED(r_.scalar_type() == y_.scalar_type() || r_.scalar_type() == at::kFloat, "residual_norm: the residual has the rows' type or float32");
+  // y_ undefined: its values are not read (the backward pass without a norm behind the block), its type is `type`
+  NormCall(const at::Tensor& y_, at::ScalarType type, const at::Tensor& r_, const at::Tensor& w_, const at::Tensor& pw_, const at::Tensor& gate_, double rs, double bs,
+           double eps, double offset) {
+    if (y_.defined()) need_cuda(y_);
+    same_device(r_, {});
+    a.dtype = dtype_code(type, "residual_norm");
+    if (y_.defined()) {
+      same_device(y_, {&r_});
+      GB_NEED(r_.sizes() == y_.sizes(), "residual_norm: rows and residual of one shape expected");
+    }
+    GB_NEED(r_.scalar_type() == type || r_.scalar_type() == at::kFloat, "residual_norm: the residual has the rows' type or float32");
     a.stream_dtype = dtype_code(r_.scalar_type(), "residual_norm");
-    GB_NEED(y_.dim() >= 1 && y_.size(-1) >= 1, "rows of at least one value expected");
-    a.H = y_.size(-1);
-    a.T = y_.numel() / a.H;
+    GB_NEED(r_.dim() >= 1 && r_.size(-1) >= 1, "rows of at least one value expected");
+    a.H = r_.size(-1);
+    a.T = r_.numel() / a.H;
     GB_NEED(a.T < (1ll << 31) && a.H < (1ll << 31), "residual_norm: too many rows or channels");
     const auto weight = [&](const at::Tensor& t, at::Tensor& to, const void*& p, int32_t& code, const char* name) {
       if (!t.defined()) return;
-      same_device(y_, {&t});
+      same_device(r_, {&t});
       GB_NEED(t.dim() == 1 && t.size(0) == a.H, std::string(name) + ": one value for each of " + std::to_string(a.H) + " channels expected");
       code = dtype_code(t.scalar_type(), name);
       to = t.contiguous();
@@ -1337,9 +1341,9 @@ struct NormCall {
     weight(pw_, pw, a.pw, a.pw_dtype, "post_weight");
     a.gate_rows = 1;
     if (gate_.defined()) {
-      same_device(y_, {&gate_});
-      GB_NEED(gate_.scalar_type() == y_.scalar_type(), "gate: the rows' type expected");
-      const int64_t rows = rows_of_gate(gate_, y_);
+      same_device(r_, {&gate_});
+      GB_NEED(gate_.scalar_type() == type, "gate: the rows' type expected");
+      const int64_t rows = rows_of_gate(gate_, r_);
       if (a.T > 0) {
         const RowsOf g(gate_);
         gate = g.t;
@@ -1350,10 +1354,16 @@ struct NormCall {
     }
     a.y_ld = a.r_ld = a.H;
     if (a.T > 0) {
-      const RowsOf yr(y_), rr(r_);
-      y = yr.t; r = rr.t;
-      a.y_ld = yr.ld; a.r_ld = rr.ld;
-      a.y = y.data_ptr(); a.r = r.data_ptr();
+      if (y_.defined()) {
+        const RowsOf yr(y_);
+        y = yr.t;
+        a.y_ld = yr.ld;
+        a.y = y.data_ptr();
+      }
+      const RowsOf rr(r_);
+      r = rr.t;
+      a.r_ld = rr.ld;
+      a.r = r.data_ptr();
     }
     a.residual_scale = (float)rs; a.branch_scale = (float)bs; a.eps = (float)eps; a.weight_offset = (float)offset;
   }
@@ -1362,9 +1372,9 @@ struct NormCall {
 struct NormBackward : torch::autograd::Node {
   SavedVariable y, w, pw, gate, stream, rstd, post_rstd;
   double rs, bs, eps, offset;
-  at::ScalarType stream_type;
+  at::ScalarType type;
   NormBackward(const at::Tensor& y_, const at::Tensor& w_, const at::Tensor& pw_, const at::Tensor& gate_, double rs_, double bs_, double eps_, double offset_)
-      : y(y_, false), w(w_, false), pw(pw_, false), gate(gate_, false), rs(rs_), bs(bs_), eps(eps_), offset(offset_) {}
+      : y(pw_.defined() || (gate_.defined() && gate_.requires_grad()) ? y_ : at::Tensor(), false), w(w_, false), pw(pw_, false), gate(gate_, false), rs(rs_), bs(bs_), eps(eps_), offset(offset_), type(y_.scalar_type()) {}
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     for (SavedVariable* v : {&y, &w, &pw, &gate, &stream, &rstd, &post_rstd}) v->reset_data();
@@ -1374,17 +1384,17 @@ struct NormBackward : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(5);
     if (!grads[0].defined() && !grads[1].defined()) return out;
-    const at::Tensor rows = y.unpack(), weight = w.unpack(), post = pw.unpack(), gates = gate.unpack(), s = stream.unpack();
-    const c10::cuda::CUDAGuard guard(rows.device());
-    const NormCall c(rows, s, weight, post, gates, rs, bs, eps, offset);      // the stream lies in the residual's place: its type alone counts
-    const auto like = [&](int i, const at::Tensor& t) {
-      if (t.defined() && task_should_compute_output(i)) out[i] = c.a.T > 0 ? fresh(t.sizes(), t.scalar_type(), t) : at::zeros(t.sizes(), t.options());
+    const at::Tensor s = stream.unpack(), rows = y.unpack(), weight = w.unpack(), post = pw.unpack(), gates = gate.unpack();
+    const c10::cuda::CUDAGuard guard(s.device());
+    const NormCall c(rows, type, s, weight, post, gates, rs, bs, eps, offset);      // the stream lies in the residual's place: its type alone counts
+    const auto like = [&](int i, const at::Tensor& t, at::ScalarType of) {
+      if (t.defined() && task_should_compute_output(i)) out[i] = c.a.T > 0 ? fresh(t.sizes(), of, t) : at::zeros(t.sizes(), t.options().dtype(of));
     };
-    like(0, rows);
-    like(1, s);
-    like(2, weight);
-    like(3, post);
-    like(4, gates);
+    like(0, s, type);
+    like(1, s, s.scalar_type());
+    if (weight.defined()) like(2, weight, weight.scalar_type());
+    if (post.defined()) like(3, post, post.scalar_type());
+    if (gates.defined()) like(4, gates, type);
     if (c.a.T == 0) return out;
     gb_residual_norm_grads g{};
     at::Tensor dh, ds;
@@ -1398,7 +1408,7 @@ struct NormBackward : torch::autograd::Node {
     g.d_y = ptr(0); g.d_r = ptr(1); g.d_w = ptr(2); g.d_pw = ptr(3); g.d_gate = ptr(4);
     Arena a;
     const int ws = a.add(L.gb_residual_norm_grad_workspace_bytes(&c.a, &g));
-    a.alloc(rows);
+    a.alloc(s);
     check(L.gb_residual_norm_grad(&c.a, &g, a.ptr(ws), a.total, current_stream()));
     return out;
   }
@@ -1416,7 +1426,7 @@ Two residual_norm(const at::Tensor& y, const at::Tensor& r, const Opt& weight, c
     const at::AutoDispatchBelowADInplaceOrView below;
     need_cuda(y);
     const c10::cuda::CUDAGuard guard(y.device());
-    const NormCall c(y, r, w, pw, g, rs, bs, eps, offset);
+    const NormCall c(y, y.scalar_type(), r, w, pw, g, rs, bs, eps, offset);
     h = fresh(y.sizes(), y.scalar_type(), y);
     stream = fresh(y.sizes(), r.scalar_type(), y);
     if (node) {
@@ -1443,7 +1453,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm_fp8(const at::Tenso
   no_tangents({&y, &r, &w, &pw, &g}, kNorms);
   need_cuda(y);
   const c10::cuda::CUDAGuard guard(y.device());
-  const NormCall c(y, r, w, pw, g, rs, bs, eps, offset);
+  const NormCall c(y, y.scalar_type(), r, w, pw, g, rs, bs, eps, offset);
   at::Tensor q = fresh(y.sizes(), at::kFloat8_e4m3fn, y), scale = fresh(with_last(y, blocks(c.a.H)), at::kFloat, y), stream = fresh(y.sizes(), r.scalar_type(), y);
   check(L.gb_residual_norm_fp8(&c.a, rule, q.data_ptr(), scale.data_ptr<float>(), stream.data_ptr(), current_stream()));
   return {q, scale, stream};

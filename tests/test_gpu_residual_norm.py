@@ -130,7 +130,7 @@ def test_gates_for_groups_of_rows(dev, H):
     from gridbook_b200 import kernels
     g = _gen(dev, H)
     for lead, shape in (((4, 33), (4, 1, H)), ((4, 33), (1, 1, H)), ((4, 33), (4, 33, H)), ((2, 3, 5), (2, 1, 1, H)), ((2, 3, 5), (2, 3, 1, H)), ((1, 7), (7, H)),
-                        ((300, 3), (300, 1, H)), ((6, 1), (6, 1, H)), ((5, 200), (H,))):
+                        ((300, 3), (300, 1, H)), ((2000, 2), (2000, 1, H)), ((1500, 3), (1500, 1, H)), ((6, 1), (6, 1, H)), ((5, 200), (H,))):
         T = torch.Size(lead).numel()
         y, r, w, pw, _ = _inputs(T, H, BF, F32, "none", True, g, dev)
         gt = torch.randn(*shape, generator=g, device=dev).to(BF)
@@ -170,6 +170,12 @@ def test_what_is_not_asked_for(dev):
                 ref = grads(s.detach(), y, w, pw, gt, dh if use_h else zero, ds if use_s else zero)
                 for n, t in zip([n for n in names if n in need], got):
                     near(t, *(summed(ref[n], T) if n in ("w", "pw", "g") else ref[n]), f"{need} {n}")
+        plain = y.clone().requires_grad_()                                   # without a norm behind the block its rows are not read again
+        h, s = kernels.residual_norm(plain, r, w, eps=EPS)
+        with torch.no_grad():
+            plain.zero_()
+        dy, = torch.autograd.grad([h, s], [plain], [dh, ds])
+        near(dy, *grads(s.detach(), y, w, None, None, dh, ds, scales=(1.0, 1.0))["y"], "y, not kept")
         h, s = kernels.residual_norm(y, r, eps=EPS)                          # neither weights nor scales nor a gate
         want = y.double() + r.double()
         near(s, want, 4 * U * (y.double().abs() + r.double().abs()), "stream")
