@@ -184,7 +184,7 @@ GB_DEVINL void store8(typename T::word* p, const F8& f) { store8<T>(p, rounded<T
 // columns were a third of the instructions: 8192 x 5120 bf16 forward 66 us, backward 116.)
 enum Form { kAny = 0, kPostGate = 1, kPost = 2, kPre = 3 };          // both norms with a gate that rows share, without a gate; the second norm alone
 
-// Weights of eight columns in shared memory, o + w; kRaw: of the rows' own type, o zero.
+// Weights of eight columns in shared memory (of the longest rows, which fill it, where they lie), o + w; kRaw: of the rows' own type, o zero.
 template <typename T, bool kRaw>
 struct Weights {
   const uint8_t* p;
@@ -202,9 +202,9 @@ struct Weights {
 // The weights' way there, by one thread; they are waited for like a row.
 GB_DEVINL void fetch_weights(const NormParams& p, uint8_t* smem, const void* gate, uint32_t gate_bytes, uint64_t* bar) {
   const auto bytes = [&](int type) { return (uint32_t)(p.H * (type == GB_DTYPE_FP32 ? 4 : 2)); };
-  gb_mbar_expect_tx(bar, (p.w ? bytes(p.w_type) : 0u) + (p.pw ? bytes(p.pw_type) : 0u) + (p.g_at != ~0u ? gate_bytes : 0u));
-  if (p.w) gb_bulk_g2s(smem + p.w_at, p.w, bytes(p.w_type), bar);
-  if (p.pw) gb_bulk_g2s(smem + p.pw_at, p.pw, bytes(p.pw_type), bar);
+  gb_mbar_expect_tx(bar, (p.w_at != ~0u ? bytes(p.w_type) : 0u) + (p.pw_at != ~0u ? bytes(p.pw_type) : 0u) + (p.g_at != ~0u ? gate_bytes : 0u));
+  if (p.w_at != ~0u) gb_bulk_g2s(smem + p.w_at, p.w, bytes(p.w_type), bar);
+  if (p.pw_at != ~0u) gb_bulk_g2s(smem + p.pw_at, p.pw, bytes(p.pw_type), bar);
   if (p.g_at != ~0u) gb_bulk_g2s(smem + p.g_at, gate, gate_bytes, bar);
 }
 template <typename R>
@@ -259,8 +259,10 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     for (int s = 1; s < p.stages; ++s)
       if ((int64_t)blockIdx.x + (int64_t)s * step < T_) fetch((int64_t)blockIdx.x + (int64_t)s * step, s);
   }
-  const bool one_gate = kKnown ? has_gate : p.g_at != ~0u;                   // the same for all rows
-  const Weights<T, kKnown> w{ring + p.w_at, p.w_type, p.offset}, pw{ring + p.pw_at, p.pw_type, p.offset};
+  constexpr bool kLong = kThreads == 1024;
+  const bool one_gate = kKnown ? has_gate : p.gate && (kLong ? p.gate_rows == p.T : p.g_at != ~0u);   // the same for all rows
+  const Weights<T, kKnown> w{kLong ? static_cast<const uint8_t*>(p.w) : ring + p.w_at, p.w_type, p.offset},
+      pw{kLong ? static_cast<const uint8_t*>(p.pw) : ring + p.pw_at, p.pw_type, p.offset};
   const Ring wheel{full, &gave_up};
   int turn = 0, i = 0, s = 0;
   uint32_t phase = 0;
@@ -284,7 +286,7 @@ norm_rows_kernel(const __grid_constant__ NormParams p) {
     if (i == 0) wheel.wait(0, kMostStages, 0, p.status, 91);
     const word* gate_row = nullptr;
     if (own_gate) gate_row = reinterpret_cast<const word*>(st + p.in_at[2]);
-    else if (one_gate) gate_row = reinterpret_cast<const word*>(ring + p.g_at);
+    else if (one_gate) gate_row = kLong ? static_cast<const word*>(p.gate) : reinterpret_cast<const word*>(ring + p.g_at);
     else if (has_gate) gate_row = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld;
     rword* out = static_cast<rword*>(p.s) + t * H;
     const uint64_t scale_r = both(p.a), scale_u = both(p.b * rp);
@@ -383,8 +385,11 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
     for (int s = 1; s < p.stages; ++s)
       if (s < mine) fetch(s, s);
   }
-  const Weights<T, kKnown> w_of{ring + p.w_at, p.w_type, p.offset}, pw_of{ring + p.pw_at, p.pw_type, p.offset};
-  const bool many_gates = !kKnown && p.gate && !own_gate && p.g_at == ~0u;      // a gate without a gradient
+  constexpr bool kLong = kV == 2;
+  const Weights<T, kKnown> w_of{kLong ? static_cast<const uint8_t*>(p.w) : ring + p.w_at, p.w_type, p.offset},
+      pw_of{kLong ? static_cast<const uint8_t*>(p.pw) : ring + p.pw_at, p.pw_type, p.offset};
+  const word* gate_own = static_cast<const word*>(p.gate) + (p.per_gate != 0 ? (int64_t)(first / rows) * p.gate_ld : 0);
+  const bool many_gates = !kKnown && p.gate && !own_gate && (kLong ? p.gates != 0 || (p.per_gate == 0 && p.gate_rows != p.T) : p.g_at == ~0u);   // not one for the block
   const Ring wheel{full, &gave_up};
   wheel.wait(0, kMostStages, 0, p.status, 92);
   F8 acc_w[kV], acc_pw[kV], acc_g[kV];
@@ -481,7 +486,7 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
           e = e * both(p.b);
           if (has_gate) {
             if (q == 0 || own_gate || many_gates) {
-              const word* from = reinterpret_cast<const word*>(own_gate ? st[q] + p.in_at[4] : ring + p.g_at);
+              const word* from = reinterpret_cast<const word*>(own_gate ? st[q] + p.in_at[4] : kLong ? reinterpret_cast<const uint8_t*>(gate_own) : ring + p.g_at);
               if (many_gates) from = static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t[q] / (uint32_t)p.gate_rows) * p.gate_ld;
               g = load8<T>(from + c);
             }
@@ -544,47 +549,71 @@ norm_rows_grad_kernel(const __grid_constant__ NormParams p) {
 // ------------------------------------------------------------------------------------------------ value by value
 constexpr int kAnyThreads = 256;
 
+// A row's inputs.  They are read by __ldg, so that several of a thread's columns are on their way past what it stores.
 template <typename T, typename R>
 struct Values {
+  using word = typename T::word;
+  using rword = typename R::word;
   const NormParams& p;
   int64_t t;
-  GB_DEVINL float y(int64_t c) const { return to_f32<T>(static_cast<const typename T::word*>(p.y)[t * p.y_ld + c]); }
-  GB_DEVINL float gate(int64_t c) const {
-    return p.gate ? to_f32<T>(static_cast<const typename T::word*>(p.gate)[t / p.gate_rows * p.gate_ld + c]) : 1.0f;
+  const word *y_row, *gate_row, *dh_row;
+  const rword *r_row, *ds_row, *s_row;
+  GB_DEVINL Values(const NormParams& params, int64_t row) : p(params), t(row) {
+    y_row = static_cast<const word*>(p.y) + t * p.y_ld;
+    gate_row = p.gate ? static_cast<const word*>(p.gate) + (int64_t)((uint32_t)t / (uint32_t)p.gate_rows) * p.gate_ld : nullptr;
+    dh_row = p.dh ? static_cast<const word*>(p.dh) + t * p.dh_ld : nullptr;
+    r_row = static_cast<const rword*>(p.r) + t * p.r_ld;
+    ds_row = p.ds ? static_cast<const rword*>(p.ds) + t * p.ds_ld : nullptr;
+    s_row = static_cast<const rword*>(p.s) + t * p.H;
   }
-  GB_DEVINL float w(int64_t c) const { return p.w ? value_of(p.w, p.w_type, c) + p.offset : 1.0f; }
-  GB_DEVINL float pw(int64_t c) const { return p.pw ? value_of(p.pw, p.pw_type, c) + p.offset : 1.0f; }
-  GB_DEVINL float x(int64_t c, float rp) const {
-    const float u = p.pw ? y(c) * (rp * pw(c)) : y(c);
-    return fmaf(p.b, u * gate(c), p.a * to_f32<R>(static_cast<const typename R::word*>(p.r)[t * p.r_ld + c]));
+  GB_DEVINL float y(int c) const { return to_f32<T>(__ldg(y_row + c)); }
+  GB_DEVINL float gate(int c) const { return gate_row ? to_f32<T>(__ldg(gate_row + c)) : 1.0f; }
+  GB_DEVINL float w(int c) const { return p.w ? value_of(p.w, p.w_type, c) + p.offset : 1.0f; }
+  GB_DEVINL float pw(int c) const { return p.pw ? value_of(p.pw, p.pw_type, c) + p.offset : 1.0f; }
+  GB_DEVINL float x_of(int c, float y, float rp) const {
+    const float u = p.pw ? y * (rp * pw(c)) : y;
+    return fmaf(p.b, u * gate(c), p.a * to_f32<R>(__ldg(r_row + c)));
   }
   // backward: p.s holds the stream
-  GB_DEVINL float x_hat(int64_t c, float rs) const { return to_f32<R>(static_cast<const typename R::word*>(p.s)[t * p.H + c]) * rs; }
-  GB_DEVINL float dh(int64_t c) const { return p.dh ? to_f32<T>(static_cast<const typename T::word*>(p.dh)[t * p.dh_ld + c]) : 0.0f; }
-  GB_DEVINL float dx(int64_t c, float rs, float m1) const {
+  GB_DEVINL float x_hat(int c, float rs) const { return to_f32<R>(__ldg(s_row + c)) * rs; }
+  GB_DEVINL float dh(int c) const { return dh_row ? to_f32<T>(__ldg(dh_row + c)) : 0.0f; }
+  GB_DEVINL float ds(int c) const { return to_f32<R>(__ldg(ds_row + c)); }
+  GB_DEVINL float dx(int c, float rs, float m1) const {
     const float d = rs * fmaf(-x_hat(c, rs), m1, dh(c) * w(c));
-    return p.ds ? d + to_f32<R>(static_cast<const typename R::word*>(p.ds)[t * p.ds_ld + c]) : d;
+    return p.ds ? d + ds(c) : d;
   }
 };
 
-template <typename T, typename R, bool kFp8>
+// kCached: the row fits shared memory in fp32, where a thread keeps its columns from pass to pass; else every pass reads them again.
+template <typename T, typename R, bool kFp8, bool kCached>
 __global__ void __launch_bounds__(kAnyThreads)
 norm_any_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ float row_s[];
   __shared__ float red[2][32];
   gb_pdl_launch_dependents();
   gb_pdl_wait();
   int turn = 0;
   const Values<T, R> v{p, (int64_t)blockIdx.x};
+  const int H = (int)p.H;
   float rp = 1.0f, sum = 0.0f;
   if (p.pw) {
-    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) sum = fmaf(v.y(c), v.y(c), sum);
+#pragma unroll 4
+    for (int c = threadIdx.x; c < H; c += kAnyThreads) {
+      const float y = v.y(c);
+      if (kCached) row_s[c] = y;
+      sum = fmaf(y, y, sum);
+    }
     rp = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
   }
   sum = 0.0f;
-  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
-    float x = v.x(c, rp);
-    static_cast<typename R::word*>(p.s)[v.t * p.H + c] = from_f32<R>(x);
-    if (!kFp8) x = as_stored<R>(x);
+  typename R::word* out = static_cast<typename R::word*>(p.s) + v.t * p.H;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < H; c += kAnyThreads) {
+    float x = v.x_of(c, kCached && p.pw ? row_s[c] : v.y(c), rp);
+    const typename R::word kept = from_f32<R>(x);
+    out[c] = kept;
+    if (!kFp8) x = to_f32<R>(kept);
+    if (kCached) row_s[c] = x;
     sum = fmaf(x, x, sum);
   }
   const float rs = rsqrtf(fmaf(block_sum(sum, red, turn), p.inv_h, p.eps));
@@ -592,26 +621,99 @@ norm_any_kernel(const __grid_constant__ NormParams p) {
     if (p.rstd) p.rstd[v.t] = rs;
     if (p.post_rstd) p.post_rstd[v.t] = rp;
   }
+  const auto again = [&](int c) {                        // (block_sum's barrier lies in front of it: other threads' columns too)
+    if (kCached) return row_s[c];
+    const float x = v.x_of(c, v.y(c), rp);
+    return kFp8 ? x : as_stored<R>(x);
+  };
   if constexpr (!kFp8) {
-    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads)
-      static_cast<typename T::word*>(p.h)[v.t * p.H + c] = from_f32<T>(as_stored<R>(v.x(c, rp)) * rs * v.w(c));
+    typename T::word* h = static_cast<typename T::word*>(p.h) + v.t * p.H;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < H; c += kAnyThreads) h[c] = from_f32<T>(again(c) * rs * v.w(c));
   } else {
-    const int64_t blocks = (p.H + kBlock - 1) / kBlock;
-    for (int64_t b0 = 0; b0 < blocks; b0 += kAnyThreads / 16) {
-      const int64_t b = b0 + threadIdx.x / 16, c = b * kBlock + (threadIdx.x & 15) * 8;
+    const int blocks = (H + kBlock - 1) / kBlock;
+    for (int b0 = 0; b0 < blocks; b0 += kAnyThreads / 16) {
+      const int b = b0 + threadIdx.x / 16, c = b * kBlock + (threadIdx.x & 15) * 8;
       float h[8], scale;
       uint32_t q[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = c + j < p.H ? v.x(c + j, rp) * rs * v.w(c + j) : 0.0f;
+      for (int j = 0; j < 8; ++j) h[j] = c + j < H ? again(c + j) * rs * v.w(c + j) : 0.0f;
       quantize_block<8, 16>(h, p.scale_rule, scale, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j < p.H) p.q[v.t * p.H + c + j] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
+        if (c + j < H) p.q[v.t * p.H + c + j] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
       if (b < blocks && (threadIdx.x & 15) == 0) p.scale[v.t * blocks + b] = scale;
     }
   }
 }
 
+// The backward pass with the row and the columns' sums in shared memory: a block walks its share of the rows, a thread has every
+// kAnyGradThreads-th column.
+constexpr int kAnyGradThreads = 512;
+
+template <typename T, typename R>
+__global__ void __launch_bounds__(kAnyGradThreads)
+norm_any_rows_grad_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ float row_s[];
+  __shared__ float red[2][32];
+  const int tid = threadIdx.x, H = (int)p.H;
+  float *d_s = row_s, *x_s = d_s + H, *w_s = x_s + H, *pw_s = w_s + H, *g_s = pw_s + H;   // dh (o + w), dx, du (o + pw) in turn; x_hat, then y_hat; sums
+  gb_pdl_launch_dependents();
+  for (int c = tid; c < H; c += kAnyGradThreads) w_s[c] = pw_s[c] = g_s[c] = 0.0f;
+  gb_pdl_wait();
+  int turn = 0;
+  const int rows = p.per_gate == 0 ? (int)p.T : (int)p.gate_rows, share = (int)blockIdx.x;
+  const int begin = p.per_gate == 0 ? share : share % p.per_gate, step = p.per_gate == 0 ? (int)gridDim.x : p.per_gate;
+  const int gates = p.gates != 0 ? p.gates : 1, first_gate = p.gates != 0 ? share : p.per_gate == 0 ? 0 : share / p.per_gate;
+  for (int i = p.gates != 0 ? share : 0; i < gates; i += (int)gridDim.x) {
+    const int gate = p.gates != 0 ? i : first_gate;
+    for (int n = begin; n < rows; n += step) {
+      const Values<T, R> v{p, (int64_t)gate * rows + n};
+      const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
+      float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll 4
+      for (int c = tid; c < H; c += kAnyGradThreads) {
+        const float xh = v.x_hat(c, rs), dh = v.dh(c), k = dh * v.w(c);
+        w_s[c] = fmaf(dh, xh, w_s[c]);
+        d_s[c] = k;
+        x_s[c] = xh;
+        m1 = fmaf(k, xh, m1);
+      }
+      m1 = block_sum(m1, red, turn) * p.inv_h;
+#pragma unroll 4
+      for (int c = tid; c < H; c += kAnyGradThreads) {
+        float dx = rs * fmaf(-x_s[c], m1, d_s[c]);
+        if (p.ds) dx += v.ds(c);
+        if (p.dr) static_cast<typename R::word*>(p.dr)[v.t * p.H + c] = from_f32<R>(p.a * dx);
+        const float u = p.pw || p.dg || p.part_g ? v.y(c) * rp : 0.0f, pw = v.pw(c), e = p.b * dx, du = e * v.gate(c);
+        if (p.dg) static_cast<typename T::word*>(p.dg)[v.t * p.H + c] = from_f32<T>(e * (u * pw));
+        g_s[c] = fmaf(e, u * pw, g_s[c]);
+        pw_s[c] = fmaf(du, u, pw_s[c]);
+        d_s[c] = du * pw;
+        x_s[c] = u;
+        m2 = fmaf(du * pw, u, m2);
+      }
+      m2 = block_sum(m2, red, turn) * p.inv_h;
+      if (p.dy)
+#pragma unroll 4
+        for (int c = tid; c < H; c += kAnyGradThreads)
+          static_cast<typename T::word*>(p.dy)[v.t * p.H + c] = from_f32<T>(p.pw ? rp * fmaf(-x_s[c], m2, d_s[c]) : d_s[c]);
+    }
+    if (p.gates != 0 && p.part_g)
+      for (int c = tid; c < H; c += kAnyGradThreads) {
+        p.part_g[(int64_t)gate * p.H + c] = g_s[c];
+        g_s[c] = 0.0f;
+      }
+  }
+  for (int c = tid; c < H; c += kAnyGradThreads) {
+    const int64_t at = (int64_t)share * p.H + c;
+    if (p.part_w) p.part_w[at] = w_s[c];
+    if (p.part_pw) p.part_pw[at] = pw_s[c];
+    if (p.part_g && p.gates == 0) p.part_g[at] = g_s[c];
+  }
+}
+
+// Rows that do not fit it.
 template <typename T, typename R>
 __global__ void __launch_bounds__(kAnyThreads)
 norm_any_grad_kernel(const __grid_constant__ NormParams p) {
@@ -623,10 +725,10 @@ norm_any_grad_kernel(const __grid_constant__ NormParams p) {
   const float rs = p.rstd[v.t], rp = p.pw ? p.post_rstd[v.t] : 1.0f;
   float m1 = 0.0f, m2 = 0.0f;
   if (p.dh)
-    for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) m1 = fmaf(v.dh(c) * v.w(c), v.x_hat(c, rs), m1);
+    for (int c = threadIdx.x; c < (int)p.H; c += kAnyThreads) m1 = fmaf(v.dh(c) * v.w(c), v.x_hat(c, rs), m1);
   m1 = block_sum(m1, red, turn) * p.inv_h;
   if (threadIdx.x == 0) p.means[v.t] = m1;
-  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
+  for (int c = threadIdx.x; c < (int)p.H; c += kAnyThreads) {
     const float dx = v.dx(c, rs, m1);
     if (p.dr) static_cast<typename R::word*>(p.dr)[v.t * p.H + c] = from_f32<R>(p.a * dx);
     if (p.dg) static_cast<typename T::word*>(p.dg)[v.t * p.H + c] = from_f32<T>(p.b * dx * (v.y(c) * (rp * v.pw(c))));
@@ -635,7 +737,7 @@ norm_any_grad_kernel(const __grid_constant__ NormParams p) {
   }
   if (!p.pw || !p.dy) return;
   m2 = block_sum(m2, red, turn) * p.inv_h;
-  for (int64_t c = threadIdx.x; c < p.H; c += kAnyThreads) {
+  for (int c = threadIdx.x; c < (int)p.H; c += kAnyThreads) {
     const float du = p.b * v.gate(c) * v.dx(c, rs, m1);
     static_cast<typename T::word*>(p.dy)[v.t * p.H + c] = from_f32<T>(rp * fmaf(-v.y(c) * rp, m2, du * v.pw(c)));
   }
@@ -771,15 +873,15 @@ Plan plan_of(int threads, int most_threads, int most_stages, uint32_t stage_byte
   return {per_sm, stages > most_stages ? most_stages : stages};
 }
 // Where the weights and a gate that a block's rows share lie behind the ring, from 0 on; their bytes.
-uint32_t place_weights(const gb_residual_norm_args* a, bool one_gate, uint32_t* w_at, uint32_t* pw_at, uint32_t* g_at) {
+uint32_t place_weights(const gb_residual_norm_args* a, bool in_shared, bool one_gate, uint32_t* w_at, uint32_t* pw_at, uint32_t* g_at) {
   uint32_t at = 0;
   const auto place = [&](bool there, int type, uint32_t* to) {
     *to = there ? at : ~0u;
     if (there) at += (uint32_t)(a->H * size_of(type));
   };
-  place(a->w != nullptr, a->w_dtype, w_at);
-  place(a->pw != nullptr, a->pw_dtype, pw_at);
-  place(one_gate, a->dtype, g_at);
+  place(in_shared && a->w != nullptr, a->w_dtype, w_at);
+  place(in_shared && a->pw != nullptr, a->pw_dtype, pw_at);
+  place(in_shared && one_gate, a->dtype, g_at);
   return at;
 }
 void behind_ring(NormParams& p, size_t ring) {
@@ -844,7 +946,7 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
   p.in_at[1] = (uint32_t)(a->H * size);
   if (full) p.in_at[2] = (uint32_t)(a->H * (size + rsize));
   p.stage_bytes = (uint32_t)(a->H * (size * (full ? 2 : 1) + rsize));
-  const uint32_t fixed = place_weights(a, a->gate && a->gate_rows == a->T && !full, &p.w_at, &p.pw_at, &p.g_at);
+  const uint32_t fixed = place_weights(a, width.most != 1024, a->gate && a->gate_rows == a->T && !full, &p.w_at, &p.pw_at, &p.g_at);
   const bool vec = width.v > 0 && a->H % 8 == 0 && whole(a->y, a->y_ld, size) && whole(a->r, a->r_ld, rsize) && whole(a->gate, a->gate_ld, size) &&
                    whole(a->w, 0, 1) && whole(a->pw, 0, 1) && whole(p.h, 0, 1) && whole(p.s, 0, 1) && whole(p.q, 0, 1) &&
                    p.stage_bytes + fixed <= (uint32_t)kRingMax - 1024;
@@ -853,8 +955,8 @@ int forward(const gb_residual_norm_args* a, NormParams p, cudaStream_t stream) {
     using T = decltype(t);
     using R = decltype(r);
     if (!vec) {
-      GB_CUDA_OK(gb_launch(norm_any_kernel<T, R, kFp8>, dim3((unsigned)a->T), dim3(kAnyThreads), 0, stream, p));
-      return GB_OK;
+      if (a->H * 4 <= kRingMax) return launch_ring<norm_any_kernel<T, R, kFp8, true>>((int)a->T, kAnyThreads, (size_t)a->H * 4, stream, p);
+      return launch_ring<norm_any_kernel<T, R, kFp8, false>>((int)a->T, kAnyThreads, 0, stream, p);
     }
     return with_width(width, [&](auto v, auto most) -> int {
       const Plan plan = plan_of(width.threads, 1024, 4, p.stage_bytes, fixed);
@@ -885,7 +987,7 @@ Shares shares_of(const gb_residual_norm_args* a, bool gate_sums, int64_t target)
 }
 
 struct GradPlan {
-  bool vec, gate_sums, gate_rows;
+  bool vec, cached, gate_sums, gate_rows;                // cached: value by value, a row and the columns' sums in shared memory
   Width width;
   Plan plan;
   Shares shares;
@@ -915,20 +1017,22 @@ GradPlan grad_plan(const gb_residual_norm_args* a, const gb_residual_norm_grads*
     r.stage_bytes = at;
     // a gate row of the block's own; there are more than one for a block only where they are more than its SM takes blocks
     const bool one_gate = a->gate && !r.gate_rows && (a->gate_rows == a->T || (r.gate_sums && a->T / a->gate_rows <= gb_sm_count()));
-    r.fixed = place_weights(a, one_gate, &r.weight_at[0], &r.weight_at[1], &r.weight_at[2]);
+    r.fixed = place_weights(a, r.width.v == 1, one_gate, &r.weight_at[0], &r.weight_at[1], &r.weight_at[2]);
     r.vec = at + r.fixed <= (uint32_t)kRingMax - 1024 && whole(a->y, a->y_ld, size) && whole(a->gate, a->gate_ld, size) && whole(a->w, 0, 1) && whole(a->pw, 0, 1) &&
             whole(g->stream, 0, 1) && whole(g->d_h, g->d_h_ld, size) && whole(g->d_stream, g->d_stream_ld, rsize) && whole(g->d_y, 0, 1) &&
             whole(g->d_r, 0, 1) && whole(g->d_gate, 0, 1);
   }
   if (r.vec) r.plan = plan_of(r.width.threads, r.width.most <= 256 ? 512 : 65536 / 96, kMostStages, r.stage_bytes, r.fixed);
   const int64_t sms = gb_sm_count();
-  r.shares = shares_of(a, r.gate_sums, r.vec ? sms * r.plan.per_sm : 64);
+  r.cached = !r.vec && a->H * 20 <= kRingMax;
+  const int64_t any_per_sm = r.cached ? std::max<int64_t>(1, std::min<int64_t>(4, kRingMax / (a->H * 20 + 1024))) : 1;
+  r.shares = shares_of(a, r.gate_sums, r.vec ? sms * r.plan.per_sm : r.cached ? sms * any_per_sm : 64);
   auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
   const int64_t sums = up(r.shares.blocks * a->H * 4);
   r.pw_at = g->d_w ? sums : 0;
   r.g_at = r.pw_at + (g->d_pw ? sums : 0);
   r.means_at = r.g_at + (r.gate_sums ? up(std::max(r.shares.blocks, r.shares.gates) * a->H * 4) : 0);
-  r.bytes = r.means_at + (r.vec ? 0 : up(a->T * 4));
+  r.bytes = r.means_at + (r.vec || r.cached ? 0 : up(a->T * 4));
   return r;
 }
 
@@ -997,7 +1101,7 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   p.part_w = g->d_w ? reinterpret_cast<float*>(ws + plan.w_at) : nullptr;
   p.part_pw = g->d_pw ? reinterpret_cast<float*>(ws + plan.pw_at) : nullptr;
   p.part_g = plan.gate_sums ? reinterpret_cast<float*>(ws + plan.g_at) : nullptr;
-  p.means = plan.vec ? nullptr : reinterpret_cast<float*>(ws + plan.means_at);
+  p.means = plan.vec || plan.cached ? nullptr : reinterpret_cast<float*>(ws + plan.means_at);
   p.per_gate = plan.shares.per_gate;
   p.gates = plan.shares.gates > plan.shares.blocks ? (int)plan.shares.gates : 0;
   const bool sums = p.part_w || p.part_pw || p.part_g;
@@ -1008,6 +1112,8 @@ int gb_residual_norm_grad(const gb_residual_norm_args* a, const gb_residual_norm
   const int rc2 = with_types(a->dtype, a->stream_dtype, [&](auto t, auto r) -> int {
     using T = decltype(t);
     using R = decltype(r);
+    if (!plan.vec && plan.cached)
+      return launch_ring<norm_any_rows_grad_kernel<T, R>>((int)plan.shares.blocks, kAnyGradThreads, (size_t)a->H * 20, st, p);
     if (!plan.vec) {
       GB_CUDA_OK(gb_launch(norm_any_grad_kernel<T, R>, dim3((unsigned)a->T), dim3(kAnyThreads), 0, st, p));
       if (!sums) return GB_OK;
