@@ -464,49 +464,83 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             v[i + 1] += to_f(b >> 16, p.fp16);
           }
         }
-        const auto send = [&](const CUtensorMap* map) {      // v as it is now
-          const uint32_t dst = out + (uint32_t)flip * kChunk;            // in turn: the chunk before last has left its buffer
-          flip ^= 1;
-          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          __syncwarp();
+        const auto put = [&](uint32_t dst) {                 // v as it is now; eight rows touch eight bank groups
 #pragma unroll
-          for (int q = 0; q < 4; ++q)                        // eight rows touch eight bank groups
+          for (int q = 0; q < 4; ++q)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                          ::"r"(dst + row_at + (((uint32_t)q ^ swz) * 16u)), "r"(pack2(v[8 * q], v[8 * q + 1], p.fp16)),
                            "r"(pack2(v[8 * q + 2], v[8 * q + 3], p.fp16)), "r"(pack2(v[8 * q + 4], v[8 * q + 5], p.fp16)),
                            "r"(pack2(v[8 * q + 6], v[8 * q + 7], p.fp16)) : "memory");
+        };
+        const auto send = [&](const CUtensorMap* map) {
+          const uint32_t dst = out + (uint32_t)flip * kChunk;            // in turn: the chunk before last has left its buffer
+          flip ^= 1;
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+          put(dst);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0 && row0 < p.M && col < p.N) tma_store_2d(map, col, row0, dst);   // what sticks out is not written
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         };
+        // Rows that TMA does not take go through the buffers too, a row at a time with the lanes along its columns: of 32 rows at once a
+        // store touches 32 sectors (4096 x 5001 x 2048 with residual 368 us).
+        const int inside = min(32, (int)min((int64_t)32, p.M - row0));
+        const bool column = col + lane < p.N;
+        const auto cell = [&](uint32_t dst, int r) { return dst + (uint32_t)r * 64u + ((((uint32_t)lane >> 3) ^ ((uint32_t)(r >> 1) & 3u)) * 16u) + ((uint32_t)lane & 7u) * 2u; };
+        const auto rows_out = [&](uint16_t* to) {
+          __syncwarp();
+          put(out);
+          __syncwarp();
+          uint16_t* at_row = to + (int64_t)row0 * p.N + col + lane;
+#pragma unroll 8
+          for (int r = 0; r < inside; ++r) {
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(cell(out, r)));
+            if (column) at_row[(int64_t)r * p.N] = w;
+          }
+        };
+        const auto residual_in = [&]() {
+          const uint16_t* from = p.r + (int64_t)row0 * p.r_ld + col + lane;
+          __syncwarp();
+#pragma unroll 8
+          for (int r = 0; r < inside; ++r) {
+            const uint16_t w = column ? __ldg(from + (int64_t)r * p.r_ld) : (uint16_t)0;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(cell(out + kChunk, r)), "h"(w) : "memory");
+          }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(rr[q].x), "=r"(rr[q].y), "=r"(rr[q].z), "=r"(rr[q].w) : "r"(out + kChunk + row_at + (((uint32_t)q ^ swz) * 16u)));
+        };
+        const auto add_residual = [&]() {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t w[4] = {rr[q].x, rr[q].y, rr[q].z, rr[q].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              v[8 * q + 2 * j] += to_f(w[j] & 0xFFFFu, p.fp16);
+              v[8 * q + 2 * j + 1] += to_f(w[j] >> 16, p.fp16);
+            }
+          }
+        };
         if (staged) {
           if (kZ) send(&map_z);
           activate(v, p.act);
           if (kRes) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t w[4] = {rr[q].x, rr[q].y, rr[q].z, rr[q].w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                v[8 * q + 2 * j] += to_f(w[j] & 0xFFFFu, p.fp16);
-                v[8 * q + 2 * j + 1] += to_f(w[j] >> 16, p.fp16);
-              }
-            }
+            add_residual();
             if (c + 1 < mine) fetch_residual(c + 1);
           }
           send(&map_d);
-        } else if (row < p.M) {
-          if (kZ) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (col + i < p.N) p.z[(int64_t)row * p.N + col + i] = pack1(v[i], p.fp16);
-          }
+        } else {
+          if (kZ) rows_out(p.z);
           activate(v, p.act);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (col + i < p.N)
-              p.d[(int64_t)row * p.N + col + i] = pack1(kRes ? v[i] + to_f(p.r[(int64_t)row * p.r_ld + col + i], p.fp16) : v[i], p.fp16);
+          if (kRes) {
+            residual_in();
+            add_residual();
+          }
+          rows_out(p.d);
         }
       }
     }
