@@ -7,11 +7,14 @@
 // pass the forward pass also stores z, rounded to the output's type: act' is taken at the rounded z, which adds half a step of it
 // times act'' to dz, less than dz's own rounding for the tensor cores does.
 //
-// Two kernels, as the other prefill GEMMs have them:
-//   linear_pair_kernel   256 x 256, 192 or 128 tiles on CTA pairs (cta_group::2), two accumulators, so that a tile's epilogue runs under
-//                        the next tile's MMAs.  The residual's tile comes by TMA into the buffers that the output leaves from, while
-//                        the MMAs run.
+// Three kernels, which of them by an estimate of their times (route_of):
+//   linear_pair_kernel   tiles of 256 rows x 128 to 256 columns on CTA pairs (cta_group::2), two accumulators, so that a tile's epilogue
+//                        runs under the next tile's MMAs; the residual comes through registers meanwhile.
 //   linear_rows_kernel   128 weight rows times up to 256 activation rows on one CTA, K sliced over a cluster: few rows, narrow layers.
+//   linear_few_kernel    one to four rows of small layers on the plain units.
+// Bound by the tensor cores at the clock that the power cap leaves where tiles fill the GPU (8192 x 34816 x 5120: 2.1 ms, 1.4 PFLOP/s, what a
+// plain library product sustains), by HBM at a few rows (16 x 34816 x 5120: 58 us, 92% of the copy rate), by launch, first fetches and the
+// last tile's epilogue in between.
 // The backward products read the same matrices where they lie, along their other axis: an operand whose rows run along the
 // contraction is the tensor core's MN-major form, tiles of 64 columns x 64 rows with the 128-byte swizzle, so that nothing
 // is transposed in memory.  dW's contraction runs over M: where its tiles are fewer than the pairs, M is split and the slices' fp32 sums
@@ -246,6 +249,10 @@ struct LinearParams {
   int* status;
   // few rows
   int rows_per_pass, box_rows, stages;
+  // one to four rows
+  const uint16_t *x, *w;
+  int64_t x_ld;
+  int K;
 };
 
 GB_DEVINL void tile_at(const LinearParams& p, int tile, int& mt, int& nt) {
@@ -734,6 +741,101 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols / 2) : "memory");
 }
 
+// ------------------------------------------------------------------------------------------------ one to four rows
+// A layer's weights are read once and multiplied on the plain fp32 units: a warp, or two to eight of them, takes a row of W, eight 16-byte
+// pieces a lane on their way at a time; the activations lie in shared memory in fp32.  It needs no clusters, tensor memory or barriers,
+// which are a third of a small layer's time in the few-rows kernel; that one is as fast or faster where a layer is larger, or has more
+// rows (its / this one's time, us, launches back to back, weights from HBM): one row of 128 x 2048 4.4 / 2.3, 128 x 7168 6.1 / 3.6, 2048 x 2048 6.0 / 4.0,
+// 4096 x 4096 9.3 / 9.9, 5120 x 17408 30.5 / 39; two rows of 1000 x 2048 5.5 / 3.9, 4096 x 4096 9.3 / 12.1; four of 256 x 2048 4.4 / 3.7.
+constexpr int kFewThreads = 256, kFewRows = 4, kFewSmem = 100 * 1024;
+constexpr int64_t kFewProducts = 1 << 22;                    // rows x weights up to which it is taken
+
+template <int kM>
+__global__ void __launch_bounds__(kFewThreads, 2)
+linear_few_kernel(const __grid_constant__ LinearParams p) {
+  extern __shared__ float4 x_s[];                            // [row][half of eight values][piece]
+  __shared__ float red[kFewThreads / 32][kM];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = p.K / 8, split = p.slices;
+  const int per_block = kFewThreads / 32 / split, mine = warp / split, part = warp - mine * split;
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  constexpr int kU = 8;
+  uint4 w[kU];
+  const auto fetch = [&](int n, int i0) {
+    const uint4* row = reinterpret_cast<const uint4*>(p.w + (int64_t)n * p.K);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = i0 + u * 32 * split;
+      w[u] = n < p.N && i < pieces ? __ldg(row + i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  int n0 = (int)blockIdx.x * per_block;
+  const int first = part * 32 + lane;
+  fetch(n0 + mine, first);
+  for (int i = threadIdx.x; i < kM * pieces; i += kFewThreads) {
+    const int m = i / pieces, at = i - m * pieces;
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.x_ld) + at);
+    x_s[(2 * m) * pieces + at] = make_float4(to_f(q.x & 0xFFFFu, p.fp16), to_f(q.x >> 16, p.fp16), to_f(q.y & 0xFFFFu, p.fp16), to_f(q.y >> 16, p.fp16));
+    x_s[(2 * m + 1) * pieces + at] = make_float4(to_f(q.z & 0xFFFFu, p.fp16), to_f(q.z >> 16, p.fp16), to_f(q.w & 0xFFFFu, p.fp16), to_f(q.w >> 16, p.fp16));
+  }
+  __syncthreads();
+  for (; n0 < p.N; n0 += (int)gridDim.x * per_block) {
+    const int n = n0 + mine;
+    float acc[kM][2];
+#pragma unroll
+    for (int m = 0; m < kM; ++m) acc[m][0] = acc[m][1] = 0.0f;
+    for (int i0 = first; i0 < pieces; i0 += kU * 32 * split) {
+      if (i0 != first) fetch(n, i0);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int i = i0 + u * 32 * split;
+        if (i >= pieces) break;
+        const float f[8] = {to_f(w[u].x & 0xFFFFu, p.fp16), to_f(w[u].x >> 16, p.fp16), to_f(w[u].y & 0xFFFFu, p.fp16), to_f(w[u].y >> 16, p.fp16),
+                            to_f(w[u].z & 0xFFFFu, p.fp16), to_f(w[u].z >> 16, p.fp16), to_f(w[u].w & 0xFFFFu, p.fp16), to_f(w[u].w >> 16, p.fp16)};
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+          const float4 a = x_s[(2 * m) * pieces + i], b = x_s[(2 * m + 1) * pieces + i];
+          acc[m][0] = fmaf(f[0], a.x, acc[m][0]); acc[m][1] = fmaf(f[1], a.y, acc[m][1]);
+          acc[m][0] = fmaf(f[2], a.z, acc[m][0]); acc[m][1] = fmaf(f[3], a.w, acc[m][1]);
+          acc[m][0] = fmaf(f[4], b.x, acc[m][0]); acc[m][1] = fmaf(f[5], b.y, acc[m][1]);
+          acc[m][0] = fmaf(f[6], b.z, acc[m][0]); acc[m][1] = fmaf(f[7], b.w, acc[m][1]);
+        }
+      }
+    }
+    fetch(n + (int)gridDim.x * per_block, first);            // the next row's, past the sums
+    float sum[kM];
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+      sum[m] = acc[m][0] + acc[m][1];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], o);
+    }
+    if (split > 1) {
+      __syncthreads();
+      if (lane == 0) {
+#pragma unroll
+        for (int m = 0; m < kM; ++m) red[warp][m] = sum[m];
+      }
+      __syncthreads();
+    }
+    float v[1] = {0.0f};
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+      if (lane == m) v[0] = sum[m];
+    if (part == 0 && lane < kM && n < p.N) {                 // lane m finishes row m
+      if (split > 1) {
+        v[0] = 0.0f;
+        for (int q = 0; q < split; ++q) v[0] += red[warp + q][lane];
+      }
+      const int64_t at = (int64_t)lane * p.N + n;
+      if (p.bias) v[0] += to_f(p.bias[n], p.fp16);
+      if (p.z) p.z[at] = pack1(v[0], p.fp16);
+      activate(v, p.act);
+      p.d[at] = pack1(p.r ? v[0] + to_f(p.r[(int64_t)lane * p.r_ld + n], p.fp16) : v[0], p.fp16);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ elementwise parts of the backward pass
 struct DzParams {
   const uint16_t *dy, *z;
@@ -868,6 +970,10 @@ int set_limits() {
   GB_PAIR(kWeightGrad, 192, kPlain);
   GB_PAIR(kWeightGrad, 128, kPlain);
 #undef GB_FORWARD
+  GB_ATTR(linear_few_kernel<1>, kFewSmem);
+  GB_ATTR(linear_few_kernel<2>, kFewSmem);
+  GB_ATTR(linear_few_kernel<3>, kFewSmem);
+  GB_ATTR(linear_few_kernel<4>, kFewSmem);
   GB_ATTR(linear_rows_kernel<false>, kRowsSmem);
   GB_ATTR(linear_rows_kernel<true>, kRowsSmem);
 #undef GB_PAIR
@@ -1025,6 +1131,27 @@ int run_rows(const Mats& m, LinearParams p, cudaStream_t stream) {   // a: activ
   return GB_OK;
 }
 
+// Warps a row of W: more than one where the rows are fewer than sixteen warps an SM and long enough.
+int run_few(const Mats& m, LinearParams p, cudaStream_t stream) {
+  p.x = static_cast<const uint16_t*>(m.a);
+  p.w = static_cast<const uint16_t*>(m.b);
+  p.x_ld = m.a_ld;
+  p.K = (int)m.K;
+  const int64_t sms = gb_sm_count();
+  p.slices = 1;
+  while (p.slices < 8 && p.N * p.slices < sms * 16 && m.K >= p.slices * 2 * 2048) p.slices *= 2;
+  const size_t smem = (size_t)p.M * (size_t)m.K * 4;
+  const int64_t blocks = ceil_div(p.N * p.slices, kFewThreads / 32), fit = std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)(220 * 1024 / (smem + 1024))));
+  const dim3 grid((unsigned)std::min(blocks, sms * fit));
+  switch (p.M) {
+    case 1: GB_CUDA_OK(gb_launch(linear_few_kernel<1>, grid, dim3(kFewThreads), smem, stream, p)); break;
+    case 2: GB_CUDA_OK(gb_launch(linear_few_kernel<2>, grid, dim3(kFewThreads), smem, stream, p)); break;
+    case 3: GB_CUDA_OK(gb_launch(linear_few_kernel<3>, grid, dim3(kFewThreads), smem, stream, p)); break;
+    default: GB_CUDA_OK(gb_launch(linear_few_kernel<4>, grid, dim3(kFewThreads), smem, stream, p)); break;
+  }
+  return GB_OK;
+}
+
 LinearParams params_of(int64_t M, int64_t N, int dtype, void* d) {
   LinearParams p = {};
   p.M = M; p.N = N;
@@ -1169,6 +1296,7 @@ int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, 
   if (r && (!aligned(r) || r_ld % 8 != 0)) p.tma = 0;
   const Mats m = {x, w, x_ld, K, K};
   const cudaStream_t st = (cudaStream_t)stream;
+  if (M <= kFewRows && M * N * K <= kFewProducts && M * K * 4 <= kFewSmem) return run_few(m, p, st);
   const int width = route_of(kWidths, M, N, K, pairs);
   if (width == 0) return run_rows<false>(m, p, st);
   if (z) return r ? run_forward<kBoth>(width, m, p, pairs, st) : run_forward<kKeepZ>(width, m, p, pairs, st);

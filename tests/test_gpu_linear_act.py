@@ -87,7 +87,7 @@ def check_grads(got, x, w, b, act, dy, name=""):
         check(got[1], dz.T @ xd, e.T @ xa + (M + 18) * ADD * (size.T @ xa), dtype, f"dw {name}")
 
 
-SHAPES = [(1, 256, 256), (1, 4096, 4096), (3, 1, 8), (7, 1000, 264), (16, 640, 1024), (130, 129, 72), (192, 512, 2048), (200, 1024, 256), (256, 8, 64), (257, 520, 520),
+SHAPES = [(1, 256, 256), (2, 300, 264), (4, 129, 1024), (1, 130, 8192), (1, 4096, 4096), (3, 1, 8), (7, 1000, 264), (16, 640, 1024), (130, 129, 72), (192, 512, 2048), (200, 1024, 256), (256, 8, 64), (257, 520, 520),
           (333, 1111, 1000), (700, 2304, 512), (1100, 1001, 136), (1500, 384, 64), (2100, 776, 200), (513, 16384, 128), (1024, 2048, 4096)]
 
 
