@@ -924,6 +924,92 @@ linear_dz_kernel(const __grid_constant__ DzParams p) {
   p.part[(int64_t)blockIdx.y * p.N + col] = sum;
 }
 
+// The relu's gradient has a step at zero, so that the sign of z there matters as its value elsewhere does not.  The tensor cores' sums
+// drop the bits behind the accumulator at every one of their K/16 steps and are off by about 5e-6 of a row's usual value at K = 7232, which turns
+// the sign of three values in 1.5 million: few, but each is a whole value of the gradient (2e-3 of an fp16 gradient's norm, ten times
+// its rounding).  So where z is kept for the backward pass, the values that such an error can carry across zero are summed up again in fp32
+// on the plain units, one in 15000 of them.  How large z is otherwise is read off its own row (a warp's 256 columns) and its own column
+// (the four rows), so that a row or a weight that is small as a whole counts as that; exact zeros stand.
+// Bound by the read of z.  No more than kMostAgain of 1024 values are summed up again, which bounds the time for values of any other spread.
+struct SignParams {
+  const uint16_t *x, *w, *bias;
+  uint16_t* z;
+  int64_t M, N, K, x_ld;
+  int fp16;
+  float reach;
+};
+constexpr int kMostAgain = 4;
+
+template <bool kVec>
+__global__ void __launch_bounds__(kDzThreads)
+linear_sign_kernel(const __grid_constant__ SignParams p) {
+  gb_pdl_launch_dependents();
+  gb_pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = (int64_t)blockIdx.x * kDzCols, c = c0 + lane * 8;
+  const int64_t step = (int64_t)gridDim.y * (kDzThreads / 32) * kDzRows;
+  for (int64_t m0 = ((int64_t)blockIdx.y * (kDzThreads / 32) + warp) * kDzRows; m0 < p.M; m0 += step) {
+    float a[kDzRows][8], row[kDzRows], col[8];
+#pragma unroll
+    for (int r = 0; r < kDzRows; ++r) {
+      const uint16_t* z = p.z + (m0 + r) * p.N + c;
+      uint32_t u[4] = {};
+      if (m0 + r < p.M) {
+        if (kVec) {
+          if (c < p.N) { const uint4 v = *reinterpret_cast<const uint4*>(z); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < p.N) u[i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
+        }
+      }
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[r][i] = fabsf(to_f(u[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16));
+        top = fmaxf(top, a[r][i]);
+      }
+      row[r] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    }
+    const bool whole = m0 + kDzRows <= p.M;                  // fewer rows say nothing of a column
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      col[i] = whole ? 0.0f : __int_as_float(0x7f800000);
+#pragma unroll
+      for (int r = 0; r < kDzRows; ++r) col[i] = fmaxf(col[i], a[r][i]);
+    }
+    uint32_t near = 0u;
+#pragma unroll
+    for (int r = 0; r < kDzRows; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (a[r][i] > 0.0f && a[r][i] < p.reach * fminf(row[r], col[i])) near |= 1u << (r * 8 + i);
+    for (int left = kMostAgain; left > 0; --left) {
+      const uint32_t who = __ballot_sync(0xffffffffu, near != 0u);
+      if (who == 0u) break;
+      const int src = __ffs(who) - 1, bit = __ffs(__shfl_sync(0xffffffffu, near, src)) - 1;
+      if (lane == src) near &= near - 1u;
+      const int64_t m = m0 + (bit >> 3), n = c0 + src * 8 + (bit & 7);
+      const uint4 *xs = reinterpret_cast<const uint4*>(p.x + m * p.x_ld), *ws = reinterpret_cast<const uint4*>(p.w + n * p.K);
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 4
+      for (int64_t k = lane; k < p.K / 8; k += 32) {
+        const uint4 f = __ldg(xs + k), g = __ldg(ws + k);
+        const uint32_t fs[4] = {f.x, f.y, f.z, f.w}, gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s0 = fmaf(to_f(fs[i] & 0xFFFFu, p.fp16), to_f(gs[i] & 0xFFFFu, p.fp16), s0);
+          s1 = fmaf(to_f(fs[i] >> 16, p.fp16), to_f(gs[i] >> 16, p.fp16), s1);
+        }
+      }
+      float s = s0 + s1;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) p.z[m * p.N + n] = pack1(p.bias ? s + to_f(p.bias[n], p.fp16) : s, p.fp16);
+    }
+  }
+}
+
 // The slices' sums, in their order, and the epilogue behind them; a thread has four neighbours of a row.
 __global__ void __launch_bounds__(256)
 linear_join_kernel(const __grid_constant__ LinearParams p) {
@@ -1272,6 +1358,22 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K, int act, bool rows_too, bool
   return g;
 }
 
+int run_signs(const Mats& m, const LinearParams& p, cudaStream_t st) {
+  SignParams s = {};
+  s.x = static_cast<const uint16_t*>(m.a);
+  s.w = static_cast<const uint16_t*>(m.b);
+  s.bias = p.bias;
+  s.z = p.z;
+  s.M = p.M; s.N = p.N; s.K = m.K; s.x_ld = m.a_ld;
+  s.fp16 = p.fp16;
+  s.reach = (float)ceil_div(m.K, 16) * 0x1p-24f;
+  const int64_t cols = ceil_div(p.N, kDzCols), rows = std::min<int64_t>(ceil_div(p.M, kDzThreads / 32 * kDzRows), std::max<int64_t>(1, (int64_t)gb_sm_count() * 16 / cols));
+  const dim3 grid((unsigned)cols, (unsigned)std::min<int64_t>(rows, 65535));
+  if (p.N % 8 == 0) GB_CUDA_OK(gb_launch(linear_sign_kernel<true>, grid, dim3(kDzThreads), 0, st, s));
+  else GB_CUDA_OK(gb_launch(linear_sign_kernel<false>, grid, dim3(kDzThreads), 0, st, s));
+  return GB_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1298,9 +1400,10 @@ int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, 
   const cudaStream_t st = (cudaStream_t)stream;
   if (M <= kFewRows && M * N * K <= kFewProducts && M * K * 4 <= kFewSmem) return run_few(m, p, st);
   const int width = route_of(kWidths, M, N, K, pairs);
-  if (width == 0) return run_rows<false>(m, p, st);
-  if (z) return r ? run_forward<kBoth>(width, m, p, pairs, st) : run_forward<kKeepZ>(width, m, p, pairs, st);
-  return r ? run_forward<kResidual>(width, m, p, pairs, st) : run_forward<kPlain>(width, m, p, pairs, st);
+  if (width == 0) rc = run_rows<false>(m, p, st);
+  else if (z) rc = r ? run_forward<kBoth>(width, m, p, pairs, st) : run_forward<kKeepZ>(width, m, p, pairs, st);
+  else rc = r ? run_forward<kResidual>(width, m, p, pairs, st) : run_forward<kPlain>(width, m, p, pairs, st);
+  return rc == GB_OK && z && act == GB_EPI_RELU ? run_signs(m, p, st) : rc;
 }
 
 int64_t gb_linear_act_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int rows, int weight, int bias, int dy_whole) {

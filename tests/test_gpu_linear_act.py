@@ -305,3 +305,30 @@ def test_past_two_to_the_31_values(dev):
     assert y.numel() > 2 ** 31
     check_forward(y[-40:], x[-40:], w, b, "relu", r[-40:])
     check_forward(y[:40], x[:40], w, b, "relu", r[:40])
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(256, 16384, 7232, HF), (256, 8200, 7232, BF), (251, 8195, 4096, HF), (40, 16384, 8192, BF)])
+def test_the_step_of_a_relu_falls_where_z_crosses_zero(dev, M, N, K, dtype):
+    """With ones as the gradient the bias' gradient counts a column's positive values, exactly up to 256 of them.  Values near zero are summed
+    up in fp32: some 2^-25 sqrt(K / 8) / sqrt(32) of z's spread off (K / 64 additions in each of two chains of a lane, whose sums are
+    sqrt(32) smaller; the sums over the lanes are less), so that less than one in ten million changes its sign; three of 4 million are allowed.  Sums
+    that drop bits at each step of the tensor cores turn a few in a million.  Some columns and rows are small as a whole, one column is
+    zero throughout."""
+    from gridbook_b200 import kernels
+    g = _gen(dev, 70 + K % 64 + M)
+    x, w, b, _ = _inputs(M, N, K, dtype, True, False, g, dev)
+    w[3::64] *= 2.0 ** -9
+    b[3::64] *= 2.0 ** -9
+    w[7], b[7] = 0.0, 0.0
+    x[5] *= 2.0 ** -6
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    y = kernels.linear_act(x, w, b, activation="relu")
+    db, = torch.autograd.grad(y, b, torch.ones_like(y))
+    with torch.no_grad():
+        turned = 0
+        for n in range(0, N, 2048):
+            z = x.double() @ w[n:n + 2048].double().T + b[n:n + 2048].double()
+            low = (z.abs() < _low(dtype)) if dtype is HF else torch.zeros_like(z, dtype=torch.bool)     # fp16 keeps no smaller z
+            off = (db[n:n + 2048].double() - (z > 0).double().sum(0)).abs()
+            turned += int((off - low.sum(0)).clamp(min=0).sum())
+    assert float(db[7]) == 0.0 and turned <= 3, turned
