@@ -930,7 +930,8 @@ linear_dz_kernel(const __grid_constant__ DzParams p) {
 // its rounding).  So where z is kept for the backward pass, the values that such an error can carry across zero are summed up again in fp32
 // on the plain units, one in 15000 of them.  How large z is otherwise is read off its own row (a warp's 256 columns) and its own column
 // (the four rows), so that a row or a weight that is small as a whole counts as that; exact zeros stand.
-// Bound by the read of z.  No more than kMostAgain of 1024 values are summed up again, which bounds the time for values of any other spread.
+// Bound by the read of z and the few rows that are summed up: 30 us for 4096 x 8192 values with K = 5120 (10 for the read alone), 6 for 411 x 3648 with K = 7232.
+// Magnitudes are compared as pairs of integers (as floats 46 us).  No more than kMostAgain of 1024 values are summed up again, which bounds the time for values of any other spread.
 struct SignParams {
   const uint16_t *x, *w, *bias;
   uint16_t* z;
@@ -949,41 +950,47 @@ linear_sign_kernel(const __grid_constant__ SignParams p) {
   const int64_t c0 = (int64_t)blockIdx.x * kDzCols, c = c0 + lane * 8;
   const int64_t step = (int64_t)gridDim.y * (kDzThreads / 32) * kDzRows;
   for (int64_t m0 = ((int64_t)blockIdx.y * (kDzThreads / 32) + warp) * kDzRows; m0 < p.M; m0 += step) {
-    float a[kDzRows][8], row[kDzRows], col[8];
+    uint32_t a[kDzRows][4], row[kDzRows], col[4];            // magnitudes in pairs, as integers: they order as the numbers do
 #pragma unroll
     for (int r = 0; r < kDzRows; ++r) {
       const uint16_t* z = p.z + (m0 + r) * p.N + c;
-      uint32_t u[4] = {};
-      if (m0 + r < p.M) {
-        if (kVec) {
-          if (c < p.N) { const uint4 v = *reinterpret_cast<const uint4*>(z); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
-        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i < p.N) u[i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
-        }
-      }
-      float top = 0.0f;
+      for (int i = 0; i < 4; ++i) a[r][i] = 0u;
+      if (m0 + r >= p.M) continue;
+      if (kVec) {
+        if (c < p.N) { const uint4 v = *reinterpret_cast<const uint4*>(z); a[r][0] = v.x; a[r][1] = v.y; a[r][2] = v.z; a[r][3] = v.w; }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[r][i] = fabsf(to_f(u[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, p.fp16));
-        top = fmaxf(top, a[r][i]);
+        for (int i = 0; i < 8; ++i)
+          if (c + i < p.N) a[r][i >> 1] |= (uint32_t)z[i] << (16 * (i & 1));
       }
-      row[r] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    }
+#pragma unroll
+    for (int r = 0; r < kDzRows; ++r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[r][i] &= 0x7FFF7FFFu;
+      const uint32_t top = __vmaxu2(__vmaxu2(a[r][0], a[r][1]), __vmaxu2(a[r][2], a[r][3]));
+      const float most = p.reach * to_f(__reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16)), p.fp16);
+      row[r] = pack2(most, most, p.fp16) & 0x7FFF7FFFu;
     }
     const bool whole = m0 + kDzRows <= p.M;                  // fewer rows say nothing of a column
+    uint32_t any = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      col[i] = whole ? 0.0f : __int_as_float(0x7f800000);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t top = __vmaxu2(__vmaxu2(a[0][i], a[1][i]), __vmaxu2(a[2][i], a[3][i]));
+      col[i] = whole ? pack2(p.reach * to_f(top & 0xFFFFu, p.fp16), p.reach * to_f(top >> 16, p.fp16), p.fp16) & 0x7FFF7FFFu : 0x7FFF7FFFu;
 #pragma unroll
-      for (int r = 0; r < kDzRows; ++r) col[i] = fmaxf(col[i], a[r][i]);
+      for (int r = 0; r < kDzRows; ++r) any |= __vcmpltu2(a[r][i], __vminu2(row[r], col[i]));
     }
+    if (!__any_sync(0xffffffffu, any != 0u)) continue;
     uint32_t near = 0u;
 #pragma unroll
     for (int r = 0; r < kDzRows; ++r)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (a[r][i] > 0.0f && a[r][i] < p.reach * fminf(row[r], col[i])) near |= 1u << (r * 8 + i);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t is = __vcmpltu2(a[r][i], __vminu2(row[r], col[i])) & __vcmpgtu2(a[r][i], 0u);
+        near |= ((is & 1u) | (is >> 16 & 1u) << 1) << (r * 8 + 2 * i);
+      }
     for (int left = kMostAgain; left > 0; --left) {
       const uint32_t who = __ballot_sync(0xffffffffu, near != 0u);
       if (who == 0u) break;
@@ -992,14 +999,22 @@ linear_sign_kernel(const __grid_constant__ SignParams p) {
       const int64_t m = m0 + (bit >> 3), n = c0 + src * 8 + (bit & 7);
       const uint4 *xs = reinterpret_cast<const uint4*>(p.x + m * p.x_ld), *ws = reinterpret_cast<const uint4*>(p.w + n * p.K);
       float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll 4
-      for (int64_t k = lane; k < p.K / 8; k += 32) {
-        const uint4 f = __ldg(xs + k), g = __ldg(ws + k);
-        const uint32_t fs[4] = {f.x, f.y, f.z, f.w}, gs[4] = {g.x, g.y, g.z, g.w};
+      constexpr int kU = 8;                                  // pieces of both rows on their way at once
+      for (int64_t k0 = lane; k0 < p.K / 8; k0 += 32 * kU) {
+        uint4 f[kU], g[kU];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s0 = fmaf(to_f(fs[i] & 0xFFFFu, p.fp16), to_f(gs[i] & 0xFFFFu, p.fp16), s0);
-          s1 = fmaf(to_f(fs[i] >> 16, p.fp16), to_f(gs[i] >> 16, p.fp16), s1);
+        for (int u = 0; u < kU; ++u) {
+          f[u] = g[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (k0 + u * 32 < p.K / 8) { f[u] = __ldg(xs + k0 + u * 32); g[u] = __ldg(ws + k0 + u * 32); }
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const uint32_t fs[4] = {f[u].x, f[u].y, f[u].z, f[u].w}, gs[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s0 = fmaf(to_f(fs[i] & 0xFFFFu, p.fp16), to_f(gs[i] & 0xFFFFu, p.fp16), s0);
+            s1 = fmaf(to_f(fs[i] >> 16, p.fp16), to_f(gs[i] >> 16, p.fp16), s1);
+          }
         }
       }
       float s = s0 + s1;
