@@ -12,6 +12,7 @@
 //                        runs under the next tile's MMAs; the residual comes through registers meanwhile.
 //   linear_rows_kernel   128 weight rows times up to 256 activation rows on one CTA, K sliced over a cluster: few rows, narrow layers.
 //   linear_few_kernel    one to four rows of small layers on the plain units.
+// linear_sign_kernel follows where a relu's z is kept, and settles the sign of values near zero.
 // Bound by the tensor cores at the clock that the power cap leaves where tiles fill the GPU (8192 x 34816 x 5120: 2.1 ms, 1.4 PFLOP/s, what a
 // plain library product sustains), by HBM at a few rows (16 x 34816 x 5120: 58 us, 92% of the copy rate), by launch, first fetches and the
 // last tile's epilogue in between.

@@ -15,6 +15,10 @@
 // rows; whole rows come by bulk copies into a ring that is some rows ahead, so that loads go on through the sums over a row.
 // A thread has the same eight (or sixteen) columns of every row: the weights' gradients add up in its registers, and a second launch
 // adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value.
+//
+// Measured, bf16, with both weights: 8192 x 5120 forward 59 us (51 at the copy rate), backward 98 and 7 for the join (77); 4096 x 7168 into E4M3
+// blocks 42 (31.5); one row 3.7, launch included.  Next to memory the instructions of a value count: issue slots are 58 to 63 % taken.  Odd rows, 8192 x 5121
+// forward and backward: 752.
 #include "gb_blocks.cuh"
 
 #include <algorithm>

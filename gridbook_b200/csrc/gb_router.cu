@@ -15,6 +15,10 @@
 //
 // A warp takes a token, its logits in registers (a block takes one past 1024 experts).  Sums over tokens are fp32: a lane's own,
 // then the block's warps, then the blocks, each in a fixed order; counts are whole numbers, added in any order.
+//
+// Bound by instructions (one exponential and some ten others a logit) and by waits for the row, not by memory.  256 experts, measured: the choice of 8192 fp32
+// rows 10.4 us and its gradient 3.9 (2.7 for the bytes of both); the loss of 65536 bf16 rows 29, the join 8, the gradient 23 (10.6), issue slots 56 to
+// 63 % taken; one token's choice 5.5 from the caller's side, which is the launch.
 #include "gb_blocks.cuh"
 
 namespace {

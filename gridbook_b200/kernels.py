@@ -776,10 +776,10 @@ _EPILOGUES = {None: nat.EPI_NONE, "none": nat.EPI_NONE, "relu": nat.EPI_RELU, "g
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
                residual: torch.Tensor | None = None) -> torch.Tensor:
-    """act(x . weight^T + bias) + residual, one kernel: ``x`` [.., K] and ``weight`` [N, K] bf16 or fp16, ``bias`` [N] and ``residual`` [.., N] of
+    """act(x . weight^T + bias) + residual: ``x`` [.., K] and ``weight`` [N, K] bf16 or fp16, ``bias`` [N] and ``residual`` [.., N] of
     their type, sums and epilogue in fp32, one rounding.  ``activation``: None, "relu", "gelu" (by erf), "gelu_tanh" or "silu".  K is a
     multiple of 8.  Differentiable in all four, by backward passes alone; with an activation the forward pass keeps its argument,
-    rounded to the type."""
+    rounded to the type (a relu's near zero by a second sum in fp32, for its sign)."""
     if activation not in _EPILOGUES:
         raise ValueError(f"linear_act: activation {activation!r}; None, relu, gelu, gelu_tanh or silu expected")
     return nat.host("16-bit linear").linear_act(x, weight, bias, _EPILOGUES[activation], residual)
