@@ -47,12 +47,13 @@ GB_DEVINL void warp_sums(float& a, float& b) {
   a = __shfl_sync(kAll, v, 0);
   b = __shfl_sync(kAll, v, 16);
 }
-// e^(v - top) from v and -top log2 e: one rounding of the exponent, two units of the function.  (expf's ten instructions for each expert
-// were half of the loss's.)
+// e^(v - top), two roundings of the exponent and two units of the function; results below 2^-126 are zero, next to the largest term's one.  The difference
+// comes first: top log2 e rounded by itself is off by as much as the exponents are for logits far from zero, and passes fp32 for those
+// at the end of its range.  (expf's ten instructions for each expert were half of the loss's.)
 constexpr float kLog2e = 1.4426950408889634f;
-GB_DEVINL float exp_from(float v, float minus_top2) {
+GB_DEVINL float exp_from(float v, float top) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(v, kLog2e, minus_top2)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((v - top) * kLog2e));
   return r;
 }
 
@@ -338,7 +339,7 @@ balance_kernel(const __grid_constant__ BalanceParams p) {
     top = over_token<kGroup, true>(top, s_red);
     if (top == -inf) continue;                             // nothing to choose from
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], -top * kLog2e); total += v[i]; }
+    for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], top); total += v[i]; }
     total = over_token<kGroup, false>(total, s_red);
     const float r = 1.0f / total, z = top + logf(total);
 #pragma unroll
@@ -477,7 +478,7 @@ balance_grad_kernel(const __grid_constant__ BalanceParams p) {
       for (int i = 0; i < kPer; ++i) v[i] = 0.0f;
     } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], -top * kLog2e); total += v[i]; dot = fmaf(v[i], f[i], dot); }
+      for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], top); total += v[i]; dot = fmaf(v[i], f[i], dot); }
       if constexpr (kGroup == 32) {
         warp_sums(total, dot);
       } else {
