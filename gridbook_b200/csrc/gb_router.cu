@@ -341,10 +341,13 @@ balance_kernel(const __grid_constant__ BalanceParams p) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { v[i] = exp_from(v[i], top); total += v[i]; }
     total = over_token<kGroup, false>(total, s_red);
-    const float r = 1.0f / total, z = top + logf(total);
+    const float r = 1.0f / total;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[i], r, acc[i]);
-    z2 = fmaf(z, z, z2);
+    if (p.z_coef != 0.0f) {                                // without a z-loss no square of it, which may pass fp32
+      const float z = top + logf(total);
+      z2 = fmaf(z, z, z2);
+    }
     ++n;
     if (lane < p.topk && (uint64_t)id < (uint64_t)p.E) atomicAdd(&s_counts[id], 1);
     for (int j = lane + kGroup; j < p.topk; j += kGroup) {
