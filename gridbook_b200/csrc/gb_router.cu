@@ -7,7 +7,7 @@
 //     w_j = scale c_j / sum over the chosen of c   (or scale c_j)
 //     softmax, renormalised:  q = w / scale;   dl_j = scale q_j (dw_j - sum q dw)
 //     softmax:                dl_e = c_e (scale dw_e - sum over the chosen of scale dw c),  dw_e = 0 for the others
-//     sigmoid, renormalised:  S = sum c;       dl_j = scale / S (dw_j - sum c dw / S) c_j (1 - c_j)
+//     sigmoid, renormalised:  q = w / scale;   dl_j = scale q_j (dw_j - sum q dw) (1 - c_j)
 //     sigmoid:                dl_j = scale dw_j c_j (1 - c_j)
 // Balance.  Over the n tokens that count (the mask's, and with a logit above -inf), p = softmax(l) and z = log sum exp l,
 //     f_e = counts_e / (n topk),  P_e = sum p_e / n,   loss = coef E sum f P + z_coef sum z^2 / n
@@ -220,12 +220,12 @@ topk_grad_kernel(const __grid_constant__ TopkParams p) {
   for (int i = 0; i < kPer; ++i) dense[i] = 0.0f;
   if (p.sigmoid) {
     const float c = id >= 0 ? 1.0f / (1.0f + expf(-l)) : 0.0f, rest = 1.0f / (1.0f + expf(l));
-    float dc = dw;
-    if (p.renormalize) {
-      const float total = warp_sum(c), dot = warp_sum(c * dw);
-      dc = total == 0.0f ? 0.0f : (dw - dot / total) / total;
+    if (p.renormalize) {                                   // shares first: dw over a sum of small scores may pass fp32, and is multiplied by them again
+      const float total = warp_sum(c), q = total == 0.0f ? 0.0f : c / total, dot = warp_sum(q * dw);
+      mine = q * (dw - dot) * rest;
+    } else {
+      mine = dw * c * rest;
     }
-    mine = dc * c * rest;
   } else {
     const float top = warp_max(id >= 0 ? l : -__int_as_float(0x7F800000));
     const float e = id >= 0 ? expf(l - top) : 0.0f;
