@@ -211,8 +211,8 @@ GB_DEVINL void slopes(float (&v)[kN], int act) {
     case GB_EPI_SILU:
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const float s = weighted(1.0f, v[i]);
-        v[i] = s * fmaf(v[i], 1.0f - s, 1.0f);
+        const float s = weighted(1.0f, v[i]), c = fminf(fmaxf(v[i], -128.0f), 128.0f);     // s is 0 or 1 past these (z kept in fp16 may be infinite)
+        v[i] = s * fmaf(c, 1.0f - s, 1.0f);
       }
       break;
     default:
