@@ -12,7 +12,7 @@
 //                        runs under the next tile's MMAs; the residual comes through registers meanwhile.
 //   linear_rows_kernel   128 weight rows times up to 256 activation rows on one CTA, K sliced over a cluster: few rows, narrow layers.
 //   linear_few_kernel    one to four rows of small layers on the plain units.
-// linear_sign_kernel follows where a relu's z is kept, and settles the sign of values near zero.
+// linear_sign_kernel follows where a relu's z is kept, and settles the sign of values near zero, in z and Y alike.
 // Bound by the tensor cores at the clock that the power cap leaves where tiles fill the GPU (8192 x 34816 x 5120: 2.1 ms, 1.4 PFLOP/s, what a
 // plain library product sustains), by HBM at a few rows (16 x 34816 x 5120: 58 us, 92% of the copy rate), by launch, first fetches and the
 // last tile's epilogue in between.
@@ -930,13 +930,14 @@ linear_dz_kernel(const __grid_constant__ DzParams p) {
 // the sign of three values in 1.5 million: few, but each is a whole value of the gradient (2e-3 of an fp16 gradient's norm, ten times
 // its rounding).  So where z is kept for the backward pass, the values that such an error can carry across zero are summed up again in fp32
 // on the plain units, one in 15000 of them.  How large z is otherwise is read off its own row (a warp's 256 columns) and its own column
-// (the four rows), so that a row or a weight that is small as a whole counts as that; exact zeros stand.
+// (the four rows), so that a row or a weight that is small as a whole counts as that; exact zeros stand.  Y is written again from the same
+// sum, so that a value has a gradient where it is above zero and nowhere else.
 // Bound by the read of z and the few rows that are summed up: 30 us for 4096 x 8192 values with K = 5120 (10 for the read alone), 6 for 411 x 3648 with K = 7232.
 // Magnitudes are compared as pairs of integers (as floats 46 us).  No more than kMostAgain of 1024 values are summed up again, which bounds the time for values of any other spread.
 struct SignParams {
-  const uint16_t *x, *w, *bias;
-  uint16_t* z;
-  int64_t M, N, K, x_ld;
+  const uint16_t *x, *w, *bias, *r;
+  uint16_t *z, *y;
+  int64_t M, N, K, x_ld, r_ld;
   int fp16;
   float reach;
 };
@@ -1021,7 +1022,12 @@ linear_sign_kernel(const __grid_constant__ SignParams p) {
       float s = s0 + s1;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) p.z[m * p.N + n] = pack1(p.bias ? s + to_f(p.bias[n], p.fp16) : s, p.fp16);
+      if (lane == 0) {
+        if (p.bias) s += to_f(p.bias[n], p.fp16);
+        const float y = s < 0.0f ? 0.0f : s;
+        p.z[m * p.N + n] = pack1(s, p.fp16);
+        p.y[m * p.N + n] = pack1(p.r ? y + to_f(p.r[m * p.r_ld + n], p.fp16) : y, p.fp16);
+      }
     }
   }
 }
@@ -1379,8 +1385,10 @@ int run_signs(const Mats& m, const LinearParams& p, cudaStream_t st) {
   s.x = static_cast<const uint16_t*>(m.a);
   s.w = static_cast<const uint16_t*>(m.b);
   s.bias = p.bias;
+  s.r = p.r;
   s.z = p.z;
-  s.M = p.M; s.N = p.N; s.K = m.K; s.x_ld = m.a_ld;
+  s.y = p.d;
+  s.M = p.M; s.N = p.N; s.K = m.K; s.x_ld = m.a_ld; s.r_ld = p.r_ld;
   s.fp16 = p.fp16;
   s.reach = (float)ceil_div(m.K, 16) * 0x1p-24f;
   const int64_t cols = ceil_div(p.N, kDzCols), rows = std::min<int64_t>(ceil_div(p.M, kDzThreads / 32 * kDzRows), std::max<int64_t>(1, (int64_t)gb_sm_count() * 16 / cols));
@@ -1402,6 +1410,7 @@ int gb_linear_act(const void* x, int64_t x_ld, const void* w, const void* bias, 
   GB_REQUIRE(act >= GB_EPI_NONE && act <= GB_EPI_SILU, "unknown activation %d", act);
   GB_REQUIRE(aligned(x) && aligned(w) && aligned(y) && aligned(z) && x_ld >= K && x_ld % 8 == 0, "operands must be rows of whole 16-byte pieces");
   GB_REQUIRE(!r || r_ld >= N, "residual rows that do not overlap expected");
+  GB_REQUIRE(!r || r != y || !z || act != GB_EPI_RELU, "a relu whose z is kept adds its residual twice: it lies elsewhere than the result");
   int pairs = 0;
   rc = ready(&pairs);
   if (rc != GB_OK) return rc;

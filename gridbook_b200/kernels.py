@@ -779,7 +779,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """act(x . weight^T + bias) + residual: ``x`` [.., K] and ``weight`` [N, K] bf16 or fp16, ``bias`` [N] and ``residual`` [.., N] of
     their type, sums and epilogue in fp32, one rounding.  ``activation``: None, "relu", "gelu" (by erf), "gelu_tanh" or "silu".  K is a
     multiple of 8.  Differentiable in all four, by backward passes alone; with an activation the forward pass keeps its argument,
-    rounded to the type (a relu's near zero by a second sum in fp32, for its sign)."""
+    rounded to the type.  A relu's near zero is summed up again in fp32 for its sign, the result with it: what is above zero has a
+    gradient and nothing else, and such values may differ from those of a call that keeps nothing, by the tensor cores' rounding."""
     if activation not in _EPILOGUES:
         raise ValueError(f"linear_act: activation {activation!r}; None, relu, gelu, gelu_tanh or silu expected")
     return nat.host("16-bit linear").linear_act(x, weight, bias, _EPILOGUES[activation], residual)

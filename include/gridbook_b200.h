@@ -490,7 +490,8 @@ GB_API int gb_moe_unpermute_grad(const void* d_out, const void* y, int dtype, co
 /* gb_linear_act: z = X W^T + bias, Y = act(z) + R: X [M, K] with rows x_ld elements apart, W [N, K], bias [N] or NULL, R [M, N] with rows
  * r_ld apart or NULL, Y [M, N], all bf16 or all fp16, sums and epilogue in fp32, one rounding.  K and x_ld are multiples of 8,
  * operands 16-byte aligned.  z (NULL: not kept) is what gb_linear_act_grad takes, [M, N]; a relu's is summed up
- * again in fp32 where it is so near zero that its sign may be off.
+ * again in fp32 where it is so near zero that its sign may be off (no more than four of 1024 values), and Y with it: R may
+ * not lie in Y's place there.
  * gb_linear_act_grad: of dY (rows dy_ld apart), dX = dz W, dW = dz^T X, dbias = column sums of dz with dz = dY act'(z) rounded to
  * the type (the column sums take it before); any of the three NULL.  The workspace's size depends on what is asked for and on
  * dy_whole: dY 16-byte aligned and dy_ld a multiple of 8. */
