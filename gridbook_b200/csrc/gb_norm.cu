@@ -11,14 +11,17 @@
 //     du = b g dx,   dg = sum over its rows of b u dx,   dpw = sum over rows of du y_hat
 //     dy = du, or (du (o + pw) - y_hat mean(du (o + pw) y_hat)) / rms y
 //
-// Bound by memory: a row is read and written once, and used in registers and shared memory in between.  Blocks stay and walk the
+// A row is read and written once, and used in registers and shared memory in between.  Blocks stay and walk the
 // rows; whole rows come by bulk copies into a ring that is some rows ahead, so that loads go on through the sums over a row.
 // A thread has the same eight (or sixteen) columns of every row: the weights' gradients add up in its registers, and a second launch
-// adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value.
+// adds the blocks' sums, in their order.  Rows that are no whole 16-byte pieces, and very long ones, go value by value; backward also
+// fp32 rows of 7571 to 8192 values with both weights and a gate for each channel, which leave no room for the weights beside one row.
 //
 // Measured, bf16, with both weights: 8192 x 5120 forward 59 us (51 at the copy rate), backward 98 and 7 for the join (77); 4096 x 7168 into E4M3
-// blocks 42 (31.5); one row 3.7, launch included.  Next to memory the instructions of a value count: issue slots are 58 to 63 % taken.  Odd rows, 8192 x 5121
-// forward and backward: 752.
+// blocks 42 (31.5); one row 3.7, launch included.  Cold, DRAM is 67, 59 and 47 % busy, issue slots 58 to 63 %, with a third of the warps that an SM
+// holds: no single pipe is full; what is left are the waits at the row's barriers with few warps beside.  Odd rows, 8192 x 5121
+// forward and backward: 752.  Backward past 5120 columns a block has 1024 threads of 64 registers, which the sums do not all fit (2048 x 16384
+// forward and backward 308, 82 at the copy rate).
 #include "gb_blocks.cuh"
 
 #include <algorithm>
@@ -183,9 +186,10 @@ GB_DEVINL void store8(typename T::word* p, const Raw8<T>& r) {
 }
 template <typename T>
 GB_DEVINL void store8(typename T::word* p, const F8& f) { store8<T>(p, rounded<T>(f)); }
-// What a launch has is known to the compiler in the forms that models have: rows of exactly kV x 8 columns a thread, weights of the rows'
-// own type with nothing added, all gradients there and asked for.  (Bounds, types and absent inputs looked at for every eight
-// columns were a third of the instructions: 8192 x 5120 bf16 forward 66 us, backward 116.)
+// What a launch has is known to the compiler in the commonest forms: rows of exactly kV x 8 columns a thread, weights of the rows'
+// own type with nothing added, all gradients there and asked for.  The others (other widths, weights around zero, fp32 weights, a gate for each
+// sequence) look at bounds, types and absent inputs for every eight columns, a third of the instructions: 8192 x 5120 bf16
+// forward 66 us, backward 116.
 enum Form { kAny = 0, kPostGate = 1, kPost = 2, kPre = 3 };          // both norms with a gate that rows share, without a gate; the second norm alone
 
 // Weights of eight columns in shared memory (of the longest rows, which fill it, where they lie), o + w; kRaw: of the rows' own type, o zero.

@@ -13,12 +13,15 @@
 //     f_e = counts_e / (n topk),  P_e = sum p_e / n,   loss = coef E sum f P + z_coef sum z^2 / n
 //     dl_te = d_loss / n p_te (coef E (f_e - sum f p_t) + 2 z_coef z_t)
 //
-// A warp takes a token, its logits in registers (a block takes one past 1024 experts).  Sums over tokens are fp32: a lane's own,
+// A warp takes a token, its logits in registers; for the loss a block takes one past 1024 experts, the choice and its gradient keep to a warp
+// with up to 128 logits a lane.  Sums over tokens are fp32: a lane's own,
 // then the block's warps, then the blocks, each in a fixed order; counts are whole numbers, added in any order.
 //
-// Bound by instructions (one exponential and some ten others a logit) and by waits for the row, not by memory.  256 experts, measured: the choice of 8192 fp32
-// rows 10.4 us and its gradient 3.9 (2.7 for the bytes of both); the loss of 65536 bf16 rows 29, the join 8, the gradient 23 (10.6), issue slots 56 to
-// 63 % taken; one token's choice 5.5 from the caller's side, which is the launch.
+// The loss is bound by instructions (one exponential and some ten others a logit) and by waits for the row, the choice by the chain of its reductions, one
+// expert behind the other, neither by memory.  256 experts, measured in a stream of calls: the choice of 8192 fp32
+// rows 9.3 us and its gradient 4.0 (2.7 for the bytes of both); the loss of 65536 bf16 rows 28 with the join (22 and 10, overlapping), its gradient 21 (10.6); cold,
+// under the profiler, 31, 14 and 28, issue slots 56 to 63 % taken; one token's choice 5.5 from the caller's side, which is the launch.  Choices of 4096 bf16 rows, top-8: of 2048
+// experts 52, of 4096 57 (as softmax without renormalising 76 and 86), their gradients 6 to 11 (34 and 37).
 #include "gb_blocks.cuh"
 
 namespace {
